@@ -693,6 +693,10 @@ int64_t gemm_choose_bn(int64_t M, int64_t N, int64_t device) {
 }  // namespace
 
 void register_elementwise(pybind11::module& m);
+void register_paged8(pybind11::module& m);
+
+int* cfb_err_ptr(int device) { return err_ptr(device); }
+int cfb_num_sms(int device) { return num_sms(device); }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("error_buffer", &error_buffer);
@@ -740,4 +744,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
              "dp_epoch_bump");
   });
   register_elementwise(m);
+  register_paged8(m);
 }

@@ -1,0 +1,122 @@
+// Device helpers shared by the 8-bit paged KV cache kernels.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "paged8.h"
+
+namespace cfb {
+
+template <typename T>
+struct P8Io;
+template <>
+struct P8Io<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ __nv_bfloat16 cast(float a) { return __float2bfloat16(a); }
+};
+template <>
+struct P8Io<__half> {
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return __half22float2(*reinterpret_cast<__half2*>(&u));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ __half cast(float a) { return __float2half(a); }
+};
+
+template <int FMT>
+__device__ __forceinline__ constexpr float p8_levels() {
+  return FMT == kP8Int8 ? 127.f : 448.f;
+}
+
+// Four codes (one word) as two f16x2: (byte 0, byte 1) and (byte 2, byte 3).  Exact:
+// an e4m3 number is an f16 number; an int8 code with its sign bit flipped is the low
+// byte of the f16 number 1024 + 128 + code.
+template <int FMT>
+__device__ __forceinline__ void p8_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == kP8Int8) {
+    w ^= 0x80808080u;
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140);
+    uint32_t b = __byte_perm(w, 0x64646464u, 0x4342);
+    __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), bias);
+    __half2 y = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+    lo = *reinterpret_cast<uint32_t*>(&x);
+    hi = *reinterpret_cast<uint32_t*>(&y);
+  } else {
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n"
+        " cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  }
+}
+
+template <int FMT>
+__device__ __forceinline__ void p8_to_float(uint32_t w, float* f) {
+  uint32_t lo, hi;
+  p8_to_half<FMT>(w, lo, hi);
+  const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo));
+  const float2 b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+  f[0] = a.x;
+  f[1] = a.y;
+  f[2] = b.x;
+  f[3] = b.y;
+}
+
+// Four scaled values (|f| <= levels up to rounding) to codes, to nearest, ties to even.
+// A NaN gives code 0: its block's scale is not finite, so its value reads as NaN anyway.
+template <int FMT>
+__device__ __forceinline__ uint32_t p8_from_float(const float* f) {
+  if constexpr (FMT == kP8Int8) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = max(-127, min(127, __float2int_rn(f[i] == f[i] ? f[i] : 0.f)));
+      r |= (static_cast<uint32_t>(c) & 0xffu) << (8 * i);
+    }
+    return r;
+  } else {
+    float g[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = f[i] == f[i] ? f[i] : 0.f;
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(g[0], g[1]), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(g[2], g[3]), __NV_SATFINITE,
+                                                 __NV_E4M3);
+    return lo | (hi << 16);
+  }
+}
+
+// Physical page of a logical one; an entry outside the pool is reported and read as page 0.
+__device__ __forceinline__ int64_t p8_page(const int32_t* row, int i, int64_t num_pages, int* err,
+                                           int site) {
+  const int p = __ldg(row + i);
+  if (static_cast<uint32_t>(p) >= static_cast<uint64_t>(num_pages)) {
+    report_error(err, kErrBounds, site);
+    return 0;
+  }
+  return p;
+}
+
+// Cached length of a sequence, held to what its page-table row can describe.
+__device__ __forceinline__ int p8_len(const int32_t* kv_lens, int seq, int max_pages, int* err,
+                                      int site) {
+  const int n = __ldg(kv_lens + seq);
+  if (n < 0 || n > max_pages * kP8Page) {
+    report_error(err, kErrBounds, site);
+    return n < 0 ? 0 : max_pages * kP8Page;
+  }
+  return n;
+}
+
+}  // namespace cfb

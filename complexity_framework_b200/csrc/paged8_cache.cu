@@ -1,0 +1,473 @@
+// The 8-bit paged KV cache: quantising append, read-back, eviction (sm_100a).
+//
+// A block is one page (16 tokens) of one head's keys or values, with one fp32 scale s;
+// a code c stands for c * s.  All three kernels move bytes: what bounds them is HBM
+// bandwidth for long inputs and launch latency for a decode step.
+#include "paged8.cuh"
+
+namespace cfb {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+// ---------------------------------------------------------------------------- append
+// For the new tokens x of a block with scale s0 (0 when it holds no older token):
+//   s = max(s0, max|x| / levels), code = round(x / s), and where s > s0 the older codes
+//   become round(code * s0 / s).
+// One warp owns a (block, head, K or V): the block's maximum is one warp reduction and
+// nothing is shared between warps.  A lane holds 8 values (16 bytes) of each of D / 16
+// loads, all issued before the reduction.  max|x| is taken on the bit patterns, which
+// order as the magnitudes do and let a NaN through to the scale.
+//
+// Blocks are enumerated without reading lengths on the host: sequence i's blocks either
+// start at item i * per_seq (per_seq bounds the blocks a chunk of max_q_len touches), or,
+// when chunks are uneven, at floor(cu_q[i] / 16) + 2 i, which leaves room for each
+// sequence's at most floor(q / 16) + 2 blocks; the host takes the smaller enumeration.
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(256)
+    p8_append_kernel(P8Cache c, P8Seqs s, const T* __restrict__ k, int64_t k_stride,
+                     const T* __restrict__ v, int64_t v_stride, int64_t N, int64_t units,
+                     int per_seq, int* err) {
+  constexpr int CH = D / 8;        // lanes of a row
+  constexpr int RPL = 32 / CH;     // rows of one load
+  constexpr int NL = kP8Page / RPL;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (unit >= units) return;
+  const int hx = static_cast<int>(unit % (2 * c.Hkv));
+  const int64_t item = unit / (2 * c.Hkv);
+  int seq;
+  int64_t j;
+  if (per_seq > 0) {
+    seq = static_cast<int>(item / per_seq);
+    j = item % per_seq;
+  } else {
+    int lo = 0, hi = s.num_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (__ldg(s.cu_q + mid) / kP8Page + 2 * static_cast<int64_t>(mid) <= item) lo = mid;
+      else hi = mid - 1;
+    }
+    seq = lo;
+    j = item - (__ldg(s.cu_q + seq) / kP8Page + 2 * static_cast<int64_t>(seq));
+  }
+  const int row0 = __ldg(s.cu_q + seq);
+  const int q_len = __ldg(s.cu_q + seq + 1) - row0;
+  const int kv = p8_len(s.kv_lens, seq, s.max_pages, err, 60);
+  const int start = kv - q_len;                       // position of row0's token
+  const int first = max(start, 0);
+  const int64_t blk = first / kP8Page + j;
+  if (q_len <= 0 || blk * kP8Page >= kv) return;
+  if (per_seq > 0 && j == per_seq - 1 && (blk + 1) * kP8Page < kv) {
+    if (lane == 0) report_error(err, kErrBounds, 59);  // the chunk is longer than max_q_len
+  }
+  if (row0 < 0 || static_cast<int64_t>(row0) + q_len > N) {
+    if (lane == 0) report_error(err, kErrBounds, 61);
+    return;
+  }
+  const int base = static_cast<int>(blk) * kP8Page;
+  const int lo = max(first, base) - base, hi = min(kv - base, kP8Page);  // new tokens of the block
+  const int h = hx >> 1, x = hx & 1;
+  const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages,
+                               static_cast<int>(blk), c.num_pages, err, 62);
+  const int64_t ph = (page * c.Hkv + h) * 2 + x;
+  float* scale = c.scales + ph;
+  uint8_t* codes = c.codes + ph * (kP8Page * D);
+  const T* src = x ? v : k;
+  const int64_t stride = x ? v_stride : k_stride;
+  const int r = lane / CH, col = (lane % CH) * 8;
+
+  uint4 in[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int t = i * RPL + r;
+    in[i] = make_uint4(0, 0, 0, 0);
+    if (t >= lo && t < hi)
+      in[i] = __ldg(reinterpret_cast<const uint4*>(
+          src + static_cast<int64_t>(row0 + base + t - start) * stride + h * D + col));
+  }
+  const float s0 = lo > 0 ? *scale : 0.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const uint32_t w[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = P8Io<T>::unpack(w[e]);
+      top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    }
+  }
+  top = __reduce_max_sync(kFull, top);
+  const float sn = __fdiv_rn(__uint_as_float(top), p8_levels<FMT>());
+  const float sc = (sn > s0 || sn != sn) ? sn : s0;
+  const float inv = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
+  const bool tiny = isinf(inv);  // a subnormal scale: divide instead
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int t = i * RPL + r;
+    if (t < lo || t >= hi) continue;
+    const uint32_t w[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 p = P8Io<T>::unpack(w[e]);
+      f[2 * e] = tiny ? __fdiv_rn(p.x, sc) : p.x * inv;
+      f[2 * e + 1] = tiny ? __fdiv_rn(p.y, sc) : p.y * inv;
+    }
+    *reinterpret_cast<uint2*>(codes + t * D + col) =
+        make_uint2(p8_from_float<FMT>(f), p8_from_float<FMT>(f + 4));
+  }
+  if (lo > 0 && sc != s0) {  // the scale grew: the older codes follow it
+    const float ratio = sc > 0.f ? __fdiv_rn(s0, sc) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int t = i * RPL + r;
+      if (t >= lo) continue;
+      uint2* at = reinterpret_cast<uint2*>(codes + t * D + col);
+      const uint2 old = *at;
+      float f[8];
+      p8_to_float<FMT>(old.x, f);
+      p8_to_float<FMT>(old.y, f + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= ratio;
+      *at = make_uint2(p8_from_float<FMT>(f), p8_from_float<FMT>(f + 4));
+    }
+  }
+  if (lane == 0 && (sc != s0 || lo == 0)) *scale = sc;
+}
+
+// ------------------------------------------------------------------------------ read
+// One warp per (layer, sequence, page, head, K or V): 16 codes a lane and load, the
+// values rounded once to the output's type.
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(256)
+    p8_read_kernel(P8Cache c, P8Seqs s, int64_t units, T* __restrict__ k_out,
+                   T* __restrict__ v_out, int* err) {
+  constexpr int NC = kP8Page * D / 16 / 32;  // 16-code chunks of a lane
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (unit >= units) return;
+  const int x = static_cast<int>(unit & 1);
+  int64_t u = unit >> 1;
+  const int h = static_cast<int>(u % c.Hkv);
+  u /= c.Hkv;
+  const int blk = static_cast<int>(u % s.max_pages);
+  u /= s.max_pages;
+  const int seq = static_cast<int>(u % s.num_seqs);
+  const int64_t layer = u / s.num_seqs;
+  const int kv = p8_len(s.kv_lens, seq, s.max_pages, err, 63);
+  const int live = min(kv - blk * kP8Page, kP8Page);  // tokens of the block, may be <= 0
+  const int64_t Lp = static_cast<int64_t>(s.max_pages) * kP8Page;
+  T* dst = (x ? v_out : k_out) +
+           (((layer * s.num_seqs + seq) * c.Hkv + h) * Lp + blk * kP8Page) * D;
+  const uint8_t* src = nullptr;
+  float sc = 0.f;
+  if (live > 0) {
+    const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages, blk,
+                                 c.num_pages, err, 64);
+    const int64_t ph = ((layer * c.num_pages + page) * c.Hkv + h) * 2 + x;
+    sc = __ldg(c.scales + ph);
+    src = c.codes + ph * (kP8Page * D);
+  }
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int e = (i * 32 + lane) * 16;
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (e / D < live) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + e));
+      float f[16];
+      p8_to_float<FMT>(w.x, f);
+      p8_to_float<FMT>(w.y, f + 4);
+      p8_to_float<FMT>(w.z, f + 8);
+      p8_to_float<FMT>(w.w, f + 12);
+      uint32_t o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = P8Io<T>::pack(f[2 * j] * sc, f[2 * j + 1] * sc);
+      a = make_uint4(o[0], o[1], o[2], o[3]);
+      b = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+    reinterpret_cast<uint4*>(dst + e)[0] = a;
+    reinterpret_cast<uint4*>(dst + e)[1] = b;
+  }
+}
+
+// ----------------------------------------------------------------------------- evict
+// Select: one CTA per (layer, sequence, head) finds the k = budget - recent largest of
+// the n = len - recent older masses by a radix select on order-preserving 32-bit keys
+// (four 8-bit digits, each a histogram in shared memory), then writes the kept indices
+// in order: everything above the k-th key, and of its equals the lowest indices.
+constexpr int kSelThreads = 256;
+constexpr int kSelKeys = 40 * 1024;  // keys held in shared memory; longer rows re-read global
+
+__device__ __forceinline__ uint32_t mass_key(float m) {
+  const uint32_t u = __float_as_uint(m + 0.f);  // -0 and 0 are one key
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+__global__ void __launch_bounds__(kSelThreads)
+    p8_select_kernel(P8Cache c, P8Seqs s, const float* __restrict__ mass, int budget, int recent,
+                     int32_t* __restrict__ keep, int cap, int* err) {
+  extern __shared__ uint32_t s_keys[];
+  __shared__ int s_hist[256];
+  __shared__ int s_scan[kSelThreads / 32][2];
+  __shared__ int s_digit, s_need;
+  const int h = blockIdx.x, seq = blockIdx.y;
+  const int64_t layer = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int len = p8_len(s.kv_lens, seq, s.max_pages, err, 65);
+  int32_t* row = keep + ((layer * s.num_seqs + seq) * c.Hkv + h) * budget;
+  if (len <= budget) {
+    for (int i = tid; i < budget; i += kSelThreads) row[i] = i < len ? i : -1;
+    return;
+  }
+  const int n = len - recent, k = budget - recent;
+  const int32_t* table = s.table + static_cast<int64_t>(seq) * s.max_pages;
+  const float* m = mass + layer * c.num_pages * c.Hkv * kP8Page;
+  auto fetch = [&](int i) {
+    const int64_t page = p8_page(table, i / kP8Page, c.num_pages, err, 66);
+    return mass_key(__ldg(m + (page * c.Hkv + h) * kP8Page + i % kP8Page));
+  };
+  const bool held = n <= cap;
+  if (held)
+    for (int i = tid; i < n; i += kSelThreads) s_keys[i] = fetch(i);
+  auto key = [&](int i) { return held ? s_keys[i] : fetch(i); };
+  uint32_t prefix = 0, mask = 0;
+  int need = k;  // of the keys that match the prefix, how many are kept
+  if (k > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += kSelThreads) s_hist[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += kSelThreads) {
+        const uint32_t u = key(i);
+        if ((u & mask) == prefix) atomicAdd(&s_hist[(u >> shift) & 255], 1);
+      }
+      __syncthreads();
+      if (warp == 0) {  // the digit whose suffix sum first reaches `need`
+        int cnt[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          cnt[i] = s_hist[255 - (lane * 8 + i)];
+          sum += cnt[i];
+        }
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(kFull, inc, o);
+          if (lane >= o) inc += y;
+        }
+        int before = inc - sum;
+        if (before < need && inc >= need) {
+          int i = 0;
+          while (before + cnt[i] < need) before += cnt[i++];
+          s_digit = 255 - (lane * 8 + i);
+          s_need = need - before;
+        }
+      }
+      __syncthreads();
+      prefix |= static_cast<uint32_t>(s_digit) << shift;
+      mask |= 0xffu << shift;
+      need = s_need;
+    }
+    // ordered write: each thread owns a contiguous stretch of the older tokens
+    const int per = (n + kSelThreads - 1) / kSelThreads;
+    const int a = min(n, tid * per), b = min(n, a + per);
+    int gt = 0, eq = 0;
+    for (int i = a; i < b; ++i) {
+      const uint32_t u = key(i);
+      gt += u > prefix;
+      eq += u == prefix;
+    }
+    int igt = gt, ieq = eq;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(kFull, igt, o), z = __shfl_up_sync(kFull, ieq, o);
+      if (lane >= o) {
+        igt += y;
+        ieq += z;
+      }
+    }
+    if (lane == 31) {
+      s_scan[warp][0] = igt;
+      s_scan[warp][1] = ieq;
+    }
+    __syncthreads();
+    gt = igt - gt;
+    eq = ieq - eq;
+    for (int w = 0; w < warp; ++w) {
+      gt += s_scan[w][0];
+      eq += s_scan[w][1];
+    }
+    for (int i = a; i < b; ++i) {
+      const uint32_t u = key(i);
+      if (u > prefix || (u == prefix && eq < need)) row[gt + min(eq, need)] = i;
+      gt += u > prefix;
+      eq += u == prefix;
+    }
+  }
+  for (int i = tid; i < recent; i += kSelThreads) row[k + i] = n + i;
+}
+
+// Move: one warp per (layer, sequence, head, new block).  The block's scale is the
+// largest among its tokens' old blocks, so a token from that block keeps its codes and
+// the others are rounded once more: code = round(code * s_old / s).
+template <int FMT, int D>
+__global__ void __launch_bounds__(256)
+    p8_move_kernel(P8Cache c, P8Seqs s, float* __restrict__ mass, int layers,
+                   const int32_t* __restrict__ dst_table, int dst_pages, int budget,
+                   const int32_t* __restrict__ keep, int64_t units, int* err) {
+  constexpr int CPR = D / 16;                 // 16-code chunks of a row
+  constexpr int NC = 2 * kP8Page * CPR / 32;  // chunks of a lane, K and V
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (unit >= units) return;
+  int64_t u = unit;
+  const int h = static_cast<int>(u % c.Hkv);
+  u /= c.Hkv;
+  const int blk = static_cast<int>(u % dst_pages);
+  u /= dst_pages;
+  const int seq = static_cast<int>(u % s.num_seqs);
+  const int64_t layer = u / s.num_seqs;
+  const int len = p8_len(s.kv_lens, seq, s.max_pages, err, 67);
+  const int kept = min(len, budget);
+  const int live = min(kept - blk * kP8Page, kP8Page);
+  if (live <= 0) return;
+  if (blk == dst_pages - 1 && kept > dst_pages * kP8Page && lane == 0)
+    report_error(err, kErrBounds, 58);  // the new pages are too few
+  const int64_t dpage = p8_page(dst_table + static_cast<int64_t>(seq) * dst_pages, blk,
+                                c.num_pages, err, 68);
+  const int64_t dph = (layer * c.num_pages + dpage) * c.Hkv + h;
+  const int32_t* row = keep + ((layer * s.num_seqs + seq) * c.Hkv + h) * budget + blk * kP8Page;
+  // lanes 0-15 look up the block's tokens
+  int64_t sph = 0;
+  int off = 0;
+  float2 sc = make_float2(0.f, 0.f);
+  float m = 0.f;
+  if (lane < live) {
+    const int i = __ldg(row + lane);
+    const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages, i / kP8Page,
+                                 c.num_pages, err, 69);
+    sph = (layer * c.num_pages + page) * c.Hkv + h;
+    off = i % kP8Page;
+    sc = __ldg(reinterpret_cast<const float2*>(c.scales) + sph);
+    if (mass != nullptr) m = mass[sph * kP8Page + off];
+  }
+  uint32_t kb = __float_as_uint(sc.x), vb = __float_as_uint(sc.y);  // scales are >= 0 or NaN
+  kb = __reduce_max_sync(kFull, kb);
+  vb = __reduce_max_sync(kFull, vb);
+  const float top[2] = {__uint_as_float(kb), __uint_as_float(vb)};
+  uint4 w[NC];
+  float ratio[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int e = i * 32 + lane;
+    const int x = e / (kP8Page * CPR), t = e / CPR % kP8Page, ch = e % CPR;
+    const int64_t p = __shfl_sync(kFull, sph, t);
+    const int o = __shfl_sync(kFull, off, t);
+    const float so = x ? __shfl_sync(kFull, sc.y, t) : __shfl_sync(kFull, sc.x, t);
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (t < live)
+      w[i] = __ldg(reinterpret_cast<const uint4*>(c.codes + ((p * 2 + x) * kP8Page + o) * D) + ch);
+    ratio[i] = so == top[x] ? 1.f : __fdiv_rn(so, top[x]);
+  }
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    if (ratio[i] != 1.f) {
+      uint32_t* q = reinterpret_cast<uint32_t*>(&w[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[4];
+        p8_to_float<FMT>(q[j], f);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) f[z] *= ratio[i];
+        q[j] = p8_from_float<FMT>(f);
+      }
+    }
+    reinterpret_cast<uint4*>(c.codes + dph * (2 * kP8Page * D))[i * 32 + lane] = w[i];
+  }
+  if (lane == 0) reinterpret_cast<float2*>(c.scales)[dph] = make_float2(top[0], top[1]);
+  if (mass != nullptr && lane < kP8Page) mass[dph * kP8Page + lane] = m;
+}
+
+template <typename T, int FMT, int D>
+void launch_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t ks, const void* v,
+                   int64_t vs, int64_t N, int64_t items, int per_seq, int* err, cudaStream_t st) {
+  const int64_t units = items * 2 * c.Hkv;
+  p8_append_kernel<T, FMT, D><<<static_cast<unsigned>((units + 7) / 8), 256, 0, st>>>(
+      c, s, static_cast<const T*>(k), ks, static_cast<const T*>(v), vs, N, units, per_seq, err);
+}
+
+}  // namespace
+
+#define CFB_P8_TYPES(CALL)                                     \
+  do {                                                         \
+    const int key_ = type * 4 + c.fmt * 2 + (c.D == 128);      \
+    switch (key_) {                                            \
+      case 0: CALL(__nv_bfloat16, kP8Int8, 64); break;         \
+      case 1: CALL(__nv_bfloat16, kP8Int8, 128); break;        \
+      case 2: CALL(__nv_bfloat16, kP8E4m3, 64); break;         \
+      case 3: CALL(__nv_bfloat16, kP8E4m3, 128); break;        \
+      case 4: CALL(__half, kP8Int8, 64); break;                \
+      case 5: CALL(__half, kP8Int8, 128); break;               \
+      case 6: CALL(__half, kP8E4m3, 64); break;                \
+      case 7: CALL(__half, kP8E4m3, 128); break;               \
+      default: return -2;                                      \
+    }                                                          \
+  } while (0)
+
+int p8_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t k_stride, const void* v,
+              int64_t v_stride, int64_t N, int max_q_len, int type, int* err,
+              cudaStream_t stream) {
+  if (N <= 0 || s.num_seqs <= 0) return 0;
+  const int64_t per_seq = (max_q_len + kP8Page - 2) / kP8Page + 1;
+  const int64_t even = per_seq * s.num_seqs, uneven = N / kP8Page + 2 * s.num_seqs;
+  const int64_t items = even <= uneven ? even : uneven;
+  if ((items * 2 * c.Hkv + 7) / 8 > 0x7fffffff) return -3;
+  const int ps = even <= uneven ? static_cast<int>(per_seq) : 0;
+#define CFB_CALL(T, F, DD) \
+  launch_append<T, F, DD>(c, s, k, k_stride, v, v_stride, N, items, ps, err, stream)
+  CFB_P8_TYPES(CFB_CALL);
+#undef CFB_CALL
+  return static_cast<int>(cudaGetLastError());
+}
+
+int p8_read(const P8Cache& c, const P8Seqs& s, int layers, void* k_out, void* v_out, int type,
+            int* err, cudaStream_t stream) {
+  const int64_t units =
+      static_cast<int64_t>(layers) * s.num_seqs * s.max_pages * c.Hkv * 2;
+  if (units <= 0) return 0;
+  if ((units + 7) / 8 > 0x7fffffff) return -3;
+  const unsigned grid = static_cast<unsigned>((units + 7) / 8);
+#define CFB_CALL(T, F, DD)                                                              \
+  p8_read_kernel<T, F, DD><<<grid, 256, 0, stream>>>(c, s, units, static_cast<T*>(k_out), \
+                                                     static_cast<T*>(v_out), err)
+  CFB_P8_TYPES(CFB_CALL);
+#undef CFB_CALL
+  return static_cast<int>(cudaGetLastError());
+}
+
+int p8_evict(const P8Cache& c, const P8Seqs& s, float* mass, int layers, const int32_t* dst_table,
+             int dst_pages, int budget, int recent, int32_t* keep, int* err,
+             cudaStream_t stream) {
+  if (s.num_seqs <= 0 || layers <= 0) return 0;
+  if (s.num_seqs > 65535 || layers > 65535) return -3;
+  const int64_t units =
+      static_cast<int64_t>(layers) * s.num_seqs * dst_pages * c.Hkv;
+  if ((units + 7) / 8 > 0x7fffffff) return -3;
+  const int longest = s.max_pages * kP8Page;
+  const int cap = longest < kSelKeys ? longest : kSelKeys;
+  const int smem = cap * 4;
+  if (cudaFuncSetAttribute(p8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
+    return static_cast<int>(cudaGetLastError());
+  p8_select_kernel<<<dim3(c.Hkv, s.num_seqs, layers), kSelThreads, smem, stream>>>(
+      c, s, mass, budget, recent, keep, cap, err);
+  const unsigned grid = static_cast<unsigned>((units + 7) / 8);
+  const int type = kP8Bf16;
+#define CFB_CALL(T, F, DD)                                                                    \
+  p8_move_kernel<F, DD><<<grid, 256, 0, stream>>>(c, s, mass, layers, dst_table, dst_pages,    \
+                                                  budget, keep, units, err)
+  CFB_P8_TYPES(CFB_CALL);
+#undef CFB_CALL
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace cfb

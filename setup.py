@@ -19,6 +19,9 @@ SOURCES = [
     "flash_fwd.cu",
     "flash_bwd.cu",
     "paged_attn.cu",
+    "bind_paged8.cpp",
+    "paged8_cache.cu",
+    "paged8_attn.cu",
     "dist_fused.cu",
     "noalloc.cu",
     "tp_fused.cu",
