@@ -151,7 +151,7 @@ void paged8_read(const Tensor& codes, const Tensor& scales, const Tensor& table,
 void paged8_attention(const Tensor& q, const Tensor& codes, const Tensor& scales,
                       const Tensor& table, const Tensor& cu_q, const Tensor& kv_lens, Tensor& out,
                       double scale, int64_t max_q_len, const c10::optional<Tensor>& mass_in,
-                      const c10::optional<Tensor>& mass_out) {
+                      const c10::optional<Tensor>& mass_out, int64_t workspace_bytes) {
   const cfb::P8Cache c = cache_of(codes, scales, false);
   const cfb::P8Seqs s = seqs_of(codes, table, kv_lens, cu_q);
   cfb::P8Attn a;
@@ -166,6 +166,7 @@ void paged8_attention(const Tensor& q, const Tensor& codes, const Tensor& scales
               "out must be contiguous, like q");
   TORCH_CHECK(max_q_len >= 1 && max_q_len * (Hq / c.Hkv) < (1ll << 30), "bad max_q_len");
   TORCH_CHECK(mass_in.has_value() == mass_out.has_value(), "mass needs both input and output");
+  TORCH_CHECK(scale > 0 && scale <= 3e38, "scale must be positive and finite");
   if (mass_out.has_value()) {
     a.mass_in = mass_of(*mass_in, codes, 0, "mass");
     a.mass_out = mass_of(*mass_out, codes, 0, "mass_out");
@@ -178,25 +179,53 @@ void paged8_attention(const Tensor& q, const Tensor& codes, const Tensor& scales
   a.scale = static_cast<float>(scale);
   if (N == 0 || s.num_seqs == 0) return;
   const c10::cuda::CUDAGuard g(codes.device());
-  a.splits = cfb::p8_attn_splits(s, c.Hkv, a.Hq / c.Hkv, a.max_q_len,
-                                 cfb_num_sms(codes.get_device()));
+  const int sms = cfb_num_sms(codes.get_device()), group = a.Hq / c.Hkv;
+  int* err = cfb_err_ptr(codes.get_device());
+  const auto stream = at::cuda::getCurrentCUDAStream();
   const auto f32 = torch::dtype(torch::kFloat32).device(codes.device());
-  Tensor ws_o, ws_lse, ws_s;
-  if (a.splits > 1) {
-    ws_o = torch::empty({N * Hq * a.splits * c.D}, f32);
-    a.ws_o = ws_o.data_ptr<float>();
+  const bool chunk = cfb::p8_is_chunk(a.max_q_len, group);
+  int64_t seqs_each = s.num_seqs;  // sequences expanded at a time, within the workspace limit
+  if (chunk) {
+    const int64_t each = static_cast<int64_t>(c.Hkv) * cfb::p8_chunk_blocks(s) * cfb::kP8Page * c.D;
+    seqs_each = std::max<int64_t>(1, std::min<int64_t>(s.num_seqs, workspace_bytes / (4 * each)));
+    cfb::p8_chunk_plan(s, c.Hkv, group, a.max_q_len, sms, &a.chunk_nq, &a.splits);
+    if (seqs_each < s.num_seqs) a.splits = 1;
+  } else {
+    a.splits = cfb::p8_attn_splits(s, c.Hkv, group, a.max_q_len, sms);
   }
-  if (a.splits > 1 || a.mass_out != nullptr) {
-    ws_lse = torch::empty({N * Hq * a.splits}, f32);
-    a.ws_lse = ws_lse.data_ptr<float>();
+  // one workspace: expanded K | V | their block scales | split outputs | log-sum-exps | scores
+  const bool mass = a.mass_out != nullptr;
+  const int64_t n_o = a.splits > 1 ? N * Hq * a.splits * c.D : 0;
+  const int64_t n_lse = a.splits > 1 || mass ? (N * Hq * a.splits + 3) / 4 * 4 : 0;
+  const int64_t blocks = cfb::p8_chunk_blocks(s);
+  const int64_t n_ks = chunk ? seqs_each * c.Hkv * blocks * 4 : 0;
+  const int64_t n_kv = chunk ? seqs_each * c.Hkv * blocks * cfb::kP8Page * c.D / 2 : 0;  // floats
+  const int64_t n_s = mass && !chunk ? N * Hq * s.max_pages * cfb::kP8Page : 0;
+  Tensor ws;
+  if (n_o + n_lse + n_ks + 2 * n_kv + n_s > 0) {
+    ws = torch::empty({2 * n_kv + n_o + n_lse + n_ks + n_s}, f32);
+    float* at = ws.data_ptr<float>();
+    a.ws_k = at;
+    a.ws_v = at + n_kv;
+    at += 2 * n_kv;
+    a.ws_par = at;
+    at += n_ks;
+    a.ws_o = n_o ? at : nullptr;
+    a.ws_lse = n_lse ? at + n_o : nullptr;
+    a.ws_s = at + n_o + n_lse;
   }
-  if (a.mass_out != nullptr) {
-    ws_s = torch::empty({N * Hq * s.max_pages * cfb::kP8Page}, f32);
-    a.ws_s = ws_s.data_ptr<float>();
+  if (!chunk) {
+    check_rc(cfb::p8_attention(c, s, a, err, stream), "paged8_attention");
+    return;
   }
-  check_rc(cfb::p8_attention(c, s, a, cfb_err_ptr(codes.get_device()),
-                             at::cuda::getCurrentCUDAStream()),
-           "paged8_attention");
+  for (int64_t i = 0; i < s.num_seqs; i += seqs_each) {
+    cfb::P8Seqs part = s;
+    part.table += i * s.max_pages;
+    part.cu_q += i;
+    part.kv_lens += i;
+    part.num_seqs = static_cast<int>(std::min<int64_t>(seqs_each, s.num_seqs - i));
+    check_rc(cfb::p8_chunk_attention(c, part, a, err, stream), "paged8_attention");
+  }
 }
 
 void paged8_evict(const Tensor& codes, const Tensor& scales, const Tensor& mass,

@@ -13,6 +13,7 @@ template <typename T>
 struct P8Io;
 template <>
 struct P8Io<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u));
   }
@@ -24,6 +25,7 @@ struct P8Io<__nv_bfloat16> {
 };
 template <>
 struct P8Io<__half> {
+  static constexpr bool kBf16 = false;
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return __half22float2(*reinterpret_cast<__half2*>(&u));
   }

@@ -53,9 +53,24 @@ struct P8Attn {
   int splits = 1;
   float* ws_o = nullptr;     // [N * Hq, splits, D] (splits > 1)
   float* ws_lse = nullptr;   // [N * Hq, splits] (splits > 1 or mass)
-  float* ws_s = nullptr;     // [N * Hq, max_pages * 16] scores (mass)
+  float* ws_s = nullptr;     // [N * Hq, max_pages * 16] scores (mass, short chunks)
+  // long chunks: keys and values as 16-bit operands, Lw = 16 * p8_chunk_blocks() tokens
+  int chunk_nq = 2;          // 128-row tiles of a CTA
+  void* ws_k = nullptr;      // [S, Hkv, Lw, D]
+  void* ws_v = nullptr;
+  void* ws_par = nullptr;    // float4 [S, Hkv, Lw / 16]
 };
 int p8_attn_splits(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_sms);
+// Joins the splits: out from ws_o and ws_lse; a row's first ws_lse becomes its total.
+int p8_combine(const P8Attn& a, int D, cudaStream_t stream);
+int p8_chunk_blocks(const P8Seqs& s);
+// Whether a call's chunks go to the tcgen05 kernels.
+bool p8_is_chunk(int max_q_len, int group);
+// Row tiles of a CTA and KV splits of the chunk kernel.
+void p8_chunk_plan(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_sms, int* nq,
+                   int* splits);
+int p8_chunk_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err,
+                       cudaStream_t stream);
 int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err,
                  cudaStream_t stream);
 

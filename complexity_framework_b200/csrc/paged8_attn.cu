@@ -268,11 +268,12 @@ __global__ void __launch_bounds__(kWarps * 32) p8_attn_kernel(const AttnParams p
       }
     // ---- w = s + log2(vs); a V block of (nearly) zeros adds to l alone
     const bool has_v = !(vs < kTinyScale);
-    if (has_v) {
+    const bool fine = vs <= 3.402823466e38f;
+    if (has_v && fine) {
       lv_last = __log2f(vs);
       rv_last = __fdividef(1.f, vs);
     }
-    const float lv = lv_last, rv = rv_last;
+    const float lv = fine ? lv_last : vs - vs, rv = rv_last;  // not finite: NaN
     const bool edge = key0 + kP8Page > min_lim;
     bool grow = false;
 #pragma unroll
@@ -281,13 +282,13 @@ __global__ void __launch_bounds__(kWarps * 32) p8_attn_kernel(const AttnParams p
       for (int e = 0; e < 4; ++e) {
         const int i = e & 1;  // row 2 t + i, token g + 8 (e / 2)
         float x = s[nb][e] * (ks * qs[nb][i]);
-        if (edge && key0 + g + 8 * (e >> 1) >= lim[nb][i]) x = -INFINITY;
+        const bool hidden = edge && key0 + g + 8 * (e >> 1) >= lim[nb][i];
         if constexpr (MASS) {
           const int r = first_row + nb * 8 + 2 * t + i;
           if (r < rows)
             p.ws_s[out_row(r) * p.s_stride + key0 + g + 8 * (e >> 1)] = x;
         }
-        s[nb][e] = x + lv;
+        s[nb][e] = hidden ? -INFINITY : x + lv;
         grow |= s[nb][e] > M[nb][i] + kGrow;
       }
     }
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(kWarps * 32) p8_attn_kernel(const AttnParams p
 template <typename T>
 __global__ void __launch_bounds__(128)
     p8_combine_kernel(const float* __restrict__ ws_o, float* __restrict__ ws_lse,
-                      T* __restrict__ out, int64_t rows, int splits, int D, int join) {
+                      T* __restrict__ out, int64_t rows, int splits, int D) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   if (row >= rows) return;
@@ -445,18 +446,16 @@ __global__ void __launch_bounds__(128)
   float den = 0.f;
   for (int s = 0; s < splits; ++s) den += ex2f(lse[s] - base);
   const float inv = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
-  if (join) {
-    for (int d = lane * 2; d < D; d += 64) {
-      float2 acc = make_float2(0.f, 0.f);
-      for (int s = 0; s < splits; ++s) {
-        const float w = ex2f(lse[s] - base);
-        if (w == 0.f) continue;
-        const float2 x = *reinterpret_cast<const float2*>(ws_o + (row * splits + s) * D + d);
-        acc.x += w * x.x;
-        acc.y += w * x.y;
-      }
-      *reinterpret_cast<uint32_t*>(out + row * D + d) = P8Io<T>::pack(acc.x * inv, acc.y * inv);
+  for (int d = lane * 2; d < D; d += 64) {
+    float2 acc = make_float2(0.f, 0.f);
+    for (int s = 0; s < splits; ++s) {
+      const float w = ex2f(lse[s] - base);
+      if (w == 0.f) continue;
+      const float2 x = *reinterpret_cast<const float2*>(ws_o + (row * splits + s) * D + d);
+      acc.x += w * x.x;
+      acc.y += w * x.y;
     }
+    *reinterpret_cast<uint32_t*>(out + row * D + d) = P8Io<T>::pack(acc.x * inv, acc.y * inv);
   }
   __syncwarp();
   if (lane == 0) lse[0] = den == 0.f ? -INFINITY : base + log2f(den);
@@ -506,10 +505,10 @@ int launch_attn(const AttnParams& p, const P8Attn& a, int rows, cudaStream_t st)
   const int rc = mass ? launch_nb<T, FMT, D, true>(p, rows, st)
                       : launch_nb<T, FMT, D, false>(p, rows, st);
   if (rc) return rc;
-  const int64_t n = a.N * a.Hq;
-  if (p.splits > 1 || mass)
-    p8_combine_kernel<T><<<static_cast<unsigned>((n + 3) / 4), 128, 0, st>>>(
-        a.ws_o, a.ws_lse, static_cast<T*>(a.out), n, p.splits, D, p.splits > 1);
+  if (p.splits > 1) {
+    const int rc = p8_combine(a, D, st);
+    if (rc) return rc;
+  }
   if (mass) {
     const int L = p.s.max_pages * kP8Page;
     p8_mass_kernel<<<dim3((L + 127) / 128, p.c.Hkv, p.s.num_seqs), 128, 0, st>>>(
@@ -520,6 +519,19 @@ int launch_attn(const AttnParams& p, const P8Attn& a, int rows, cudaStream_t st)
 }
 
 }  // namespace
+
+int p8_combine(const P8Attn& a, int D, cudaStream_t st) {
+  const int64_t n = a.N * a.Hq;
+  const int64_t grid = (n + 3) / 4;
+  if (grid > 0x7fffffff) return -3;
+  if (a.type == kP8Bf16)
+    p8_combine_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), 128, 0, st>>>(
+        a.ws_o, a.ws_lse, static_cast<__nv_bfloat16*>(a.out), n, a.splits, D);
+  else
+    p8_combine_kernel<__half><<<static_cast<unsigned>(grid), 128, 0, st>>>(
+        a.ws_o, a.ws_lse, static_cast<__half*>(a.out), n, a.splits, D);
+  return 0;
+}
 
 int p8_attn_splits(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_sms) {
   const int rows = max_q_len * group;

@@ -1,0 +1,860 @@
+// Attention over the 8-bit paged KV cache (sm_100a): long chunks of new tokens.
+//
+// With hundreds of rows (new tokens x grouped heads) for each KV head the work is bound by
+// the tensor cores and by exponentials, not by the cache's bytes, so it goes to tcgen05.
+// Every CTA of a KV head needs the same keys and values as 16-bit operands.  Converting
+// them in each CTA costs about as many instruction slots as its softmax; they are expanded
+// once instead, into a workspace that TMA reads back from L2:
+//   K as its codes in q's type, V as its codes in f16: both exact.  The block scales stay
+//   in fp32 and cost nothing: K's multiplies the softmax scale, log2 of V's is added in the
+//   exponent, so that P carries it (w = s + log2 vs, P = 2^(w - M), l = sum P / vs; see
+//   paged8_attn.cu), and P is rounded to f16.
+//
+// p8_chunk_kernel: one CTA per (NQ x 128 rows, KV head, sequence, KV split).  A row tile
+// packs floor(128 / G) tokens x G heads, so all the heads of a group share each K/V tile.
+//   warps 0 .. 4 NQ - 1  softmax, one row per thread: S from TMEM, running maximum with a
+//                        lazy rescale (only when it grows by more than 2^8), P back to TMEM
+//   next warp            TMA producer: Q once, then K / V tiles through a ring
+//   last warp            MMA issuer: O_x += P_x V, then S_x = Q_x K^T of the next tile
+// p8_chunk_mass_kernel: weights summed over the rows need each row's final log-sum-exp, so
+// they are recomputed: one CTA per (128 keys, KV head, sequence) walks the row tiles with
+// S^T = K Q^T (a thread owns a key), adding 2^(s - lse) in row order: no atomics, the same
+// bits every time.
+#include "paged8.cuh"
+
+#include "flash.h"
+
+namespace cfb {
+namespace {
+
+constexpr int kT = 128;               // rows of a tile, keys of a tile
+constexpr float kRescaleLog2 = 8.f;
+constexpr float kTinyScale = 7.888609e-31f;  // 2^-100: blocks below it count as zeros
+
+__device__ __forceinline__ float ex2c(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// kind::f16 instruction descriptor, fp32 accumulators: A and B both bf16 or both f16.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc16(int M, int N, bool b_mn) {
+  return (1u << 4) | (sizeof(T) == 2 && P8Io<T>::kBf16 ? (1u << 7) | (1u << 10) : 0u) |
+         ((b_mn ? 1u : 0u) << 16) | ((static_cast<uint32_t>(N) >> 3) << 17) |
+         ((static_cast<uint32_t>(M) >> 4) << 24);
+}
+
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > kWaitBoundNs) return;
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                          int* err, int code, int site) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code, site));
+}
+
+// ---------------------------------------------------------------------------- expand
+// One warp per (sequence, block, head, K or V) of the workspace
+//   k_ws, v_ws [S, Hkv, Lw, D],  par [S, Hkv, Lw / 16],  Lw a multiple of 128,
+// where par holds (ks * scale * log2 e, log2 vs, 1 / vs) of a block.  Tokens past the
+// sequence, up to the end of its last 128-key tile, become zeros.  A block whose V scale is
+// not finite gets V = 0 and a NaN K scale: the rows that see the block read NaN, and the rows
+// that do not are not reached by 0 * NaN.  A scale of (nearly) zero becomes zero codes with a
+// harmless scale: 1 for K, so that no masked score meets -inf * 0, and 2^-24 for V, so that
+// the block does not raise the bound of w.
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(256)
+    p8_expand_kernel(P8Cache c, P8Seqs s, int blocks, int64_t units, float scale_log2,
+                     T* __restrict__ k_ws, __half* __restrict__ v_ws, float4* __restrict__ par,
+                     int* err) {
+  constexpr int NC = kP8Page * D / 16 / 32;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (unit >= units) return;
+  const int x = static_cast<int>(unit & 1);
+  int64_t u = unit >> 1;
+  const int h = static_cast<int>(u % c.Hkv);
+  u /= c.Hkv;
+  const int blk = static_cast<int>(u % blocks);
+  const int seq = static_cast<int>(u / blocks);
+  const int kv = p8_len(s.kv_lens, seq, s.max_pages, err, 80);
+  if (blk * kP8Page >= (kv + kT - 1) / kT * kT) return;
+  const int64_t sh = static_cast<int64_t>(seq) * c.Hkv + h;
+  int live = min(kv - blk * kP8Page, kP8Page);
+  uint4* dst = reinterpret_cast<uint4*>(
+      (x ? reinterpret_cast<uint16_t*>(v_ws) : reinterpret_cast<uint16_t*>(k_ws)) +
+      (sh * blocks + blk) * (kP8Page * D));
+  const uint8_t* src = nullptr;
+  float4 f = make_float4(scale_log2, -24.f, 16777216.f, 0.f);
+  if (live > 0) {
+    const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages, blk,
+                                 c.num_pages, err, 81);
+    const int64_t ph = page * c.Hkv + h;
+    const float2 sc = __ldg(reinterpret_cast<const float2*>(c.scales) + ph);
+    const bool fine = fabsf(sc.y) <= 3.402823466e38f;
+    if (!(sc.x < kTinyScale)) f.x = sc.x * scale_log2;
+    if (!fine) f.x = __uint_as_float(0x7fc00000u);
+    if (fine && sc.y >= kTinyScale) {
+      f.y = log2f(sc.y);
+      f.z = __fdiv_rn(1.f, sc.y);
+    }
+    if (x == 0 ? sc.x < kTinyScale : !fine || sc.y < kTinyScale) live = 0;
+    src = c.codes + (ph * 2 + x) * (kP8Page * D);
+  }
+  if (x == 0 && lane == 0) par[sh * blocks + blk] = f;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int e = (i * 32 + lane) * 16;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    uint32_t o[8] = {};
+    if (e / D < live) {
+      w = __ldg(reinterpret_cast<const uint4*>(src + e));
+      const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p8_to_half<FMT>(in[j], o[2 * j], o[2 * j + 1]);
+        if (P8Io<T>::kBf16 && x == 0) {
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const float2 v = __half22float2(*reinterpret_cast<__half2*>(&o[2 * j + z]));
+            o[2 * j + z] = pack_bf16x2(v.x, v.y);
+          }
+        }
+      }
+    }
+    dst[2 * (i * 32 + lane)] = make_uint4(o[0], o[1], o[2], o[3]);
+    dst[2 * (i * 32 + lane) + 1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+// --------------------------------------------------------------------------- forward
+struct ChunkParams {
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  int max_pages, blocks;       // page-table width; workspace blocks of a sequence
+  const float4* par;           // block scales of the workspace
+  void* out;
+  float* lse;                  // [N * Hq, splits], log2 units (splits > 1, or for the weights)
+  float* ws_o;                 // [N * Hq, splits, D] (splits > 1)
+  int64_t N;
+  int Hq, Hkv, G, splits, row_ctas;
+  int* err;
+};
+
+template <int D, int NQ>
+struct ChunkCfg {
+  static constexpr int STAGES = D == 64 ? (NQ == 2 ? 4 : 2) : 2;
+  static constexpr int CHUNKS = D / 64;
+  static constexpr int Q_BYTES = kT * D * 2;
+  static constexpr int K_BYTES = kT * D * 2;
+  static constexpr int SMEM = NQ * Q_BYTES + STAGES * 2 * K_BYTES + 1024 + 512;
+  static constexpr uint32_t T_O = NQ * 128;
+  static constexpr uint32_t TMEM = NQ == 2 ? 512 : 256;
+  static constexpr int PRODUCER = 4 * NQ, MMA = 4 * NQ + 1;
+  static constexpr int THREADS = (4 * NQ + 2) * 32;
+  static_assert(T_O + NQ * D <= TMEM, "TMEM budget");
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+struct ChunkBars {
+  uint64_t q_full;
+  uint64_t kv_full[4];
+  uint64_t kv_empty[4];
+  uint64_t s_full[2];
+  uint64_t p_full[2];
+  uint64_t o_full[2];
+  uint64_t mma_done;
+  uint32_t tmem;
+  int abort;
+};
+
+template <typename T, int D, int NQ, int POLY>
+__global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
+    p8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
+                    const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV, const ChunkParams p) {
+  using Cfg = ChunkCfg<D, NQ>;
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + NQ * Cfg::Q_BYTES;
+  uint8_t* sV = sK + STAGES * Cfg::K_BYTES;
+  ChunkBars* bars = reinterpret_cast<ChunkBars*>(sV + STAGES * Cfg::K_BYTES);
+  volatile int* abort_flag = &bars->abort;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  // the last row tiles see the most keys: they go first
+  const int split = blockIdx.x % p.splits;
+  const int rc = p.row_ctas - 1 - static_cast<int>(blockIdx.x / p.splits);
+  const int h = blockIdx.y, seq = blockIdx.z;
+  const int row0 = __ldg(p.cu_q + seq), q_len = __ldg(p.cu_q + seq + 1) - row0;
+  if (row0 < 0 || q_len < 0 || static_cast<int64_t>(row0) + q_len > p.N) {
+    if (threadIdx.x == 0) report_error(p.err, kErrBounds, 82);
+    return;
+  }
+  const int kv = p8_len(p.kv_lens, seq, p.max_pages, p.err, 83);
+  const int TT = kT / p.G;                 // tokens of a row tile
+  const int tok0 = rc * NQ * TT;
+  if (rc == p.row_ctas - 1 && q_len > tok0 + NQ * TT && threadIdx.x == 0)
+    report_error(p.err, kErrBounds, 84);   // a chunk longer than max_q_len
+  if (tok0 >= q_len) return;
+  const int start = kv - q_len;
+  // key tiles of row tile x, and this split's share of them
+  auto tiles_of = [&](int x) {
+    const int t0 = tok0 + x * TT;
+    if (t0 >= q_len) return 0;
+    const int last = min(q_len, t0 + TT) - 1;
+    return (max(0, start + last + 1) + kT - 1) / kT;
+  };
+  int tiles = 0;
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) tiles = max(tiles, tiles_of(x));
+  const int per = (tiles + p.splits - 1) / p.splits;
+  const int j0 = split * per;
+  auto nkv_of = [&](int x) { return max(0, min(tiles_of(x), j0 + per) - j0); };
+  int nkv = 0;
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) nkv = max(nkv, nkv_of(x));
+  const int64_t sh = static_cast<int64_t>(seq) * p.Hkv + h;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&bars->kv_full[s], 1);
+      mbar_init(&bars->kv_empty[s], 1);
+    }
+    for (int x = 0; x < NQ; ++x) {
+      mbar_init(&bars->s_full[x], 1);
+      mbar_init(&bars->p_full[x], 4);
+      mbar_init(&bars->o_full[x], 1);
+    }
+    mbar_init(&bars->mma_done, 1);
+    bars->abort = 0;
+    fence_barrier_init();
+  }
+  {  // rows of a tile past its TT * G are no token's: zeros
+    const int used = TT * p.G;
+    const int rows = kT - used;
+    for (int i = threadIdx.x; i < NQ * Cfg::CHUNKS * rows * 8; i += blockDim.x) {
+      const int t = i / (rows * 8), r = i % (rows * 8);
+      *reinterpret_cast<uint4*>(sQ + t * (kT * 128) + used * 128 + r * 16) =
+          make_uint4(0, 0, 0, 0);
+    }
+    if (rows > 0) fence_proxy_async_shared();
+  }
+  if (warp == Cfg::MMA) tmem_alloc(&bars->tmem, Cfg::TMEM);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+
+  if (warp == Cfg::PRODUCER) {
+    if (nkv > 0 && elect_one()) {
+      int live = 0;
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) live += nkv_of(x) > 0;
+      mbar_arrive_expect_tx(&bars->q_full, live * Cfg::CHUNKS * TT * p.G * 128);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+        if (nkv_of(x) > 0)
+#pragma unroll
+          for (int c = 0; c < Cfg::CHUNKS; ++c)
+            tma_load_4d(sQ + x * Cfg::Q_BYTES + c * kT * 128, &tmQ, &bars->q_full, c * 64, 0, h,
+                        row0 + tok0 + x * TT);
+      int issued = 0;
+      for (int j = 0; j < nkv; ++j) {
+        const int st = j % STAGES;
+        if (!mbar_wait(&bars->kv_empty[st], ((j / STAGES) & 1) ^ 1, abort_flag, p.err,
+                       kErrTimeoutEmpty, 85))
+          break;
+        mbar_arrive_expect_tx(&bars->kv_full[st], 2 * Cfg::K_BYTES);
+#pragma unroll
+        for (int c = 0; c < Cfg::CHUNKS; ++c) {
+          tma_load_4d(sK + st * Cfg::K_BYTES + c * kT * 128, &tmK, &bars->kv_full[st], c * 64,
+                      (j0 + j) * kT, h, seq);
+          tma_load_4d(sV + st * Cfg::K_BYTES + c * kT * 128, &tmV, &bars->kv_full[st], c * 64,
+                      (j0 + j) * kT, h, seq);
+        }
+        ++issued;
+      }
+      drain(&bars->q_full, 0);
+      for (int j = issued - STAGES < 0 ? 0 : issued - STAGES; j < issued; ++j)
+        drain(&bars->kv_full[j % STAGES], (j / STAGES) & 1);
+    }
+  } else if (warp == Cfg::MMA) {
+    if (nkv > 0 && elect_one()) {
+      constexpr uint32_t IDESC_S = idesc16<T>(kT, kT, false);
+      constexpr uint32_t IDESC_PV = idesc16<__half>(kT, D, true);
+      int nkv_x[NQ];
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) nkv_x[x] = nkv_of(x);
+      bool ok = mbar_wait(&bars->q_full, 0, abort_flag, p.err, kErrTimeoutFull, 86);
+      auto issue_pv = [&](int x, int jp) -> bool {
+        if (!mbar_wait(&bars->p_full[x], jp & 1, abort_flag, p.err, kErrTimeoutFull, 87))
+          return false;
+        tc_fence_after();
+        const uint32_t v_base = smem_u32(sV + (jp % STAGES) * Cfg::K_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < kT / 16; ++kk)
+          umma_bf16_ts(tmem + Cfg::T_O + x * D, tmem + x * 128 + kk * 8,
+                       sw128_desc(v_base + kk * 2048, kT * 128, 1024), IDESC_PV,
+                       (jp > 0 || kk > 0) ? 1u : 0u);
+        return true;
+      };
+      for (int j = 0; j <= nkv && ok; ++j) {
+        const int st = j % STAGES;
+        if (j < nkv && !mbar_wait(&bars->kv_full[st], (j / STAGES) & 1, abort_flag, p.err,
+                                  kErrTimeoutFull, 88)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t k_base = smem_u32(sK + st * Cfg::K_BYTES);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          if (j > 0 && j - 1 < nkv_x[x]) {
+            if (!issue_pv(x, j - 1)) {
+              ok = false;
+              break;
+            }
+            if (j - 1 == nkv_x[x] - 1) umma_commit(&bars->o_full[x]);
+          }
+          if (j < nkv_x[x]) {
+            const uint32_t q_base = smem_u32(sQ + x * Cfg::Q_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
+              umma_bf16(tmem + x * 128, sw128_desc(q_base + off, 16, 1024),
+                        sw128_desc(k_base + off, 16, 1024), IDESC_S, kk != 0 ? 1u : 0u);
+            }
+            umma_commit(&bars->s_full[x]);
+          }
+        }
+        if (!ok) break;
+        if (j > 0) umma_commit(&bars->kv_empty[(j - 1) % STAGES]);
+      }
+      umma_commit(&bars->mma_done);
+      drain(&bars->mma_done, 0);
+    }
+  } else {
+    const int x = warp >> 2, wq = warp & 3;
+    const int r = wq * 32 + lane;
+    const int tok = tok0 + x * TT + r / p.G;
+    const bool mine = r < TT * p.G && tok < q_len;
+    const int lim = mine ? start + tok + 1 : 0;   // keys this row sees
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t t_s = tmem + x * 128 + lane_off;
+    const uint32_t t_o = tmem + Cfg::T_O + x * D + lane_off;
+    const int n = nkv_of(x);
+    const float4* par = p.par + sh * p.blocks;
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n && ok; ++j) {
+      const float4* pj = par + (j0 + j) * (kT / kP8Page);
+      if (!wait_warp(&bars->s_full[x], j & 1, abort_flag, p.err, kErrTimeoutTmem, 89)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float s[kT];
+#pragma unroll
+      for (int c = 0; c < kT; c += 32) tmem_ld32(t_s + c, s + c);
+      tmem_wait_ld();
+      const int kmax = lim - (j0 + j) * kT;
+      if (kmax < kT) {
+#pragma unroll
+        for (int c = 0; c < kT; ++c)
+          if (c >= kmax) s[c] = -INFINITY;
+      }
+      // block maxima of w (scales are not negative), then the row's
+      float mx = -INFINITY, all = 0.f;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const float4 f = __ldg(pj + b);
+        float a0 = s[16 * b], a1 = s[16 * b + 1];
+#pragma unroll
+        for (int c = 2; c < 16; c += 2) {
+          a0 = fmaxf(a0, s[16 * b + c]);
+          a1 = fmaxf(a1, s[16 * b + c + 1]);
+        }
+        mx = fmaxf(mx, fmaf(fmaxf(a0, a1), f.x, f.y));
+        all += f.x;
+      }
+      if (!(all <= 3.402823466e38f)) {  // a block that is not finite: NaN for the rows that see it
+#pragma unroll
+        for (int c = 0; c < kT; ++c) {
+          const float f = __ldg(&pj[c / 16].x);
+          if (f != f && s[c] != -INFINITY) {
+            l = f;
+            s[c] = -INFINITY;
+          }
+        }
+      }
+      const float m_new = fmaxf(m_used, mx);
+      const bool grow = m_new > m_used + kRescaleLog2;
+      if (__any_sync(0xffffffffu, grow && m_used != -INFINITY)) {
+        const float alpha = (grow && m_used != -INFINITY) ? ex2c(m_used - m_new) : 1.f;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          uint32_t u[32];
+          tmem_ld32(t_o + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * alpha);
+          tmem_st16(t_o + c, u);
+          tmem_st16(t_o + c + 16, u + 16);
+        }
+        tmem_wait_st();
+      }
+      if (grow) {
+        if (m_used != -INFINITY) l *= ex2c(m_used - m_new);
+        m_used = m_new;
+      }
+      const float msub = m_used == -INFINITY ? 0.f : m_used;
+      float2 l2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < kT; c += 32) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int hb = 0; hb < 32; hb += 16) {
+          const float4 f = __ldg(pj + (c + hb) / 16);
+          const float kf = f.x == f.x ? f.x : 1.f;  // all masked then
+          const float nm = f.y - msub;
+          float2 rs[2] = {};
+#pragma unroll
+          for (int i = hb; i < hb + 16; i += 2) {
+            const float2 xv = fma2(make_float2(s[c + i], s[c + i + 1]), make_float2(kf, kf),
+                                   make_float2(nm, nm));
+            const float2 pv = ((i >> 1) % 8) < POLY ? exp2_poly2(xv)
+                                                    : make_float2(ex2c(xv.x), ex2c(xv.y));
+            rs[(i >> 1) & 1] = add2(rs[(i >> 1) & 1], pv);
+            pk[i / 2] = P8Io<__half>::pack(pv.x, pv.y);
+          }
+          l2 = fma2(add2(rs[0], rs[1]), make_float2(f.z, f.z), l2);
+        }
+        tmem_st16(t_s + c / 2, pk);
+      }
+      l += l2.x + l2.y;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->p_full[x]);
+    }
+    const int64_t orow = static_cast<int64_t>(row0 + tok) * p.Hq + h * p.G + r % p.G;
+    if (n > 0) {
+      if (ok && wait_warp(&bars->o_full[x], 0, abort_flag, p.err, kErrTimeoutTmem, 90)) {
+        tc_fence_after();
+        const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld32(t_o + c, o);
+          tmem_wait_ld();
+          if (!mine) continue;
+          if (p.splits == 1) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * D + c);
+#pragma unroll
+            for (int u = 0; u < 32; u += 8)
+              dst[u / 8] = make_uint4(P8Io<T>::pack(o[u] * inv, o[u + 1] * inv),
+                                      P8Io<T>::pack(o[u + 2] * inv, o[u + 3] * inv),
+                                      P8Io<T>::pack(o[u + 4] * inv, o[u + 5] * inv),
+                                      P8Io<T>::pack(o[u + 6] * inv, o[u + 7] * inv));
+          } else {
+            float4* dst =
+                reinterpret_cast<float4*>(p.ws_o + (orow * p.splits + split) * D + c);
+#pragma unroll
+            for (int u = 0; u < 32; u += 4)
+              dst[u / 4] = make_float4(o[u] * inv, o[u + 1] * inv, o[u + 2] * inv, o[u + 3] * inv);
+          }
+        }
+      }
+    } else if (mine && p.splits == 1) {  // no visible key
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * D);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+    }
+    if (mine && p.lse != nullptr)
+      p.lse[orow * p.splits + split] = l == 0.f ? -INFINITY : m_used + log2f(l);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == Cfg::MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::TMEM);
+  }
+}
+
+// --------------------------------------------------------------------------- weights
+struct MassParams {
+  const int32_t* table;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  int max_pages, blocks;
+  int64_t num_pages;
+  const float4* par;
+  const float* lse;            // [N * Hq], row stride lse_stride
+  int64_t lse_stride;
+  const float* mass_in;
+  float* mass_out;
+  int64_t N;
+  int Hq, Hkv, G;
+  int* err;
+};
+
+template <int D>
+struct MassCfg {
+  static constexpr int STAGES = 3;
+  static constexpr int CHUNKS = D / 64;
+  static constexpr int TILE = kT * D * 2;
+  static constexpr int SMEM = (1 + STAGES) * TILE + 1024 + 512 + 2 * kT * 8 + kT * 4;
+  static constexpr int THREADS = 320;
+};
+
+struct MassBars {
+  uint64_t k_full;
+  uint64_t q_full[3];
+  uint64_t q_empty[3];
+  uint64_t s_full[2];
+  uint64_t s_empty[2];
+  uint64_t mma_done;
+  uint32_t tmem;
+  int abort;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
+    p8_chunk_mass_kernel(const __grid_constant__ CUtensorMap tmQ,
+                         const __grid_constant__ CUtensorMap tmK, const MassParams p) {
+  using Cfg = MassCfg<D>;
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sK = smem;
+  uint8_t* sQ = sK + Cfg::TILE;
+  float* s_lse = reinterpret_cast<float*>(sQ + STAGES * Cfg::TILE);  // [2][128]
+  int* s_lim = reinterpret_cast<int*>(s_lse + 2 * kT);               // [2][128]
+  float* s_w = reinterpret_cast<float*>(s_lim + 2 * kT);             // [128]
+  MassBars* bars = reinterpret_cast<MassBars*>(s_w + kT);
+  volatile int* abort_flag = &bars->abort;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int h = blockIdx.y, seq = blockIdx.z;
+  const int k0 = blockIdx.x * kT;
+  const int row0 = __ldg(p.cu_q + seq), q_len = __ldg(p.cu_q + seq + 1) - row0;
+  if (row0 < 0 || q_len < 0 || static_cast<int64_t>(row0) + q_len > p.N) {
+    if (threadIdx.x == 0) report_error(p.err, kErrBounds, 91);
+    return;
+  }
+  const int kv = p8_len(p.kv_lens, seq, p.max_pages, p.err, 92);
+  if (k0 >= kv) return;
+  const int start = kv - q_len, TT = kT / p.G;
+  const int i0 = max(0, k0 - start) / TT;               // first row tile that sees the keys
+  const int n = max(0, (q_len + TT - 1) / TT - i0);      // row tiles
+  const int64_t sh = static_cast<int64_t>(seq) * p.Hkv + h;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->k_full, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&bars->q_full[s], 1);
+      mbar_init(&bars->q_empty[s], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&bars->s_full[x], 1);
+      mbar_init(&bars->s_empty[x], 4);
+    }
+    mbar_init(&bars->mma_done, 1);
+    bars->abort = 0;
+    fence_barrier_init();
+  }
+  {
+    const int used = TT * p.G, rows = kT - used;
+    for (int i = threadIdx.x; i < STAGES * Cfg::CHUNKS * rows * 8; i += blockDim.x) {
+      const int t = i / (rows * 8), r = i % (rows * 8);
+      *reinterpret_cast<uint4*>(sQ + t * (kT * 128) + used * 128 + r * 16) =
+          make_uint4(0, 0, 0, 0);
+    }
+    if (rows > 0) fence_proxy_async_shared();
+  }
+  if (warp == 9) tmem_alloc(&bars->tmem, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+
+  if (warp == 8) {
+    if (elect_one()) {
+      mbar_arrive_expect_tx(&bars->k_full, Cfg::TILE);
+#pragma unroll
+      for (int c = 0; c < Cfg::CHUNKS; ++c)
+        tma_load_4d(sK + c * kT * 128, &tmK, &bars->k_full, c * 64, k0, h, seq);
+      int issued = 0;
+      for (int i = 0; i < n; ++i) {
+        const int st = i % STAGES;
+        if (!mbar_wait(&bars->q_empty[st], ((i / STAGES) & 1) ^ 1, abort_flag, p.err,
+                       kErrTimeoutEmpty, 93))
+          break;
+        mbar_arrive_expect_tx(&bars->q_full[st], Cfg::CHUNKS * TT * p.G * 128);
+#pragma unroll
+        for (int c = 0; c < Cfg::CHUNKS; ++c)
+          tma_load_4d(sQ + st * Cfg::TILE + c * kT * 128, &tmQ, &bars->q_full[st], c * 64, 0, h,
+                      row0 + (i0 + i) * TT);
+        ++issued;
+      }
+      drain(&bars->k_full, 0);
+      for (int i = issued - STAGES < 0 ? 0 : issued - STAGES; i < issued; ++i)
+        drain(&bars->q_full[i % STAGES], (i / STAGES) & 1);
+    }
+  } else if (warp == 9) {
+    if (elect_one()) {
+      constexpr uint32_t IDESC = idesc16<T>(kT, kT, false);
+      bool ok = mbar_wait(&bars->k_full, 0, abort_flag, p.err, kErrTimeoutFull, 94);
+      const uint32_t k_base = smem_u32(sK);
+      for (int i = 0; i < n && ok; ++i) {
+        const int st = i % STAGES, x = i & 1;
+        if (!mbar_wait(&bars->q_full[st], (i / STAGES) & 1, abort_flag, p.err, kErrTimeoutFull,
+                       95) ||
+            !mbar_wait(&bars->s_empty[x], ((i >> 1) & 1) ^ 1, abort_flag, p.err, kErrTimeoutTmem,
+                       96)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t q_base = smem_u32(sQ + st * Cfg::TILE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
+          umma_bf16(tmem + x * 128, sw128_desc(k_base + off, 16, 1024),
+                    sw128_desc(q_base + off, 16, 1024), IDESC, kk != 0 ? 1u : 0u);
+        }
+        umma_commit(&bars->s_full[x]);
+        umma_commit(&bars->q_empty[st]);
+      }
+      umma_commit(&bars->mma_done);
+      drain(&bars->mma_done, 0);
+    }
+  } else {
+    const int x = warp >> 2, wq = warp & 3;
+    const int r = wq * 32 + lane;                       // key of this thread; also its column
+    const int key = k0 + r;
+    const float kf = key < kv ? __ldg(&p.par[sh * p.blocks + key / kP8Page].x) : 0.f;
+    const uint32_t t_s = tmem + x * 128 + (static_cast<uint32_t>(wq * 32) << 16);
+    float2 acc[2] = {};
+    bool ok = true;  // a warp that gave up still meets the others at their barriers
+    for (int i = x; i < n; i += 2) {
+      // column r of this row tile: its log-sum-exp and last visible key
+      const int tok = (i0 + i) * TT + r / p.G;
+      const bool row = r < TT * p.G && tok < q_len;
+      float le = INFINITY;
+      if (row) {
+        le = __ldg(p.lse + (static_cast<int64_t>(row0 + tok) * p.Hq + h * p.G + r % p.G) *
+                               p.lse_stride);
+        if (le == -INFINITY) le = INFINITY;              // a row without keys weighs nothing
+      }
+      named_bar_sync(1 + x, 128);                         // the previous tile's values are read
+      s_lse[x * kT + r] = -le;
+      s_lim[x * kT + r] = row ? start + tok : -1;
+      named_bar_sync(1 + x, 128);
+      const bool edge = k0 + kT - 1 > start + (i0 + i) * TT || (i0 + i + 1) * TT > q_len;
+      ok = ok && wait_warp(&bars->s_full[x], (i >> 1) & 1, abort_flag, p.err, kErrTimeoutTmem, 97);
+      if (!ok) continue;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < kT; c += 32) {
+        float s[32];
+        tmem_ld32(t_s + c, s);
+        tmem_wait_ld();
+        if (c == kT - 32) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->s_empty[x]);
+        }
+#pragma unroll
+        for (int u = 0; u < 32; u += 4) {
+          const float4 nl = *reinterpret_cast<const float4*>(s_lse + x * kT + c + u);
+          const float2 a = fma2(make_float2(s[u], s[u + 1]), make_float2(kf, kf),
+                                make_float2(nl.x, nl.y));
+          const float2 b = fma2(make_float2(s[u + 2], s[u + 3]), make_float2(kf, kf),
+                                make_float2(nl.z, nl.w));
+          float2 ea = make_float2(ex2c(a.x), ex2c(a.y)), eb = make_float2(ex2c(b.x), ex2c(b.y));
+          if (edge) {
+            const int4 li = *reinterpret_cast<const int4*>(s_lim + x * kT + c + u);
+            if (key > li.x) ea.x = 0.f;
+            if (key > li.y) ea.y = 0.f;
+            if (key > li.z) eb.x = 0.f;
+            if (key > li.w) eb.y = 0.f;
+          }
+          acc[0] = add2(acc[0], ea);
+          acc[1] = add2(acc[1], eb);
+        }
+      }
+    }
+    const float w = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+    if (x == 1) s_w[r] = w;
+    named_bar_sync(3, 256);
+    if (x == 0 && key < kv) {
+      const int64_t page = p8_page(p.table + static_cast<int64_t>(seq) * p.max_pages,
+                                   key / kP8Page, p.num_pages, p.err, 98);
+      const int64_t at = (page * p.Hkv + h) * kP8Page + key % kP8Page;
+      p.mass_out[at] = p.mass_in[at] + (w + s_w[r]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+template <typename T, int FMT, int D>
+int launch_expand(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int blocks, int* err,
+                  cudaStream_t st) {
+  const int64_t units = static_cast<int64_t>(s.num_seqs) * blocks * c.Hkv * 2;
+  if ((units + 7) / 8 > 0x7fffffff) return -3;
+  p8_expand_kernel<T, FMT, D><<<static_cast<unsigned>((units + 7) / 8), 256, 0, st>>>(
+      c, s, blocks, units, a.scale * 1.4426950408889634f, static_cast<T*>(a.ws_k),
+      static_cast<__half*>(a.ws_v), static_cast<float4*>(a.ws_par), err);
+  return 0;
+}
+
+template <typename T, int D, int NQ, int POLY>
+int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+               ChunkParams p, int max_q_len, int num_seqs, cudaStream_t st) {
+  using Cfg = ChunkCfg<D, NQ>;
+  auto kern = p8_chunk_kernel<T, D, NQ, POLY>;
+  const int per_cta = NQ * (kT / p.G);
+  p.row_ctas = (max_q_len + per_cta - 1) / per_cta;
+  const int64_t gx = static_cast<int64_t>(p.row_ctas) * p.splits;
+  if (gx > 0x7fffffff) return -3;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM))
+    return static_cast<int>(cudaGetLastError());
+  kern<<<dim3(static_cast<unsigned>(gx), p.Hkv, num_seqs), Cfg::THREADS, Cfg::SMEM, st>>>(tq, tk,
+                                                                                          tv, p);
+  return 0;
+}
+
+template <typename T, int D>
+int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, cudaStream_t st) {
+  const int blocks = p8_chunk_blocks(s);
+  int rc = c.fmt == kP8Int8 ? launch_expand<T, kP8Int8, D>(c, s, a, blocks, err, st)
+                            : launch_expand<T, kP8E4m3, D>(c, s, a, blocks, err, st);
+  if (rc) return rc;
+  const int G = a.Hq / c.Hkv, TT = kT / G;
+  CUtensorMap tq, tk, tv;
+  {
+    const int64_t dims[4] = {D, G, c.Hkv, a.N};
+    const int64_t strides[3] = {D * 2, static_cast<int64_t>(G) * D * 2, a.q_stride * 2};
+    const int box[4] = {64, G, 1, TT};
+    rc = make_tmap_nd(&tq, a.q, 4, dims, strides, box, false, true);
+  }
+  const int64_t Lw = static_cast<int64_t>(blocks) * kP8Page;
+  Bhsd k, v;
+  k.p = a.ws_k;
+  v.p = a.ws_v;
+  k.ss = v.ss = D;
+  k.sh = v.sh = Lw * D;
+  k.sb = v.sb = Lw * D * c.Hkv;
+  if (!rc) rc = make_bhsd_map(&tk, k, s.num_seqs, c.Hkv, static_cast<int>(Lw), D, kT);
+  if (!rc) rc = make_bhsd_map(&tv, v, s.num_seqs, c.Hkv, static_cast<int>(Lw), D, kT);
+  if (rc) return rc;
+  ChunkParams p;
+  p.cu_q = s.cu_q;
+  p.kv_lens = s.kv_lens;
+  p.max_pages = s.max_pages;
+  p.blocks = blocks;
+  p.par = static_cast<const float4*>(a.ws_par);
+  p.out = a.out;
+  p.lse = a.ws_lse;
+  p.ws_o = a.ws_o;
+  p.N = a.N;
+  p.Hq = a.Hq;
+  p.Hkv = c.Hkv;
+  p.G = G;
+  p.splits = a.splits;
+  p.row_ctas = 0;
+  p.err = err;
+  const bool mass = a.mass_out != nullptr;
+  // the cubic's error (8e-5) is below half an ulp of f16's P, not below what the weights
+  // are held to
+  const bool poly = !mass;
+  if (a.chunk_nq == 2)
+    rc = poly ? launch_fwd<T, D, 2, 2>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st)
+              : launch_fwd<T, D, 2, 0>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st);
+  else
+    rc = poly ? launch_fwd<T, D, 1, 2>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st)
+              : launch_fwd<T, D, 1, 0>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st);
+  if (rc) return rc;
+  if (p.splits > 1) {
+    rc = p8_combine(a, c.D, st);
+    if (rc) return rc;
+  }
+  if (mass) {
+    using Cfg = MassCfg<D>;
+    MassParams m;
+    m.table = s.table;
+    m.cu_q = s.cu_q;
+    m.kv_lens = s.kv_lens;
+    m.max_pages = s.max_pages;
+    m.blocks = blocks;
+    m.num_pages = c.num_pages;
+    m.par = p.par;
+    m.lse = a.ws_lse;
+    m.lse_stride = p.splits;
+    m.mass_in = a.mass_in;
+    m.mass_out = a.mass_out;
+    m.N = a.N;
+    m.Hq = a.Hq;
+    m.Hkv = c.Hkv;
+    m.G = G;
+    m.err = err;
+    auto kern = p8_chunk_mass_kernel<T, D>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM))
+      return static_cast<int>(cudaGetLastError());
+    kern<<<dim3(static_cast<unsigned>((s.max_pages * kP8Page + kT - 1) / kT), c.Hkv, s.num_seqs),
+           Cfg::THREADS, Cfg::SMEM, st>>>(tq, tk, m);
+  }
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace
+
+bool p8_is_chunk(int max_q_len, int group) {
+  return static_cast<int64_t>(max_q_len) * group > 64 && group <= kT / 2;
+}
+
+void p8_chunk_plan(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_sms, int* nq,
+                   int* splits) {
+  const int TT = kT / group;
+  const int64_t heads = static_cast<int64_t>(Hkv) * s.num_seqs;
+  const int64_t pairs = (max_q_len + 2 * TT - 1) / (2 * TT) * heads;
+  *nq = pairs >= num_sms ? 2 : 1;
+  const int64_t ctas = *nq == 2 ? pairs : (max_q_len + TT - 1) / TT * heads;
+  // fill the SMs, at least four key tiles each
+  const int64_t tiles = (static_cast<int64_t>(s.max_pages) * kP8Page + kT - 1) / kT;
+  int64_t sp = num_sms / ctas;
+  if (sp > tiles / 4) sp = tiles / 4;
+  *splits = static_cast<int>(sp < 1 ? 1 : sp);
+}
+
+int p8_chunk_blocks(const P8Seqs& s) {
+  constexpr int per = kT / kP8Page;
+  return (s.max_pages + per - 1) / per * per;
+}
+
+int p8_chunk_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err,
+                       cudaStream_t stream) {
+  if (a.N <= 0 || s.num_seqs <= 0) return 0;
+  if (s.num_seqs > 65535 || c.Hkv > 65535 || a.Hq / c.Hkv > kT) return -3;
+  if (a.type == kP8Bf16)
+    return c.D == 128 ? launch_chunk<__nv_bfloat16, 128>(c, s, a, err, stream)
+                      : launch_chunk<__nv_bfloat16, 64>(c, s, a, err, stream);
+  return c.D == 128 ? launch_chunk<__half, 128>(c, s, a, err, stream)
+                    : launch_chunk<__half, 64>(c, s, a, err, stream);
+}
+
+}  // namespace cfb

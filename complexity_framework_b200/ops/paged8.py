@@ -134,13 +134,18 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                      page_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, *,
                      scale: float, max_q_len: int, mass: Optional[torch.Tensor] = None,
                      mass_out: Optional[torch.Tensor] = None,
-                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     out: Optional[torch.Tensor] = None,
+                     workspace_bytes: int = 4 << 30) -> torch.Tensor:
     """Causal attention of ``q`` ``[N, Hq, D]`` over one layer of the cache -> ``[N, Hq, D]``.
 
     With ``mass`` the softmax weights every cached token receives from this call are added to
     it: in place, or into ``mass_out`` (which takes the tokens of this call's sequences only).
+    Long chunks expand keys and values to 16 bits first, in a workspace of at most
+    ``workspace_bytes`` (or one sequence's, where that is more).
     """
     _no_grad(q)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("scale must be positive and finite")
     if mass is None and mass_out is not None:
         raise ValueError("mass_out needs mass")
     if mass is not None and mass_out is None:
@@ -149,7 +154,8 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         require().paged8_attention(_rows(q), codes, scales, page_table, cu_q, kv_lens, out,
-                                   float(scale), int(max_q_len), mass, mass_out)
+                                   float(scale), int(max_q_len), mass, mass_out,
+                                   int(workspace_bytes))
         return out
     _check_cpu(codes, scales)
     H, D = codes.shape[1], codes.shape[4]
@@ -163,8 +169,6 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
         rows = cu[i + 1] - cu[i]
         if rows > max_q_len:
             raise ValueError("a chunk is longer than max_q_len")
-        if rows == 0:
-            continue
         blocks = -(-n // PAGE)
         pages = page_table[i, :blocks].long()
         x = codes[pages].float() * scales[pages][..., None, None]

@@ -22,6 +22,7 @@ SOURCES = [
     "bind_paged8.cpp",
     "paged8_cache.cu",
     "paged8_attn.cu",
+    "paged8_chunk.cu",
     "dist_fused.cu",
     "noalloc.cu",
     "tp_fused.cu",

@@ -238,6 +238,20 @@ def test_chunks(lens, new, hq, hkv, d, dtype, io, mass):
     run_attention(lens, new, hq, hkv, d, dtype, io, mass=mass, seed=4)
 
 
+def test_chunk_in_parts():
+    """A workspace too small for all sequences: they are expanded one after another."""
+    L = Layer([300, 129, 200], 2, 64, INT8, "cuda", seed=1)
+    cu = torch.tensor([0, 100, 150, 350], dtype=torch.int32, device="cuda")
+    q = torch.randn(350, 8, 64, device="cuda").bfloat16()
+    m = torch.zeros(2, L.num_pages, 2, PAGE, device="cuda")
+    outs = [ops().paged8_attention(q, L.codes, L.scales, L.table, cu, L.kv_lens, scale=0.125,
+                                   max_q_len=200, mass=m[i], workspace_bytes=ws)
+            for i, ws in enumerate((4 << 30, 1))]
+    clean()
+    assert (outs[0].float() - outs[1].float()).abs().max() < 2.0 ** -6  # other splits, same sums
+    assert torch.allclose(m[0], m[1], rtol=1e-4, atol=1e-6)
+
+
 def test_peaked_and_large_scores():
     """Scores far apart (one key takes all the weight), large and tiny q: no overflow."""
     for qs in (100.0, 1e-6, 2e4):
@@ -266,11 +280,22 @@ def test_unwritten_tail_is_not_read():
         run_attention([50, 83], [new, new], 8, 2, 128, FP8, torch.bfloat16, layer=L, mass=True)
 
 
-def test_later_nan_block_is_masked():
+def test_zero_key_blocks():
+    """Blocks of zero keys (scale 0), one of them the last and partly empty."""
+    for new in (1, 70):
+        L = Layer([100], 2, 64, INT8, "cuda", seed=9)
+        for b in (1, 6):
+            L.scales[int(L.table[0, b]), :, 0] = 0
+            L.codes[int(L.table[0, b]), :, 0] = 0
+        run_attention([100], [new], 4, 2, 64, INT8, torch.bfloat16, layer=L, mass=True)
+
+
+@pytest.mark.parametrize("heads", [1, 8])
+def test_later_nan_block_is_masked(heads):
     """A block that is not finite is seen by the rows at or after it only."""
     for dtype in (INT8, FP8):
         L = Layer([64], 1, 64, dtype, "cuda", seed=2)
-        q = torch.randn(20, 4, 64, device="cuda").bfloat16()
+        q = torch.randn(20, heads, 64, device="cuda").bfloat16()
         args = (torch.tensor([0, 20], dtype=torch.int32, device="cuda"), L.kv_lens)
         good = ops().paged8_attention(q, L.codes, L.scales, L.table, *args, scale=0.125,
                                       max_q_len=20)
@@ -448,7 +473,7 @@ def test_refusals():
            lambda: at(codes=L.codes[:, :, :, :8]), lambda: at(scales=L.scales.half()),
            lambda: at(scales=L.scales[:-1]), lambda: at(table=L.table.long()),
            lambda: at(table=L.table[:1]), lambda: at(cu=cu[:2]), lambda: at(lens=L.kv_lens.cpu()),
-           lambda: at(max_q_len=0), lambda: at(mass=torch.zeros(1, 2, 16, device="cuda")),
+           lambda: at(max_q_len=0), lambda: at(scale=0.0), lambda: at(scale=float("nan")), lambda: at(mass=torch.zeros(1, 2, 16, device="cuda")),
            lambda: at(out=torch.empty_like(q, dtype=torch.float16)),
            lambda: p8.paged8_append(k, k[:1], L.codes, L.scales, L.table, cu, L.kv_lens,
                                     max_q_len=1),
