@@ -82,16 +82,21 @@ int type_of(torch::ScalarType t, const char* name) {
   return t == torch::kBFloat16 ? cfb::kP8Bf16 : cfb::kP8Half;
 }
 
-// [N, H, D] whose rows of H * D elements are dense, 16-byte aligned and any distance apart.
-int64_t rows_of(const Tensor& t, const Tensor& codes, int64_t D, const char* name) {
+// [N, H, D] whose rows of H * D elements are dense, 16-byte aligned and any distance apart
+// (a slice of a fused projection is one); other layouts are copied.
+Tensor rows_of(const Tensor& t, const Tensor& codes, int64_t D, const char* name) {
   same_device(t, codes, name);
   TORCH_CHECK(t.dim() == 3 && t.size(2) == D, name, " must be [tokens, heads, ", D, "]");
   TORCH_CHECK(t.size(0) <= 0x7fffffff, name, ": too many tokens");
-  TORCH_CHECK((t.size(2) == 1 || t.stride(2) == 1) && (t.size(1) == 1 || t.stride(1) == D) &&
-                  (t.size(0) <= 1 || t.stride(0) % 8 == 0) &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              name, " must have dense, 16-byte aligned rows");
-  return t.size(0) > 1 ? t.stride(0) : t.size(1) * D;
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()),
+              "the 8-bit KV cache operators have no gradient; call them under torch.no_grad()");
+  const bool dense = t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == D) &&
+                     (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= 0)) &&
+                     reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return dense ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+int64_t row_stride(const Tensor& t) {
+  return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2);
 }
 
 void check_rc(int rc, const char* what) {
@@ -109,57 +114,64 @@ float* mass_of(const Tensor& m, const Tensor& codes, int64_t lead, const char* n
   return m.data_ptr<float>();
 }
 
-void paged8_append(const Tensor& k, const Tensor& v, const Tensor& codes, const Tensor& scales,
+void paged8_append(const Tensor& k_in, const Tensor& v_in, const Tensor& codes, const Tensor& scales,
                    const Tensor& table, const Tensor& cu_q, const Tensor& kv_lens,
                    int64_t max_q_len) {
   const cfb::P8Cache c = cache_of(codes, scales, false);
   const cfb::P8Seqs s = seqs_of(codes, table, kv_lens, cu_q);
-  const int64_t ks = rows_of(k, codes, c.D, "k"), vs = rows_of(v, codes, c.D, "v");
+  const Tensor k = rows_of(k_in, codes, c.D, "k"), v = rows_of(v_in, codes, c.D, "v");
   TORCH_CHECK(k.size(1) == c.Hkv && k.sizes() == v.sizes(), "k and v must be [tokens, ", c.Hkv,
               ", ", c.D, "]");
   TORCH_CHECK(k.scalar_type() == v.scalar_type(), "k and v must have one dtype");
   TORCH_CHECK(max_q_len >= 1 && max_q_len <= (1 << 30), "max_q_len must be positive");
   const int type = type_of(k.scalar_type(), "k and v");
   const c10::cuda::CUDAGuard g(codes.device());
-  check_rc(cfb::p8_append(c, s, k.data_ptr(), ks, v.data_ptr(), vs, k.size(0),
+  check_rc(cfb::p8_append(c, s, k.data_ptr(), row_stride(k), v.data_ptr(), row_stride(v),
+                          k.size(0),
                           static_cast<int>(max_q_len), type, cfb_err_ptr(codes.get_device()),
                           at::cuda::getCurrentCUDAStream()),
            "paged8_append");
 }
 
-void paged8_read(const Tensor& codes, const Tensor& scales, const Tensor& table,
-                 const Tensor& kv_lens, Tensor& k_out, Tensor& v_out) {
+std::tuple<Tensor, Tensor> paged8_read(const Tensor& codes, const Tensor& scales,
+                                       const Tensor& table, const Tensor& kv_lens,
+                                       torch::ScalarType dtype) {
   const bool layered = codes.dim() == 6;
   const cfb::P8Cache c = cache_of(codes, scales, layered);
   const cfb::P8Seqs s = seqs_of(codes, table, kv_lens, c10::nullopt);
   const int64_t layers = layered ? codes.size(0) : 1;
-  for (const Tensor* t : {&k_out, &v_out}) {
-    same_device(*t, codes, "out");
-    TORCH_CHECK(t->is_contiguous() && t->numel() == layers * s.num_seqs * c.Hkv * s.max_pages *
-                                                        cfb::kP8Page * static_cast<int64_t>(c.D),
-                "out must be contiguous [(layers,) seqs, kv_heads, max_pages * 16, head_dim]");
-  }
-  TORCH_CHECK(k_out.scalar_type() == v_out.scalar_type(), "outputs must have one dtype");
   TORCH_CHECK(layers <= 65535, "too many layers");
-  const int type = type_of(k_out.scalar_type(), "out");
+  const int type = type_of(dtype, "dtype");
   const c10::cuda::CUDAGuard g(codes.device());
-  check_rc(cfb::p8_read(c, s, static_cast<int>(layers), k_out.data_ptr(), v_out.data_ptr(), type,
+  const int64_t L = static_cast<int64_t>(s.max_pages) * cfb::kP8Page;
+  const auto opt = codes.options().dtype(dtype);
+  const auto make = [&] {
+    return layered ? torch::empty({layers, s.num_seqs, c.Hkv, L, c.D}, opt)
+                   : torch::empty({s.num_seqs, c.Hkv, L, c.D}, opt);
+  };
+  Tensor k = make(), v = make();
+  check_rc(cfb::p8_read(c, s, static_cast<int>(layers), k.data_ptr(), v.data_ptr(), type,
                         cfb_err_ptr(codes.get_device()), at::cuda::getCurrentCUDAStream()),
            "paged8_read");
+  return {k, v};
 }
 
-void paged8_attention(const Tensor& q, const Tensor& codes, const Tensor& scales,
-                      const Tensor& table, const Tensor& cu_q, const Tensor& kv_lens, Tensor& out,
-                      double scale, int64_t max_q_len, const c10::optional<Tensor>& mass_in,
-                      const c10::optional<Tensor>& mass_out, int64_t workspace_bytes) {
+Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& scales,
+                        const Tensor& table, const Tensor& cu_q, const Tensor& kv_lens,
+                        const c10::optional<Tensor>& out_in, double scale, int64_t max_q_len,
+                        const c10::optional<Tensor>& mass_in,
+                        const c10::optional<Tensor>& mass_out, int64_t workspace_bytes) {
   const cfb::P8Cache c = cache_of(codes, scales, false);
   const cfb::P8Seqs s = seqs_of(codes, table, kv_lens, cu_q);
   cfb::P8Attn a;
-  a.q_stride = rows_of(q, codes, c.D, "q");
+  const Tensor q = rows_of(q_in, codes, c.D, "q");
+  a.q_stride = row_stride(q);
   a.type = type_of(q.scalar_type(), "q");
   const int64_t Hq = q.size(1), N = q.size(0);
   TORCH_CHECK(Hq >= 1 && Hq % c.Hkv == 0, "query heads (", Hq, ") must be a multiple of KV heads (",
               c.Hkv, ")");
+  const c10::cuda::CUDAGuard g(codes.device());
+  const Tensor out = out_in.has_value() ? *out_in : torch::empty({N, Hq, c.D}, q.options());
   same_device(out, codes, "out");
   TORCH_CHECK(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() &&
                   out.is_contiguous() && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
@@ -177,8 +189,7 @@ void paged8_attention(const Tensor& q, const Tensor& codes, const Tensor& scales
   a.Hq = static_cast<int>(Hq);
   a.max_q_len = static_cast<int>(max_q_len);
   a.scale = static_cast<float>(scale);
-  if (N == 0 || s.num_seqs == 0) return;
-  const c10::cuda::CUDAGuard g(codes.device());
+  if (N == 0 || s.num_seqs == 0) return out;
   const int sms = cfb_num_sms(codes.get_device()), group = a.Hq / c.Hkv;
   int* err = cfb_err_ptr(codes.get_device());
   const auto stream = at::cuda::getCurrentCUDAStream();
@@ -216,7 +227,7 @@ void paged8_attention(const Tensor& q, const Tensor& codes, const Tensor& scales
   }
   if (!chunk) {
     check_rc(cfb::p8_attention(c, s, a, err, stream), "paged8_attention");
-    return;
+    return out;
   }
   for (int64_t i = 0; i < s.num_seqs; i += seqs_each) {
     cfb::P8Seqs part = s;
@@ -226,11 +237,12 @@ void paged8_attention(const Tensor& q, const Tensor& codes, const Tensor& scales
     part.num_seqs = static_cast<int>(std::min<int64_t>(seqs_each, s.num_seqs - i));
     check_rc(cfb::p8_chunk_attention(c, part, a, err, stream), "paged8_attention");
   }
+  return out;
 }
 
-void paged8_evict(const Tensor& codes, const Tensor& scales, const Tensor& mass,
-                  const Tensor& table, const Tensor& kv_lens, const Tensor& dst_table,
-                  int64_t budget, int64_t recent, Tensor& keep) {
+Tensor paged8_evict(const Tensor& codes, const Tensor& scales, const Tensor& mass,
+                    const Tensor& table, const Tensor& kv_lens, const Tensor& dst_table,
+                    int64_t budget, int64_t recent) {
   const bool layered = codes.dim() == 6;
   const cfb::P8Cache c = cache_of(codes, scales, layered);
   const cfb::P8Seqs s = seqs_of(codes, table, kv_lens, c10::nullopt);
@@ -243,14 +255,15 @@ void paged8_evict(const Tensor& codes, const Tensor& scales, const Tensor& mass,
                   dst_table.size(1) <= (1 << 26),
               "dst_table must have one row for each sequence");
   TORCH_CHECK(layers <= 65535, "too many layers");
-  ints(keep, codes, keep.dim(), "keep");
-  TORCH_CHECK(keep.numel() == layers * s.num_seqs * c.Hkv * budget, "keep has the wrong size");
   const c10::cuda::CUDAGuard g(codes.device());
+  Tensor keep = layered ? torch::empty({layers, s.num_seqs, c.Hkv, budget}, table.options())
+                        : torch::empty({s.num_seqs, c.Hkv, budget}, table.options());
   check_rc(cfb::p8_evict(c, s, m, static_cast<int>(layers), dst,
                          static_cast<int>(dst_table.size(1)), static_cast<int>(budget),
                          static_cast<int>(recent), keep.data_ptr<int32_t>(),
                          cfb_err_ptr(codes.get_device()), at::cuda::getCurrentCUDAStream()),
            "paged8_evict");
+  return keep;
 }
 
 }  // namespace

@@ -39,14 +39,6 @@ def _no_grad(*tensors: torch.Tensor) -> None:
                            "call them under torch.no_grad()")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``[N, H, D]`` with dense 16-byte aligned rows (a slice of a fused projection is one)."""
-    if t.dim() == 3 and (t.stride(2) != 1 or t.stride(1) != t.shape[2] or t.stride(0) % 8
-                         or t.data_ptr() % 16):
-        return t.contiguous()
-    return t
-
-
 def _check_cpu(codes: torch.Tensor, scales: torch.Tensor) -> None:
     if codes.dtype not in LEVELS:
         raise ValueError("codes must be int8 or float8_e4m3fn")
@@ -67,11 +59,10 @@ def paged8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales:
     bounds the new tokens of a sequence.  A block with a value that is not finite reads as NaN
     or infinity throughout.
     """
-    _no_grad(k, v)
     if codes.is_cuda:
-        require().paged8_append(_rows(k), _rows(v), codes, scales, page_table, cu_q, kv_lens,
-                                int(max_q_len))
+        require().paged8_append(k, v, codes, scales, page_table, cu_q, kv_lens, max_q_len)
         return
+    _no_grad(k, v)
     _check_cpu(codes, scales)
     if k.shape != v.shape or k.shape[1] != codes.shape[1] or k.shape[2] != codes.shape[4]:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] of the cache")
@@ -110,15 +101,12 @@ def paged8_read(codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Ten
                 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """The cached values ``(k, v)``, each ``[(layers,) S, Hkv, max_pages * 16, D]``, of one layer
     or (with a leading dimension of ``codes`` and ``scales``) of all; 0 past ``kv_lens``."""
+    if codes.is_cuda:
+        return require().paged8_read(codes, scales, page_table, kv_lens, dtype)
+    _check_cpu(codes, scales)
     lead = codes.shape[:-5]
     S, P = page_table.shape
     H, D = codes.shape[-4], codes.shape[-1]
-    if codes.is_cuda:
-        k = torch.empty(*lead, S, H, P * PAGE, D, dtype=dtype, device=codes.device)
-        v = torch.empty_like(k)
-        require().paged8_read(codes, scales, page_table, kv_lens, k, v)
-        return k, v
-    _check_cpu(codes, scales)
     t = page_table.long()
     if lead:
         x = codes[:, t].float() * scales[:, t][..., None, None]
@@ -143,7 +131,6 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     Long chunks expand keys and values to 16 bits first, in a workspace of at most
     ``workspace_bytes`` (or one sequence's, where that is more).
     """
-    _no_grad(q)
     if not 0.0 < scale < float("inf"):
         raise ValueError("scale must be positive and finite")
     if mass is None and mass_out is not None:
@@ -151,12 +138,9 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     if mass is not None and mass_out is None:
         mass_out = mass
     if codes.is_cuda:
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        require().paged8_attention(_rows(q), codes, scales, page_table, cu_q, kv_lens, out,
-                                   float(scale), int(max_q_len), mass, mass_out,
-                                   int(workspace_bytes))
-        return out
+        return require().paged8_attention(q, codes, scales, page_table, cu_q, kv_lens, out, scale,
+                                          max_q_len, mass, mass_out, workspace_bytes)
+    _no_grad(q)
     _check_cpu(codes, scales)
     H, D = codes.shape[1], codes.shape[4]
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] % H:
@@ -202,16 +186,15 @@ def paged8_evict(codes: torch.Tensor, scales: torch.Tensor, mass: torch.Tensor,
     must not be among the new ones.  Returns the kept indices
     ``[(layers,) S, Hkv, budget]`` int32, -1 past a sequence's kept tokens.
     """
-    lead = codes.shape[:-5]
-    S, H, D = page_table.shape[0], codes.shape[-4], codes.shape[-1]
     if not 0 <= recent <= budget or budget < 1:
         raise ValueError("need 0 <= recent <= budget and budget >= 1")
-    keep = torch.empty(*lead, S, H, budget, dtype=torch.int32, device=codes.device)
     if codes.is_cuda:
-        require().paged8_evict(codes, scales, mass, page_table, kv_lens, dst_table, int(budget),
-                               int(recent), keep)
-        return keep
+        return require().paged8_evict(codes, scales, mass, page_table, kv_lens, dst_table, budget,
+                                      recent)
     _check_cpu(codes, scales)
+    lead = codes.shape[:-5]
+    S, H, D = page_table.shape[0], codes.shape[-4], codes.shape[-1]
+    keep = torch.empty(*lead, S, H, budget, dtype=torch.int32, device=codes.device)
     layers = codes.shape[0] if lead else 1
     cs, ss, ms, ks = [x if lead else x[None] for x in (codes, scales, mass, keep)]
     ks.fill_(-1)
