@@ -194,41 +194,40 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
   int* err = cfb_err_ptr(codes.get_device());
   const auto stream = at::cuda::getCurrentCUDAStream();
   const auto f32 = torch::dtype(torch::kFloat32).device(codes.device());
-  const bool chunk = cfb::p8_is_chunk(a.max_q_len, group);
-  int64_t seqs_each = s.num_seqs;  // sequences expanded at a time, within the workspace limit
-  if (chunk) {
-    const int64_t each = static_cast<int64_t>(c.Hkv) * cfb::p8_chunk_blocks(s) * cfb::kP8Page * c.D;
-    seqs_each = std::max<int64_t>(1, std::min<int64_t>(s.num_seqs, workspace_bytes / (4 * each)));
-    cfb::p8_chunk_plan(s, c.Hkv, group, a.max_q_len, sms, &a.chunk_nq, &a.splits);
-    if (seqs_each < s.num_seqs) a.splits = 1;
-  } else {
-    a.splits = cfb::p8_attn_splits(s, c.Hkv, group, a.max_q_len, sms);
-  }
-  // one workspace: expanded K | V | their block scales | split outputs | log-sum-exps | scores
   const bool mass = a.mass_out != nullptr;
-  const int64_t n_o = a.splits > 1 ? N * Hq * a.splits * c.D : 0;
-  const int64_t n_lse = a.splits > 1 || mass ? (N * Hq * a.splits + 3) / 4 * 4 : 0;
-  const int64_t blocks = cfb::p8_chunk_blocks(s);
-  const int64_t n_ks = chunk ? seqs_each * c.Hkv * blocks * 4 : 0;
-  const int64_t n_kv = chunk ? seqs_each * c.Hkv * blocks * cfb::kP8Page * c.D / 2 : 0;  // floats
-  const int64_t n_s = mass && !chunk ? N * Hq * s.max_pages * cfb::kP8Page : 0;
-  Tensor ws;
-  if (n_o + n_lse + n_ks + 2 * n_kv + n_s > 0) {
-    ws = torch::empty({2 * n_kv + n_o + n_lse + n_ks + n_s}, f32);
-    float* at = ws.data_ptr<float>();
-    a.ws_k = at;
-    a.ws_v = at + n_kv;
-    at += 2 * n_kv;
-    a.ws_par = at;
-    at += n_ks;
-    a.ws_o = n_o ? at : nullptr;
-    a.ws_lse = n_lse ? at + n_o : nullptr;
-    a.ws_s = at + n_o + n_lse;
-  }
-  if (!chunk) {
-    check_rc(cfb::p8_attention(c, s, a, err, stream), "paged8_attention");
+  TORCH_CHECK(group <= 128, "at most 128 query heads for each KV head");
+  TORCH_CHECK(s.num_seqs * static_cast<int64_t>(c.Hkv) <= 65535 &&
+                  c.num_pages * c.Hkv <= 0x7fffffff,
+              "too many sequences or pages");
+  if (!cfb::p8_is_chunk(a.max_q_len, group)) {
+    const cfb::P8AttnPlan plan = cfb::p8_attn_plan(c, s, group, a.max_q_len, mass, sms);
+    Tensor ws;
+    if (plan.floats() > 0) ws = torch::empty({plan.floats()}, f32);
+    check_rc(cfb::p8_attention(c, s, a, plan, plan.floats() > 0 ? ws.data_ptr<float>() : nullptr,
+                               err, stream),
+             "paged8_attention");
     return out;
   }
+  const int64_t blocks = cfb::p8_chunk_blocks(s);
+  const int64_t each = static_cast<int64_t>(c.Hkv) * blocks * cfb::kP8Page * c.D;
+  // sequences expanded at a time, within the workspace limit
+  const int64_t seqs_each =
+      std::max<int64_t>(1, std::min<int64_t>(s.num_seqs, workspace_bytes / (4 * each)));
+  cfb::p8_chunk_plan(s, c.Hkv, group, a.max_q_len, sms, &a.chunk_nq, &a.splits);
+  if (seqs_each < s.num_seqs) a.splits = 1;
+  // one workspace: expanded K | V | their block scales | split outputs | log-sum-exps
+  const int64_t n_kv = seqs_each * each / 2;  // floats
+  const int64_t n_par = seqs_each * c.Hkv * blocks * 4;
+  const int64_t n_o = a.splits > 1 ? N * Hq * a.splits * c.D : 0;
+  const int64_t n_lse = a.splits > 1 || mass ? N * Hq * a.splits : 0;
+  Tensor ws = torch::empty({2 * n_kv + n_par + n_o + n_lse}, f32);
+  float* at = ws.data_ptr<float>();
+  a.ws_k = at;
+  a.ws_v = at + n_kv;
+  a.ws_par = at + 2 * n_kv;
+  at += 2 * n_kv + n_par;
+  a.ws_o = n_o ? at : nullptr;
+  a.ws_lse = n_lse ? at + n_o : nullptr;
   for (int64_t i = 0; i < s.num_seqs; i += seqs_each) {
     cfb::P8Seqs part = s;
     part.table += i * s.max_pages;

@@ -50,18 +50,32 @@ struct P8Attn {
   float scale = 1.f;
   const float* mass_in = nullptr;  // with mass_out: mass_out = mass_in + weights
   float* mass_out = nullptr;
+  // long chunks only
   int splits = 1;
   float* ws_o = nullptr;     // [N * Hq, splits, D] (splits > 1)
   float* ws_lse = nullptr;   // [N * Hq, splits] (splits > 1 or mass)
-  float* ws_s = nullptr;     // [N * Hq, max_pages * 16] scores (mass, short chunks)
-  // long chunks: keys and values as 16-bit operands, Lw = 16 * p8_chunk_blocks() tokens
   int chunk_nq = 2;          // 128-row tiles of a CTA
+  // keys and values as 16-bit operands, Lw = 16 * p8_chunk_blocks() tokens
   void* ws_k = nullptr;      // [S, Hkv, Lw, D]
   void* ws_v = nullptr;
   void* ws_par = nullptr;    // float4 [S, Hkv, Lw / 16]
 };
-int p8_attn_splits(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_sms);
-// Joins the splits: out from ws_o and ws_lse; a row's first ws_lse becomes its total.
+
+// Decode and short chunks: how the work is dealt out, and the workspace in floats.
+struct P8AttnPlan {
+  int nb = 1;                // 8-row tiles of a CTA
+  int row_tiles = 1;         // row tiles of the longest chunk
+  int chunk = 1, splits = 1; // pages of a CTA, CTAs of the longest (sequence, KV head, row tile)
+  int64_t n_o = 0, n_lse = 0, n_s = 0;
+  int64_t floats() const { return n_o + n_lse + n_s; }
+};
+P8AttnPlan p8_attn_plan(const P8Cache& c, const P8Seqs& s, int group, int max_q_len, bool mass,
+                        int num_sms);
+int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, const P8AttnPlan& plan,
+                 float* ws, int* err, cudaStream_t stream);
+
+// Long chunks.  Joins the splits: out from ws_o and ws_lse; a row's first ws_lse becomes its
+// total.
 int p8_combine(const P8Attn& a, int D, cudaStream_t stream);
 int p8_chunk_blocks(const P8Seqs& s);
 // Whether a call's chunks go to the tcgen05 kernels.
@@ -71,8 +85,6 @@ void p8_chunk_plan(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_s
                    int* splits);
 int p8_chunk_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err,
                        cudaStream_t stream);
-int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err,
-                 cudaStream_t stream);
 
 // Keeps `budget` tokens of each sequence and moves them to the pages of dst_table
 // [S, dst_pages]; keep [layers, S, Hkv, budget] int32.

@@ -5,24 +5,38 @@
 // for each row (new token, query head) over the cached tokens j at or before its position.
 //
 // A step reads every cached byte once and does little else, so the kernel is built to keep
-// bytes in flight: codes go from global memory straight into tensor-core fragments, with
-// no shared memory, barrier or wait between.  Both products take the cache as the A operand
-// of m16n8k16 and the rows of one KV head (tokens x grouped heads) as its 8 columns,
+// bytes in flight and instructions few.  Each warp streams pages of one KV head (32 * D
+// contiguous bytes) through its own ring in shared memory (cp.async, no barrier); both
+// products take the cache as the A operand of m16n8k16 and the rows of the KV head (tokens x
+// grouped heads) as its 8 columns,
 //   S^T[16 tokens, 8 rows] = K[16, D] Q^T      O^T[D, 8 rows] += V^T[D, 16] P^T,
-// which wastes nothing on the usual groups of up to eight query heads.  A contraction may
-// visit its axis in any order that both operands share, and an output axis may be dealt to
-// rows at will; the orders below are chosen so that each lane's share of a page is whole
-// 16-byte pieces of it (D = 64: 8-byte pieces of V).  tcgen05 needs 64 rows and operands
-// in shared memory: eight times the work and a staging pass for a kernel that waits on HBM.
+// which wastes nothing on the usual groups of up to eight query heads.  tcgen05 needs 64 rows
+// and 16-bit operands in shared memory: eight times the work and a conversion pass for a
+// kernel that waits on HBM.  A contraction may visit its axis in any order that both operands
+// share, and an output axis may be dealt to rows at will: the orders are chosen so that a
+// lane's share of a page is whole 16-byte pieces (D = 64: 8-byte pieces of V), and the ring is
+// swizzled so that a quarter warp's pieces lie in distinct banks.
 //
-// Codes become f16 exactly; q is scaled by a power of two per row into f16 range, where a
-// bf16 q is exact too.  Scores, maxima, sums and the output accumulate in fp32; the
-// probabilities are rounded to f16 (11 bits, against 8 of bf16).
-// V's block scale cannot be taken out of the sum over blocks, so it goes into the
-// exponent: with w_j = s_j + log2 vs[b(j)] and M a running bound of w,
+// Codes become f16 exactly: an e4m3 number is an f16 number; an int8 code c becomes the f16
+// subnormal (c + 128) 2^-24, which is its byte with the sign bit flipped and needs one byte
+// permutation for two codes.  The offset comes out again exactly where it went in: 128 sum(q)
+// is subtracted from the score, 128 sum(P) (an MMA against ones, so of the rounded P) from the
+// output.  q is scaled by a power of two per row into f16 range, where a bf16 q is exact too.
+// Scores, maxima, sums and the output accumulate in fp32; the probabilities are rounded to
+// f16 (11 bits, against 8 of bf16).
+// V's block scale cannot be taken out of the sum over blocks, so it goes into the exponent:
+// with w_j = s_j + log2 vs[b(j)] and M a running bound of w,
 //   P_j = 2^(w_j - M),  O = sum P_j cV_j,  l = sum P_j / vs[b(j)],  o = O / l.
 // M moves only when some w exceeds it by more than 2^8 (then by a warp-wide maximum), which
 // leaves one vote per page in the usual case.
+//
+// One CTA takes `chunk` pages of one item (sequence, KV head, row tile); the host picks the
+// chunk for a few waves of CTAs from the page table's width, and CTAs past a sequence's own
+// length leave at once.  The hardware deals CTAs to SMs as they free up: SMs run up to 18%
+// apart on equal work, so equal static shares (tried) wait for the slowest one.  Items of more
+// than one chunk leave normalised partial outputs, which p8_finish_kernel joins.
+#include <algorithm>
+
 #include "paged8.cuh"
 
 namespace cfb {
@@ -30,8 +44,14 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 4;
-constexpr float kGrow = 8.f;           // log2 of how far P may exceed 1
+constexpr int kStages = 4;                   // pages of a warp's ring: two used, two in flight
+constexpr int kWholePages = 32;              // up to here an item is one CTA's
+constexpr int kMinPages = 32, kMaxPages = 64;  // chunk of a CTA otherwise
+constexpr int kMaxRows = 64;                 // rows of a KV head (longer chunks: paged8_chunk.cu)
+constexpr float kGrow = 8.f;                 // log2 of how far P may exceed 1
+constexpr float kNone = -1e30f;              // M before any visible key
 constexpr float kTinyScale = 7.888609e-31f;  // 2^-100: V blocks below it count as zeros
+constexpr float kTwo24 = 16777216.f;
 
 struct AttnParams {
   P8Cache c;
@@ -40,12 +60,15 @@ struct AttnParams {
   int64_t q_stride;
   void* out;
   int64_t N;
-  int Hq, G, splits, row_tiles;
+  int Hq, G;
+  int row_tiles;               // of the longest chunk of new tokens
+  int chunk, splits;           // pages of a CTA, CTAs of the longest item
   float scale_log2;
-  float* ws_o;
-  float* ws_lse;
-  float* ws_s;
-  int64_t s_stride;
+  float* ws_o;                 // [items, splits, R, D] partial outputs (splits > 1)
+  float* ws_lse;               // [items, splits, R] (splits > 1 or mass)
+  float* ws_s;                 // [items, R, max_pages * 16] scores (mass)
+  const float* mass_in;
+  float* mass_out;
   int* err;
 };
 
@@ -62,18 +85,25 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
-               : "=r"(v.x), "=r"(v.y)
-               : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ float ex2f(float x) {
@@ -85,226 +115,362 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
   __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-
-// One lane's share of a page: g = lane / 4, t = lane % 4.
-//   k[i][h]: token g + 8 i, bytes [64 h + 16 t, + 16)   -> k-steps 4 h .. 4 h + 3
-//   v[i]:    token {2t, 2t+1, 2t+8, 2t+9}[i], bytes [g D / 8, + D / 8)
-template <int D>
-struct PageFrag {
-  static constexpr int KH = D / 64;
-  static constexpr int VW = D / 32;  // words of one token's piece
-  uint4 k[2][KH];
-  uint32_t v[4][VW];
-  __device__ __forceinline__ void load(const uint8_t* p, int g, int t) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int h = 0; h < KH; ++h) k[i][h] = ld_stream16(p + (g + 8 * i) * D + 64 * h + 16 * t);
-    const uint8_t* pv = p + kP8Page * D + g * (D / 8);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
-      if constexpr (D == 128) {
-        const uint4 x = ld_stream16(pv + tok * D);
-        v[i][0] = x.x;
-        v[i][1] = x.y;
-        v[i][2] = x.z;
-        v[i][3] = x.w;
-      } else {
-        const uint2 x = ld_stream8(pv + tok * D);
-        v[i][0] = x.x;
-        v[i][1] = x.y;
-      }
-    }
-  }
-};
-
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-// NB: 8-row column tiles of a CTA (8 * NB rows of one KV head).
+// Four codes as two f16x2 A-operand registers, (byte 0, byte 1) and (byte 2, byte 3):
+// e4m3 as its value; int8 (sign bit flipped by the caller) as (c + 128) 2^-24.
+template <int FMT>
+__device__ __forceinline__ void operand(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == kP8Int8) {
+    lo = __byte_perm(w, 0u, 0x4140);
+    hi = __byte_perm(w, 0u, 0x4342);
+  } else {
+    p8_to_half<FMT>(w, lo, hi);
+  }
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t flip(uint32_t w) {
+  return FMT == kP8Int8 ? w ^ 0x80808080u : w;
+}
+
+template <int D, int NB>
+struct AttnCfg {
+  static constexpr int R = 8 * NB;
+  static constexpr int PAGE_BYTES = 2 * kP8Page * D;
+  static constexpr int RING = kWarps * kStages * PAGE_BYTES;
+  static constexpr int JOIN = kWarps * R * D * 4;              // reuses the ring
+  static constexpr int QF = RING > JOIN ? RING : JOIN;         // q fragments
+  static constexpr int ROWS = QF + NB * D * 16;                // per-row values
+  static constexpr int SMEM = ROWS + (2 + 2 * kWarps) * R * 4;
+  static constexpr int MIN_CTAS = NB <= 2 ? 3 : 2;
+  static_assert(SMEM * MIN_CTAS <= 224 * 1024, "shared memory");
+};
+
+struct SeqInfo {
+  int row0, q_len, kv, rows;  // rows of a KV head: tokens x G
+};
+
+template <int R>
+__device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int seq) {
+  SeqInfo i;
+  i.row0 = __ldg(p.s.cu_q + seq);
+  i.q_len = __ldg(p.s.cu_q + seq + 1) - i.row0;
+  i.kv = p8_len(p.s.kv_lens, seq, p.s.max_pages, p.err, 72);
+  if (i.row0 < 0 || i.q_len < 0 || static_cast<int64_t>(i.row0) + i.q_len > p.N) {
+    report_error(p.err, kErrBounds, 70);
+    i.q_len = 0;
+  }
+  if (static_cast<int64_t>(i.q_len) * p.G > p.row_tiles * R) {  // longer than max_q_len
+    report_error(p.err, kErrBounds, 71);
+    i.rows = p.row_tiles * R;
+  } else {
+    i.rows = i.q_len * p.G;
+  }
+  return i;
+}
+
+// mass_out[j] = mass_in[j] + sum over rows of 2^(s_j - lse), in row order.  sj: the token's
+// scores, row stride Lp; r0: the first row that sees it.
+__device__ __forceinline__ void add_mass(const AttnParams& p, const int32_t* table, int h, int j,
+                                         const float* sj, int64_t Lp, int r0, int rows,
+                                         const float* lse) {
+  const int64_t pg = p8_page(table, j / kP8Page, p.c.num_pages, p.err, 75);
+  const int64_t at = (pg * p.c.Hkv + h) * kP8Page + j % kP8Page;
+  const float before = p.mass_in[at];
+  float w = 0.f;
+#pragma unroll 4
+  for (int r = r0; r < rows; ++r) w += ex2f(sj[r * Lp] - lse[r]);
+  p.mass_out[at] = before + w;
+}
+
+// NB: 8-row column tiles of a CTA (R = 8 * NB rows of one KV head).
 template <typename T, int FMT, int D, int NB, bool MASS>
-__global__ void __launch_bounds__(kWarps * 32) p8_attn_kernel(const AttnParams p) {
-  constexpr int R = 8 * NB;
+__global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
+    p8_attn_kernel(const AttnParams p) {
+  using Cfg = AttnCfg<D, NB>;
+  constexpr int R = Cfg::R;
   constexpr int KH = D / 64, KS = D / 16, MT = D / 16;
-  constexpr int DL = D / 8;  // output dims of a lane
-  __shared__ float s_m[kWarps][R], s_l[kWarps][R];
-  __shared__ __align__(16) float s_o[kWarps][R][D];
+  constexpr int DL = D / 8;              // output dims of a lane
+  constexpr int VW = D / 32;             // words of a lane's piece of one token's V
+  constexpr int PB = Cfg::PAGE_BYTES;
+  constexpr int HALF = kP8Page / 2 * D;  // bytes of eight tokens
+  constexpr bool kInt8 = FMT == kP8Int8;
+  constexpr int U = NB <= 2 ? 2 : 1;     // pages of an iteration: two hide each other's latency
+  constexpr int AHEAD = kStages / U - 1; // groups of pages in flight beyond the current one
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* s_o = reinterpret_cast<float*>(smem);                        // [kWarps][R][D]
+  float* s_qs = reinterpret_cast<float*>(smem + Cfg::ROWS);           // [R]
+  float* s_qb = s_qs + R;                                             // [R]
+  float* s_m = s_qb + R;                                              // [kWarps][R]
+  float* s_l = s_m + kWarps * R;                                      // [kWarps][R]
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * (kStages * PB);
+  const uint32_t qf = smem_u32(smem + Cfg::QF);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // p8_finish_kernel waits
 
   const int split = blockIdx.x % p.splits, rt = blockIdx.x / p.splits;
   const int h = blockIdx.y, seq = blockIdx.z;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int g = lane >> 2, t = lane & 3;
-  const int row0 = __ldg(p.s.cu_q + seq);
-  const int q_len = __ldg(p.s.cu_q + seq + 1) - row0;
-  if (row0 < 0 || q_len < 0 || static_cast<int64_t>(row0) + q_len > p.N) {
-    if (threadIdx.x == 0) report_error(p.err, kErrBounds, 70);
+  const SeqInfo si = seq_info<R>(p, seq);
+  const int rows = si.rows, first_row = rt * R;
+  // row r is token r / G and head r % G; it sees the keys [0, start + token + 1)
+  const int start = si.kv - si.q_len;
+  const int32_t* table = p.s.table + static_cast<int64_t>(seq) * p.s.max_pages;
+  const int64_t Lp = static_cast<int64_t>(p.s.max_pages) * kP8Page;
+  const int64_t item = (static_cast<int64_t>(seq) * p.c.Hkv + h) * p.row_tiles + rt;
+  if (first_row >= rows) {
+    if (MASS && p.splits == 1 && p.row_tiles == 1)  // cached tokens, none of them new
+      for (int j = threadIdx.x; j < si.kv; j += kWarps * 32)
+        add_mass(p, table, h, j, nullptr, 0, 0, 0, nullptr);
     return;
   }
-  const int rows = q_len * p.G;       // rows of this KV head
-  const int first_row = rt * R;
-  if (rt == p.row_tiles - 1 && rows > first_row + R && threadIdx.x == 0)
-    report_error(p.err, kErrBounds, 71);  // a chunk longer than max_q_len
-  if (first_row >= rows) return;
-  const int kv = p8_len(p.s.kv_lens, seq, p.s.max_pages, p.err, 72);
-  // row r is token r / G and head r % G; its visible keys are [0, start + token + 1)
-  const int start = kv - q_len;
   const int last_tok = (min(rows, first_row + R) - 1) / p.G;
   const int n_keys = max(0, start + last_tok + 1);
+  const int min_lim = start + first_row / p.G + 1;  // every row of the tile sees these keys
   const int n_pages = (n_keys + kP8Page - 1) / kP8Page;
-  // even ranges of this row tile's own pages, at least two pages a warp
-  const int per = max(2 * kWarps, (n_pages + p.splits - 1) / p.splits);
-  const int p_begin = split * per, p_end = min(n_pages, p_begin + per);
-  auto out_row = [&](int r) {  // row of out / ws (token-major, Hq heads)
-    return static_cast<int64_t>(row0 + r / p.G) * p.Hq + h * p.G + r % p.G;
-  };
-  if (p_begin >= p_end && split > 0) {
-    for (int r = threadIdx.x; r < R; r += blockDim.x)
-      if (first_row + r < rows) p.ws_lse[out_row(first_row + r) * p.splits + split] = -INFINITY;
-    return;
-  }
-  const int32_t* table = p.s.table + static_cast<int64_t>(seq) * p.s.max_pages;
-  const int first = p_begin + warp;
+  const int page = split * p.chunk;
+  if (page >= n_pages && split > 0) return;
+  const int p_end = min(n_pages, page + p.chunk);
+  const bool uncut = n_pages <= p.chunk;
+  const int first = page + warp;
   const int count = first < p_end ? (p_end - first + kWarps - 1) / kWarps : 0;
 
-  // Pages of this warp, 32 at a time: lane i looks up the i-th (pool offset, scales).
-  int64_t ids = 0, ids_next = 0;
-  float2 sc = make_float2(0.f, 0.f), sc_next = sc;
-  auto lookup = [&](int j) -> int64_t {
-    return j < count ? p8_page(table, first + kWarps * j, p.c.num_pages, p.err, 73) * p.c.Hkv + h
-                     : 0;
-  };
-  auto scales_of = [&](int j, int64_t ph) {
-    return j < count ? __ldg(reinterpret_cast<const float2*>(p.c.scales) + ph)
-                     : make_float2(0.f, 0.f);
-  };
-  ids = lookup(lane);
-  sc = scales_of(lane, ids);
-  if (count > 32) {
-    ids_next = lookup(32 + lane);
-    sc_next = scales_of(32 + lane, ids_next);
-  }
-  PageFrag<D> cur, nxt;
-  if (count > 0) cur.load(p.c.codes + __shfl_sync(kFull, ids, 0) * (2 * kP8Page * D), g, t);
-
-  // q as B fragments in f16, scaled by a power of two per row
-  uint32_t qb[NB][KS][2];
-  float qs[NB][2];   // of rows 2 t, 2 t + 1: scale * log2(e) * the power of two undone
-  int lim[NB][2];    // their visible keys
+  // constant lane offsets in a page of the ring (see the bank comment above)
+  uint32_t cp_off[2], k_off[2], v_off[2];
+  {
+    const int l8 = lane >> 3, c8 = lane & 7;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int r = first_row + nb * 8 + g;
+    for (int i = 0; i < 2; ++i) {
+      const int sw = D == 128 ? i * 4 + l8 : (2 * l8) & 7;
+      cp_off[i] = l8 * 128 + ((c8 ^ sw) * 16);
+      if (D == 128) {
+        k_off[i] = g * 128 + (((2 * t + i) ^ g) * 16);
+        const int r = 2 * t + i;
+        v_off[i] = kP8Page * D + r * 128 + ((g ^ r) * 16);
+      } else {
+        k_off[i] = (g >> 1) * 128 + ((((g & 1) * 4 + t) ^ ((2 * (g >> 1)) & 7)) * 16);
+        v_off[i] = kP8Page * D + t * 128 + (((i * 4 + (g >> 1)) ^ (2 * t)) * 16) + (g & 1) * 8;
+      }
+    }
+  }
+
+  // Pages of this warp (at most 32): lane i holds the i-th one's place and scales (K's; log2
+  // and reciprocal of V's, the reciprocal negative for a block of zeros).
+  int id = 0;
+  float ks_i = 0.f, lv_i = 0.f, rv_i = 1.f;
+  if (lane < count) {
+    id = static_cast<int>(p8_page(table, first + kWarps * lane, p.c.num_pages, p.err, 73) *
+                              p.c.Hkv + h);
+    const float2 sc = __ldg(reinterpret_cast<const float2*>(p.c.scales) + id);
+    const bool tiny = sc.y < kTinyScale, fine = sc.y <= 3.402823466e38f;
+    ks_i = sc.x;
+    lv_i = tiny ? -24.f : fine ? __log2f(sc.y) : sc.y - sc.y;  // not finite: NaN
+    rv_i = tiny ? -kTwo24 : fine ? __fdividef(1.f, sc.y) : 1.f;
+  }
+  auto issue = [&](int q) {  // pages U q, ..
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = U * q + u;
+      if (j < count) {
+        const uint8_t* src =
+            p.c.codes + static_cast<int64_t>(__shfl_sync(kFull, id, j)) * PB + lane * 16;
+        const uint32_t dst = ring + (j % kStages) * PB;
+#pragma unroll
+        for (int i = 0; i < PB / 512; ++i) cp_async16(dst + cp_off[i & 1] + i * 512, src + i * 512);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int q = 0; q < AHEAD; ++q) issue(q);
+
+  // ---- q: warp nb turns its eight rows into f16 B fragments in shared memory
+  if (warp < NB) {
+    const int r = first_row + warp * 8 + g;
     const bool live = r < rows;
     const T* qr = static_cast<const T*>(p.q) +
-                  static_cast<int64_t>(row0 + (live ? r / p.G : 0)) * p.q_stride +
-                  (h * p.G + (live ? r % p.G : 0)) * D;
-    float f[KS][4];
+                  static_cast<int64_t>(si.row0 + (live ? r / p.G : 0)) * p.q_stride +
+                  (h * p.G + (live ? r % p.G : 0)) * D + t * (D / 4);
+    uint4 u[D / 32];
     uint32_t top = 0;
 #pragma unroll
-    for (int hh = 0; hh < KH; ++hh)
+    for (int i = 0; i < D / 32; ++i)
+      u[i] = live ? __ldg(reinterpret_cast<const uint4*>(qr) + i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (live) u = __ldg(reinterpret_cast<const uint4*>(qr + 64 * hh + 16 * t) + c);
+    for (int i = 0; i < D / 32; ++i) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 x = P8Io<T>::unpack(word_of(u, e));
-          float* d = &f[hh * 4 + c * 2 + (e >> 1)][(e & 1) * 2];
-          d[0] = x.x;
-          d[1] = x.y;
-          top = max(top,
-                    max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = P8Io<T>::unpack(word_of(u[i], e));
+        top = max(top,
+                  max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
       }
+    }
     top = max(top, __shfl_xor_sync(kFull, top, 1));
     top = max(top, __shfl_xor_sync(kFull, top, 2));
     // 2^-e with 2^e the largest power of two in the row's magnitude
     const int ex = min(max(static_cast<int>(top >> 23), 27), 227);
     const float down = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
     const float up = __uint_as_float(static_cast<uint32_t>(ex) << 23) * p.scale_log2;
+    float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      qb[nb][k][0] = half2_of(f[k][0] * down, f[k][1] * down);
-      qb[nb][k][1] = half2_of(f[k][2] * down, f[k][3] * down);
+    for (int i = 0; i < D / 32; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = P8Io<T>::unpack(word_of(u[i], e));
+        w[e] = half2_of(x.x * down, x.y * down);
+        const float2 y = __half22float2(*reinterpret_cast<__half2*>(&w[e]));
+        sum += y.x + y.y;
+      }
+      *reinterpret_cast<uint4*>(smem + Cfg::QF + ((i * NB + warp) * 32 + lane) * 16) =
+          make_uint4(w[0], w[1], w[2], w[3]);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      qs[nb][i] = __shfl_sync(kFull, up, (2 * t + i) * 4);
-      const int rr = first_row + nb * 8 + 2 * t + i;
-      lim[nb][i] = rr < rows ? start + rr / p.G + 1 : 0;
+    sum += __shfl_xor_sync(kFull, sum, 1);
+    sum += __shfl_xor_sync(kFull, sum, 2);
+    if (t == 0) {
+      s_qs[warp * 8 + g] = kInt8 ? up * kTwo24 : up;
+      s_qb[warp * 8 + g] = kInt8 ? -128.f * sum * up : 0.f;
     }
   }
+  __syncthreads();
+  float qs[NB][2], qb[NB][2];  // of rows 2 t, 2 t + 1
+  int lim[NB][2];              // their visible keys
+  uint4 qr[NB == 1 ? KS / 2 : 1];
+  if constexpr (NB == 1) {
+#pragma unroll
+    for (int i = 0; i < KS / 2; ++i) qr[i] = lds16(qf + (i * 32 + lane) * 16);
+  }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = nb * 8 + 2 * t + i;
+      qs[nb][i] = s_qs[r];
+      qb[nb][i] = s_qb[r];
+      lim[nb][i] = first_row + r < rows ? start + (first_row + r) / p.G + 1 : 0;
+    }
+  float* sp = nullptr;         // scores of row 2 t, token g
+  if constexpr (MASS) sp = p.ws_s + (item * R + 2 * t) * Lp + g;
 
-  float o[NB][MT][4];
+  float o[NB][MT][4], ps[NB][4];
   float M[NB][2], l[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
     for (int j = 0; j < MT; ++j) o[nb][j][0] = o[nb][j][1] = o[nb][j][2] = o[nb][j][3] = 0.f;
-    M[nb][0] = M[nb][1] = -INFINITY;
+    ps[nb][0] = ps[nb][1] = ps[nb][2] = ps[nb][3] = 0.f;
+    M[nb][0] = M[nb][1] = kNone;
     l[nb][0] = l[nb][1] = 0.f;
   }
-  const int min_lim = start + first_row / p.G + 1;  // every row of the tile sees these keys
-  float lv_last = 0.f, rv_last = 1.f;
 
-  auto page_step = [&](PageFrag<D>& f, int j) {
-    const float ks = __shfl_sync(kFull, sc.x, j & 31), vs = __shfl_sync(kFull, sc.y, j & 31);
-    const int key0 = (first + kWarps * j) * kP8Page;
+  for (int j = 0; j < count; j += U) {
+    issue(j / U + AHEAD);
+    cp_async_wait<AHEAD>();  // this lane's share of pages j .. j + U - 1 has landed
+    __syncwarp();
+    uint32_t st[U];
+    float lv[U], rv[U], s[U][NB][4];
+    int key0[U];
     // ---- S^T = K Q^T
-    float s[NB][4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+    for (int u = 0; u < U; ++u) {
+      st[u] = ring + ((j + u) % kStages) * PB;
+      // past the warp's last page every key is hidden
+      key0[u] = j + u < count ? (first + kWarps * (j + u)) * kP8Page : 1 << 30;
 #pragma unroll
-    for (int hh = 0; hh < KH; ++hh)
+      for (int nb = 0; nb < NB; ++nb)
+        s[u][nb][0] = s[u][nb][1] = s[u][nb][2] = s[u][nb][3] = 0.f;
+    }
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t a0, a1, a2, a3;
-        p8_to_half<FMT>(word_of(f.k[0][hh], w), a0, a2);
-        p8_to_half<FMT>(word_of(f.k[1][hh], w), a1, a3);
+    for (int hh = 0; hh < KH; ++hh) {
+      uint4 ka[U], kb[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        ka[u] = lds16(st[u] + k_off[hh]);
+        kb[u] = lds16(st[u] + k_off[hh] + HALF);
+      }
+#pragma unroll
+      for (int w2 = 0; w2 < 2; ++w2) {
+        uint4 qv[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          if constexpr (NB == 1)
+            qv[nb] = qr[hh * 2 + w2];
+          else
+            qv[nb] = lds16(qf + (((hh * 2 + w2) * NB + nb) * 32 + lane) * 16);
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            uint32_t a0, a1, a2, a3;
+            operand<FMT>(flip<FMT>(word_of(ka[u], 2 * w2 + w)), a0, a2);
+            operand<FMT>(flip<FMT>(word_of(kb[u], 2 * w2 + w)), a1, a3);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              mma_f16(s[u][nb], a0, a1, a2, a3, word_of(qv[nb], 2 * w), word_of(qv[nb], 2 * w + 1));
+          }
+      }
+    }
+    // ---- w = s + log2(vs)
+    bool edge = false, grow = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = (j + u) & 31;
+      const float ks = __shfl_sync(kFull, ks_i, at);
+      lv[u] = __shfl_sync(kFull, lv_i, at);
+      rv[u] = __shfl_sync(kFull, rv_i, at);
+      edge |= key0[u] + kP8Page > min_lim;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = e & 1;  // row 2 t + i, token g + 8 (e / 2)
+          const float y = fmaf(s[u][nb][e], qs[nb][i], qb[nb][i]);
+          if constexpr (MASS) {
+            const float x = y * ks;
+            if (lim[nb][i] > 0 && (u == 0 || j + u < count))
+              sp[(nb * 8 + i) * Lp + key0[u] + 8 * (e >> 1)] = x;
+            s[u][nb][e] = x + lv[u];
+          } else {
+            s[u][nb][e] = fmaf(y, ks, lv[u]);
+          }
+        }
+    }
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-          mma_f16(s[nb], a0, a1, a2, a3, qb[nb][hh * 4 + w][0], qb[nb][hh * 4 + w][1]);
-      }
-    // ---- w = s + log2(vs); a V block of (nearly) zeros adds to l alone
-    const bool has_v = !(vs < kTinyScale);
-    const bool fine = vs <= 3.402823466e38f;
-    if (has_v && fine) {
-      lv_last = __log2f(vs);
-      rv_last = __fdividef(1.f, vs);
-    }
-    const float lv = fine ? lv_last : vs - vs, rv = rv_last;  // not finite: NaN
-    const bool edge = key0 + kP8Page > min_lim;
-    bool grow = false;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = e & 1;  // row 2 t + i, token g + 8 (e / 2)
-        float x = s[nb][e] * (ks * qs[nb][i]);
-        const bool hidden = edge && key0 + g + 8 * (e >> 1) >= lim[nb][i];
-        if constexpr (MASS) {
-          const int r = first_row + nb * 8 + 2 * t + i;
-          if (r < rows)
-            p.ws_s[out_row(r) * p.s_stride + key0 + g + 8 * (e >> 1)] = x;
-        }
-        s[nb][e] = hidden ? -INFINITY : x + lv;
-        grow |= s[nb][e] > M[nb][i] + kGrow;
-      }
+          for (int e = 0; e < 4; ++e)
+            if (key0[u] + g + 8 * (e >> 1) >= lim[nb][e & 1]) s[u][nb][e] = -INFINITY;
     }
+    float mx[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float m = fmaxf(s[0][nb][i], s[0][nb][2 + i]);
+        if constexpr (U == 2) m = fmaxf(m, fmaxf(s[U - 1][nb][i], s[U - 1][nb][2 + i]));
+        mx[nb][i] = m;
+        grow |= m > M[nb][i] + kGrow;
+      }
     if (__any_sync(kFull, grow)) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float m = fmaxf(s[nb][i], s[nb][2 + i]);
+          float m = mx[nb][i];
           m = fmaxf(m, __shfl_xor_sync(kFull, m, 4));
           m = fmaxf(m, __shfl_xor_sync(kFull, m, 8));
           m = fmaxf(m, __shfl_xor_sync(kFull, m, 16));
           m = fmaxf(m, M[nb][i]);
-          const float a = M[nb][i] == -INFINITY ? 0.f : ex2f(M[nb][i] - m);
+          const float a = ex2f(M[nb][i] - m);
           M[nb][i] = m;
           l[nb][i] *= a;
+          ps[nb][i] *= a;
 #pragma unroll
           for (int jj = 0; jj < MT; ++jj) {
             o[nb][jj][i] *= a;
@@ -312,62 +478,77 @@ __global__ void __launch_bounds__(kWarps * 32) p8_attn_kernel(const AttnParams p
           }
         }
     }
-    uint32_t pb[NB][2];
+    uint32_t pb[U][NB][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float e4[4];
+    for (int u = 0; u < U; ++u) {
+      const float rl = fabsf(rv[u]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float base = M[nb][i] == -INFINITY ? 0.f : M[nb][i];  // nothing visible yet
-        e4[i] = ex2f(s[nb][i] - base);
-        e4[2 + i] = ex2f(s[nb][2 + i] - base);
-        const float sum = e4[i] + e4[2 + i];
-        l[nb][i] += sum == 0.f ? 0.f : sum * rv;
+      for (int nb = 0; nb < NB; ++nb) {
+        float e4[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          e4[i] = ex2f(s[u][nb][i] - M[nb][i]);
+          e4[2 + i] = ex2f(s[u][nb][2 + i] - M[nb][i]);
+          l[nb][i] = fmaf(e4[i] + e4[2 + i], rl, l[nb][i]);
+        }
+        pb[u][nb][0] = transpose8x8(half2_of(e4[0], e4[1]));
+        pb[u][nb][1] = transpose8x8(half2_of(e4[2], e4[3]));
       }
-      pb[nb][0] = has_v ? transpose8x8(half2_of(e4[0], e4[1])) : 0u;
-      pb[nb][1] = has_v ? transpose8x8(half2_of(e4[2], e4[3])) : 0u;
+      if (rv[u] < 0.f) {  // a V block of zeros adds to l alone
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) pb[u][nb][0] = pb[u][nb][1] = 0u;
+      }
     }
-    // ---- O^T += V^T P^T; codes past the last visible key are never looked at
-    const int live = n_keys - key0;
-    if (live < kP8Page) {
+    // ---- O^T += V^T P^T
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (2 * t + (i & 1) + 8 * (i >> 1) >= live)
+    for (int u = 0; u < U; ++u) {
+      uint32_t v[4][VW];         // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-          for (int w = 0; w < PageFrag<D>::VW; ++w) f.v[i][w] = 0u;
-    }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = st[u] + v_off[i & 1] + (i >> 1) * HALF;
+        if constexpr (D == 128) {
+          const uint4 x = lds16(a);
 #pragma unroll
-    for (int w = 0; w < PageFrag<D>::VW; ++w) {
+          for (int w = 0; w < 4; ++w) v[i][w] = flip<FMT>(word_of(x, w));
+        } else {
+          const uint2 x = lds8(a);
+          v[i][0] = flip<FMT>(x.x);
+          v[i][1] = flip<FMT>(x.y);
+        }
+      }
+      if constexpr (!kInt8) {  // codes past the last visible key may be NaN
+        const int live = n_keys - key0[u];
+        if (live < kP8Page) {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {  // bytes 4 w + 2 hf, + 1 of the piece
-        const uint32_t sel = hf == 0 ? 0x5140 : 0x7362;
-        uint32_t a0, a1, a2, a3;
-        p8_to_half<FMT>(__byte_perm(f.v[0][w], f.v[1][w], sel), a0, a1);
-        p8_to_half<FMT>(__byte_perm(f.v[2][w], f.v[3][w], sel), a2, a3);
+          for (int i = 0; i < 4; ++i)
+            if (2 * t + (i & 1) + 8 * (i >> 1) >= live)
+#pragma unroll
+              for (int w = 0; w < VW; ++w) v[i][w] = 0u;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {  // bytes 4 w + 2 hf, + 1 of the piece
+          const uint32_t sel = hf == 0 ? 0x5140 : 0x7362;
+          uint32_t a0, a1, a2, a3;
+          operand<FMT>(__byte_perm(v[0][w], v[1][w], sel), a0, a1);
+          operand<FMT>(__byte_perm(v[2][w], v[3][w], sel), a2, a3);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            mma_f16(o[nb][2 * w + hf], a0, a1, a2, a3, pb[u][nb][0], pb[u][nb][1]);
+        }
+      if constexpr (kInt8) {
+        constexpr uint32_t kOnes = 0x3c003c00u;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-          mma_f16(o[nb][2 * w + hf], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
+          mma_f16(ps[nb], kOnes, kOnes, kOnes, kOnes, pb[u][nb][0], pb[u][nb][1]);
       }
     }
-  };
-  auto fetch = [&](PageFrag<D>& f, int j) {  // page j's codes; j in the current or next 32
-    const int64_t ph = __shfl_sync(kFull, (j & ~31) == 0 || (j & 31) ? ids : ids_next, j & 31);
-    f.load(p.c.codes + ph * (2 * kP8Page * D), g, t);
-  };
-  for (int j = 0; j < count; j += 2) {
-    if (j + 1 < count) fetch(nxt, j + 1);
-    page_step(cur, j);
-    if (j + 1 < count) {
-      if (j + 2 < count) fetch(cur, j + 2);
-      page_step(nxt, j + 1);
-    }
-    if (((j + 2) & 31) == 0) {  // the next 32 pages become current
-      ids = ids_next;
-      sc = sc_next;
-      ids_next = lookup(j + 2 + 32 + lane);
-      sc_next = scales_of(j + 2 + 32 + lane, ids_next);
-    }
+    __syncwarp();  // every lane is done with these stages before they are refilled
   }
+  cp_async_wait<0>();
+  __syncthreads();  // the ring becomes the join's buffer
 
   // ---- join the warps
 #pragma unroll
@@ -380,56 +561,170 @@ __global__ void __launch_bounds__(kWarps * 32) p8_attn_kernel(const AttnParams p
       x += __shfl_xor_sync(kFull, x, 16);
       const int r = nb * 8 + 2 * t + i;
       if (g == 0) {
-        s_m[warp][r] = M[nb][i];
-        s_l[warp][r] = x;
+        s_m[warp * R + r] = M[nb][i];
+        s_l[warp * R + r] = x;
       }
+      const float off = -128.f * ps[nb][i];
+      auto val = [&](int j, int z) {
+        return kInt8 ? fmaf(o[nb][j][z + i], kTwo24, off) : o[nb][j][z + i];
+      };
       // dims g D / 8 + 2 j (+ 1): element j of the lane's piece, two per m-tile
+      if (first_row + r < rows) {
 #pragma unroll
-      for (int j = 0; j < MT; j += 2)
-        *reinterpret_cast<float4*>(&s_o[warp][r][g * DL + 2 * j]) =
-            make_float4(o[nb][j][i], o[nb][j][2 + i], o[nb][j + 1][i], o[nb][j + 1][2 + i]);
+        for (int j = 0; j < MT; j += 2)
+          *reinterpret_cast<float4*>(s_o + (warp * R + r) * D + g * DL + 2 * j) =
+              make_float4(val(j, 0), val(j, 2), val(j + 1, 0), val(j + 1, 2));
+      }
     }
   __syncthreads();
-  for (int e = threadIdx.x; e < R * (D / 4); e += blockDim.x) {
+  const int64_t slot = item * p.splits + split;
+  for (int e = threadIdx.x; e < R * (D / 4); e += kWarps * 32) {
     const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-    if (first_row + r >= rows) continue;
-    float m = -INFINITY;
+    if (first_row + r >= rows) break;
+    float m = s_m[r];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_m[w][r]);
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w * R + r]);
     float den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (s_m[w][r] == -INFINITY && s_l[w][r] == 0.f) continue;
-      const float x = ex2f(s_m[w][r] - m);
-      const float4 y = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
-      den += s_l[w][r] * x;
-      acc.x += y.x * x;
-      acc.y += y.y * x;
-      acc.z += y.z * x;
-      acc.w += y.w * x;
+      const float x = ex2f(s_m[w * R + r] - m);
+      const float4 y = *reinterpret_cast<const float4*>(s_o + (w * R + r) * D + d);
+      den = fmaf(s_l[w * R + r], x, den);
+      acc.x = fmaf(y.x, x, acc.x);
+      acc.y = fmaf(y.y, x, acc.y);
+      acc.z = fmaf(y.z, x, acc.z);
+      acc.w = fmaf(y.w, x, acc.w);
     }
     const float inv = den == 0.f ? 0.f : __fdiv_rn(1.f, den);  // no visible key: 0
     acc.x *= inv;
     acc.y *= inv;
     acc.z *= inv;
     acc.w *= inv;
-    const int64_t orow = out_row(first_row + r);
-    if (p.splits == 1) {
+    if (uncut) {
+      const int64_t orow = static_cast<int64_t>(si.row0 + (first_row + r) / p.G) * p.Hq +
+                           h * p.G + (first_row + r) % p.G;
       uint2 u;
       u.x = P8Io<T>::pack(acc.x, acc.y);
       u.y = P8Io<T>::pack(acc.z, acc.w);
       *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + orow * D + d) = u;
     } else {
-      *reinterpret_cast<float4*>(p.ws_o + (orow * p.splits + split) * D + d) = acc;
+      *reinterpret_cast<float4*>(p.ws_o + (slot * R + r) * D + d) = acc;
     }
-    if (d == 0 && p.ws_lse != nullptr)
-      p.ws_lse[orow * p.splits + split] = den == 0.f ? -INFINITY : m + log2f(den);
+    if (d == 0 && (MASS || !uncut)) {
+      const float lse = den == 0.f ? -INFINITY : m + log2f(den);
+      if (MASS && p.splits == 1 && p.row_tiles == 1)
+        s_qs[r] = lse;
+      else
+        p.ws_lse[slot * R + r] = lse;
+    }
+  }
+  if constexpr (MASS) {
+    if (p.splits == 1 && p.row_tiles == 1) {  // this CTA has every row and key of the head
+      __syncthreads();
+      for (int j = threadIdx.x; j < si.kv; j += kWarps * 32)
+        add_mass(p, table, h, j, p.ws_s + item * R * Lp + j, Lp, max(0, j - start) * p.G, rows,
+                 s_qs);
+    }
   }
 }
 
-// Joins the splits of a row: out = sum 2^(lse_s - L) o_s with L = log2 sum 2^lse_s, and
-// leaves L in the row's first lse slot for the weights.
+// Joins the chunks of an item: out = sum 2^(lse_c - L) o_c with L = log2 sum 2^lse_c, in the
+// order of its pages.  `wpr` warps share a row (eight where there are many chunks).  With
+// mass, further CTAs of kTokens tokens of a (sequence, KV head) add the weights.  Launched so
+// that its start overlaps the end of p8_attn_kernel, which it waits for.
+constexpr int kTokens = 512;
+template <typename T, int D, int NB, bool MASS>
+__global__ void __launch_bounds__(256)
+    p8_finish_kernel(const AttnParams p, int join_ctas, int wpr) {
+  constexpr int R = 8 * NB;
+  constexpr int VL = D / 32;  // dims of a lane
+  __shared__ float s_lse[kMaxRows];
+  __shared__ float s_acc[8][D];
+  const int seq = blockIdx.y / p.c.Hkv, h = blockIdx.y % p.c.Hkv;
+  const SeqInfo si = seq_info<R>(p, seq);  // inputs, complete before p8_attn_kernel began
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int start = si.kv - si.q_len;
+  const int64_t item0 = static_cast<int64_t>(blockIdx.y) * p.row_tiles;
+  auto chunks_of = [&](int rt) {
+    const int last_tok = (min(si.rows, (rt + 1) * R) - 1) / p.G;
+    const int n_pages = (max(0, start + last_tok + 1) + kP8Page - 1) / kP8Page;
+    return max(1, (n_pages + p.chunk - 1) / p.chunk);
+  };
+  // a row's L, by one warp
+  auto total_lse = [&](const float* lse, int n) {
+    float m = -INFINITY;
+    for (int c = lane; c < n; c += 32) m = fmaxf(m, lse[c * R]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+    const float base = m == -INFINITY ? 0.f : m;
+    float den = 0.f;
+    for (int c = lane; c < n; c += 32) den += ex2f(lse[c * R] - base);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(kFull, den, o);
+    return den == 0.f ? -INFINITY : base + log2f(den);
+  };
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (static_cast<int>(blockIdx.x) < join_ctas) {
+    const int rr = (blockIdx.x * 8 + warp) / wpr, part = warp % wpr;
+    const int rt = rr / R, r = rr % R;
+    const int n = rr < si.rows ? chunks_of(rt) : 0;
+    float acc[VL] = {};
+    if (n > 1) {
+      const int64_t slot = (item0 + rt) * p.splits;
+      const float* lse = p.ws_lse + slot * R + r;
+      float L = total_lse(lse, n);
+      if (L == -INFINITY) L = 0.f;
+      const float* src = p.ws_o + (slot * R + r) * D + lane * VL;
+#pragma unroll 4
+      for (int c = part; c < n; c += wpr) {
+        const float w = ex2f(lse[c * R] - L);
+        float x[VL];
+        if constexpr (VL == 4)
+          *reinterpret_cast<float4*>(x) =
+              *reinterpret_cast<const float4*>(src + static_cast<int64_t>(c) * R * D);
+        else
+          *reinterpret_cast<float2*>(x) =
+              *reinterpret_cast<const float2*>(src + static_cast<int64_t>(c) * R * D);
+#pragma unroll
+        for (int i = 0; i < VL; ++i) acc[i] = fmaf(w, x[i], acc[i]);
+      }
+    }
+    if (wpr > 1) {  // all eight warps have one row
+#pragma unroll
+      for (int i = 0; i < VL; ++i) s_acc[warp][lane * VL + i] = acc[i];
+      __syncthreads();
+      if (warp > 0) return;
+#pragma unroll
+      for (int i = 0; i < VL; ++i)
+        for (int w = 1; w < 8; ++w) acc[i] += s_acc[w][lane * VL + i];
+    }
+    if (n > 1) {
+      const int64_t orow = static_cast<int64_t>(si.row0 + rr / p.G) * p.Hq + h * p.G + rr % p.G;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + orow * D + lane * VL);
+#pragma unroll
+      for (int i = 0; i < VL; i += 2) dst[i / 2] = P8Io<T>::pack(acc[i], acc[i + 1]);
+    }
+    return;
+  }
+  if constexpr (MASS) {
+    const int j0 = (blockIdx.x - join_ctas) * kTokens;
+    if (j0 >= si.kv) return;
+    for (int r = warp; r < si.rows; r += 8) {
+      const float L = total_lse(p.ws_lse + (item0 + r / R) * p.splits * R + r % R, chunks_of(r / R));
+      if (lane == 0) s_lse[r] = L;
+    }
+    __syncthreads();
+    const int32_t* table = p.s.table + static_cast<int64_t>(seq) * p.s.max_pages;
+    const int64_t Lp = static_cast<int64_t>(p.s.max_pages) * kP8Page;
+    for (int j = j0 + threadIdx.x; j < min(si.kv, j0 + kTokens); j += 256)
+      add_mass(p, table, h, j, p.ws_s + item0 * R * Lp + j, Lp, max(0, j - start) * p.G, si.rows,
+               s_lse);
+  }
+}
+
+// Joins the splits of a row of a long chunk: out = sum 2^(lse_s - L) o_s with
+// L = log2 sum 2^lse_s, and leaves L in the row's first lse slot for the weights.
 template <typename T>
 __global__ void __launch_bounds__(128)
     p8_combine_kernel(const float* __restrict__ ws_o, float* __restrict__ ws_lse,
@@ -461,61 +756,44 @@ __global__ void __launch_bounds__(128)
   if (lane == 0) lse[0] = den == 0.f ? -INFINITY : base + log2f(den);
 }
 
-// mass_out[j] = mass_in[j] + sum over the KV head's rows of 2^(s_j - L), in row order.
-__global__ void __launch_bounds__(128)
-    p8_mass_kernel(P8Cache c, P8Seqs s, const float* __restrict__ ws_s, int64_t s_stride,
-                   const float* __restrict__ lse, int splits, int Hq, int G,
-                   const float* __restrict__ mass_in, float* __restrict__ mass_out, int* err) {
-  const int seq = blockIdx.z, h = blockIdx.y;
-  const int kv = p8_len(s.kv_lens, seq, s.max_pages, err, 74);
-  const int j = blockIdx.x * blockDim.x + threadIdx.x;
-  if (j >= kv) return;
-  const int row0 = __ldg(s.cu_q + seq), q_len = __ldg(s.cu_q + seq + 1) - row0;
-  const int start = kv - q_len;
-  const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages, j / kP8Page,
-                               c.num_pages, err, 75);
-  float w = 0.f;
-  for (int tok = max(0, j - start); tok < q_len; ++tok)
-    for (int g = 0; g < G; ++g) {
-      const int64_t row = static_cast<int64_t>(row0 + tok) * Hq + h * G + g;
-      w += ex2f(ws_s[row * s_stride + j] - lse[row * splits]);
-    }
-  const int64_t at = (page * c.Hkv + h) * kP8Page + j % kP8Page;
-  mass_out[at] = mass_in[at] + w;
-}
-
-template <typename T, int FMT, int D, bool MASS>
-int launch_nb(const AttnParams& p, int rows, cudaStream_t st) {
-  AttnParams a = p;
-  const int nb = rows <= 8 ? 1 : 2;
-  a.row_tiles = (rows + 8 * nb - 1) / (8 * nb);
-  const int64_t gx = static_cast<int64_t>(a.splits) * a.row_tiles;
-  if (gx > 0x7fffffff) return -3;
-  const dim3 grid(static_cast<unsigned>(gx), a.c.Hkv, a.s.num_seqs);
-  if (nb == 1)
-    p8_attn_kernel<T, FMT, D, 1, MASS><<<grid, kWarps * 32, 0, st>>>(a);
-  else
-    p8_attn_kernel<T, FMT, D, 2, MASS><<<grid, kWarps * 32, 0, st>>>(a);
-  return 0;
+template <typename T, int FMT, int D, int NB, bool MASS>
+int launch_nb(const AttnParams& p, cudaStream_t st) {
+  using Cfg = AttnCfg<D, NB>;
+  auto kern = p8_attn_kernel<T, FMT, D, NB, MASS>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM))
+    return static_cast<int>(cudaGetLastError());
+  kern<<<dim3(p.splits * p.row_tiles, p.c.Hkv, p.s.num_seqs), kWarps * 32, Cfg::SMEM, st>>>(p);
+  if (p.splits == 1 && !(MASS && p.row_tiles > 1)) return 0;
+  const int wpr = p.splits > 16 ? 8 : 1;
+  const int join = p.splits > 1 ? p.row_tiles * NB * wpr : 0;
+  const int tokens = MASS ? (p.s.max_pages * kP8Page + kTokens - 1) / kTokens : 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(join + tokens, p.c.Hkv * p.s.num_seqs);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, p8_finish_kernel<T, D, NB, MASS>, p, join, wpr));
 }
 
 template <typename T, int FMT, int D>
-int launch_attn(const AttnParams& p, const P8Attn& a, int rows, cudaStream_t st) {
-  const bool mass = a.mass_out != nullptr;
-  const int rc = mass ? launch_nb<T, FMT, D, true>(p, rows, st)
-                      : launch_nb<T, FMT, D, false>(p, rows, st);
-  if (rc) return rc;
-  if (p.splits > 1) {
-    const int rc = p8_combine(a, D, st);
-    if (rc) return rc;
+int launch_attn(const AttnParams& p, int nb, cudaStream_t st) {
+  const bool mass = p.mass_out != nullptr;
+#define CFB_NB(NBV)                                                       \
+  case NBV:                                                               \
+    return mass ? launch_nb<T, FMT, D, NBV, true>(p, st)            \
+                : launch_nb<T, FMT, D, NBV, false>(p, st);
+  switch (nb) {
+    CFB_NB(1)
+    CFB_NB(2)
+    CFB_NB(3)
+    CFB_NB(4)
+    default: return -2;
   }
-  if (mass) {
-    const int L = p.s.max_pages * kP8Page;
-    p8_mass_kernel<<<dim3((L + 127) / 128, p.c.Hkv, p.s.num_seqs), 128, 0, st>>>(
-        p.c, p.s, a.ws_s, p.s_stride, a.ws_lse, p.splits, a.Hq, p.G, a.mass_in, a.mass_out,
-        p.err);
-  }
-  return 0;
+#undef CFB_NB
 }
 
 }  // namespace
@@ -533,21 +811,37 @@ int p8_combine(const P8Attn& a, int D, cudaStream_t st) {
   return 0;
 }
 
-int p8_attn_splits(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_sms) {
+P8AttnPlan p8_attn_plan(const P8Cache& c, const P8Seqs& s, int group, int max_q_len, bool mass,
+                        int num_sms) {
+  P8AttnPlan pl;
   const int rows = max_q_len * group;
-  const int per_tile = rows <= 8 ? 8 : 16;
-  const int64_t ctas = static_cast<int64_t>((rows + per_tile - 1) / per_tile) * Hkv * s.num_seqs;
-  // about six CTAs for each SM, and at least two pages for each warp
-  int64_t sp = (6 * static_cast<int64_t>(num_sms) + ctas - 1) / ctas;
-  const int64_t most = (s.max_pages + 2 * kWarps - 1) / (2 * kWarps);
-  if (sp > most) sp = most;
-  return static_cast<int>(sp < 1 ? 1 : sp);
+  // as few row tiles as 32 rows of a CTA allow: a tile reads and converts all its pages
+  pl.row_tiles = (rows + 31) / 32;
+  pl.nb = ((rows + pl.row_tiles - 1) / pl.row_tiles + 7) / 8;
+  const int64_t items = static_cast<int64_t>(s.num_seqs) * c.Hkv * pl.row_tiles;
+  const int R = 8 * pl.nb;
+  if (s.max_pages <= kWholePages) {
+    pl.chunk = kWholePages;
+  } else {  // about three waves of CTAs, were all sequences as long as the table is wide
+    const int64_t ctas = 3 * static_cast<int64_t>(num_sms) * (pl.nb <= 2 ? 3 : 2);
+    const int64_t chunk = (items * s.max_pages + ctas - 1) / ctas;
+    pl.chunk = static_cast<int>(std::min<int64_t>(std::max<int64_t>(chunk, kMinPages), kMaxPages));
+  }
+  pl.splits = (s.max_pages + pl.chunk - 1) / pl.chunk;
+  if (pl.splits > 1) pl.n_o = items * pl.splits * R * c.D;
+  if (pl.splits > 1 || mass) pl.n_lse = items * pl.splits * R;
+  if (mass) pl.n_s = items * R * s.max_pages * kP8Page;
+  return pl;
 }
 
-int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err,
-                 cudaStream_t stream) {
+int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, const P8AttnPlan& plan,
+                 float* ws, int* err, cudaStream_t stream) {
   if (a.N <= 0 || s.num_seqs <= 0) return 0;
-  if (s.num_seqs > 65535 || c.Hkv > 65535) return -3;
+  const int64_t heads = static_cast<int64_t>(s.num_seqs) * c.Hkv;
+  if (heads > 65535 || c.num_pages * c.Hkv > 0x7fffffff ||
+      static_cast<int64_t>(plan.splits) * plan.row_tiles > 0x7fffffff ||
+      plan.chunk > 32 * kWarps || static_cast<int64_t>(a.max_q_len) * (a.Hq / c.Hkv) > kMaxRows)
+    return -3;
   AttnParams p;
   p.c = c;
   p.s = s;
@@ -557,25 +851,26 @@ int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err,
   p.N = a.N;
   p.Hq = a.Hq;
   p.G = a.Hq / c.Hkv;
-  p.splits = a.splits;
-  p.row_tiles = 1;
+  p.row_tiles = plan.row_tiles;
+  p.chunk = plan.chunk;
+  p.splits = plan.splits;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  p.ws_o = a.ws_o;
-  p.ws_lse = a.ws_lse;
-  p.ws_s = a.ws_s;
-  p.s_stride = static_cast<int64_t>(s.max_pages) * kP8Page;
+  p.ws_o = ws;
+  p.ws_lse = p.ws_o + plan.n_o;
+  p.ws_s = p.ws_lse + plan.n_lse;
+  p.mass_in = a.mass_in;
+  p.mass_out = a.mass_out;
   p.err = err;
-  const int rows = a.max_q_len * p.G;
   int rc = 0;
   switch (a.type * 4 + c.fmt * 2 + (c.D == 128)) {
-    case 0: rc = launch_attn<__nv_bfloat16, kP8Int8, 64>(p, a, rows, stream); break;
-    case 1: rc = launch_attn<__nv_bfloat16, kP8Int8, 128>(p, a, rows, stream); break;
-    case 2: rc = launch_attn<__nv_bfloat16, kP8E4m3, 64>(p, a, rows, stream); break;
-    case 3: rc = launch_attn<__nv_bfloat16, kP8E4m3, 128>(p, a, rows, stream); break;
-    case 4: rc = launch_attn<__half, kP8Int8, 64>(p, a, rows, stream); break;
-    case 5: rc = launch_attn<__half, kP8Int8, 128>(p, a, rows, stream); break;
-    case 6: rc = launch_attn<__half, kP8E4m3, 64>(p, a, rows, stream); break;
-    case 7: rc = launch_attn<__half, kP8E4m3, 128>(p, a, rows, stream); break;
+    case 0: rc = launch_attn<__nv_bfloat16, kP8Int8, 64>(p, plan.nb, stream); break;
+    case 1: rc = launch_attn<__nv_bfloat16, kP8Int8, 128>(p, plan.nb, stream); break;
+    case 2: rc = launch_attn<__nv_bfloat16, kP8E4m3, 64>(p, plan.nb, stream); break;
+    case 3: rc = launch_attn<__nv_bfloat16, kP8E4m3, 128>(p, plan.nb, stream); break;
+    case 4: rc = launch_attn<__half, kP8Int8, 64>(p, plan.nb, stream); break;
+    case 5: rc = launch_attn<__half, kP8Int8, 128>(p, plan.nb, stream); break;
+    case 6: rc = launch_attn<__half, kP8E4m3, 64>(p, plan.nb, stream); break;
+    case 7: rc = launch_attn<__half, kP8E4m3, 128>(p, plan.nb, stream); break;
     default: return -2;
   }
   return rc ? rc : static_cast<int>(cudaGetLastError());

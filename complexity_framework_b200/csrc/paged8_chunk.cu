@@ -824,7 +824,7 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
 }  // namespace
 
 bool p8_is_chunk(int max_q_len, int group) {
-  return static_cast<int64_t>(max_q_len) * group > 64 && group <= kT / 2;
+  return static_cast<int64_t>(max_q_len) * group > 64;
 }
 
 void p8_chunk_plan(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_sms, int* nq,

@@ -205,7 +205,7 @@ def run_attention(lens, new, hq, hkv, d, dtype, io, seed=0, mass=False, width=No
 DECODE = [
     ([1], 4, 2, 64), ([15, 16, 17, 0, 31], 8, 8, 128), ([700, 1, 333, 129], 32, 8, 128),
     ([257, 64], 14, 2, 64), ([90, 260], 8, 1, 128), ([130], 10, 1, 64), ([200, 5], 16, 1, 128),
-    ([45], 24, 1, 64),
+    ([45], 24, 1, 64), ([70, 33], 80, 2, 64), ([1000, 1, 40], 33, 1, 128),
 ]
 
 
@@ -216,11 +216,28 @@ def test_decode(lens, hq, hkv, d, dtype, io):
     run_attention(lens, [1] * len(lens), hq, hkv, d, dtype, io, mass=io == torch.bfloat16)
 
 
+def test_sequences_without_new_tokens():
+    """They have no rows; their weights pass through.  Table widths of both work splits."""
+    for width in (8, 200):
+        for new in ([1, 0, 2], [0, 100, 0]):
+            run_attention([100, 37, 120], new, 4, 2, 64, INT8, torch.bfloat16, mass=True,
+                          width=width)
+
+
+def test_many_sequences():
+    """More sequences than one pass of the work split's sums takes, uneven ones among them."""
+    lens = [(7 * i) % 50 for i in range(300)]
+    run_attention(lens, [1] * 300, 2, 1, 64, INT8, torch.bfloat16, mass=True, width=60)
+    run_attention(lens, [3] * 300, 2, 1, 64, FP8, torch.bfloat16, width=4)
+
+
 def test_decode_long_split():
     """Many splits, page-table rows wider than the sequences, more than 32 pages a warp."""
     run_attention([9000, 70, 3100], [1, 1, 1], 4, 1, 128, INT8, torch.bfloat16, mass=True,
                   width=1000)
     run_attention([9001] * 40, [1] * 40, 4, 4, 64, FP8, torch.bfloat16, width=563)
+    run_attention([5000, 0, 900, 2111], [5, 1, 7, 3], 8, 2, 128, INT8, torch.bfloat16, mass=True,
+                  width=400)
 
 
 CHUNKS = [
