@@ -209,15 +209,21 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
   const int g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * (kStages * PB);
   const uint32_t qf = smem_u32(smem + Cfg::QF);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // p8_finish_kernel waits
+  // started while the kernel before it ends, and lets the next one start: both ends wait
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int split = blockIdx.x % p.splits, rt = blockIdx.x / p.splits;
   const int h = blockIdx.y, seq = blockIdx.z;
+  // a page-table entry for each lane, read together with the lengths that say whether it counts
+  const int32_t* table = p.s.table + static_cast<int64_t>(seq) * p.s.max_pages;
+  const int page = split * p.chunk, first = page + warp;
+  const int entry = first + kWarps * lane;
+  int id = entry < p.s.max_pages ? __ldg(table + entry) : 0;
   const SeqInfo si = seq_info<R>(p, seq);
   const int rows = si.rows, first_row = rt * R;
   // row r is token r / G and head r % G; it sees the keys [0, start + token + 1)
   const int start = si.kv - si.q_len;
-  const int32_t* table = p.s.table + static_cast<int64_t>(seq) * p.s.max_pages;
   const int64_t Lp = static_cast<int64_t>(p.s.max_pages) * kP8Page;
   const int64_t item = (static_cast<int64_t>(seq) * p.c.Hkv + h) * p.row_tiles + rt;
   if (first_row >= rows) {
@@ -230,11 +236,9 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
   const int n_keys = max(0, start + last_tok + 1);
   const int min_lim = start + first_row / p.G + 1;  // every row of the tile sees these keys
   const int n_pages = (n_keys + kP8Page - 1) / kP8Page;
-  const int page = split * p.chunk;
   if (page >= n_pages && split > 0) return;
   const int p_end = min(n_pages, page + p.chunk);
   const bool uncut = n_pages <= p.chunk;
-  const int first = page + warp;
   const int count = first < p_end ? (p_end - first + kWarps - 1) / kWarps : 0;
 
   // constant lane offsets in a page of the ring (see the bank comment above)
@@ -258,11 +262,13 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
 
   // Pages of this warp (at most 32): lane i holds the i-th one's place and scales (K's; log2
   // and reciprocal of V's, the reciprocal negative for a block of zeros).
-  int id = 0;
   float ks_i = 0.f, lv_i = 0.f, rv_i = 1.f;
   if (lane < count) {
-    id = static_cast<int>(p8_page(table, first + kWarps * lane, p.c.num_pages, p.err, 73) *
-                              p.c.Hkv + h);
+    if (static_cast<uint32_t>(id) >= static_cast<uint64_t>(p.c.num_pages)) {
+      report_error(p.err, kErrBounds, 73);  // not followed: page 0 is read instead
+      id = 0;
+    }
+    id = id * p.c.Hkv + h;
     const float2 sc = __ldg(reinterpret_cast<const float2*>(p.c.scales) + id);
     const bool tiny = sc.y < kTinyScale, fine = sc.y <= 3.402823466e38f;
     ks_i = sc.x;
@@ -665,6 +671,7 @@ __global__ void __launch_bounds__(256)
     return den == 0.f ? -INFINITY : base + log2f(den);
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (static_cast<int>(blockIdx.x) < join_ctas) {
     const int rr = (blockIdx.x * 8 + warp) / wpr, part = warp % wpr;
     const int rt = rr / R, r = rr % R;
@@ -673,21 +680,35 @@ __global__ void __launch_bounds__(256)
     if (n > 1) {
       const int64_t slot = (item0 + rt) * p.splits;
       const float* lse = p.ws_lse + slot * R + r;
+      const float* src = p.ws_o + (slot * R + r) * D + lane * VL;
+      // four chunks at a time, the first four before L is known
+      float x[4][VL], ls[4];
+      auto fetch = [&](int c0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int c = c0 + k * wpr;
+          if (c >= n) break;
+          ls[k] = lse[c * R];
+          if constexpr (VL == 4)
+            *reinterpret_cast<float4*>(x[k]) =
+                *reinterpret_cast<const float4*>(src + static_cast<int64_t>(c) * R * D);
+          else
+            *reinterpret_cast<float2*>(x[k]) =
+                *reinterpret_cast<const float2*>(src + static_cast<int64_t>(c) * R * D);
+        }
+      };
+      fetch(part);
       float L = total_lse(lse, n);
       if (L == -INFINITY) L = 0.f;
-      const float* src = p.ws_o + (slot * R + r) * D + lane * VL;
-#pragma unroll 4
-      for (int c = part; c < n; c += wpr) {
-        const float w = ex2f(lse[c * R] - L);
-        float x[VL];
-        if constexpr (VL == 4)
-          *reinterpret_cast<float4*>(x) =
-              *reinterpret_cast<const float4*>(src + static_cast<int64_t>(c) * R * D);
-        else
-          *reinterpret_cast<float2*>(x) =
-              *reinterpret_cast<const float2*>(src + static_cast<int64_t>(c) * R * D);
+      for (int c0 = part; c0 < n; c0 += 4 * wpr) {
+        if (c0 != part) fetch(c0);
 #pragma unroll
-        for (int i = 0; i < VL; ++i) acc[i] = fmaf(w, x[i], acc[i]);
+        for (int k = 0; k < 4; ++k) {
+          if (c0 + k * wpr >= n) break;
+          const float w = ex2f(ls[k] - L);
+#pragma unroll
+          for (int i = 0; i < VL; ++i) acc[i] = fmaf(w, x[k][i], acc[i]);
+        }
       }
     }
     if (wpr > 1) {  // all eight warps have one row
@@ -762,20 +783,25 @@ int launch_nb(const AttnParams& p, cudaStream_t st) {
   auto kern = p8_attn_kernel<T, FMT, D, NB, MASS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM))
     return static_cast<int>(cudaGetLastError());
-  kern<<<dim3(p.splits * p.row_tiles, p.c.Hkv, p.s.num_seqs), kWarps * 32, Cfg::SMEM, st>>>(p);
-  if (p.splits == 1 && !(MASS && p.row_tiles > 1)) return 0;
-  const int wpr = p.splits > 16 ? 8 : 1;
-  const int join = p.splits > 1 ? p.row_tiles * NB * wpr : 0;
-  const int tokens = MASS ? (p.s.max_pages * kP8Page + kTokens - 1) / kTokens : 0;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(join + tokens, p.c.Hkv * p.s.num_seqs);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3(p.splits * p.row_tiles, p.c.Hkv, p.s.num_seqs);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess || (p.splits == 1 && !(MASS && p.row_tiles > 1)))
+    return static_cast<int>(e);
+  const int wpr = p.splits > 16 ? 8 : 1;
+  const int join = p.splits > 1 ? p.row_tiles * NB * wpr : 0;
+  const int tokens = MASS ? (p.s.max_pages * kP8Page + kTokens - 1) / kTokens : 0;
+  cfg.gridDim = dim3(join + tokens, p.c.Hkv * p.s.num_seqs);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, p8_finish_kernel<T, D, NB, MASS>, p, join, wpr));
 }
 
