@@ -3,6 +3,7 @@
 // checked in the kernels and reported through the per-device error word.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "paged8.h"
@@ -13,6 +14,10 @@ int cfb_num_sms(int device);
 namespace {
 
 using torch::Tensor;
+
+Tensor empty(at::IntArrayRef sizes, torch::ScalarType dtype, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
 
 void same_device(const Tensor& t, const Tensor& codes, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.get_device() == codes.get_device(), name,
@@ -144,10 +149,9 @@ std::tuple<Tensor, Tensor> paged8_read(const Tensor& codes, const Tensor& scales
   const int type = type_of(dtype, "dtype");
   const c10::cuda::CUDAGuard g(codes.device());
   const int64_t L = static_cast<int64_t>(s.max_pages) * cfb::kP8Page;
-  const auto opt = codes.options().dtype(dtype);
   const auto make = [&] {
-    return layered ? torch::empty({layers, s.num_seqs, c.Hkv, L, c.D}, opt)
-                   : torch::empty({s.num_seqs, c.Hkv, L, c.D}, opt);
+    return layered ? empty({layers, s.num_seqs, c.Hkv, L, c.D}, dtype, codes)
+                   : empty({s.num_seqs, c.Hkv, L, c.D}, dtype, codes);
   };
   Tensor k = make(), v = make();
   check_rc(cfb::p8_read(c, s, static_cast<int>(layers), k.data_ptr(), v.data_ptr(), type,
@@ -171,7 +175,7 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
   TORCH_CHECK(Hq >= 1 && Hq % c.Hkv == 0, "query heads (", Hq, ") must be a multiple of KV heads (",
               c.Hkv, ")");
   const c10::cuda::CUDAGuard g(codes.device());
-  const Tensor out = out_in.has_value() ? *out_in : torch::empty({N, Hq, c.D}, q.options());
+  const Tensor out = out_in.has_value() ? *out_in : empty({N, Hq, c.D}, q.scalar_type(), codes);
   same_device(out, codes, "out");
   TORCH_CHECK(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() &&
                   out.is_contiguous() && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
@@ -193,7 +197,6 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
   const int sms = cfb_num_sms(codes.get_device()), group = a.Hq / c.Hkv;
   int* err = cfb_err_ptr(codes.get_device());
   const auto stream = at::cuda::getCurrentCUDAStream();
-  const auto f32 = torch::dtype(torch::kFloat32).device(codes.device());
   const bool mass = a.mass_out != nullptr;
   TORCH_CHECK(group <= 128, "at most 128 query heads for each KV head");
   TORCH_CHECK(s.num_seqs * static_cast<int64_t>(c.Hkv) <= 65535 &&
@@ -202,7 +205,7 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
   if (!cfb::p8_is_chunk(a.max_q_len, group)) {
     const cfb::P8AttnPlan plan = cfb::p8_attn_plan(c, s, group, a.max_q_len, mass, sms);
     Tensor ws;
-    if (plan.floats() > 0) ws = torch::empty({plan.floats()}, f32);
+    if (plan.floats() > 0) ws = empty({plan.floats()}, torch::kFloat32, codes);
     check_rc(cfb::p8_attention(c, s, a, plan, plan.floats() > 0 ? ws.data_ptr<float>() : nullptr,
                                err, stream),
              "paged8_attention");
@@ -220,7 +223,7 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
   const int64_t n_par = seqs_each * c.Hkv * blocks * 4;
   const int64_t n_o = a.splits > 1 ? N * Hq * a.splits * c.D : 0;
   const int64_t n_lse = a.splits > 1 || mass ? N * Hq * a.splits : 0;
-  Tensor ws = torch::empty({2 * n_kv + n_par + n_o + n_lse}, f32);
+  const Tensor ws = empty({2 * n_kv + n_par + n_o + n_lse}, torch::kFloat32, codes);
   float* at = ws.data_ptr<float>();
   a.ws_k = at;
   a.ws_v = at + n_kv;
@@ -255,8 +258,9 @@ Tensor paged8_evict(const Tensor& codes, const Tensor& scales, const Tensor& mas
               "dst_table must have one row for each sequence");
   TORCH_CHECK(layers <= 65535, "too many layers");
   const c10::cuda::CUDAGuard g(codes.device());
-  Tensor keep = layered ? torch::empty({layers, s.num_seqs, c.Hkv, budget}, table.options())
-                        : torch::empty({s.num_seqs, c.Hkv, budget}, table.options());
+  const Tensor keep = layered
+                          ? empty({layers, s.num_seqs, c.Hkv, budget}, torch::kInt32, codes)
+                          : empty({s.num_seqs, c.Hkv, budget}, torch::kInt32, codes);
   check_rc(cfb::p8_evict(c, s, m, static_cast<int>(layers), dst,
                          static_cast<int>(dst_table.size(1)), static_cast<int>(budget),
                          static_cast<int>(recent), keep.data_ptr<int32_t>(),

@@ -4,6 +4,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "paged8.h"
 
@@ -97,6 +99,44 @@ __device__ __forceinline__ uint32_t p8_from_float(const float* f) {
                                                  __NV_E4M3);
     return lo | (hi << 16);
   }
+}
+
+// Kernels of these operators are launched with programmatic stream serialisation: their
+// launch overlaps the end of the kernel before, whose results they may read after the wait.
+__device__ __forceinline__ void p8_grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <typename... KArgs, typename... Args>
+int p8_launch(void (*kern)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t stream,
+              Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = stream;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
+}
+
+// Opts a kernel in to its shared memory, once for each device.
+template <auto Kern>
+int p8_opt_in(int smem) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
+  e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
 }
 
 // Physical page of a logical one; an entry outside the pool is reported and read as page 0.

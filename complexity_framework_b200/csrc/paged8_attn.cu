@@ -171,18 +171,20 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int seq) {
   return i;
 }
 
-// mass_out[j] = mass_in[j] + sum over rows of 2^(s_j - lse), in row order.  sj: the token's
-// scores, row stride Lp; r0: the first row that sees it.
-__device__ __forceinline__ void add_mass(const AttnParams& p, const int32_t* table, int h, int j,
-                                         const float* sj, int64_t Lp, int r0, int rows,
-                                         const float* lse) {
+// Where a token's mass is kept.
+__device__ __forceinline__ int64_t mass_at(const AttnParams& p, const int32_t* table, int h,
+                                           int j) {
   const int64_t pg = p8_page(table, j / kP8Page, p.c.num_pages, p.err, 75);
-  const int64_t at = (pg * p.c.Hkv + h) * kP8Page + j % kP8Page;
-  const float before = p.mass_in[at];
+  return (pg * p.c.Hkv + h) * kP8Page + j % kP8Page;
+}
+// The weight a token receives: sum over rows of 2^(s_j - lse), in row order.  sj: the token's
+// scores, row stride Lp; r0: the first row that sees it.
+__device__ __forceinline__ float weight_of(const float* sj, int64_t Lp, int r0, int rows,
+                                           const float* lse) {
   float w = 0.f;
 #pragma unroll 4
   for (int r = r0; r < rows; ++r) w += ex2f(sj[r * Lp] - lse[r]);
-  p.mass_out[at] = before + w;
+  return w;
 }
 
 // NB: 8-row column tiles of a CTA (R = 8 * NB rows of one KV head).
@@ -209,9 +211,7 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
   const int g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * (kStages * PB);
   const uint32_t qf = smem_u32(smem + Cfg::QF);
-  // started while the kernel before it ends, and lets the next one start: both ends wait
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  p8_grid_wait();
 
   const int split = blockIdx.x % p.splits, rt = blockIdx.x / p.splits;
   const int h = blockIdx.y, seq = blockIdx.z;
@@ -228,8 +228,10 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
   const int64_t item = (static_cast<int64_t>(seq) * p.c.Hkv + h) * p.row_tiles + rt;
   if (first_row >= rows) {
     if (MASS && p.splits == 1 && p.row_tiles == 1)  // cached tokens, none of them new
-      for (int j = threadIdx.x; j < si.kv; j += kWarps * 32)
-        add_mass(p, table, h, j, nullptr, 0, 0, 0, nullptr);
+      for (int j = threadIdx.x; j < si.kv; j += kWarps * 32) {
+        const int64_t at = mass_at(p, table, h, j);
+        p.mass_out[at] = p.mass_in[at];
+      }
     return;
   }
   const int last_tok = (min(rows, first_row + R) - 1) / p.G;
@@ -628,9 +630,11 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
   if constexpr (MASS) {
     if (p.splits == 1 && p.row_tiles == 1) {  // this CTA has every row and key of the head
       __syncthreads();
-      for (int j = threadIdx.x; j < si.kv; j += kWarps * 32)
-        add_mass(p, table, h, j, p.ws_s + item * R * Lp + j, Lp, max(0, j - start) * p.G, rows,
-                 s_qs);
+      for (int j = threadIdx.x; j < si.kv; j += kWarps * 32) {
+        const int64_t at = mass_at(p, table, h, j);
+        p.mass_out[at] = p.mass_in[at] + weight_of(p.ws_s + item * R * Lp + j, Lp,
+                                                   max(0, j - start) * p.G, rows, s_qs);
+      }
     }
   }
 }
@@ -670,8 +674,20 @@ __global__ void __launch_bounds__(256)
     for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(kFull, den, o);
     return den == 0.f ? -INFINITY : base + log2f(den);
   };
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int j0 = (static_cast<int>(blockIdx.x) - join_ctas) * kTokens;
+  int64_t at[kTokens / 256];
+  float before[kTokens / 256];
+  if constexpr (MASS) {  // the masses so far are inputs as well
+#pragma unroll
+    for (int i = 0; i < kTokens / 256; ++i) {
+      const int j = j0 + i * 256 + threadIdx.x;
+      if (j0 >= 0 && j < si.kv) {
+        at[i] = mass_at(p, p.s.table + static_cast<int64_t>(seq) * p.s.max_pages, h, j);
+        before[i] = p.mass_in[at[i]];
+      }
+    }
+  }
+  p8_grid_wait();
   if (static_cast<int>(blockIdx.x) < join_ctas) {
     const int rr = (blockIdx.x * 8 + warp) / wpr, part = warp % wpr;
     const int rt = rr / R, r = rr % R;
@@ -729,18 +745,20 @@ __global__ void __launch_bounds__(256)
     return;
   }
   if constexpr (MASS) {
-    const int j0 = (blockIdx.x - join_ctas) * kTokens;
     if (j0 >= si.kv) return;
     for (int r = warp; r < si.rows; r += 8) {
       const float L = total_lse(p.ws_lse + (item0 + r / R) * p.splits * R + r % R, chunks_of(r / R));
       if (lane == 0) s_lse[r] = L;
     }
     __syncthreads();
-    const int32_t* table = p.s.table + static_cast<int64_t>(seq) * p.s.max_pages;
     const int64_t Lp = static_cast<int64_t>(p.s.max_pages) * kP8Page;
-    for (int j = j0 + threadIdx.x; j < min(si.kv, j0 + kTokens); j += 256)
-      add_mass(p, table, h, j, p.ws_s + item0 * R * Lp + j, Lp, max(0, j - start) * p.G, si.rows,
-               s_lse);
+#pragma unroll
+    for (int i = 0; i < kTokens / 256; ++i) {
+      const int j = j0 + i * 256 + threadIdx.x;
+      if (j < si.kv)
+        p.mass_out[at[i]] = before[i] + weight_of(p.ws_s + item0 * R * Lp + j, Lp,
+                                                  max(0, j - start) * p.G, si.rows, s_lse);
+    }
   }
 }
 
@@ -780,29 +798,17 @@ __global__ void __launch_bounds__(128)
 template <typename T, int FMT, int D, int NB, bool MASS>
 int launch_nb(const AttnParams& p, cudaStream_t st) {
   using Cfg = AttnCfg<D, NB>;
-  auto kern = p8_attn_kernel<T, FMT, D, NB, MASS>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM))
-    return static_cast<int>(cudaGetLastError());
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cfg.stream = st;
-  cfg.gridDim = dim3(p.splits * p.row_tiles, p.c.Hkv, p.s.num_seqs);
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = Cfg::SMEM;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  if (e != cudaSuccess || (p.splits == 1 && !(MASS && p.row_tiles > 1)))
-    return static_cast<int>(e);
+  constexpr auto kern = p8_attn_kernel<T, FMT, D, NB, MASS>;
+  int rc = p8_opt_in<kern>(Cfg::SMEM);
+  if (rc) return rc;
+  rc = p8_launch(kern, dim3(p.splits * p.row_tiles, p.c.Hkv, p.s.num_seqs), kWarps * 32, Cfg::SMEM,
+                 st, p);
+  if (rc || (p.splits == 1 && !(MASS && p.row_tiles > 1))) return rc;
   const int wpr = p.splits > 16 ? 8 : 1;
   const int join = p.splits > 1 ? p.row_tiles * NB * wpr : 0;
   const int tokens = MASS ? (p.s.max_pages * kP8Page + kTokens - 1) / kTokens : 0;
-  cfg.gridDim = dim3(join + tokens, p.c.Hkv * p.s.num_seqs);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, p8_finish_kernel<T, D, NB, MASS>, p, join, wpr));
+  return p8_launch(p8_finish_kernel<T, D, NB, MASS>, dim3(join + tokens, p.c.Hkv * p.s.num_seqs),
+                   256, 0, st, p, join, wpr);
 }
 
 template <typename T, int FMT, int D>

@@ -24,7 +24,7 @@ constexpr unsigned kFull = 0xffffffffu;
 // when chunks are uneven, at floor(cu_q[i] / 16) + 2 i, which leaves room for each
 // sequence's at most floor(q / 16) + 2 blocks; the host takes the smaller enumeration.
 template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
     p8_append_kernel(P8Cache c, P8Seqs s, const T* __restrict__ k, int64_t k_stride,
                      const T* __restrict__ v, int64_t v_stride, int64_t N, int64_t units,
                      int per_seq, int* err) {
@@ -33,6 +33,7 @@ __global__ void __launch_bounds__(256)
   constexpr int NL = kP8Page / RPL;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  p8_grid_wait();
   if (unit >= units) return;
   const int hx = static_cast<int>(unit % (2 * c.Hkv));
   const int64_t item = unit / (2 * c.Hkv);
@@ -68,11 +69,6 @@ __global__ void __launch_bounds__(256)
   const int base = static_cast<int>(blk) * kP8Page;
   const int lo = max(first, base) - base, hi = min(kv - base, kP8Page);  // new tokens of the block
   const int h = hx >> 1, x = hx & 1;
-  const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages,
-                               static_cast<int>(blk), c.num_pages, err, 62);
-  const int64_t ph = (page * c.Hkv + h) * 2 + x;
-  float* scale = c.scales + ph;
-  uint8_t* codes = c.codes + ph * (kP8Page * D);
   const T* src = x ? v : k;
   const int64_t stride = x ? v_stride : k_stride;
   const int r = lane / CH, col = (lane % CH) * 8;
@@ -86,6 +82,12 @@ __global__ void __launch_bounds__(256)
       in[i] = __ldg(reinterpret_cast<const uint4*>(
           src + static_cast<int64_t>(row0 + base + t - start) * stride + h * D + col));
   }
+  // after the loads: its check waits for the table
+  const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages,
+                               static_cast<int>(blk), c.num_pages, err, 62);
+  const int64_t ph = (page * c.Hkv + h) * 2 + x;
+  float* scale = c.scales + ph;
+  uint8_t* codes = c.codes + ph * (kP8Page * D);
   const float s0 = lo > 0 ? *scale : 0.f;
   uint32_t top = 0;
 #pragma unroll
@@ -137,15 +139,16 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------------------ read
-// One warp per (layer, sequence, page, head, K or V): 16 codes a lane and load, the
-// values rounded once to the output's type.
+// One warp per (layer, sequence, page, head, K or V): 8 codes a lane and load, so that its
+// 16-byte stores are dense; the values are rounded once to the output's type.
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256)
     p8_read_kernel(P8Cache c, P8Seqs s, int64_t units, T* __restrict__ k_out,
                    T* __restrict__ v_out, int* err) {
-  constexpr int NC = kP8Page * D / 16 / 32;  // 16-code chunks of a lane
+  constexpr int NC = kP8Page * D / 8 / 32;  // 8-code pieces of a lane
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  p8_grid_wait();
   if (unit >= units) return;
   const int x = static_cast<int>(unit & 1);
   int64_t u = unit >> 1;
@@ -169,25 +172,24 @@ __global__ void __launch_bounds__(256)
     sc = __ldg(c.scales + ph);
     src = c.codes + ph * (kP8Page * D);
   }
+  uint2 w[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int e = (i * 32 + lane) * 16;
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (e / D < live) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + e));
-      float f[16];
-      p8_to_float<FMT>(w.x, f);
-      p8_to_float<FMT>(w.y, f + 4);
-      p8_to_float<FMT>(w.z, f + 8);
-      p8_to_float<FMT>(w.w, f + 12);
-      uint32_t o[8];
+    const int e = (i * 32 + lane) * 8;
+    w[i] = e / D < live ? __ldg(reinterpret_cast<const uint2*>(src + e)) : make_uint2(0, 0);
+  }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = P8Io<T>::pack(f[2 * j] * sc, f[2 * j + 1] * sc);
-      a = make_uint4(o[0], o[1], o[2], o[3]);
-      b = make_uint4(o[4], o[5], o[6], o[7]);
+  for (int i = 0; i < NC; ++i) {
+    const int e = (i * 32 + lane) * 8;
+    uint4 a = make_uint4(0, 0, 0, 0);
+    if (e / D < live) {
+      float f[8];
+      p8_to_float<FMT>(w[i].x, f);
+      p8_to_float<FMT>(w[i].y, f + 4);
+      a = make_uint4(P8Io<T>::pack(f[0] * sc, f[1] * sc), P8Io<T>::pack(f[2] * sc, f[3] * sc),
+                     P8Io<T>::pack(f[4] * sc, f[5] * sc), P8Io<T>::pack(f[6] * sc, f[7] * sc));
     }
-    reinterpret_cast<uint4*>(dst + e)[0] = a;
-    reinterpret_cast<uint4*>(dst + e)[1] = b;
+    *reinterpret_cast<uint4*>(dst + e) = a;
   }
 }
 
@@ -214,6 +216,7 @@ __global__ void __launch_bounds__(kSelThreads)
   const int h = blockIdx.x, seq = blockIdx.y;
   const int64_t layer = blockIdx.z;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  p8_grid_wait();
   const int len = p8_len(s.kv_lens, seq, s.max_pages, err, 65);
   int32_t* row = keep + ((layer * s.num_seqs + seq) * c.Hkv + h) * budget;
   if (len <= budget) {
@@ -319,6 +322,7 @@ __global__ void __launch_bounds__(256)
   constexpr int NC = 2 * kP8Page * CPR / 32;  // chunks of a lane, K and V
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  p8_grid_wait();
   if (unit >= units) return;
   int64_t u = unit;
   const int h = static_cast<int>(u % c.Hkv);
@@ -389,11 +393,12 @@ __global__ void __launch_bounds__(256)
 }
 
 template <typename T, int FMT, int D>
-void launch_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t ks, const void* v,
+int launch_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t ks, const void* v,
                    int64_t vs, int64_t N, int64_t items, int per_seq, int* err, cudaStream_t st) {
   const int64_t units = items * 2 * c.Hkv;
-  p8_append_kernel<T, FMT, D><<<static_cast<unsigned>((units + 7) / 8), 256, 0, st>>>(
-      c, s, static_cast<const T*>(k), ks, static_cast<const T*>(v), vs, N, units, per_seq, err);
+  return p8_launch(p8_append_kernel<T, FMT, D>, dim3(static_cast<unsigned>((units + 7) / 8)), 256,
+                   0, st, c, s, static_cast<const T*>(k), ks, static_cast<const T*>(v), vs, N,
+                   units, per_seq, err);
 }
 
 }  // namespace
@@ -423,11 +428,12 @@ int p8_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t k_stride
   const int64_t items = even <= uneven ? even : uneven;
   if ((items * 2 * c.Hkv + 7) / 8 > 0x7fffffff) return -3;
   const int ps = even <= uneven ? static_cast<int>(per_seq) : 0;
+  int rc = 0;
 #define CFB_CALL(T, F, DD) \
-  launch_append<T, F, DD>(c, s, k, k_stride, v, v_stride, N, items, ps, err, stream)
+  rc = launch_append<T, F, DD>(c, s, k, k_stride, v, v_stride, N, items, ps, err, stream)
   CFB_P8_TYPES(CFB_CALL);
 #undef CFB_CALL
-  return static_cast<int>(cudaGetLastError());
+  return rc ? rc : static_cast<int>(cudaGetLastError());
 }
 
 int p8_read(const P8Cache& c, const P8Seqs& s, int layers, void* k_out, void* v_out, int type,
@@ -437,12 +443,13 @@ int p8_read(const P8Cache& c, const P8Seqs& s, int layers, void* k_out, void* v_
   if (units <= 0) return 0;
   if ((units + 7) / 8 > 0x7fffffff) return -3;
   const unsigned grid = static_cast<unsigned>((units + 7) / 8);
-#define CFB_CALL(T, F, DD)                                                              \
-  p8_read_kernel<T, F, DD><<<grid, 256, 0, stream>>>(c, s, units, static_cast<T*>(k_out), \
-                                                     static_cast<T*>(v_out), err)
+  int rc = 0;
+#define CFB_CALL(T, F, DD)                                                                      \
+  rc = p8_launch(p8_read_kernel<T, F, DD>, dim3(grid), 256, 0, stream, c, s, units,              \
+                 static_cast<T*>(k_out), static_cast<T*>(v_out), err)
   CFB_P8_TYPES(CFB_CALL);
 #undef CFB_CALL
-  return static_cast<int>(cudaGetLastError());
+  return rc ? rc : static_cast<int>(cudaGetLastError());
 }
 
 int p8_evict(const P8Cache& c, const P8Seqs& s, float* mass, int layers, const int32_t* dst_table,
@@ -456,18 +463,19 @@ int p8_evict(const P8Cache& c, const P8Seqs& s, float* mass, int layers, const i
   const int longest = s.max_pages * kP8Page;
   const int cap = longest < kSelKeys ? longest : kSelKeys;
   const int smem = cap * 4;
-  if (cudaFuncSetAttribute(p8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
-    return static_cast<int>(cudaGetLastError());
-  p8_select_kernel<<<dim3(c.Hkv, s.num_seqs, layers), kSelThreads, smem, stream>>>(
-      c, s, mass, budget, recent, keep, cap, err);
+  int rc = p8_opt_in<p8_select_kernel>(kSelKeys * 4);
+  if (!rc)
+    rc = p8_launch(p8_select_kernel, dim3(c.Hkv, s.num_seqs, layers), kSelThreads, smem, stream, c,
+                   s, mass, budget, recent, keep, cap, err);
+  if (rc) return rc;
   const unsigned grid = static_cast<unsigned>((units + 7) / 8);
   const int type = kP8Bf16;
-#define CFB_CALL(T, F, DD)                                                                    \
-  p8_move_kernel<F, DD><<<grid, 256, 0, stream>>>(c, s, mass, layers, dst_table, dst_pages,    \
-                                                  budget, keep, units, err)
+#define CFB_CALL(T, F, DD)                                                                      \
+  rc = p8_launch(p8_move_kernel<F, DD>, dim3(grid), 256, 0, stream, c, s, mass, layers, dst_table, \
+                 dst_pages, budget, keep, units, err)
   CFB_P8_TYPES(CFB_CALL);
 #undef CFB_CALL
-  return static_cast<int>(cudaGetLastError());
+  return rc ? rc : static_cast<int>(cudaGetLastError());
 }
 
 }  // namespace cfb

@@ -69,9 +69,10 @@ __global__ void __launch_bounds__(256)
     p8_expand_kernel(P8Cache c, P8Seqs s, int blocks, int64_t units, float scale_log2,
                      T* __restrict__ k_ws, __half* __restrict__ v_ws, float4* __restrict__ par,
                      int* err) {
-  constexpr int NC = kP8Page * D / 16 / 32;
+  constexpr int NC = kP8Page * D / 8 / 32;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  p8_grid_wait();
   if (unit >= units) return;
   const int x = static_cast<int>(unit & 1);
   int64_t u = unit >> 1;
@@ -104,28 +105,27 @@ __global__ void __launch_bounds__(256)
     src = c.codes + (ph * 2 + x) * (kP8Page * D);
   }
   if (x == 0 && lane == 0) par[sh * blocks + blk] = f;
+  uint2 w[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int e = (i * 32 + lane) * 16;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    uint32_t o[8] = {};
-    if (e / D < live) {
-      w = __ldg(reinterpret_cast<const uint4*>(src + e));
-      const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    const int e = (i * 32 + lane) * 8;
+    w[i] = e / D < live ? __ldg(reinterpret_cast<const uint2*>(src + e)) : make_uint2(0, 0);
+  }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p8_to_half<FMT>(in[j], o[2 * j], o[2 * j + 1]);
-        if (P8Io<T>::kBf16 && x == 0) {
+  for (int i = 0; i < NC; ++i) {
+    uint32_t o[4] = {};
+    if ((i * 32 + lane) * 8 / D < live) {
+      p8_to_half<FMT>(w[i].x, o[0], o[1]);
+      p8_to_half<FMT>(w[i].y, o[2], o[3]);
+      if (P8Io<T>::kBf16 && x == 0) {
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const float2 v = __half22float2(*reinterpret_cast<__half2*>(&o[2 * j + z]));
-            o[2 * j + z] = pack_bf16x2(v.x, v.y);
-          }
+        for (int z = 0; z < 4; ++z) {
+          const float2 v = __half22float2(*reinterpret_cast<__half2*>(&o[z]));
+          o[z] = pack_bf16x2(v.x, v.y);
         }
       }
     }
-    dst[2 * (i * 32 + lane)] = make_uint4(o[0], o[1], o[2], o[3]);
-    dst[2 * (i * 32 + lane) + 1] = make_uint4(o[4], o[5], o[6], o[7]);
+    dst[i * 32 + lane] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -716,10 +716,10 @@ int launch_expand(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int blocks
                   cudaStream_t st) {
   const int64_t units = static_cast<int64_t>(s.num_seqs) * blocks * c.Hkv * 2;
   if ((units + 7) / 8 > 0x7fffffff) return -3;
-  p8_expand_kernel<T, FMT, D><<<static_cast<unsigned>((units + 7) / 8), 256, 0, st>>>(
-      c, s, blocks, units, a.scale * 1.4426950408889634f, static_cast<T*>(a.ws_k),
-      static_cast<__half*>(a.ws_v), static_cast<float4*>(a.ws_par), err);
-  return 0;
+  return p8_launch(p8_expand_kernel<T, FMT, D>, dim3(static_cast<unsigned>((units + 7) / 8)), 256,
+                   0, st, c, s, blocks, units, a.scale * 1.4426950408889634f,
+                   static_cast<T*>(a.ws_k), static_cast<__half*>(a.ws_v),
+                   static_cast<float4*>(a.ws_par), err);
 }
 
 template <typename T, int D, int NQ, int POLY>
