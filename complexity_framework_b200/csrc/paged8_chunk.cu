@@ -20,6 +20,8 @@
 // they are recomputed: one CTA per (128 keys, KV head, sequence) walks the row tiles with
 // S^T = K Q^T (a thread owns a key), adding 2^(s - lse) in row order: no atomics, the same
 // bits every time.
+#include <type_traits>
+
 #include "paged8.cuh"
 
 #include "flash.h"
@@ -53,6 +55,26 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                           int* err, int code, int site) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code, site));
+}
+
+// 16 columns of TMEM into registers, and the wait that makes them readable: the registers
+// pass through the wait, so no use of them can move before it.
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 
 // ---------------------------------------------------------------------------- expand
@@ -139,7 +161,7 @@ struct ChunkParams {
   float* lse;                  // [N * Hq, splits], log2 units (splits > 1, or for the weights)
   float* ws_o;                 // [N * Hq, splits, D] (splits > 1)
   int64_t N;
-  int Hq, Hkv, G, splits, row_ctas;
+  int Hq, Hkv, G, splits, row_ctas, num_seqs;
   int* err;
 };
 
@@ -149,7 +171,7 @@ struct ChunkCfg {
   static constexpr int CHUNKS = D / 64;
   static constexpr int Q_BYTES = kT * D * 2;
   static constexpr int K_BYTES = kT * D * 2;
-  static constexpr int SMEM = NQ * Q_BYTES + STAGES * 2 * K_BYTES + 1024 + 512;
+  static constexpr int SMEM = NQ * Q_BYTES + STAGES * 2 * K_BYTES + 1024 + 256 + 4 * NQ * 128;
   static constexpr uint32_t T_O = NQ * 128;
   static constexpr uint32_t TMEM = NQ == 2 ? 512 : 256;
   static constexpr int PRODUCER = 4 * NQ, MMA = 4 * NQ + 1;
@@ -158,7 +180,7 @@ struct ChunkCfg {
   static_assert(SMEM <= 232448, "shared memory");
 };
 
-struct ChunkBars {
+struct alignas(16) ChunkBars {
   uint64_t q_full;
   uint64_t kv_full[4];
   uint64_t kv_empty[4];
@@ -169,6 +191,7 @@ struct ChunkBars {
   uint32_t tmem;
   int abort;
 };
+static_assert(sizeof(ChunkBars) % 16 == 0 && sizeof(ChunkBars) <= 256, "block scales follow");
 
 template <typename T, int D, int NQ, int POLY>
 __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
@@ -187,10 +210,11 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
   volatile int* abort_flag = &bars->abort;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-  // the last row tiles see the most keys: they go first
-  const int split = blockIdx.x % p.splits;
-  const int rc = p.row_ctas - 1 - static_cast<int>(blockIdx.x / p.splits);
-  const int h = blockIdx.y, seq = blockIdx.z;
+  // the last row tiles see the most keys: those of all sequences go first
+  const unsigned each = p.splits * p.Hkv * p.num_seqs;
+  const int rc = p.row_ctas - 1 - static_cast<int>(blockIdx.x / each);
+  const int rest = blockIdx.x % each;
+  const int split = rest % p.splits, h = rest / p.splits % p.Hkv, seq = rest / p.splits / p.Hkv;
   const int row0 = __ldg(p.cu_q + seq), q_len = __ldg(p.cu_q + seq + 1) - row0;
   if (row0 < 0 || q_len < 0 || static_cast<int64_t>(row0) + q_len > p.N) {
     if (threadIdx.x == 0) report_error(p.err, kErrBounds, 82);
@@ -350,96 +374,95 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
     const uint32_t t_s = tmem + x * 128 + lane_off;
     const uint32_t t_o = tmem + Cfg::T_O + x * D + lane_off;
     const int n = nkv_of(x);
-    const float4* par = p.par + sh * p.blocks;
-    float m_used = -INFINITY, l = 0.f;
+    const float4* par = p.par + sh * p.blocks + j0 * (kT / kP8Page);
+    float4* s_par = reinterpret_cast<float4*>(bars + 1) + warp * (kT / kP8Page);
+    // rows that are no token's never see a key and never ask for a rescale
+    float m_used = mine ? -INFINITY : 0.f, l = 0.f;
     bool ok = true;
+    float4 next = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (n > 0 && lane < kT / kP8Page) next = __ldg(par + lane);
     for (int j = 0; j < n && ok; ++j) {
-      const float4* pj = par + (j0 + j) * (kT / kP8Page);
+      // the tile's block scales, through this warp's own corner of shared memory
+      const bool bad = __any_sync(0xffffffffu, next.x != next.x);
+      if (lane < kT / kP8Page) {
+        s_par[lane] = next;
+        if (j + 1 < n) next = __ldg(par + (j + 1) * (kT / kP8Page) + lane);
+      }
+      __syncwarp();
       if (!wait_warp(&bars->s_full[x], j & 1, abort_flag, p.err, kErrTimeoutTmem, 89)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      float s[kT];
+      const int kmax = lim - (j0 + j) * kT;  // keys of the tile that this row sees
+      const bool edge = __any_sync(0xffffffffu, kmax < kT);
+      // One pass over S computes P against the bound in use and the row's maximum; only
+      // where the maximum turns out too far above the bound is the bound moved and the pass
+      // repeated (always in a row's first tile, seldom later).
+      uint32_t pk[kT / 2];
+      float sum;
+      bool nan_row = false;
+      auto pass = [&](auto masked, float msub) {
+        float2 mx2 = make_float2(-INFINITY, -INFINITY), l2 = make_float2(0.f, 0.f);
+        uint32_t buf[2][16];
+        tmem_ld16_async(t_s, buf[0]);
 #pragma unroll
-      for (int c = 0; c < kT; c += 32) tmem_ld32(t_s + c, s + c);
-      tmem_wait_ld();
-      const int kmax = lim - (j0 + j) * kT;
-      if (kmax < kT) {
+        for (int b = 0; b < kT / 16; ++b) {
+          uint32_t(&cur)[16] = buf[b & 1];
+          tmem_wait16(cur);
+          if (b + 1 < kT / 16) tmem_ld16_async(t_s + (b + 1) * 16, buf[(b + 1) & 1]);
+          const float4 f = s_par[b];
+          float kf = f.x, nm = f.y - msub;
+          if (bad && kf != kf) {  // NaN for the rows that see the block, nothing for the others
+            nan_row |= b * 16 < kmax;
+            kf = 1.f;
+            nm = -INFINITY;
+          }
+          float2 rs = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < kT; ++c)
-          if (c >= kmax) s[c] = -INFINITY;
-      }
-      // block maxima of w (scales are not negative), then the row's
-      float mx = -INFINITY, all = 0.f;
-#pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        const float4 f = __ldg(pj + b);
-        float a0 = s[16 * b], a1 = s[16 * b + 1];
-#pragma unroll
-        for (int c = 2; c < 16; c += 2) {
-          a0 = fmaxf(a0, s[16 * b + c]);
-          a1 = fmaxf(a1, s[16 * b + c + 1]);
+          for (int i = 0; i < 16; i += 2) {
+            float2 sv = make_float2(__uint_as_float(cur[i]), __uint_as_float(cur[i + 1]));
+            if constexpr (decltype(masked)::value) {
+              if (b * 16 + i >= kmax) sv.x = -INFINITY;
+              if (b * 16 + i + 1 >= kmax) sv.y = -INFINITY;
+            }
+            const float2 xv = fma2(sv, make_float2(kf, kf), make_float2(nm, nm));
+            mx2.x = fmaxf(mx2.x, xv.x);
+            mx2.y = fmaxf(mx2.y, xv.y);
+            const float2 pv = (i >> 1) < POLY ? exp2_poly2(xv) : make_float2(ex2c(xv.x), ex2c(xv.y));
+            rs = add2(rs, pv);
+            pk[b * 8 + i / 2] = P8Io<__half>::pack(pv.x, pv.y);
+          }
+          l2 = fma2(rs, make_float2(f.z, f.z), l2);
         }
-        mx = fmaxf(mx, fmaf(fmaxf(a0, a1), f.x, f.y));
-        all += f.x;
-      }
-      if (!(all <= 3.402823466e38f)) {  // a block that is not finite: NaN for the rows that see it
+        sum = l2.x + l2.y;
+        return fmaxf(mx2.x, mx2.y);
+      };
+      for (int tries = 0; tries < 4; ++tries) {  // two are enough for finite scores
+        const float msub = m_used == -INFINITY ? 0.f : m_used;
+        // the maximum, relative to the bound
+        const float mx = edge ? pass(std::true_type{}, msub) : pass(std::false_type{}, msub);
+        const bool grow = m_used == -INFINITY ? mx > -INFINITY : mx > kRescaleLog2;
+        if (!__any_sync(0xffffffffu, grow)) break;
+        const bool had = m_used != -INFINITY;
+        const float alpha = grow && had ? ex2c(-mx) : 1.f;
+        if (grow) m_used = msub + mx;
+        l *= alpha;
+        if (__any_sync(0xffffffffu, grow && had)) {  // O_x holds the earlier tiles' P V
 #pragma unroll
-        for (int c = 0; c < kT; ++c) {
-          const float f = __ldg(&pj[c / 16].x);
-          if (f != f && s[c] != -INFINITY) {
-            l = f;
-            s[c] = -INFINITY;
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld16_async(t_o + c, o);
+            tmem_wait16(o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(t_o + c, o);
           }
         }
       }
-      const float m_new = fmaxf(m_used, mx);
-      const bool grow = m_new > m_used + kRescaleLog2;
-      if (__any_sync(0xffffffffu, grow && m_used != -INFINITY)) {
-        const float alpha = (grow && m_used != -INFINITY) ? ex2c(m_used - m_new) : 1.f;
+      l += nan_row ? __uint_as_float(0x7fc00000u) : sum;
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          uint32_t u[32];
-          tmem_ld32(t_o + c, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * alpha);
-          tmem_st16(t_o + c, u);
-          tmem_st16(t_o + c + 16, u + 16);
-        }
-        tmem_wait_st();
-      }
-      if (grow) {
-        if (m_used != -INFINITY) l *= ex2c(m_used - m_new);
-        m_used = m_new;
-      }
-      const float msub = m_used == -INFINITY ? 0.f : m_used;
-      float2 l2 = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int c = 0; c < kT; c += 32) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int hb = 0; hb < 32; hb += 16) {
-          const float4 f = __ldg(pj + (c + hb) / 16);
-          const float kf = f.x == f.x ? f.x : 1.f;  // all masked then
-          const float nm = f.y - msub;
-          float2 rs[2] = {};
-#pragma unroll
-          for (int i = hb; i < hb + 16; i += 2) {
-            const float2 xv = fma2(make_float2(s[c + i], s[c + i + 1]), make_float2(kf, kf),
-                                   make_float2(nm, nm));
-            const float2 pv = ((i >> 1) % 8) < POLY ? exp2_poly2(xv)
-                                                    : make_float2(ex2c(xv.x), ex2c(xv.y));
-            rs[(i >> 1) & 1] = add2(rs[(i >> 1) & 1], pv);
-            pk[i / 2] = P8Io<__half>::pack(pv.x, pv.y);
-          }
-          l2 = fma2(add2(rs[0], rs[1]), make_float2(f.z, f.z), l2);
-        }
-        tmem_st16(t_s + c / 2, pk);
-      }
-      l += l2.x + l2.y;
+      for (int c = 0; c < kT / 2; c += 16) tmem_st16(t_s + c, pk + c);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -726,15 +749,15 @@ template <typename T, int D, int NQ, int POLY>
 int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                ChunkParams p, int max_q_len, int num_seqs, cudaStream_t st) {
   using Cfg = ChunkCfg<D, NQ>;
-  auto kern = p8_chunk_kernel<T, D, NQ, POLY>;
+  constexpr auto kern = p8_chunk_kernel<T, D, NQ, POLY>;
   const int per_cta = NQ * (kT / p.G);
   p.row_ctas = (max_q_len + per_cta - 1) / per_cta;
-  const int64_t gx = static_cast<int64_t>(p.row_ctas) * p.splits;
+  p.num_seqs = num_seqs;
+  const int64_t gx = static_cast<int64_t>(p.row_ctas) * p.splits * p.Hkv * num_seqs;
   if (gx > 0x7fffffff) return -3;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM))
-    return static_cast<int>(cudaGetLastError());
-  kern<<<dim3(static_cast<unsigned>(gx), p.Hkv, num_seqs), Cfg::THREADS, Cfg::SMEM, st>>>(tq, tk,
-                                                                                          tv, p);
+  const int rc = p8_opt_in<kern>(Cfg::SMEM);
+  if (rc) return rc;
+  kern<<<static_cast<unsigned>(gx), Cfg::THREADS, Cfg::SMEM, st>>>(tq, tk, tv, p);
   return 0;
 }
 
