@@ -218,6 +218,7 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
       std::max<int64_t>(1, std::min<int64_t>(s.num_seqs, workspace_bytes / (4 * each)));
   cfb::p8_chunk_plan(s, c.Hkv, group, a.max_q_len, sms, &a.chunk_nq, &a.splits);
   if (seqs_each < s.num_seqs) a.splits = 1;
+  a.num_sms = sms;
   // one workspace: expanded K | V | their block scales | split outputs | log-sum-exps
   const int64_t n_kv = seqs_each * each / 2;  // floats
   const int64_t n_par = seqs_each * c.Hkv * blocks * 4;

@@ -55,6 +55,7 @@ struct P8Attn {
   float* ws_o = nullptr;     // [N * Hq, splits, D] (splits > 1)
   float* ws_lse = nullptr;   // [N * Hq, splits] (splits > 1 or mass)
   int chunk_nq = 2;          // 128-row tiles of a CTA
+  int num_sms = 148;
   // keys and values as 16-bit operands, Lw = 16 * p8_chunk_blocks() tokens
   void* ws_k = nullptr;      // [S, Hkv, Lw, D]
   void* ws_v = nullptr;

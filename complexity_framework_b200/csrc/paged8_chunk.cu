@@ -14,12 +14,17 @@
 // packs floor(128 / G) tokens x G heads, so all the heads of a group share each K/V tile.
 //   warps 0 .. 4 NQ - 1  softmax, one row per thread: S from TMEM, running maximum with a
 //                        lazy rescale (only when it grows by more than 2^8), P back to TMEM
-//   next warp            TMA producer: Q once, then K / V tiles through a ring
-//   last warp            MMA issuer: O_x += P_x V, then S_x = Q_x K^T of the next tile
+//   next warp            TMA producer: Q once, then K and V tiles through rings of their own
+//   last warp            MMA issuer: S_x = Q_x K^T of the next tile, then O_x += P_x V
+// Key tiles are 64 wide so that TMEM (512 columns) holds two S of each row tile beside O:
+// the next S is there when a softmax warp ends a tile.  With 128-wide tiles and one S the
+// chain S -> P -> O -> S left the softmax warps idle for 40% of a tile (4100 cycles for 128
+// keys of two row tiles, of which their exponentials need 2100).
 // p8_chunk_mass_kernel: weights summed over the rows need each row's final log-sum-exp, so
 // they are recomputed: one CTA per (128 keys, KV head, sequence) walks the row tiles with
-// S^T = K Q^T (a thread owns a key), adding 2^(s - lse) in row order: no atomics, the same
-// bits every time.
+// S^T = K Q^T (a thread owns a key), adding 2^(s - lse) in a fixed order: no atomics, the same
+// bits every time.  Where that leaves SMs idle a cluster shares the row tiles of a key tile
+// and its first CTA adds the others' sums up over distributed shared memory.
 #include <type_traits>
 
 #include "paged8.cuh"
@@ -29,7 +34,8 @@
 namespace cfb {
 namespace {
 
-constexpr int kT = 128;               // rows of a tile, keys of a tile
+constexpr int kT = 128;               // rows of a tile
+constexpr int kKeys = 64;             // keys of a tile of the forward kernel
 constexpr float kRescaleLog2 = 8.f;
 constexpr float kTinyScale = 7.888609e-31f;  // 2^-100: blocks below it count as zeros
 
@@ -57,6 +63,12 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code, site));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // 16 columns of TMEM into registers, and the wait that makes them readable: the registers
 // pass through the wait, so no use of them can move before it.
 __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
@@ -75,6 +87,27 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
                  "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// After a wait: no use of these registers can move before this point.
+__device__ __forceinline__ void tmem_ready32(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
 
 // ---------------------------------------------------------------------------- expand
@@ -167,34 +200,38 @@ struct ChunkParams {
 
 template <int D, int NQ>
 struct ChunkCfg {
-  static constexpr int STAGES = D == 64 ? (NQ == 2 ? 4 : 2) : 2;
+  static constexpr int STAGES = NQ == 1 && D == 128 ? 2 : 4;  // of K, and of V
+  static constexpr int CTAS = NQ == 1 ? 2 : 1;        // on an SM
   static constexpr int CHUNKS = D / 64;
   static constexpr int Q_BYTES = kT * D * 2;
-  static constexpr int K_BYTES = kT * D * 2;
-  static constexpr int SMEM = NQ * Q_BYTES + STAGES * 2 * K_BYTES + 1024 + 256 + 4 * NQ * 128;
-  static constexpr uint32_t T_O = NQ * 128;
-  static constexpr uint32_t TMEM = NQ == 2 ? 512 : 256;
-  static constexpr int PRODUCER = 4 * NQ, MMA = 4 * NQ + 1;
-  static constexpr int THREADS = (4 * NQ + 2) * 32;
+  static constexpr int K_BYTES = kKeys * D * 2;
+  static constexpr int BLOCKS = kKeys / kP8Page;      // scale blocks of a key tile
+  static constexpr int SOFT = 4 * NQ;                 // softmax warps
+  static constexpr int SMEM =
+      NQ * Q_BYTES + STAGES * 2 * K_BYTES + 1024 + 512 + SOFT * 2 * BLOCKS * 16;
+  static constexpr uint32_t T_O = NQ * 2 * kKeys;     // two S of each row tile, then O
+  static constexpr uint32_t TMEM = T_O + NQ * D <= 256 ? 256 : 512;
+  static constexpr int PRODUCER = SOFT, MMA = SOFT + 1;
+  static constexpr int THREADS = (SOFT + 2) * 32;
   static_assert(T_O + NQ * D <= TMEM, "TMEM budget");
-  static_assert(SMEM <= 232448, "shared memory");
+  static_assert(CTAS * (SMEM + 1024) <= 233472, "shared memory");
 };
 
 struct alignas(16) ChunkBars {
   uint64_t q_full;
-  uint64_t kv_full[4];
-  uint64_t kv_empty[4];
-  uint64_t s_full[2];
-  uint64_t p_full[2];
-  uint64_t o_full[2];
+  uint64_t k_full[4], k_empty[4];
+  uint64_t v_full[4], v_empty[4];
+  uint64_t s_full[2][2];   // [row tile][S buffer]
+  uint64_t p_full[2][2];
+  uint64_t o_full[2][2];   // O += P V; two, as the next may be done before this one is awaited
   uint64_t mma_done;
   uint32_t tmem;
   int abort;
 };
-static_assert(sizeof(ChunkBars) % 16 == 0 && sizeof(ChunkBars) <= 256, "block scales follow");
+static_assert(sizeof(ChunkBars) % 16 == 0 && sizeof(ChunkBars) <= 512, "block scales follow");
 
 template <typename T, int D, int NQ, int POLY>
-__global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
+__global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CTAS))
     p8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                     const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const ChunkParams p) {
@@ -210,11 +247,23 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
   volatile int* abort_flag = &bars->abort;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-  // the last row tiles see the most keys: those of all sequences go first
-  const unsigned each = p.splits * p.Hkv * p.num_seqs;
-  const int rc = p.row_ctas - 1 - static_cast<int>(blockIdx.x / each);
-  const int rest = blockIdx.x % each;
-  const int split = rest % p.splits, h = rest / p.splits % p.Hkv, seq = rest / p.splits / p.Hkv;
+  // The most work first, so that no long CTA starts late: the longest sequence (of the first
+  // 32; more of them even out by themselves), and in it the last row tiles, which see the
+  // most keys.
+  const unsigned each = p.splits * p.Hkv * p.row_ctas;
+  int seq = static_cast<int>(blockIdx.x / each);
+  const int rest = static_cast<int>(blockIdx.x % each);
+  const int rc = p.row_ctas - 1 - rest / (p.splits * p.Hkv);
+  const int split = rest % p.splits, h = rest / p.splits % p.Hkv;
+  if (p.num_seqs <= 32) {
+    const int len = lane < p.num_seqs ? __ldg(p.kv_lens + lane) : -1;
+    int rank = 0;
+    for (int i = 0; i < p.num_seqs; ++i) {
+      const int other = __shfl_sync(0xffffffffu, len, i);
+      rank += other > len || (other == len && i < lane);
+    }
+    seq = __ffs(__ballot_sync(0xffffffffu, lane < p.num_seqs && rank == seq)) - 1;
+  }
   const int row0 = __ldg(p.cu_q + seq), q_len = __ldg(p.cu_q + seq + 1) - row0;
   if (row0 < 0 || q_len < 0 || static_cast<int64_t>(row0) + q_len > p.N) {
     if (threadIdx.x == 0) report_error(p.err, kErrBounds, 82);
@@ -232,7 +281,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
     const int t0 = tok0 + x * TT;
     if (t0 >= q_len) return 0;
     const int last = min(q_len, t0 + TT) - 1;
-    return (max(0, start + last + 1) + kT - 1) / kT;
+    return (max(0, start + last + 1) + kKeys - 1) / kKeys;
   };
   int tiles = 0;
 #pragma unroll
@@ -248,13 +297,17 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&bars->kv_full[s], 1);
-      mbar_init(&bars->kv_empty[s], 1);
+      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->k_empty[s], 1);
+      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->v_empty[s], 1);
     }
     for (int x = 0; x < NQ; ++x) {
-      mbar_init(&bars->s_full[x], 1);
-      mbar_init(&bars->p_full[x], 4);
-      mbar_init(&bars->o_full[x], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->s_full[x][b], 1);
+        mbar_init(&bars->p_full[x][b], 4);
+        mbar_init(&bars->o_full[x][b], 1);
+      }
     }
     mbar_init(&bars->mma_done, 1);
     bars->abort = 0;
@@ -289,77 +342,90 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
           for (int c = 0; c < Cfg::CHUNKS; ++c)
             tma_load_4d(sQ + x * Cfg::Q_BYTES + c * kT * 128, &tmQ, &bars->q_full, c * 64, 0, h,
                         row0 + tok0 + x * TT);
-      int issued = 0;
-      for (int j = 0; j < nkv; ++j) {
+      // K runs one tile ahead: a K stage is free once the tile's scores are computed
+      int issued_k = 0, issued_v = 0;
+      auto load = [&](int j, const CUtensorMap* map, uint8_t* tiles, uint64_t* full,
+                      uint64_t* empty, int& issued) -> bool {
+        if (j >= nkv) return true;
         const int st = j % STAGES;
-        if (!mbar_wait(&bars->kv_empty[st], ((j / STAGES) & 1) ^ 1, abort_flag, p.err,
-                       kErrTimeoutEmpty, 85))
-          break;
-        mbar_arrive_expect_tx(&bars->kv_full[st], 2 * Cfg::K_BYTES);
+        if (!mbar_wait(&empty[st], ((j / STAGES) & 1) ^ 1, abort_flag, p.err, kErrTimeoutEmpty, 85))
+          return false;
+        mbar_arrive_expect_tx(&full[st], Cfg::K_BYTES);
 #pragma unroll
-        for (int c = 0; c < Cfg::CHUNKS; ++c) {
-          tma_load_4d(sK + st * Cfg::K_BYTES + c * kT * 128, &tmK, &bars->kv_full[st], c * 64,
-                      (j0 + j) * kT, h, seq);
-          tma_load_4d(sV + st * Cfg::K_BYTES + c * kT * 128, &tmV, &bars->kv_full[st], c * 64,
-                      (j0 + j) * kT, h, seq);
-        }
+        for (int c = 0; c < Cfg::CHUNKS; ++c)
+          tma_load_4d(tiles + st * Cfg::K_BYTES + c * kKeys * 128, map, &full[st], c * 64,
+                      (j0 + j) * kKeys, h, seq);
         ++issued;
-      }
+        return true;
+      };
+      bool ok = load(0, &tmK, sK, bars->k_full, bars->k_empty, issued_k);
+      for (int j = 0; j < nkv && ok; ++j)
+        ok = load(j + 1, &tmK, sK, bars->k_full, bars->k_empty, issued_k) &&
+             load(j, &tmV, sV, bars->v_full, bars->v_empty, issued_v);
       drain(&bars->q_full, 0);
-      for (int j = issued - STAGES < 0 ? 0 : issued - STAGES; j < issued; ++j)
-        drain(&bars->kv_full[j % STAGES], (j / STAGES) & 1);
+      for (int j = issued_k - STAGES < 0 ? 0 : issued_k - STAGES; j < issued_k; ++j)
+        drain(&bars->k_full[j % STAGES], (j / STAGES) & 1);
+      for (int j = issued_v - STAGES < 0 ? 0 : issued_v - STAGES; j < issued_v; ++j)
+        drain(&bars->v_full[j % STAGES], (j / STAGES) & 1);
     }
   } else if (warp == Cfg::MMA) {
     if (nkv > 0 && elect_one()) {
-      constexpr uint32_t IDESC_S = idesc16<T>(kT, kT, false);
+      constexpr uint32_t IDESC_S = idesc16<T>(kT, kKeys, false);
       constexpr uint32_t IDESC_PV = idesc16<__half>(kT, D, true);
       int nkv_x[NQ];
 #pragma unroll
       for (int x = 0; x < NQ; ++x) nkv_x[x] = nkv_of(x);
-      bool ok = mbar_wait(&bars->q_full, 0, abort_flag, p.err, kErrTimeoutFull, 86);
-      auto issue_pv = [&](int x, int jp) -> bool {
-        if (!mbar_wait(&bars->p_full[x], jp & 1, abort_flag, p.err, kErrTimeoutFull, 87))
-          return false;
-        tc_fence_after();
-        const uint32_t v_base = smem_u32(sV + (jp % STAGES) * Cfg::K_BYTES);
-#pragma unroll
-        for (int kk = 0; kk < kT / 16; ++kk)
-          umma_bf16_ts(tmem + Cfg::T_O + x * D, tmem + x * 128 + kk * 8,
-                       sw128_desc(v_base + kk * 2048, kT * 128, 1024), IDESC_PV,
-                       (jp > 0 || kk > 0) ? 1u : 0u);
-        return true;
-      };
-      for (int j = 0; j <= nkv && ok; ++j) {
+      // S_x(j) = Q_x K_j^T into buffer j & 1: its P_x(j - 2) was consumed by an MMA issued before
+      auto issue_s = [&](int j) -> bool {
+        if (j >= nkv) return true;
         const int st = j % STAGES;
-        if (j < nkv && !mbar_wait(&bars->kv_full[st], (j / STAGES) & 1, abort_flag, p.err,
-                                  kErrTimeoutFull, 88)) {
-          ok = false;
-          break;
-        }
+        if (!mbar_wait(&bars->k_full[st], (j / STAGES) & 1, abort_flag, p.err, kErrTimeoutFull, 88))
+          return false;
         tc_fence_after();
         const uint32_t k_base = smem_u32(sK + st * Cfg::K_BYTES);
 #pragma unroll
         for (int x = 0; x < NQ; ++x) {
-          if (j > 0 && j - 1 < nkv_x[x]) {
-            if (!issue_pv(x, j - 1)) {
-              ok = false;
-              break;
-            }
-            if (j - 1 == nkv_x[x] - 1) umma_commit(&bars->o_full[x]);
-          }
-          if (j < nkv_x[x]) {
-            const uint32_t q_base = smem_u32(sQ + x * Cfg::Q_BYTES);
+          if (j >= nkv_x[x]) continue;
+          const uint32_t q_base = smem_u32(sQ + x * Cfg::Q_BYTES);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
-              umma_bf16(tmem + x * 128, sw128_desc(q_base + off, 16, 1024),
-                        sw128_desc(k_base + off, 16, 1024), IDESC_S, kk != 0 ? 1u : 0u);
-            }
-            umma_commit(&bars->s_full[x]);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16(tmem + (2 * x + (j & 1)) * kKeys,
+                      sw128_desc(q_base + (kk >> 2) * (kT * 128) + (kk & 3) * 32, 16, 1024),
+                      sw128_desc(k_base + (kk >> 2) * (kKeys * 128) + (kk & 3) * 32, 16, 1024),
+                      IDESC_S, kk != 0 ? 1u : 0u);
+          umma_commit(&bars->s_full[x][j & 1]);
         }
+        umma_commit(&bars->k_empty[st]);
+        return true;
+      };
+      bool ok = mbar_wait(&bars->q_full, 0, abort_flag, p.err, kErrTimeoutFull, 86);
+      if (ok) {
+        tc_fence_after();
+        ok = issue_s(0);
+      }
+      for (int j = 0; j < nkv && ok; ++j) {
+        const int st = j % STAGES;
+        ok = issue_s(j + 1) && mbar_wait(&bars->v_full[st], (j / STAGES) & 1, abort_flag, p.err,
+                                         kErrTimeoutFull, 79);
         if (!ok) break;
-        if (j > 0) umma_commit(&bars->kv_empty[(j - 1) % STAGES]);
+        const uint32_t v_base = smem_u32(sV + st * Cfg::K_BYTES);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          if (j >= nkv_x[x]) continue;
+          if (!mbar_wait(&bars->p_full[x][j & 1], (j >> 1) & 1, abort_flag, p.err, kErrTimeoutFull,
+                         87)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            umma_bf16_ts(tmem + Cfg::T_O + x * D, tmem + (2 * x + (j & 1)) * kKeys + kk * 8,
+                         sw128_desc(v_base + kk * 2048, kKeys * 128, 1024), IDESC_PV,
+                         (j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&bars->o_full[x][j & 1]);
+        }
+        if (ok) umma_commit(&bars->v_empty[st]);
       }
       umma_commit(&bars->mma_done);
       drain(&bars->mma_done, 0);
@@ -371,72 +437,89 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
     const bool mine = r < TT * p.G && tok < q_len;
     const int lim = mine ? start + tok + 1 : 0;   // keys this row sees
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
-    const uint32_t t_s = tmem + x * 128 + lane_off;
     const uint32_t t_o = tmem + Cfg::T_O + x * D + lane_off;
     const int n = nkv_of(x);
-    const float4* par = p.par + sh * p.blocks + j0 * (kT / kP8Page);
-    float4* s_par = reinterpret_cast<float4*>(bars + 1) + warp * (kT / kP8Page);
+    constexpr int BL = Cfg::BLOCKS;
+    const float4* par = p.par + sh * p.blocks + j0 * BL;
+    // the tiles' block scales, through this warp's own corner of shared memory: an
+    // asynchronous copy one tile ahead, for which no register waits
+    float4* s_par2 = reinterpret_cast<float4*>(bars + 1) + warp * (2 * BL);
+    auto fetch_par = [&](int j) {
+      if (j < n && lane < BL)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(
+                         smem_u32(s_par2 + (j & 1) * BL + lane)),
+                     "l"(par + j * BL + lane)
+                     : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     // rows that are no token's never see a key and never ask for a rescale
     float m_used = mine ? -INFINITY : 0.f, l = 0.f;
     bool ok = true;
-    float4 next = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (n > 0 && lane < kT / kP8Page) next = __ldg(par + lane);
+    fetch_par(0);
     for (int j = 0; j < n && ok; ++j) {
-      // the tile's block scales, through this warp's own corner of shared memory
-      const bool bad = __any_sync(0xffffffffu, next.x != next.x);
-      if (lane < kT / kP8Page) {
-        s_par[lane] = next;
-        if (j + 1 < n) next = __ldg(par + (j + 1) * (kT / kP8Page) + lane);
-      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();
-      if (!wait_warp(&bars->s_full[x], j & 1, abort_flag, p.err, kErrTimeoutTmem, 89)) {
+      const float4* s_par = s_par2 + (j & 1) * BL;
+      const float k_scale = s_par[lane % BL].x;
+      const bool bad = __any_sync(0xffffffffu, k_scale != k_scale);
+      fetch_par(j + 1);
+      if (!wait_warp(&bars->s_full[x][j & 1], (j >> 1) & 1, abort_flag, p.err, kErrTimeoutTmem,
+                     89)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const int kmax = lim - (j0 + j) * kT;  // keys of the tile that this row sees
-      const bool edge = __any_sync(0xffffffffu, kmax < kT);
+      const uint32_t t_s = tmem + (2 * x + (j & 1)) * kKeys + lane_off;
+      const int kmax = lim - (j0 + j) * kKeys;  // keys of the tile that this row sees
+      const bool edge = __any_sync(0xffffffffu, kmax < kKeys);
       // One pass over S computes P against the bound in use and the row's maximum; only
       // where the maximum turns out too far above the bound is the bound moved and the pass
       // repeated (always in a row's first tile, seldom later).
-      uint32_t pk[kT / 2];
+      uint32_t pk[kKeys / 2];
       float sum;
       bool nan_row = false;
       auto pass = [&](auto masked, float msub) {
-        float2 mx2 = make_float2(-INFINITY, -INFINITY), l2 = make_float2(0.f, 0.f);
-        uint32_t buf[2][16];
-        tmem_ld16_async(t_s, buf[0]);
+        float mx = -INFINITY;
+        float2 l2 = make_float2(0.f, 0.f);
+        uint32_t buf[kKeys / 32][32];
 #pragma unroll
-        for (int b = 0; b < kT / 16; ++b) {
-          uint32_t(&cur)[16] = buf[b & 1];
-          tmem_wait16(cur);
-          if (b + 1 < kT / 16) tmem_ld16_async(t_s + (b + 1) * 16, buf[(b + 1) & 1]);
-          const float4 f = s_par[b];
-          float kf = f.x, nm = f.y - msub;
-          if (bad && kf != kf) {  // NaN for the rows that see the block, nothing for the others
-            nan_row |= b * 16 < kmax;
-            kf = 1.f;
-            nm = -INFINITY;
-          }
-          float2 rs = make_float2(0.f, 0.f);
+        for (int c = 0; c < kKeys / 32; ++c) tmem_ld32_async(t_s + c * 32, buf[c]);
+        tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float2 sv = make_float2(__uint_as_float(cur[i]), __uint_as_float(cur[i + 1]));
-            if constexpr (decltype(masked)::value) {
-              if (b * 16 + i >= kmax) sv.x = -INFINITY;
-              if (b * 16 + i + 1 >= kmax) sv.y = -INFINITY;
+        for (int c = 0; c < kKeys / 32; ++c) tmem_ready32(buf[c]);
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) {
+          uint32_t(&cur)[32] = buf[c];
+#pragma unroll
+          for (int b = 2 * c; b < 2 * c + 2; ++b) {
+            const float4 f = s_par[b];
+            float kf = f.x, nm = f.y - msub;
+            if (bad && kf != kf) {  // NaN for the rows that see the block, nothing for the others
+              nan_row |= b * 16 < kmax;
+              kf = 1.f;
+              nm = -INFINITY;
             }
-            const float2 xv = fma2(sv, make_float2(kf, kf), make_float2(nm, nm));
-            mx2.x = fmaxf(mx2.x, xv.x);
-            mx2.y = fmaxf(mx2.y, xv.y);
-            const float2 pv = (i >> 1) < POLY ? exp2_poly2(xv) : make_float2(ex2c(xv.x), ex2c(xv.y));
-            rs = add2(rs, pv);
-            pk[b * 8 + i / 2] = P8Io<__half>::pack(pv.x, pv.y);
+            float2 rs = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const int u = (b & 1) * 16 + i;
+              float2 sv = make_float2(__uint_as_float(cur[u]), __uint_as_float(cur[u + 1]));
+              if constexpr (decltype(masked)::value) {
+                if (b * 16 + i >= kmax) sv.x = -INFINITY;
+                if (b * 16 + i + 1 >= kmax) sv.y = -INFINITY;
+              }
+              const float2 xv = fma2(sv, make_float2(kf, kf), make_float2(nm, nm));
+              mx = max3(mx, xv.x, xv.y);
+              const float2 pv =
+                  (i >> 1) < POLY ? exp2_poly2(xv) : make_float2(ex2c(xv.x), ex2c(xv.y));
+              rs = add2(rs, pv);
+              pk[b * 8 + i / 2] = P8Io<__half>::pack(pv.x, pv.y);
+            }
+            l2 = fma2(rs, make_float2(f.z, f.z), l2);
           }
-          l2 = fma2(rs, make_float2(f.z, f.z), l2);
         }
         sum = l2.x + l2.y;
-        return fmaxf(mx2.x, mx2.y);
+        return mx;
       };
       for (int tries = 0; tries < 4; ++tries) {  // two are enough for finite scores
         const float msub = m_used == -INFINITY ? 0.f : m_used;
@@ -448,7 +531,14 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
         const float alpha = grow && had ? ex2c(-mx) : 1.f;
         if (grow) m_used = msub + mx;
         l *= alpha;
-        if (__any_sync(0xffffffffu, grow && had)) {  // O_x holds the earlier tiles' P V
+        if (__any_sync(0xffffffffu, grow && had)) {
+          // O_x holds the earlier tiles' P V, once the last of them is done
+          if (!wait_warp(&bars->o_full[x][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, p.err,
+                         kErrTimeoutTmem, 78)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D; c += 16) {
             uint32_t o[16];
@@ -460,17 +550,19 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, 1)
           }
         }
       }
+      if (!ok) break;
       l += nan_row ? __uint_as_float(0x7fc00000u) : sum;
 #pragma unroll
-      for (int c = 0; c < kT / 2; c += 16) tmem_st16(t_s + c, pk + c);
+      for (int c = 0; c < kKeys / 2; c += 16) tmem_st16(t_s + c, pk + c);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full[x]);
+      if (lane == 0) mbar_arrive(&bars->p_full[x][j & 1]);
     }
     const int64_t orow = static_cast<int64_t>(row0 + tok) * p.Hq + h * p.G + r % p.G;
     if (n > 0) {
-      if (ok && wait_warp(&bars->o_full[x], 0, abort_flag, p.err, kErrTimeoutTmem, 90)) {
+      if (ok && wait_warp(&bars->o_full[x][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, p.err,
+                          kErrTimeoutTmem, 90)) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
 #pragma unroll
@@ -526,6 +618,7 @@ struct MassParams {
   float* mass_out;
   int64_t N;
   int Hq, Hkv, G;
+  int parts;                   // CTAs of a key tile's cluster
   int* err;
 };
 
@@ -567,7 +660,8 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
   volatile int* abort_flag = &bars->abort;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int h = blockIdx.y, seq = blockIdx.z;
-  const int k0 = blockIdx.x * kT;
+  const int part = static_cast<int>(cluster_ctarank());
+  const int k0 = static_cast<int>(blockIdx.x) / p.parts * kT;
   const int row0 = __ldg(p.cu_q + seq), q_len = __ldg(p.cu_q + seq + 1) - row0;
   if (row0 < 0 || q_len < 0 || static_cast<int64_t>(row0) + q_len > p.N) {
     if (threadIdx.x == 0) report_error(p.err, kErrBounds, 91);
@@ -576,8 +670,9 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
   const int kv = p8_len(p.kv_lens, seq, p.max_pages, p.err, 92);
   if (k0 >= kv) return;
   const int start = kv - q_len, TT = kT / p.G;
-  const int i0 = max(0, k0 - start) / TT;               // first row tile that sees the keys
-  const int n = max(0, (q_len + TT - 1) / TT - i0);      // row tiles
+  // this CTA's row tiles: part, part + parts, .. of those that see the keys
+  const int i0 = max(0, k0 - start) / TT + part;
+  const int n = max(0, ((q_len + TT - 1) / TT - i0 + p.parts - 1) / p.parts);
   const int64_t sh = static_cast<int64_t>(seq) * p.Hkv + h;
 
   if (threadIdx.x == 0) {
@@ -625,7 +720,7 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
 #pragma unroll
         for (int c = 0; c < Cfg::CHUNKS; ++c)
           tma_load_4d(sQ + st * Cfg::TILE + c * kT * 128, &tmQ, &bars->q_full[st], c * 64, 0, h,
-                      row0 + (i0 + i) * TT);
+                      row0 + (i0 + i * p.parts) * TT);
         ++issued;
       }
       drain(&bars->k_full, 0);
@@ -668,21 +763,28 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
     const uint32_t t_s = tmem + x * 128 + (static_cast<uint32_t>(wq * 32) << 16);
     float2 acc[2] = {};
     bool ok = true;  // a warp that gave up still meets the others at their barriers
+    // column r of a row tile: its log-sum-exp (one tile ahead) and last visible key
+    const int my_tok = r / p.G;
+    const float* my_lse = p.lse + (static_cast<int64_t>(row0 + my_tok) * p.Hq + h * p.G + r % p.G) *
+                                      p.lse_stride;
+    auto is_row = [&](int i) {
+      return r < TT * p.G && (i0 + i * p.parts) * TT + my_tok < q_len;
+    };
+    auto fetch = [&](int i) {
+      return i < n && is_row(i)
+                 ? __ldg(my_lse + static_cast<int64_t>(i0 + i * p.parts) * TT * p.Hq * p.lse_stride)
+                 : INFINITY;
+    };
+    float next = fetch(x);
     for (int i = x; i < n; i += 2) {
-      // column r of this row tile: its log-sum-exp and last visible key
-      const int tok = (i0 + i) * TT + r / p.G;
-      const bool row = r < TT * p.G && tok < q_len;
-      float le = INFINITY;
-      if (row) {
-        le = __ldg(p.lse + (static_cast<int64_t>(row0 + tok) * p.Hq + h * p.G + r % p.G) *
-                               p.lse_stride);
-        if (le == -INFINITY) le = INFINITY;              // a row without keys weighs nothing
-      }
+      const float le = next == -INFINITY ? INFINITY : next;  // a row without keys weighs nothing
+      next = fetch(i + 2);
       named_bar_sync(1 + x, 128);                         // the previous tile's values are read
       s_lse[x * kT + r] = -le;
-      s_lim[x * kT + r] = row ? start + tok : -1;
+      s_lim[x * kT + r] = is_row(i) ? start + (i0 + i * p.parts) * TT + my_tok : -1;
       named_bar_sync(1 + x, 128);
-      const bool edge = k0 + kT - 1 > start + (i0 + i) * TT || (i0 + i + 1) * TT > q_len;
+      const int t0 = (i0 + i * p.parts) * TT;
+      const bool edge = k0 + kT - 1 > start + t0 || t0 + TT > q_len;
       ok = ok && wait_warp(&bars->s_full[x], (i >> 1) & 1, abort_flag, p.err, kErrTimeoutTmem, 97);
       if (!ok) continue;
       tc_fence_after();
@@ -719,12 +821,7 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
     const float w = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
     if (x == 1) s_w[r] = w;
     named_bar_sync(3, 256);
-    if (x == 0 && key < kv) {
-      const int64_t page = p8_page(p.table + static_cast<int64_t>(seq) * p.max_pages,
-                                   key / kP8Page, p.num_pages, p.err, 98);
-      const int64_t at = (page * p.Hkv + h) * kP8Page + key % kP8Page;
-      p.mass_out[at] = p.mass_in[at] + (w + s_w[r]);
-    }
+    if (x == 0) s_w[r] += w;
   }
   tc_fence_before();
   __syncthreads();
@@ -732,6 +829,24 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
+  __syncwarp();
+  cluster_sync_all();  // every part's sums are in its shared memory
+  if (part == 0 && threadIdx.x < kT && k0 + static_cast<int>(threadIdx.x) < kv) {
+    const int key = k0 + threadIdx.x;
+    float w = s_w[threadIdx.x];
+    for (int i = 1; i < p.parts; ++i) {
+      float y;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                   : "=f"(y) : "r"(mapa_shared(smem_u32(s_w + threadIdx.x), i)) : "memory");
+      w += y;
+    }
+    const int64_t page = p8_page(p.table + static_cast<int64_t>(seq) * p.max_pages, key / kP8Page,
+                                 p.num_pages, p.err, 98);
+    const int64_t at = (page * p.Hkv + h) * kP8Page + key % kP8Page;
+    p.mass_out[at] = p.mass_in[at] + w;
+  }
+  __syncwarp();
+  cluster_sync_all();  // nobody leaves while its sums are read
 }
 
 template <typename T, int FMT, int D>
@@ -782,8 +897,8 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
   k.ss = v.ss = D;
   k.sh = v.sh = Lw * D;
   k.sb = v.sb = Lw * D * c.Hkv;
-  if (!rc) rc = make_bhsd_map(&tk, k, s.num_seqs, c.Hkv, static_cast<int>(Lw), D, kT);
-  if (!rc) rc = make_bhsd_map(&tv, v, s.num_seqs, c.Hkv, static_cast<int>(Lw), D, kT);
+  if (!rc) rc = make_bhsd_map(&tk, k, s.num_seqs, c.Hkv, static_cast<int>(Lw), D, kKeys);
+  if (!rc) rc = make_bhsd_map(&tv, v, s.num_seqs, c.Hkv, static_cast<int>(Lw), D, kKeys);
   if (rc) return rc;
   ChunkParams p;
   p.cu_q = s.cu_q;
@@ -818,6 +933,9 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
   }
   if (mass) {
     using Cfg = MassCfg<D>;
+    CUtensorMap tkm;
+    rc = make_bhsd_map(&tkm, k, s.num_seqs, c.Hkv, static_cast<int>(Lw), D, kT);
+    if (rc) return rc;
     MassParams m;
     m.table = s.table;
     m.cu_q = s.cu_q;
@@ -835,11 +953,28 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
     m.Hkv = c.Hkv;
     m.G = G;
     m.err = err;
-    auto kern = p8_chunk_mass_kernel<T, D>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM))
-      return static_cast<int>(cudaGetLastError());
-    kern<<<dim3(static_cast<unsigned>((s.max_pages * kP8Page + kT - 1) / kT), c.Hkv, s.num_seqs),
-           Cfg::THREADS, Cfg::SMEM, st>>>(tq, tk, m);
+    constexpr auto kern = p8_chunk_mass_kernel<T, D>;
+    rc = p8_opt_in<kern>(Cfg::SMEM);
+    if (rc) return rc;
+    const int key_tiles = (s.max_pages * kP8Page + kT - 1) / kT;
+    const int64_t ctas = static_cast<int64_t>(key_tiles) * c.Hkv * s.num_seqs;
+    const int row_tiles = (a.max_q_len + TT - 1) / TT;
+    m.parts = 1;
+    while (m.parts < 8 && 2 * m.parts * ctas <= 2 * a.num_sms && 4 * m.parts <= row_tiles)
+      m.parts *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = m.parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.stream = st;
+    cfg.gridDim = dim3(key_tiles * m.parts, c.Hkv, s.num_seqs);
+    cfg.blockDim = dim3(Cfg::THREADS);
+    cfg.dynamicSmemBytes = Cfg::SMEM;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tq, tkm, m);
+    if (e != cudaSuccess) return static_cast<int>(e);
   }
   return static_cast<int>(cudaGetLastError());
 }
@@ -855,12 +990,13 @@ void p8_chunk_plan(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_s
   const int TT = kT / group;
   const int64_t heads = static_cast<int64_t>(Hkv) * s.num_seqs;
   const int64_t pairs = (max_q_len + 2 * TT - 1) / (2 * TT) * heads;
+  // two row tiles share the keys of a CTA once that still fills the SMs
   *nq = pairs >= num_sms ? 2 : 1;
-  const int64_t ctas = *nq == 2 ? pairs : (max_q_len + TT - 1) / TT * heads;
-  // fill the SMs, at least four key tiles each
-  const int64_t tiles = (static_cast<int64_t>(s.max_pages) * kP8Page + kT - 1) / kT;
-  int64_t sp = num_sms / ctas;
-  if (sp > tiles / 4) sp = tiles / 4;
+  // one row tile a CTA: two CTAs on an SM, at least eight key tiles each
+  const int64_t ctas = (max_q_len + TT - 1) / TT * heads;
+  const int64_t tiles = (static_cast<int64_t>(s.max_pages) * kP8Page + kKeys - 1) / kKeys;
+  int64_t sp = *nq == 2 ? 1 : 2 * num_sms / ctas;
+  if (sp > tiles / 8) sp = tiles / 8;
   *splits = static_cast<int>(sp < 1 ? 1 : sp);
 }
 
