@@ -219,12 +219,13 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
   cfb::p8_chunk_plan(s, c.Hkv, group, a.max_q_len, sms, &a.chunk_nq, &a.splits);
   if (seqs_each < s.num_seqs) a.splits = 1;
   a.num_sms = sms;
-  // one workspace: expanded K | V | their block scales | split outputs | log-sum-exps
+  // one workspace: expanded K | V | their block scales | split outputs | log-sum-exps | totals
   const int64_t n_kv = seqs_each * each / 2;  // floats
   const int64_t n_par = seqs_each * c.Hkv * blocks * 4;
   const int64_t n_o = a.splits > 1 ? N * Hq * a.splits * c.D : 0;
   const int64_t n_lse = a.splits > 1 || mass ? N * Hq * a.splits : 0;
-  const Tensor ws = empty({2 * n_kv + n_par + n_o + n_lse}, torch::kFloat32, codes);
+  const int64_t n_total = a.splits > 1 && mass ? N * Hq : 0;
+  const Tensor ws = empty({2 * n_kv + n_par + n_o + n_lse + n_total}, torch::kFloat32, codes);
   float* at = ws.data_ptr<float>();
   a.ws_k = at;
   a.ws_v = at + n_kv;
@@ -232,6 +233,7 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
   at += 2 * n_kv + n_par;
   a.ws_o = n_o ? at : nullptr;
   a.ws_lse = n_lse ? at + n_o : nullptr;
+  a.ws_total = n_total ? at + n_o + n_lse : nullptr;
   for (int64_t i = 0; i < s.num_seqs; i += seqs_each) {
     cfb::P8Seqs part = s;
     part.table += i * s.max_pages;

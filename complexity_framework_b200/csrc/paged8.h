@@ -54,6 +54,7 @@ struct P8Attn {
   int splits = 1;
   float* ws_o = nullptr;     // [N * Hq, splits, D] (splits > 1)
   float* ws_lse = nullptr;   // [N * Hq, splits] (splits > 1 or mass)
+  float* ws_total = nullptr; // [N * Hq] (splits > 1 and mass)
   int chunk_nq = 2;          // 128-row tiles of a CTA
   int num_sms = 148;
   // keys and values as 16-bit operands, Lw = 16 * p8_chunk_blocks() tokens
@@ -75,8 +76,7 @@ P8AttnPlan p8_attn_plan(const P8Cache& c, const P8Seqs& s, int group, int max_q_
 int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, const P8AttnPlan& plan,
                  float* ws, int* err, cudaStream_t stream);
 
-// Long chunks.  Joins the splits: out from ws_o and ws_lse; a row's first ws_lse becomes its
-// total.
+// Long chunks.  Joins the splits: out, and each row's total, from ws_o and ws_lse.
 int p8_combine(const P8Attn& a, int D, cudaStream_t stream);
 int p8_chunk_blocks(const P8Seqs& s);
 // Whether a call's chunks go to the tcgen05 kernels.

@@ -762,37 +762,56 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Joins the splits of a row of a long chunk: out = sum 2^(lse_s - L) o_s with
-// L = log2 sum 2^lse_s, and leaves L in the row's first lse slot for the weights.
-template <typename T>
-__global__ void __launch_bounds__(128)
-    p8_combine_kernel(const float* __restrict__ ws_o, float* __restrict__ ws_lse,
-                      T* __restrict__ out, int64_t rows, int splits, int D) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
+// Joins the splits of a long chunk's rows: out = sum 2^(lse_s - L) o_s with
+// L = log2 sum 2^lse_s, which goes to `total` where the weights need it.  A thread has four
+// dims of a row; all it reads is on its way before it is looked at.
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+    p8_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_lse,
+                      float* __restrict__ total, T* __restrict__ out, int64_t rows, int splits) {
+  constexpr int kMost = 4;  // splits read ahead
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = at / (D / 4);
+  const int d = static_cast<int>(at % (D / 4)) * 4;
+  p8_grid_wait();
   if (row >= rows) return;
-  float* lse = ws_lse + row * splits;
-  float m = -INFINITY;
-  for (int s = lane; s < splits; s += 32) m = fmaxf(m, lse[s]);
+  const float* lse = ws_lse + row * splits;
+  const float* o = ws_o + row * splits * D + d;
+  float ls[kMost];
+  float4 x[kMost];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+  for (int s = 0; s < kMost; ++s)
+    if (s < splits) {
+      ls[s] = lse[s];
+      x[s] = *reinterpret_cast<const float4*>(o + s * D);
+    }
+  float m = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < kMost; ++s)
+    if (s < splits) m = fmaxf(m, ls[s]);
+  for (int s = kMost; s < splits; ++s) m = fmaxf(m, lse[s]);
   const float base = m == -INFINITY ? 0.f : m;
   float den = 0.f;
-  for (int s = 0; s < splits; ++s) den += ex2f(lse[s] - base);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float l, const float4& y) {
+    const float w = ex2f(l - base);
+    if (w == 0.f) return;  // a split without keys of this row left nothing to read
+    den += w;
+    acc.x = fmaf(w, y.x, acc.x);
+    acc.y = fmaf(w, y.y, acc.y);
+    acc.z = fmaf(w, y.z, acc.z);
+    acc.w = fmaf(w, y.w, acc.w);
+  };
+#pragma unroll
+  for (int s = 0; s < kMost; ++s)
+    if (s < splits) add(ls[s], x[s]);
+  for (int s = kMost; s < splits; ++s) add(lse[s], *reinterpret_cast<const float4*>(o + s * D));
   const float inv = den == 0.f ? 0.f : __fdiv_rn(1.f, den);
-  for (int d = lane * 2; d < D; d += 64) {
-    float2 acc = make_float2(0.f, 0.f);
-    for (int s = 0; s < splits; ++s) {
-      const float w = ex2f(lse[s] - base);
-      if (w == 0.f) continue;
-      const float2 x = *reinterpret_cast<const float2*>(ws_o + (row * splits + s) * D + d);
-      acc.x += w * x.x;
-      acc.y += w * x.y;
-    }
-    *reinterpret_cast<uint32_t*>(out + row * D + d) = P8Io<T>::pack(acc.x * inv, acc.y * inv);
-  }
-  __syncwarp();
-  if (lane == 0) lse[0] = den == 0.f ? -INFINITY : base + log2f(den);
+  uint2 u;
+  u.x = P8Io<T>::pack(acc.x * inv, acc.y * inv);
+  u.y = P8Io<T>::pack(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(out + row * D + d) = u;
+  if (total != nullptr && d == 0) total[row] = den == 0.f ? -INFINITY : base + log2f(den);
 }
 
 template <typename T, int FMT, int D, int NB, bool MASS>
@@ -832,15 +851,19 @@ int launch_attn(const AttnParams& p, int nb, cudaStream_t st) {
 
 int p8_combine(const P8Attn& a, int D, cudaStream_t st) {
   const int64_t n = a.N * a.Hq;
-  const int64_t grid = (n + 3) / 4;
+  const int64_t grid = (n * (D / 4) + 255) / 256;
   if (grid > 0x7fffffff) return -3;
-  if (a.type == kP8Bf16)
-    p8_combine_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), 128, 0, st>>>(
-        a.ws_o, a.ws_lse, static_cast<__nv_bfloat16*>(a.out), n, a.splits, D);
-  else
-    p8_combine_kernel<__half><<<static_cast<unsigned>(grid), 128, 0, st>>>(
-        a.ws_o, a.ws_lse, static_cast<__half*>(a.out), n, a.splits, D);
-  return 0;
+  const dim3 g(static_cast<unsigned>(grid));
+#define CFB_COMBINE(T, DD)                                                                  \
+  return p8_launch(p8_combine_kernel<T, DD>, g, 256, 0, st, a.ws_o, a.ws_lse, a.ws_total,   \
+                   static_cast<T*>(a.out), n, a.splits)
+  if (a.type == kP8Bf16) {
+    if (D == 128) CFB_COMBINE(__nv_bfloat16, 128);
+    CFB_COMBINE(__nv_bfloat16, 64);
+  }
+  if (D == 128) CFB_COMBINE(__half, 128);
+  CFB_COMBINE(__half, 64);
+#undef CFB_COMBINE
 }
 
 P8AttnPlan p8_attn_plan(const P8Cache& c, const P8Seqs& s, int group, int max_q_len, bool mass,

@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CT
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
+  p8_grid_wait();  // the setup above overlaps the expansion's end
 
   if (warp == Cfg::PRODUCER) {
     if (nkv > 0 && elect_one()) {
@@ -612,8 +613,7 @@ struct MassParams {
   int max_pages, blocks;
   int64_t num_pages;
   const float4* par;
-  const float* lse;            // [N * Hq], row stride lse_stride
-  int64_t lse_stride;
+  const float* lse;            // [N * Hq]
   const float* mass_in;
   float* mass_out;
   int64_t N;
@@ -625,18 +625,21 @@ struct MassParams {
 template <int D>
 struct MassCfg {
   static constexpr int STAGES = 3;
+  static constexpr int GROUPS = 4;             // of four warps; each has a score tile of its own
   static constexpr int CHUNKS = D / 64;
   static constexpr int TILE = kT * D * 2;
-  static constexpr int SMEM = (1 + STAGES) * TILE + 1024 + 512 + 2 * kT * 8 + kT * 4;
-  static constexpr int THREADS = 320;
+  static constexpr int SMEM = (1 + STAGES) * TILE + 1024 + 512 + GROUPS * kT * 12;
+  static constexpr int PRODUCER = 4 * GROUPS, MMA = PRODUCER + 1;
+  static constexpr int THREADS = (MMA + 1) * 32;
+  static constexpr uint32_t TMEM = GROUPS * kT;
 };
 
 struct MassBars {
   uint64_t k_full;
   uint64_t q_full[3];
   uint64_t q_empty[3];
-  uint64_t s_full[2];
-  uint64_t s_empty[2];
+  uint64_t s_full[4];
+  uint64_t s_empty[4];
   uint64_t mma_done;
   uint32_t tmem;
   int abort;
@@ -653,10 +656,11 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sK = smem;
   uint8_t* sQ = sK + Cfg::TILE;
-  float* s_lse = reinterpret_cast<float*>(sQ + STAGES * Cfg::TILE);  // [2][128]
-  int* s_lim = reinterpret_cast<int*>(s_lse + 2 * kT);               // [2][128]
-  float* s_w = reinterpret_cast<float*>(s_lim + 2 * kT);             // [128]
-  MassBars* bars = reinterpret_cast<MassBars*>(s_w + kT);
+  constexpr int GR = Cfg::GROUPS;
+  float* s_lse = reinterpret_cast<float*>(sQ + STAGES * Cfg::TILE);  // [GR][128]
+  int* s_lim = reinterpret_cast<int*>(s_lse + GR * kT);              // [GR][128]
+  float* s_w = reinterpret_cast<float*>(s_lim + GR * kT);            // [GR][128]
+  MassBars* bars = reinterpret_cast<MassBars*>(s_w + GR * kT);
   volatile int* abort_flag = &bars->abort;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int h = blockIdx.y, seq = blockIdx.z;
@@ -681,7 +685,7 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
       mbar_init(&bars->q_full[s], 1);
       mbar_init(&bars->q_empty[s], 1);
     }
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < GR; ++x) {
       mbar_init(&bars->s_full[x], 1);
       mbar_init(&bars->s_empty[x], 4);
     }
@@ -698,13 +702,14 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
     }
     if (rows > 0) fence_proxy_async_shared();
   }
-  if (warp == 9) tmem_alloc(&bars->tmem, 256);
+  if (warp == Cfg::MMA) tmem_alloc(&bars->tmem, Cfg::TMEM);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
+  p8_grid_wait();
 
-  if (warp == 8) {
+  if (warp == Cfg::PRODUCER) {
     if (elect_one()) {
       mbar_arrive_expect_tx(&bars->k_full, Cfg::TILE);
 #pragma unroll
@@ -727,16 +732,16 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
       for (int i = issued - STAGES < 0 ? 0 : issued - STAGES; i < issued; ++i)
         drain(&bars->q_full[i % STAGES], (i / STAGES) & 1);
     }
-  } else if (warp == 9) {
+  } else if (warp == Cfg::MMA) {
     if (elect_one()) {
       constexpr uint32_t IDESC = idesc16<T>(kT, kT, false);
       bool ok = mbar_wait(&bars->k_full, 0, abort_flag, p.err, kErrTimeoutFull, 94);
       const uint32_t k_base = smem_u32(sK);
       for (int i = 0; i < n && ok; ++i) {
-        const int st = i % STAGES, x = i & 1;
+        const int st = i % STAGES, x = i % GR;
         if (!mbar_wait(&bars->q_full[st], (i / STAGES) & 1, abort_flag, p.err, kErrTimeoutFull,
                        95) ||
-            !mbar_wait(&bars->s_empty[x], ((i >> 1) & 1) ^ 1, abort_flag, p.err, kErrTimeoutTmem,
+            !mbar_wait(&bars->s_empty[x], ((i / GR) & 1) ^ 1, abort_flag, p.err, kErrTimeoutTmem,
                        96)) {
           ok = false;
           break;
@@ -765,27 +770,27 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
     bool ok = true;  // a warp that gave up still meets the others at their barriers
     // column r of a row tile: its log-sum-exp (one tile ahead) and last visible key
     const int my_tok = r / p.G;
-    const float* my_lse = p.lse + (static_cast<int64_t>(row0 + my_tok) * p.Hq + h * p.G + r % p.G) *
-                                      p.lse_stride;
+    const float* my_lse =
+        p.lse + static_cast<int64_t>(row0 + my_tok) * p.Hq + h * p.G + r % p.G;
     auto is_row = [&](int i) {
       return r < TT * p.G && (i0 + i * p.parts) * TT + my_tok < q_len;
     };
     auto fetch = [&](int i) {
       return i < n && is_row(i)
-                 ? __ldg(my_lse + static_cast<int64_t>(i0 + i * p.parts) * TT * p.Hq * p.lse_stride)
+                 ? __ldg(my_lse + static_cast<int64_t>(i0 + i * p.parts) * TT * p.Hq)
                  : INFINITY;
     };
     float next = fetch(x);
-    for (int i = x; i < n; i += 2) {
+    for (int i = x; i < n; i += GR) {
       const float le = next == -INFINITY ? INFINITY : next;  // a row without keys weighs nothing
-      next = fetch(i + 2);
+      next = fetch(i + GR);
       named_bar_sync(1 + x, 128);                         // the previous tile's values are read
       s_lse[x * kT + r] = -le;
       s_lim[x * kT + r] = is_row(i) ? start + (i0 + i * p.parts) * TT + my_tok : -1;
       named_bar_sync(1 + x, 128);
       const int t0 = (i0 + i * p.parts) * TT;
       const bool edge = k0 + kT - 1 > start + t0 || t0 + TT > q_len;
-      ok = ok && wait_warp(&bars->s_full[x], (i >> 1) & 1, abort_flag, p.err, kErrTimeoutTmem, 97);
+      ok = ok && wait_warp(&bars->s_full[x], (i / GR) & 1, abort_flag, p.err, kErrTimeoutTmem, 97);
       if (!ok) continue;
       tc_fence_after();
 #pragma unroll
@@ -819,27 +824,29 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
       }
     }
     const float w = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
-    if (x == 1) s_w[r] = w;
-    named_bar_sync(3, 256);
-    if (x == 0) s_w[r] += w;
+    s_w[x * kT + r] = w;
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == Cfg::MMA) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, Cfg::TMEM);
   }
   __syncwarp();
   cluster_sync_all();  // every part's sums are in its shared memory
   if (part == 0 && threadIdx.x < kT && k0 + static_cast<int>(threadIdx.x) < kv) {
     const int key = k0 + threadIdx.x;
-    float w = s_w[threadIdx.x];
-    for (int i = 1; i < p.parts; ++i) {
-      float y;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                   : "=f"(y) : "r"(mapa_shared(smem_u32(s_w + threadIdx.x), i)) : "memory");
-      w += y;
-    }
+    float w = 0.f;
+    for (int i = 0; i < p.parts; ++i)
+#pragma unroll
+      for (int x = 0; x < GR; ++x) {
+        float y;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                     : "=f"(y)
+                     : "r"(mapa_shared(smem_u32(s_w + x * kT + threadIdx.x), i))
+                     : "memory");
+        w += y;
+      }
     const int64_t page = p8_page(p.table + static_cast<int64_t>(seq) * p.max_pages, key / kP8Page,
                                  p.num_pages, p.err, 98);
     const int64_t at = (page * p.Hkv + h) * kP8Page + key % kP8Page;
@@ -872,8 +879,7 @@ int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
   if (gx > 0x7fffffff) return -3;
   const int rc = p8_opt_in<kern>(Cfg::SMEM);
   if (rc) return rc;
-  kern<<<static_cast<unsigned>(gx), Cfg::THREADS, Cfg::SMEM, st>>>(tq, tk, tv, p);
-  return 0;
+  return p8_launch(kern, dim3(static_cast<unsigned>(gx)), Cfg::THREADS, Cfg::SMEM, st, tq, tk, tv, p);
 }
 
 template <typename T, int D>
@@ -944,8 +950,7 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
     m.blocks = blocks;
     m.num_pages = c.num_pages;
     m.par = p.par;
-    m.lse = a.ws_lse;
-    m.lse_stride = p.splits;
+    m.lse = p.splits > 1 ? a.ws_total : a.ws_lse;
     m.mass_in = a.mass_in;
     m.mass_out = a.mass_out;
     m.N = a.N;
@@ -960,15 +965,17 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
     const int64_t ctas = static_cast<int64_t>(key_tiles) * c.Hkv * s.num_seqs;
     const int row_tiles = (a.max_q_len + TT - 1) / TT;
     m.parts = 1;
-    while (m.parts < 8 && 2 * m.parts * ctas <= 2 * a.num_sms && 4 * m.parts <= row_tiles)
+    while (m.parts < 8 && 2 * m.parts * ctas <= a.num_sms && 8 * m.parts <= row_tiles)
       m.parts *= 2;
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = m.parts;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     cfg.stream = st;
     cfg.gridDim = dim3(key_tiles * m.parts, c.Hkv, s.num_seqs);
     cfg.blockDim = dim3(Cfg::THREADS);
