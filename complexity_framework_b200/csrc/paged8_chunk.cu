@@ -19,7 +19,9 @@
 // Key tiles are 64 wide so that TMEM (512 columns) holds two S of each row tile beside O:
 // the next S is there when a softmax warp ends a tile.  With 128-wide tiles and one S the
 // chain S -> P -> O -> S left the softmax warps idle for 40% of a tile (4100 cycles for 128
-// keys of two row tiles, of which their exponentials need 2100).
+// keys of two row tiles, of which their exponentials need 2100).  A cubic on the FMA pipe for
+// a share of the exponentials gains nothing here (140.9 us with a quarter of them, 142.8
+// without): issue slots are as scarce as the exponential unit.
 // p8_chunk_mass_kernel: weights summed over the rows need each row's final log-sum-exp, so
 // they are recomputed: one CTA per (128 keys, KV head, sequence) walks the row tiles with
 // S^T = K Q^T (a thread owns a key), adding 2^(s - lse) in a fixed order: no atomics, the same
@@ -230,7 +232,7 @@ struct alignas(16) ChunkBars {
 };
 static_assert(sizeof(ChunkBars) % 16 == 0 && sizeof(ChunkBars) <= 512, "block scales follow");
 
-template <typename T, int D, int NQ, int POLY>
+template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CTAS))
     p8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ,
                     const __grid_constant__ CUtensorMap tmK,
@@ -458,18 +460,16 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CT
     bool ok = true;
     fetch_par(0);
     for (int j = 0; j < n && ok; ++j) {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      __syncwarp();
-      const float4* s_par = s_par2 + (j & 1) * BL;
-      const float k_scale = s_par[lane % BL].x;
-      const bool bad = __any_sync(0xffffffffu, k_scale != k_scale);
-      fetch_par(j + 1);
       if (!wait_warp(&bars->s_full[x][j & 1], (j >> 1) & 1, abort_flag, p.err, kErrTimeoutTmem,
                      89)) {
         ok = false;
         break;
       }
       tc_fence_after();
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+      const float4* s_par = s_par2 + (j & 1) * BL;
+      fetch_par(j + 1);
       const uint32_t t_s = tmem + (2 * x + (j & 1)) * kKeys + lane_off;
       const int kmax = lim - (j0 + j) * kKeys;  // keys of the tile that this row sees
       const bool edge = __any_sync(0xffffffffu, kmax < kKeys);
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CT
           for (int b = 2 * c; b < 2 * c + 2; ++b) {
             const float4 f = s_par[b];
             float kf = f.x, nm = f.y - msub;
-            if (bad && kf != kf) {  // NaN for the rows that see the block, nothing for the others
+            if (kf != kf) {  // NaN for the rows that see the block, nothing for the others
               nan_row |= b * 16 < kmax;
               kf = 1.f;
               nm = -INFINITY;
@@ -511,8 +511,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CT
               }
               const float2 xv = fma2(sv, make_float2(kf, kf), make_float2(nm, nm));
               mx = max3(mx, xv.x, xv.y);
-              const float2 pv =
-                  (i >> 1) < POLY ? exp2_poly2(xv) : make_float2(ex2c(xv.x), ex2c(xv.y));
+              const float2 pv = make_float2(ex2c(xv.x), ex2c(xv.y));
               rs = add2(rs, pv);
               pk[b * 8 + i / 2] = P8Io<__half>::pack(pv.x, pv.y);
             }
@@ -867,11 +866,11 @@ int launch_expand(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int blocks
                    static_cast<float4*>(a.ws_par), err);
 }
 
-template <typename T, int D, int NQ, int POLY>
+template <typename T, int D, int NQ>
 int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                ChunkParams p, int max_q_len, int num_seqs, cudaStream_t st) {
   using Cfg = ChunkCfg<D, NQ>;
-  constexpr auto kern = p8_chunk_kernel<T, D, NQ, POLY>;
+  constexpr auto kern = p8_chunk_kernel<T, D, NQ>;
   const int per_cta = NQ * (kT / p.G);
   p.row_ctas = (max_q_len + per_cta - 1) / per_cta;
   p.num_seqs = num_seqs;
@@ -923,15 +922,8 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
   p.row_ctas = 0;
   p.err = err;
   const bool mass = a.mass_out != nullptr;
-  // the cubic's error (8e-5) is below half an ulp of f16's P, not below what the weights
-  // are held to
-  const bool poly = !mass;
-  if (a.chunk_nq == 2)
-    rc = poly ? launch_fwd<T, D, 2, 2>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st)
-              : launch_fwd<T, D, 2, 0>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st);
-  else
-    rc = poly ? launch_fwd<T, D, 1, 2>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st)
-              : launch_fwd<T, D, 1, 0>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st);
+  rc = a.chunk_nq == 2 ? launch_fwd<T, D, 2>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st)
+                       : launch_fwd<T, D, 1>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st);
   if (rc) return rc;
   if (p.splits > 1) {
     rc = p8_combine(a, c.D, st);
