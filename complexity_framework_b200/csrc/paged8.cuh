@@ -77,25 +77,22 @@ __device__ __forceinline__ void p8_to_float(uint32_t w, float* f) {
   f[3] = b.y;
 }
 
-// Four scaled values (|f| <= levels up to rounding) to codes, to nearest, ties to even.
-// A NaN gives code 0: its block's scale is not finite, so its value reads as NaN anyway.
+// Four scaled values, finite and |f| <= levels up to rounding, to codes: to nearest, ties to
+// even.  int8 rounds in the adder: f + 1.5 * 2^23 has the integer in its low byte.  (The
+// conversion instruction runs at an eighth of the adder's rate, and an append would wait on it.)
 template <int FMT>
 __device__ __forceinline__ uint32_t p8_from_float(const float* f) {
   if constexpr (FMT == kP8Int8) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = max(-127, min(127, __float2int_rn(f[i] == f[i] ? f[i] : 0.f)));
-      r |= (static_cast<uint32_t>(c) & 0xffu) << (8 * i);
-    }
-    return r;
+    constexpr float kRound = 12582912.f;
+    const uint32_t a = __float_as_uint(__fadd_rn(f[0], kRound));
+    const uint32_t b = __float_as_uint(__fadd_rn(f[1], kRound));
+    const uint32_t c = __float_as_uint(__fadd_rn(f[2], kRound));
+    const uint32_t d = __float_as_uint(__fadd_rn(f[3], kRound));
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
   } else {
-    float g[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = f[i] == f[i] ? f[i] : 0.f;
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(g[0], g[1]), __NV_SATFINITE,
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE,
                                                  __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(g[2], g[3]), __NV_SATFINITE,
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE,
                                                  __NV_E4M3);
     return lo | (hi << 16);
   }
@@ -139,15 +136,17 @@ int p8_opt_in(int smem) {
   return 0;
 }
 
-// Physical page of a logical one; an entry outside the pool is reported and read as page 0.
-__device__ __forceinline__ int64_t p8_page(const int32_t* row, int i, int64_t num_pages, int* err,
-                                           int site) {
-  const int p = __ldg(row + i);
+// A page id read from a table; one outside the pool is reported and read as page 0.
+__device__ __forceinline__ int64_t p8_checked(int p, int64_t num_pages, int* err, int site) {
   if (static_cast<uint32_t>(p) >= static_cast<uint64_t>(num_pages)) {
     report_error(err, kErrBounds, site);
     return 0;
   }
   return p;
+}
+__device__ __forceinline__ int64_t p8_page(const int32_t* row, int i, int64_t num_pages, int* err,
+                                           int site) {
+  return p8_checked(__ldg(row + i), num_pages, err, site);
 }
 
 // Cached length of a sequence, held to what its page-table row can describe.

@@ -266,10 +266,7 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
   // and reciprocal of V's, the reciprocal negative for a block of zeros).
   float ks_i = 0.f, lv_i = 0.f, rv_i = 1.f;
   if (lane < count) {
-    if (static_cast<uint32_t>(id) >= static_cast<uint64_t>(p.c.num_pages)) {
-      report_error(p.err, kErrBounds, 73);  // not followed: page 0 is read instead
-      id = 0;
-    }
+    id = static_cast<int>(p8_checked(id, p.c.num_pages, p.err, 73));
     id = id * p.c.Hkv + h;
     const float2 sc = __ldg(reinterpret_cast<const float2*>(p.c.scales) + id);
     const bool tiny = sc.y < kTinyScale, fine = sc.y <= 3.402823466e38f;
@@ -436,14 +433,11 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
         for (int e = 0; e < 4; ++e) {
           const int i = e & 1;  // row 2 t + i, token g + 8 (e / 2)
           const float y = fmaf(s[u][nb][e], qs[nb][i], qb[nb][i]);
-          if constexpr (MASS) {
-            const float x = y * ks;
+          // one rounding either way, so that the output does not depend on the weights' being kept
+          s[u][nb][e] = fmaf(y, ks, lv[u]);
+          if constexpr (MASS)
             if (lim[nb][i] > 0 && (u == 0 || j + u < count))
-              sp[(nb * 8 + i) * Lp + key0[u] + 8 * (e >> 1)] = x;
-            s[u][nb][e] = x + lv[u];
-          } else {
-            s[u][nb][e] = fmaf(y, ks, lv[u]);
-          }
+              sp[(nb * 8 + i) * Lp + key0[u] + 8 * (e >> 1)] = y * ks;
         }
     }
     if (edge) {

@@ -19,38 +19,35 @@ constexpr unsigned kFull = 0xffffffffu;
 // loads, all issued before the reduction.  max|x| is taken on the bit patterns, which
 // order as the magnitudes do and let a NaN through to the scale.
 //
-// Blocks are enumerated without reading lengths on the host: sequence i's blocks either
-// start at item i * per_seq (per_seq bounds the blocks a chunk of max_q_len touches), or,
-// when chunks are uneven, at floor(cu_q[i] / 16) + 2 i, which leaves room for each
-// sequence's at most floor(q / 16) + 2 blocks; the host takes the smaller enumeration.
+// Blocks are enumerated without reading lengths on the host: sequence i either has a row of
+// the grid, as long as the blocks a chunk of max_q_len can touch, or, when chunks are uneven,
+// the items from floor(cu_q[i] / 16) + 2 i on, which leaves room for its at most
+// floor(q / 16) + 2 blocks; the host takes the smaller enumeration.
+// A block with a value that is not finite has a scale that is not, and codes of 0.
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256, 3)
     p8_append_kernel(P8Cache c, P8Seqs s, const T* __restrict__ k, int64_t k_stride,
-                     const T* __restrict__ v, int64_t v_stride, int64_t N, int64_t units,
+                     const T* __restrict__ v, int64_t v_stride, int64_t N, unsigned units,
                      int per_seq, int* err) {
   constexpr int CH = D / 8;        // lanes of a row
   constexpr int RPL = 32 / CH;     // rows of one load
   constexpr int NL = kP8Page / RPL;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const unsigned unit = blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
   p8_grid_wait();
   if (unit >= units) return;
   const int hx = static_cast<int>(unit % (2 * c.Hkv));
-  const int64_t item = unit / (2 * c.Hkv);
-  int seq;
-  int64_t j;
-  if (per_seq > 0) {
-    seq = static_cast<int>(item / per_seq);
-    j = item % per_seq;
-  } else {
+  int64_t j = unit / (2 * c.Hkv);
+  int seq = blockIdx.y;
+  if (per_seq == 0) {
     int lo = 0, hi = s.num_seqs - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (__ldg(s.cu_q + mid) / kP8Page + 2 * static_cast<int64_t>(mid) <= item) lo = mid;
+      if (__ldg(s.cu_q + mid) / kP8Page + 2 * static_cast<int64_t>(mid) <= j) lo = mid;
       else hi = mid - 1;
     }
     seq = lo;
-    j = item - (__ldg(s.cu_q + seq) / kP8Page + 2 * static_cast<int64_t>(seq));
+    j -= __ldg(s.cu_q + seq) / kP8Page + 2 * static_cast<int64_t>(seq);
   }
   const int row0 = __ldg(s.cu_q + seq);
   const int q_len = __ldg(s.cu_q + seq + 1) - row0;
@@ -102,7 +99,8 @@ __global__ void __launch_bounds__(256, 3)
   top = __reduce_max_sync(kFull, top);
   const float sn = __fdiv_rn(__uint_as_float(top), p8_levels<FMT>());
   const float sc = (sn > s0 || sn != sn) ? sn : s0;
-  const float inv = sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
+  const bool fine = sc <= 3.402823466e38f;
+  const float inv = fine && sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
   const bool tiny = isinf(inv);  // a subnormal scale: divide instead
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
@@ -116,11 +114,12 @@ __global__ void __launch_bounds__(256, 3)
       f[2 * e] = tiny ? __fdiv_rn(p.x, sc) : p.x * inv;
       f[2 * e + 1] = tiny ? __fdiv_rn(p.y, sc) : p.y * inv;
     }
-    *reinterpret_cast<uint2*>(codes + t * D + col) =
-        make_uint2(p8_from_float<FMT>(f), p8_from_float<FMT>(f + 4));
+    uint2 w2 = make_uint2(p8_from_float<FMT>(f), p8_from_float<FMT>(f + 4));
+    if (!fine) w2 = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(codes + t * D + col) = w2;
   }
   if (lo > 0 && sc != s0) {  // the scale grew: the older codes follow it
-    const float ratio = sc > 0.f ? __fdiv_rn(s0, sc) : 0.f;
+    const float ratio = fine && sc > 0.f ? __fdiv_rn(s0, sc) : 0.f;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int t = i * RPL + r;
@@ -143,21 +142,18 @@ __global__ void __launch_bounds__(256, 3)
 // 16-byte stores are dense; the values are rounded once to the output's type.
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256)
-    p8_read_kernel(P8Cache c, P8Seqs s, int64_t units, T* __restrict__ k_out,
+    p8_read_kernel(P8Cache c, P8Seqs s, unsigned units, T* __restrict__ k_out,
                    T* __restrict__ v_out, int* err) {
   constexpr int NC = kP8Page * D / 8 / 32;  // 8-code pieces of a lane
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const unsigned unit = blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  const int x = unit & 1, h = (unit >> 1) % c.Hkv, blk = (unit >> 1) / c.Hkv;
+  const int seq = blockIdx.y;
+  const int64_t layer = blockIdx.z;
   p8_grid_wait();
   if (unit >= units) return;
-  const int x = static_cast<int>(unit & 1);
-  int64_t u = unit >> 1;
-  const int h = static_cast<int>(u % c.Hkv);
-  u /= c.Hkv;
-  const int blk = static_cast<int>(u % s.max_pages);
-  u /= s.max_pages;
-  const int seq = static_cast<int>(u % s.num_seqs);
-  const int64_t layer = u / s.num_seqs;
+  // the table's entry beside the length that says whether it counts
+  const int entry = __ldg(s.table + static_cast<int64_t>(seq) * s.max_pages + blk);
   const int kv = p8_len(s.kv_lens, seq, s.max_pages, err, 63);
   const int live = min(kv - blk * kP8Page, kP8Page);  // tokens of the block, may be <= 0
   const int64_t Lp = static_cast<int64_t>(s.max_pages) * kP8Page;
@@ -166,8 +162,7 @@ __global__ void __launch_bounds__(256)
   const uint8_t* src = nullptr;
   float sc = 0.f;
   if (live > 0) {
-    const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages, blk,
-                                 c.num_pages, err, 64);
+    const int64_t page = p8_checked(entry, c.num_pages, err, 64);
     const int64_t ph = ((layer * c.num_pages + page) * c.Hkv + h) * 2 + x;
     sc = __ldg(c.scales + ph);
     src = c.codes + ph * (kP8Page * D);
@@ -196,9 +191,12 @@ __global__ void __launch_bounds__(256)
 // ----------------------------------------------------------------------------- evict
 // Select: one CTA per (layer, sequence, head) finds the k = budget - recent largest of
 // the n = len - recent older masses by a radix select on order-preserving 32-bit keys
-// (four 8-bit digits, each a histogram in shared memory), then writes the kept indices
-// in order: everything above the k-th key, and of its equals the lowest indices.
+// (digits of 11, 11 and 10 bits, each a histogram in shared memory; it ends early once a
+// digit's keys are all kept), then writes the kept indices in order: everything above the
+// k-th key, and of its equals the lowest indices.  The first digit covers the exponent and
+// two bits more: masses crowd into few exponents, and the histogram's atomics would queue.
 constexpr int kSelThreads = 256;
+constexpr int kSelBins = 2048;
 constexpr int kSelKeys = 40 * 1024;  // keys held in shared memory; longer rows re-read global
 
 __device__ __forceinline__ uint32_t mass_key(float m) {
@@ -206,16 +204,40 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+// Exclusive sums over the CTA's threads of two counts, in thread order.
+__device__ __forceinline__ int2 sums_before(int2 v, int2 (&s_part)[kSelThreads / 32]) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int2 inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(kFull, inc.x, o), b = __shfl_up_sync(kFull, inc.y, o);
+    if (lane >= o) {
+      inc.x += a;
+      inc.y += b;
+    }
+  }
+  if (lane == 31) s_part[warp] = inc;
+  __syncthreads();
+  int2 r = make_int2(inc.x - v.x, inc.y - v.y);
+#pragma unroll
+  for (int w = 0; w < kSelThreads / 32; ++w)
+    if (w < warp) {
+      r.x += s_part[w].x;
+      r.y += s_part[w].y;
+    }
+  return r;
+}
+
 __global__ void __launch_bounds__(kSelThreads)
     p8_select_kernel(P8Cache c, P8Seqs s, const float* __restrict__ mass, int budget, int recent,
                      int32_t* __restrict__ keep, int cap, int* err) {
   extern __shared__ uint32_t s_keys[];
-  __shared__ int s_hist[256];
-  __shared__ int s_scan[kSelThreads / 32][2];
-  __shared__ int s_digit, s_need;
+  __shared__ int s_hist[kSelBins];
+  __shared__ int2 s_part[2][kSelThreads / 32];
+  __shared__ int s_digit, s_need, s_count;
   const int h = blockIdx.x, seq = blockIdx.y;
   const int64_t layer = blockIdx.z;
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int tid = threadIdx.x;
   p8_grid_wait();
   const int len = p8_len(s.kv_lens, seq, s.max_pages, err, 65);
   int32_t* row = keep + ((layer * s.num_seqs + seq) * c.Hkv + h) * budget;
@@ -224,6 +246,8 @@ __global__ void __launch_bounds__(kSelThreads)
     return;
   }
   const int n = len - recent, k = budget - recent;
+  for (int i = tid; i < recent; i += kSelThreads) row[k + i] = n + i;
+  if (k == 0) return;
   const int32_t* table = s.table + static_cast<int64_t>(seq) * s.max_pages;
   const float* m = mass + layer * c.num_pages * c.Hkv * kP8Page;
   auto fetch = [&](int i) {
@@ -231,83 +255,71 @@ __global__ void __launch_bounds__(kSelThreads)
     return mass_key(__ldg(m + (page * c.Hkv + h) * kP8Page + i % kP8Page));
   };
   const bool held = n <= cap;
-  if (held)
+  if (held) {
+#pragma unroll 4
     for (int i = tid; i < n; i += kSelThreads) s_keys[i] = fetch(i);
+  }
   auto key = [&](int i) { return held ? s_keys[i] : fetch(i); };
   uint32_t prefix = 0, mask = 0;
   int need = k;  // of the keys that match the prefix, how many are kept
-  if (k > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelThreads) s_hist[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kSelThreads) {
-        const uint32_t u = key(i);
-        if ((u & mask) == prefix) atomicAdd(&s_hist[(u >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (warp == 0) {  // the digit whose suffix sum first reaches `need`
-        int cnt[8], sum = 0;
+  int shift = 32;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          cnt[i] = s_hist[255 - (lane * 8 + i)];
-          sum += cnt[i];
-        }
-        int inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(kFull, inc, o);
-          if (lane >= o) inc += y;
-        }
-        int before = inc - sum;
-        if (before < need && inc >= need) {
-          int i = 0;
-          while (before + cnt[i] < need) before += cnt[i++];
-          s_digit = 255 - (lane * 8 + i);
-          s_need = need - before;
-        }
-      }
-      __syncthreads();
-      prefix |= static_cast<uint32_t>(s_digit) << shift;
-      mask |= 0xffu << shift;
-      need = s_need;
-    }
-    // ordered write: each thread owns a contiguous stretch of the older tokens
-    const int per = (n + kSelThreads - 1) / kSelThreads;
-    const int a = min(n, tid * per), b = min(n, a + per);
-    int gt = 0, eq = 0;
-    for (int i = a; i < b; ++i) {
+  for (int digit = 0; digit < 3; ++digit) {
+    const int bits = digit < 2 ? 11 : 10, bins = 1 << bits;
+    shift -= bits;
+    for (int i = tid; i < bins; i += kSelThreads) s_hist[i] = 0;
+    __syncthreads();  // also: the keys are there
+    for (int i = tid; i < n; i += kSelThreads) {
       const uint32_t u = key(i);
-      gt += u > prefix;
-      eq += u == prefix;
-    }
-    int igt = gt, ieq = eq;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(kFull, igt, o), z = __shfl_up_sync(kFull, ieq, o);
-      if (lane >= o) {
-        igt += y;
-        ieq += z;
-      }
-    }
-    if (lane == 31) {
-      s_scan[warp][0] = igt;
-      s_scan[warp][1] = ieq;
+      if ((u & mask) == prefix) atomicAdd(&s_hist[(u >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
-    gt = igt - gt;
-    eq = ieq - eq;
-    for (int w = 0; w < warp; ++w) {
-      gt += s_scan[w][0];
-      eq += s_scan[w][1];
+    // the digit at which the count from the top first reaches `need`
+    const int each = bins / kSelThreads;
+    int cnt[8], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      cnt[i] = i < each ? s_hist[bins - 1 - (tid * each + i)] : 0;
+      sum += cnt[i];
     }
-    for (int i = a; i < b; ++i) {
-      const uint32_t u = key(i);
-      if (u > prefix || (u == prefix && eq < need)) row[gt + min(eq, need)] = i;
-      gt += u > prefix;
-      eq += u == prefix;
+    int before = sums_before(make_int2(sum, 0), s_part[digit & 1]).x;
+    if (before < need && before + sum >= need) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (before < need && before + cnt[i] >= need) {
+          s_digit = bins - 1 - (tid * each + i);
+          s_need = need - before;
+          s_count = cnt[i];
+          before = need;  // found
+        } else {
+          before += cnt[i];
+        }
     }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(s_digit) << shift;
+    mask |= static_cast<uint32_t>(bins - 1) << shift;
+    need = s_need;
+    if (s_count == need) break;  // all that match are kept
   }
-  for (int i = tid; i < recent; i += kSelThreads) row[k + i] = n + i;
+  // ordered write: each thread owns a contiguous stretch of the older tokens
+  const int per = (n + kSelThreads - 1) / kSelThreads;
+  const int a = min(n, tid * per), b = min(n, a + per);
+  int gt = 0, eq = 0;
+  for (int i = a; i < b; ++i) {
+    const uint32_t u = key(i) & mask;
+    gt += u > prefix;
+    eq += u == prefix;
+  }
+  __syncthreads();  // the partial sums of the last digit are read
+  const int2 at = sums_before(make_int2(gt, eq), s_part[0]);
+  gt = at.x;
+  eq = at.y;
+  for (int i = a; i < b; ++i) {
+    const uint32_t u = key(i) & mask;
+    if (u > prefix || (u == prefix && eq < need)) row[gt + min(eq, need)] = i;
+    gt += u > prefix;
+    eq += u == prefix;
+  }
 }
 
 // Move: one warp per (layer, sequence, head, new block).  The block's scale is the
@@ -317,20 +329,15 @@ template <int FMT, int D>
 __global__ void __launch_bounds__(256)
     p8_move_kernel(P8Cache c, P8Seqs s, float* __restrict__ mass, int layers,
                    const int32_t* __restrict__ dst_table, int dst_pages, int budget,
-                   const int32_t* __restrict__ keep, int64_t units, int* err) {
+                   const int32_t* __restrict__ keep, unsigned units, int* err) {
   constexpr int CPR = D / 16;                 // 16-code chunks of a row
   constexpr int NC = 2 * kP8Page * CPR / 32;  // chunks of a lane, K and V
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const unsigned unit = blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  const int h = unit % c.Hkv, blk = unit / c.Hkv, seq = blockIdx.y;
+  const int64_t layer = blockIdx.z;
   p8_grid_wait();
   if (unit >= units) return;
-  int64_t u = unit;
-  const int h = static_cast<int>(u % c.Hkv);
-  u /= c.Hkv;
-  const int blk = static_cast<int>(u % dst_pages);
-  u /= dst_pages;
-  const int seq = static_cast<int>(u % s.num_seqs);
-  const int64_t layer = u / s.num_seqs;
   const int len = p8_len(s.kv_lens, seq, s.max_pages, err, 67);
   const int kept = min(len, budget);
   const int live = min(kept - blk * kP8Page, kP8Page);
@@ -372,6 +379,7 @@ __global__ void __launch_bounds__(256)
     if (t < live)
       w[i] = __ldg(reinterpret_cast<const uint4*>(c.codes + ((p * 2 + x) * kP8Page + o) * D) + ch);
     ratio[i] = so == top[x] ? 1.f : __fdiv_rn(so, top[x]);
+    if (ratio[i] != ratio[i]) ratio[i] = 0.f;  // a scale that is not a number: codes of 0
   }
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
@@ -394,11 +402,11 @@ __global__ void __launch_bounds__(256)
 
 template <typename T, int FMT, int D>
 int launch_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t ks, const void* v,
-                   int64_t vs, int64_t N, int64_t items, int per_seq, int* err, cudaStream_t st) {
-  const int64_t units = items * 2 * c.Hkv;
-  return p8_launch(p8_append_kernel<T, FMT, D>, dim3(static_cast<unsigned>((units + 7) / 8)), 256,
-                   0, st, c, s, static_cast<const T*>(k), ks, static_cast<const T*>(v), vs, N,
-                   units, per_seq, err);
+                  int64_t vs, int64_t N, unsigned units, int per_seq, int* err, cudaStream_t st) {
+  return p8_launch(p8_append_kernel<T, FMT, D>,
+                   dim3((units + 7) / 8, per_seq > 0 ? s.num_seqs : 1), 256, 0, st, c, s,
+                   static_cast<const T*>(k), ks, static_cast<const T*>(v), vs, N, units, per_seq,
+                   err);
 }
 
 }  // namespace
@@ -426,11 +434,13 @@ int p8_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t k_stride
   const int64_t per_seq = (max_q_len + kP8Page - 2) / kP8Page + 1;
   const int64_t even = per_seq * s.num_seqs, uneven = N / kP8Page + 2 * s.num_seqs;
   const int64_t items = even <= uneven ? even : uneven;
-  if ((items * 2 * c.Hkv + 7) / 8 > 0x7fffffff) return -3;
   const int ps = even <= uneven ? static_cast<int>(per_seq) : 0;
+  const int64_t units = (ps ? per_seq : items) * 2 * c.Hkv;
+  if (units > 0x7fffffff) return -3;
   int rc = 0;
-#define CFB_CALL(T, F, DD) \
-  rc = launch_append<T, F, DD>(c, s, k, k_stride, v, v_stride, N, items, ps, err, stream)
+#define CFB_CALL(T, F, DD)                                                                       \
+  rc = launch_append<T, F, DD>(c, s, k, k_stride, v, v_stride, N, static_cast<unsigned>(units), ps, \
+                               err, stream)
   CFB_P8_TYPES(CFB_CALL);
 #undef CFB_CALL
   return rc ? rc : static_cast<int>(cudaGetLastError());
@@ -438,15 +448,14 @@ int p8_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t k_stride
 
 int p8_read(const P8Cache& c, const P8Seqs& s, int layers, void* k_out, void* v_out, int type,
             int* err, cudaStream_t stream) {
-  const int64_t units =
-      static_cast<int64_t>(layers) * s.num_seqs * s.max_pages * c.Hkv * 2;
-  if (units <= 0) return 0;
-  if ((units + 7) / 8 > 0x7fffffff) return -3;
-  const unsigned grid = static_cast<unsigned>((units + 7) / 8);
+  const int64_t units = static_cast<int64_t>(s.max_pages) * c.Hkv * 2;
+  if (layers <= 0 || s.num_seqs <= 0) return 0;
+  if (units > 0x7fffffff) return -3;
+  const dim3 grid(static_cast<unsigned>((units + 7) / 8), s.num_seqs, layers);
   int rc = 0;
-#define CFB_CALL(T, F, DD)                                                                      \
-  rc = p8_launch(p8_read_kernel<T, F, DD>, dim3(grid), 256, 0, stream, c, s, units,              \
-                 static_cast<T*>(k_out), static_cast<T*>(v_out), err)
+#define CFB_CALL(T, F, DD)                                                              \
+  rc = p8_launch(p8_read_kernel<T, F, DD>, grid, 256, 0, stream, c, s,                   \
+                 static_cast<unsigned>(units), static_cast<T*>(k_out), static_cast<T*>(v_out), err)
   CFB_P8_TYPES(CFB_CALL);
 #undef CFB_CALL
   return rc ? rc : static_cast<int>(cudaGetLastError());
@@ -457,9 +466,8 @@ int p8_evict(const P8Cache& c, const P8Seqs& s, float* mass, int layers, const i
              cudaStream_t stream) {
   if (s.num_seqs <= 0 || layers <= 0) return 0;
   if (s.num_seqs > 65535 || layers > 65535) return -3;
-  const int64_t units =
-      static_cast<int64_t>(layers) * s.num_seqs * dst_pages * c.Hkv;
-  if ((units + 7) / 8 > 0x7fffffff) return -3;
+  const int64_t units = static_cast<int64_t>(dst_pages) * c.Hkv;
+  if (units > 0x7fffffff) return -3;
   const int longest = s.max_pages * kP8Page;
   const int cap = longest < kSelKeys ? longest : kSelKeys;
   const int smem = cap * 4;
@@ -468,11 +476,11 @@ int p8_evict(const P8Cache& c, const P8Seqs& s, float* mass, int layers, const i
     rc = p8_launch(p8_select_kernel, dim3(c.Hkv, s.num_seqs, layers), kSelThreads, smem, stream, c,
                    s, mass, budget, recent, keep, cap, err);
   if (rc) return rc;
-  const unsigned grid = static_cast<unsigned>((units + 7) / 8);
+  const dim3 grid(static_cast<unsigned>((units + 7) / 8), s.num_seqs, layers);
   const int type = kP8Bf16;
-#define CFB_CALL(T, F, DD)                                                                      \
-  rc = p8_launch(p8_move_kernel<F, DD>, dim3(grid), 256, 0, stream, c, s, mass, layers, dst_table, \
-                 dst_pages, budget, keep, units, err)
+#define CFB_CALL(T, F, DD)                                                                  \
+  rc = p8_launch(p8_move_kernel<F, DD>, grid, 256, 0, stream, c, s, mass, layers, dst_table, \
+                 dst_pages, budget, keep, static_cast<unsigned>(units), err)
   CFB_P8_TYPES(CFB_CALL);
 #undef CFB_CALL
   return rc ? rc : static_cast<int>(cudaGetLastError());

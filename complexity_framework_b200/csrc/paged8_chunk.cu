@@ -123,20 +123,18 @@ __device__ __forceinline__ void tmem_ready32(uint32_t (&r)[32]) {
 // the block does not raise the bound of w.
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256)
-    p8_expand_kernel(P8Cache c, P8Seqs s, int blocks, int64_t units, float scale_log2,
+    p8_expand_kernel(P8Cache c, P8Seqs s, int blocks, unsigned units, float scale_log2,
                      T* __restrict__ k_ws, __half* __restrict__ v_ws, float4* __restrict__ par,
                      int* err) {
   constexpr int NC = kP8Page * D / 8 / 32;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const unsigned unit = blockIdx.x * 8 + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  const int x = unit & 1, h = (unit >> 1) % c.Hkv, blk = (unit >> 1) / c.Hkv;
+  const int seq = blockIdx.y;
   p8_grid_wait();
   if (unit >= units) return;
-  const int x = static_cast<int>(unit & 1);
-  int64_t u = unit >> 1;
-  const int h = static_cast<int>(u % c.Hkv);
-  u /= c.Hkv;
-  const int blk = static_cast<int>(u % blocks);
-  const int seq = static_cast<int>(u / blocks);
+  const int entry = __ldg(s.table + static_cast<int64_t>(seq) * s.max_pages +
+                          min(blk, s.max_pages - 1));
   const int kv = p8_len(s.kv_lens, seq, s.max_pages, err, 80);
   if (blk * kP8Page >= (kv + kT - 1) / kT * kT) return;
   const int64_t sh = static_cast<int64_t>(seq) * c.Hkv + h;
@@ -147,8 +145,7 @@ __global__ void __launch_bounds__(256)
   const uint8_t* src = nullptr;
   float4 f = make_float4(scale_log2, -24.f, 16777216.f, 0.f);
   if (live > 0) {
-    const int64_t page = p8_page(s.table + static_cast<int64_t>(seq) * s.max_pages, blk,
-                                 c.num_pages, err, 81);
+    const int64_t page = p8_checked(entry, c.num_pages, err, 81);
     const int64_t ph = page * c.Hkv + h;
     const float2 sc = __ldg(reinterpret_cast<const float2*>(c.scales) + ph);
     const bool fine = fabsf(sc.y) <= 3.402823466e38f;
@@ -858,10 +855,11 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
 template <typename T, int FMT, int D>
 int launch_expand(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int blocks, int* err,
                   cudaStream_t st) {
-  const int64_t units = static_cast<int64_t>(s.num_seqs) * blocks * c.Hkv * 2;
-  if ((units + 7) / 8 > 0x7fffffff) return -3;
-  return p8_launch(p8_expand_kernel<T, FMT, D>, dim3(static_cast<unsigned>((units + 7) / 8)), 256,
-                   0, st, c, s, blocks, units, a.scale * 1.4426950408889634f,
+  const int64_t units = static_cast<int64_t>(blocks) * c.Hkv * 2;
+  if (units > 0x7fffffff) return -3;
+  return p8_launch(p8_expand_kernel<T, FMT, D>,
+                   dim3(static_cast<unsigned>((units + 7) / 8), s.num_seqs), 256, 0, st, c, s,
+                   blocks, static_cast<unsigned>(units), a.scale * 1.4426950408889634f,
                    static_cast<T*>(a.ws_k), static_cast<__half*>(a.ws_v),
                    static_cast<float4*>(a.ws_par), err);
 }
