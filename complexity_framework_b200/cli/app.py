@@ -72,12 +72,18 @@ def cmd_train(argv: List[str]) -> None:
     TrainRunner().main(argv)
 
 
+def _engine_config(a):
+    from ..inference.engine import InferenceConfig
+
+    return InferenceConfig(kv_cache_dtype=a.kv_cache_dtype, kv_evict_budget=a.kv_evict_budget)
+
+
 def cmd_generate(a) -> None:
     from ..inference.engine import GenerationConfig, InferenceEngine
 
     dev = _device(a.device)
     model, tok = _load_model(a.model, dev), _tokenizer(a.tokenizer)
-    eng = InferenceEngine(model)
+    eng = InferenceEngine(model, _engine_config(a))
     gen = GenerationConfig(max_new_tokens=a.max_new_tokens, do_sample=a.temperature > 0,
                            temperature=a.temperature or 1.0, top_p=a.top_p, top_k=a.top_k,
                            eos_token_id=tok.eos_token_id, seed=a.seed)
@@ -96,7 +102,7 @@ def cmd_chat(a) -> None:
 
     dev = _device(a.device)
     model, tok = _load_model(a.model, dev), _tokenizer(a.tokenizer)
-    eng, tpl = InferenceEngine(model), ChatTemplate(a.format)
+    eng, tpl = InferenceEngine(model, _engine_config(a)), ChatTemplate(a.format)
     msgs = [Message("system", a.system)] if a.system else []
     for line in sys.stdin:
         msgs.append(Message("user", line.strip()))
@@ -116,7 +122,7 @@ def cmd_bench_infer(a) -> None:
     V = model.config.vocab_size
     g = torch.Generator().manual_seed(0)
     prompts = [torch.randint(0, V, (a.prompt_len,), generator=g).tolist() for _ in range(a.batch)]
-    eng = InferenceEngine(model)
+    eng = InferenceEngine(model, _engine_config(a))
     gen = GenerationConfig(max_new_tokens=a.new_tokens)
     eng.generate_tokens(prompts[:1], GenerationConfig(max_new_tokens=2))  # warm-up
     if dev.type == "cuda":
@@ -141,7 +147,7 @@ def cmd_serve(a) -> None:
 
     dev = _device(a.device)
     serve(_load_model(a.model, dev), _tokenizer(a.tokenizer), host=a.host, port=a.port,
-          model_name=Path(a.model).name)
+          config=_engine_config(a), model_name=Path(a.model).name)
 
 
 def cmd_convert(a) -> None:
@@ -332,8 +338,15 @@ def build_parser() -> argparse.ArgumentParser:
         p.add_argument("--tokenizer", default=None)
         p.add_argument("--device", default=None)
 
+    def cache_args(p):
+        p.add_argument("--kv-cache-dtype", choices=["int8", "fp8"], default=None,
+                       help="hold the KV cache in 8 bits")
+        p.add_argument("--kv-evict-budget", type=int, default=0,
+                       help="cached tokens kept for a sequence (8-bit cache; 0: all)")
+
     g = sub.add_parser("generate")
     model_args(g)
+    cache_args(g)
     g.add_argument("--prompt", required=True)
     g.add_argument("--max-new-tokens", type=int, default=64)
     g.add_argument("--temperature", type=float, default=0.0)
@@ -343,16 +356,19 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--stream", action="store_true")
     c = sub.add_parser("chat")
     model_args(c)
+    cache_args(c)
     c.add_argument("--system", default=None)
     c.add_argument("--format", default="complexity", choices=["complexity", "chatml", "llama"])
     c.add_argument("--max-new-tokens", type=int, default=256)
     b = sub.add_parser("bench-infer")
     model_args(b)
+    cache_args(b)
     b.add_argument("--batch", type=int, default=32)
     b.add_argument("--prompt-len", type=int, default=512)
     b.add_argument("--new-tokens", type=int, default=128)
     s = sub.add_parser("serve")
     model_args(s)
+    cache_args(s)
     s.add_argument("--host", default="127.0.0.1")
     s.add_argument("--port", type=int, default=8000)
     cv = sub.add_parser("convert")

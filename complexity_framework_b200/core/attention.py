@@ -344,11 +344,12 @@ class GroupedQueryAttention(nn.Module):
             cos_h, sin_h = self.rotary_emb.tables(cache.max_position + 1, x.device)
             q = torch.empty(N, self.num_heads, self.head_dim, device=x.device, dtype=x.dtype)
             norm = self.use_qk_norm
+            slots, k, v = cache.rope_target(layer_idx)
             require().paged_qkv_rope(kqv.view(N, -1), self.q_norm.weight if norm else None,
                                      self.k_norm.weight if norm else None, cos_h, sin_h,
-                                     cache.positions, cache.slots, q, cache.pool.k[layer_idx],
-                                     cache.pool.v[layer_idx],
+                                     cache.positions, slots, q, k, v,
                                      float(self.q_norm.eps) if norm else 0.0)
+            cache.rope_done(layer_idx, k, v)
             o = cache.attend(layer_idx, q, self.attn_scale)
             if getattr(self, "tp_group", None) is not None:
                 return self._tp_out(o.reshape(N, qd), residual, N, True)

@@ -121,7 +121,7 @@ float* mass_of(const Tensor& m, const Tensor& codes, int64_t lead, const char* n
 
 void paged8_append(const Tensor& k_in, const Tensor& v_in, const Tensor& codes, const Tensor& scales,
                    const Tensor& table, const Tensor& cu_q, const Tensor& kv_lens,
-                   int64_t max_q_len) {
+                   int64_t max_q_len, const c10::optional<Tensor>& mass) {
   const cfb::P8Cache c = cache_of(codes, scales, false);
   const cfb::P8Seqs s = seqs_of(codes, table, kv_lens, cu_q);
   const Tensor k = rows_of(k_in, codes, c.D, "k"), v = rows_of(v_in, codes, c.D, "v");
@@ -130,10 +130,11 @@ void paged8_append(const Tensor& k_in, const Tensor& v_in, const Tensor& codes, 
   TORCH_CHECK(k.scalar_type() == v.scalar_type(), "k and v must have one dtype");
   TORCH_CHECK(max_q_len >= 1 && max_q_len <= (1 << 30), "max_q_len must be positive");
   const int type = type_of(k.scalar_type(), "k and v");
+  float* m = mass.has_value() ? mass_of(*mass, codes, 0, "mass") : nullptr;
   const c10::cuda::CUDAGuard g(codes.device());
   check_rc(cfb::p8_append(c, s, k.data_ptr(), row_stride(k), v.data_ptr(), row_stride(v),
                           k.size(0),
-                          static_cast<int>(max_q_len), type, cfb_err_ptr(codes.get_device()),
+                          static_cast<int>(max_q_len), type, m, cfb_err_ptr(codes.get_device()),
                           at::cuda::getCurrentCUDAStream()),
            "paged8_append");
 }

@@ -33,8 +33,10 @@ struct P8Seqs {
 };
 
 // Quantises the new tokens' k, v [N, Hkv, D] (row strides in elements) into their blocks.
+// Their mass (where there is one) becomes 0.
 int p8_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t k_stride, const void* v,
-              int64_t v_stride, int64_t N, int max_q_len, int type, int* err, cudaStream_t stream);
+              int64_t v_stride, int64_t N, int max_q_len, int type, float* mass, int* err,
+              cudaStream_t stream);
 
 // k_out, v_out [layers, S, Hkv, max_pages * 16, D]: the cached values, 0 past kv_lens.
 int p8_read(const P8Cache& c, const P8Seqs& s, int layers, void* k_out, void* v_out, int type,

@@ -28,7 +28,7 @@ template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256, 3)
     p8_append_kernel(P8Cache c, P8Seqs s, const T* __restrict__ k, int64_t k_stride,
                      const T* __restrict__ v, int64_t v_stride, int64_t N, unsigned units,
-                     int per_seq, int* err) {
+                     int per_seq, float* __restrict__ mass, int* err) {
   constexpr int CH = D / 8;        // lanes of a row
   constexpr int RPL = 32 / CH;     // rows of one load
   constexpr int NL = kP8Page / RPL;
@@ -135,6 +135,8 @@ __global__ void __launch_bounds__(256, 3)
     }
   }
   if (lane == 0 && (sc != s0 || lo == 0)) *scale = sc;
+  if (mass != nullptr && x == 0 && lane >= lo && lane < hi)
+    mass[(page * c.Hkv + h) * kP8Page + lane] = 0.f;
 }
 
 // ------------------------------------------------------------------------------ read
@@ -402,11 +404,12 @@ __global__ void __launch_bounds__(256)
 
 template <typename T, int FMT, int D>
 int launch_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t ks, const void* v,
-                  int64_t vs, int64_t N, unsigned units, int per_seq, int* err, cudaStream_t st) {
+                  int64_t vs, int64_t N, unsigned units, int per_seq, float* mass, int* err,
+                  cudaStream_t st) {
   return p8_launch(p8_append_kernel<T, FMT, D>,
                    dim3((units + 7) / 8, per_seq > 0 ? s.num_seqs : 1), 256, 0, st, c, s,
                    static_cast<const T*>(k), ks, static_cast<const T*>(v), vs, N, units, per_seq,
-                   err);
+                   mass, err);
 }
 
 }  // namespace
@@ -428,7 +431,7 @@ int launch_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t ks, 
   } while (0)
 
 int p8_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t k_stride, const void* v,
-              int64_t v_stride, int64_t N, int max_q_len, int type, int* err,
+              int64_t v_stride, int64_t N, int max_q_len, int type, float* mass, int* err,
               cudaStream_t stream) {
   if (N <= 0 || s.num_seqs <= 0) return 0;
   const int64_t per_seq = (max_q_len + kP8Page - 2) / kP8Page + 1;
@@ -440,7 +443,7 @@ int p8_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t k_stride
   int rc = 0;
 #define CFB_CALL(T, F, DD)                                                                       \
   rc = launch_append<T, F, DD>(c, s, k, k_stride, v, v_stride, N, static_cast<unsigned>(units), ps, \
-                               err, stream)
+                               mass, err, stream)
   CFB_P8_TYPES(CFB_CALL);
 #undef CFB_CALL
   return rc ? rc : static_cast<int>(cudaGetLastError());

@@ -5,12 +5,14 @@ from .engine import (DecodingStrategy, GenerationConfig, InferenceConfig, Infere
 from .decoding import (LayerSkipDraft, SlidingWindowCache, SpeculativeDecoder, SpeculativeStats,
                        beam_search, paged_logits)
 from .paged import KVCache, OutOfPages, PagedBatch, PagePool, SeqChunk
+from .paged8 import Paged8Batch, Paged8Pool, StaticDecode8Batch
 from . import chat_template  # noqa: F401  (template contract: inference.chat_template)
 
 PagedKVCache = PagePool
 
 __all__ = ["AsyncBatcher", "BatchConfig", "ContinuousBatcher", "DecodingStrategy",
            "GenerationConfig", "InferenceConfig", "InferenceEngine", "KVCache", "OutOfPages",
-           "PagedBatch", "PagedKVCache", "PagePool", "Request", "RequestStatus", "SeqChunk",
+           "Paged8Batch", "Paged8Pool", "PagedBatch", "PagedKVCache", "PagePool", "Request", "RequestStatus", "SeqChunk",
            "forward_paged", "sample_next", "LayerSkipDraft", "SlidingWindowCache",
-           "SpeculativeDecoder", "SpeculativeStats", "beam_search", "paged_logits"]
+           "SpeculativeDecoder", "SpeculativeStats", "StaticDecode8Batch", "beam_search",
+           "paged_logits"]

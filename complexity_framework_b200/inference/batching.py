@@ -55,6 +55,8 @@ class BatchConfig:
     prefill_chunk_size: int = 512
     dynamic_batching: bool = True
     timeout_seconds: float = 60.0
+    kv_cache_dtype: Optional[str] = None   # see InferenceConfig
+    kv_evict_budget: int = 0
 
 
 class ContinuousBatcher:
@@ -63,7 +65,9 @@ class ContinuousBatcher:
         icfg = InferenceConfig(max_cache_length=self.config.max_sequence_length,
                                max_batch_size=self.config.max_batch_size, page_size=page_size,
                                max_tokens_per_step=self.config.max_tokens_per_batch or 8192,
-                               prefill_chunk_size=self.config.prefill_chunk_size)
+                               prefill_chunk_size=self.config.prefill_chunk_size,
+                               kv_cache_dtype=self.config.kv_cache_dtype,
+                               kv_evict_budget=self.config.kv_evict_budget)
         self.engine = InferenceEngine(model, icfg)
         self.requests: Dict[str, Request] = {}
         self._eng_ids: Dict[int, str] = {}

@@ -23,7 +23,8 @@ from typing import Dict, Iterator, List, Optional, Sequence, Union
 
 import torch
 
-from .paged import PagedBatch, PagePool, SeqChunk
+from .paged import OutOfPages, PagedBatch, PagePool, SeqChunk
+from .paged8 import Paged8Pool
 
 
 class DecodingStrategy(Enum):
@@ -74,6 +75,14 @@ class InferenceConfig:
     # padded batch size (CUDA only)
     cuda_graph_decode: bool = True
     decode_graph_buckets: Sequence[int] = (1, 2, 4, 8, 16, 32, 64, 128, 256)
+    # "int8" or "fp8": keys and values in 8 bits (``inference.paged8``); None: the model's dtype
+    kv_cache_dtype: Optional[str] = None
+    # with an 8-bit cache: cut a sequence that holds ``kv_evict_slack`` tokens more than
+    # ``kv_evict_budget`` to that budget, keeping the last ``kv_evict_recent`` tokens and
+    # those that received the most attention; 0: keep everything
+    kv_evict_budget: int = 0
+    kv_evict_recent: int = 64
+    kv_evict_slack: int = 256
 
 
 @dataclass
@@ -155,8 +164,20 @@ class InferenceEngine:
         # KV heads held by this rank (fewer than the config's under tensor parallelism)
         kv_heads = getattr(getattr(model.layers[0], "self_attn", None), "num_kv_heads",
                            mc.num_key_value_heads)
-        self.pool = PagePool(mc.num_hidden_layers, kv_heads, mc.head_dim, pages,
-                             self.config.page_size, dtype=self.dtype, device=self.device)
+        cfg = self.config
+        if cfg.kv_evict_budget and cfg.kv_cache_dtype is None:
+            raise ValueError("kv_evict_budget needs an 8-bit cache (kv_cache_dtype)")
+        if cfg.kv_evict_budget < 0 or (cfg.kv_evict_budget and not (
+                0 <= cfg.kv_evict_recent <= cfg.kv_evict_budget and cfg.kv_evict_slack >= 1)):
+            raise ValueError("need 0 <= kv_evict_recent <= kv_evict_budget and a positive slack")
+        if cfg.kv_cache_dtype is None:
+            self.pool = PagePool(mc.num_hidden_layers, kv_heads, mc.head_dim, pages,
+                                 cfg.page_size, dtype=self.dtype, device=self.device)
+        else:
+            self.pool = Paged8Pool(mc.num_hidden_layers, kv_heads, mc.head_dim, pages,
+                                   cfg.page_size, dtype=self.dtype, device=self.device,
+                                   kv_dtype=cfg.kv_cache_dtype,
+                                   track_mass=cfg.kv_evict_budget > 0)
         self._ids = itertools.count()
         self._graphs: Dict[int, tuple] = {}
         self.requests: Dict[int, _Req] = {}
@@ -210,14 +231,12 @@ class InferenceEngine:
 
     def _decode_graph(self, size: int):
         """(static batch, graph, next-token buffer) for a padded decode batch."""
-        from .paged import StaticDecodeBatch
-
         got = self._graphs.get(size)
         if got is not None:
             return got
         cfg = self.config
         max_pages = -(-cfg.max_cache_length // cfg.page_size)
-        sb = StaticDecodeBatch(self.pool, size, max_pages, cfg.max_cache_length - 1)
+        sb = self.pool.static_batch(size, max_pages, cfg.max_cache_length - 1)
         sb.fill([])
 
         def body():
@@ -278,9 +297,26 @@ class InferenceEngine:
         self.stats["graph_steps"] = self.stats.get("graph_steps", 0) + 1
         return finished
 
+    def _evict(self) -> None:
+        """Cut the sequences that outgrew the cache budget.  Where no pages are free to move
+        the kept tokens to, they stay whole until some are."""
+        cfg = self.config
+        over = [s for s, n in self.pool.lengths.items()
+                if n >= cfg.kv_evict_budget + cfg.kv_evict_slack]
+        while over:
+            try:
+                self.pool.evict(over, cfg.kv_evict_budget, cfg.kv_evict_recent)
+            except OutOfPages:
+                over = over[:len(over) // 2]  # fewer at a time: the old pages come back
+                continue
+            self.stats["evictions"] = self.stats.get("evictions", 0) + len(over)
+            break
+
     @torch.no_grad()
     def step(self) -> List[int]:
         """Run one batched forward; returns ids of requests that finished."""
+        if self.config.kv_evict_budget:
+            self._evict()
         if self._graph_eligible():
             return self._graph_decode_step()
         budget = self.config.max_tokens_per_step
@@ -313,7 +349,7 @@ class InferenceEngine:
                 break
         if not chunks:
             return []
-        batch = PagedBatch(self.pool, chunks)
+        batch = self.pool.batch(chunks)
         ids = torch.tensor(toks, dtype=torch.long, device=self.device)
         hidden = forward_paged(self.model, ids, batch)
         batch.commit()

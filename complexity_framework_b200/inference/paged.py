@@ -114,6 +114,12 @@ class PagePool:
     def get_seq_len(self, seq_id: int) -> int:
         return self.lengths[seq_id]
 
+    def batch(self, chunks: Sequence["SeqChunk"]) -> "PagedBatch":
+        return PagedBatch(self, chunks)
+
+    def static_batch(self, size: int, max_pages: int, max_position: int) -> "StaticDecodeBatch":
+        return StaticDecodeBatch(self, size, max_pages, max_position)
+
 
 @dataclass
 class SeqChunk:
@@ -183,6 +189,13 @@ class PagedBatch:
         vf = P.v[layer].view(-1, P.num_kv_heads, P.head_dim)
         kf.index_copy_(0, self.slots, k.to(P.dtype))
         vf.index_copy_(0, self.slots, v.to(P.dtype))
+
+    def rope_target(self, layer: int):
+        """(slots, k, v) that the QK-norm + RoPE kernel writes the new tokens to."""
+        return self.slots, self.pool.k[layer], self.pool.v[layer]
+
+    def rope_done(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        pass  # written in place
 
     def attend(self, layer: int, q: torch.Tensor, scale: float) -> torch.Tensor:
         """Causal attention of q [N, Hq, D] over each sequence's cached keys -> [N, Hq, D]."""

@@ -50,17 +50,17 @@ def _check_cpu(codes: torch.Tensor, scales: torch.Tensor) -> None:
 
 def paged8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                   page_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, *,
-                  max_q_len: int) -> None:
+                  max_q_len: int, mass: Optional[torch.Tensor] = None) -> None:
     """Quantise the new tokens' ``k``, ``v`` ``[N, Hkv, D]`` into one layer, in place.
 
     A block's scale is the largest magnitude among its new tokens over the largest code, or
     its present scale where that is larger and the block holds older tokens; the older codes
     are rounded anew when the scale grows.  ``kv_lens`` counts the new tokens; ``max_q_len``
-    bounds the new tokens of a sequence.  A block with a value that is not finite reads as NaN
+    bounds the new tokens of a sequence; the new tokens' ``mass`` starts at 0.  A block with a value that is not finite reads as NaN
     or infinity throughout.
     """
     if codes.is_cuda:
-        require().paged8_append(k, v, codes, scales, page_table, cu_q, kv_lens, max_q_len)
+        require().paged8_append(k, v, codes, scales, page_table, cu_q, kv_lens, max_q_len, mass)
         return
     _no_grad(k, v)
     _check_cpu(codes, scales)
@@ -83,17 +83,25 @@ def paged8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales:
             older = lo - b * PAGE
             s0 = scales[page] if older else torch.zeros_like(scales[page])
             s = torch.maximum(new.abs().amax((-1, -2)) / levels, s0)
-            div = torch.where(s == 0, torch.ones_like(s), s)[..., None, None]
+            # the kernel's arithmetic, to the bit: a product with the reciprocal, or a quotient
+            # where the scale is subnormal; codes of 0 where it is 0 or not finite
+            fine = (s > 0) & torch.isfinite(s)
+            div = torch.where(fine, s, torch.ones_like(s))[..., None, None]
+            x = torch.where(torch.isinf(1 / div), new / div, new * (1 / div))
+            fine = fine[..., None, None]
             block = codes[page].float()
             if older:
-                ratio = s0[..., None, None] / div
-                block[:, :, :older] *= ratio
-            block[:, :, older:older + hi - lo] = new / div
+                ratio = torch.where(fine, s0[..., None, None] / div, 0.0)
+                block[:, :, :older] *= torch.where(s[..., None, None] == s0[..., None, None], 1.0,
+                                                   ratio)
+            block[:, :, older:older + hi - lo] = torch.where(fine, x, 0.0)
             block = torch.nan_to_num(block)
             if codes.dtype == torch.int8:
                 block = block.round().clamp(-levels, levels)
             codes[page] = block.to(codes.dtype)
             scales[page] = s
+            if mass is not None:
+                mass[page][:, older:older + hi - lo] = 0
 
 
 def paged8_read(codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor,

@@ -120,6 +120,21 @@ def test_append_strided_rows_and_steps(dtype):
     assert (x - want).abs().max() <= 16 * step
 
 
+def test_append_resets_the_new_tokens_mass():
+    L = Layer([20, 0, 33], 2, 64, INT8, "cuda", seed=3)
+    mass = torch.ones(L.num_pages, 2, PAGE, device="cuda")
+    k = torch.randn(10, 2, 64, device="cuda").bfloat16()
+    ops().paged8_append(k, k, L.codes, L.scales, L.table,
+                        torch.tensor([0, 6, 7, 10], dtype=torch.int32, device="cuda"), L.kv_lens,
+                        max_q_len=6, mass=mass)
+    clean()
+    want = torch.ones(L.num_pages, 2, PAGE)
+    for i, (lo, hi) in {0: (14, 20), 2: (30, 33)}.items():
+        for j in range(lo, hi):
+            want[int(L.table[i, j // PAGE]), :, j % PAGE] = 0
+    assert torch.equal(mass.cpu(), want)
+
+
 def test_append_extremes():
     """Zero blocks, subnormal magnitudes, infinities and NaN: other blocks are untouched."""
     hkv, d = 2, 64
