@@ -70,6 +70,7 @@ struct P8AttnPlan {
   int nb = 1;                // 8-row tiles of a CTA
   int row_tiles = 1;         // row tiles of the longest chunk
   int chunk = 1, splits = 1; // pages of a CTA, CTAs of the longest (sequence, KV head, row tile)
+  int score_rows = 4;        // rows of a token's kept scores (mass)
   int64_t n_o = 0, n_lse = 0, n_s = 0;
   int64_t floats() const { return n_o + n_lse + n_s; }
 };

@@ -66,7 +66,8 @@ struct AttnParams {
   float scale_log2;
   float* ws_o;                 // [items, splits, R, D] partial outputs (splits > 1)
   float* ws_lse;               // [items, splits, R] (splits > 1 or mass)
-  float* ws_s;                 // [items, R, max_pages * 16] scores (mass)
+  float* ws_s;                 // [items, max_pages * 16, RS] scores (mass)
+  int RS;                      // rows of a token's scores: 4 where those are enough, else R
   const float* mass_in;
   float* mass_out;
   int* err;
@@ -177,13 +178,23 @@ __device__ __forceinline__ int64_t mass_at(const AttnParams& p, const int32_t* t
   const int64_t pg = p8_page(table, j / kP8Page, p.c.num_pages, p.err, 75);
   return (pg * p.c.Hkv + h) * kP8Page + j % kP8Page;
 }
-// The weight a token receives: sum over rows of 2^(s_j - lse), in row order.  sj: the token's
-// scores, row stride Lp; r0: the first row that sees it.
-__device__ __forceinline__ float weight_of(const float* sj, int64_t Lp, int r0, int rows,
+// The weight a token receives: sum over rows of 2^(s_j - lse), in row order.  s: the token's
+// scores of the head's first row tile, the next tile's `tile` floats on; r0: the first row that
+// sees the token.
+template <int R>
+__device__ __forceinline__ float weight_of(const float* s, int64_t tile, int r0, int rows,
                                            const float* lse) {
   float w = 0.f;
-#pragma unroll 4
-  for (int r = r0; r < rows; ++r) w += ex2f(sj[r * Lp] - lse[r]);
+  for (int b = 0; b < rows; b += R, s += tile)
+#pragma unroll 2
+    for (int r = 0; r < min(R, rows - b); r += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(s + r);
+      const int at = b + r;
+      if (at >= r0) w += ex2f(x.x - lse[at]);
+      if (at + 1 >= r0 && at + 1 < rows) w += ex2f(x.y - lse[at + 1]);
+      if (at + 2 >= r0 && at + 2 < rows) w += ex2f(x.z - lse[at + 2]);
+      if (at + 3 >= r0 && at + 3 < rows) w += ex2f(x.w - lse[at + 3]);
+    }
   return w;
 }
 
@@ -356,8 +367,8 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
       qb[nb][i] = s_qb[r];
       lim[nb][i] = first_row + r < rows ? start + (first_row + r) / p.G + 1 : 0;
     }
-  float* sp = nullptr;         // scores of row 2 t, token g
-  if constexpr (MASS) sp = p.ws_s + (item * R + 2 * t) * Lp + g;
+  float* sp = nullptr;         // scores of token g, rows 2 t and on
+  if constexpr (MASS) sp = p.ws_s + (item * Lp + g) * p.RS + 2 * t;
 
   float o[NB][MT][4], ps[NB][4];
   float M[NB][2], l[NB][2];
@@ -428,17 +439,23 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
       rv[u] = __shfl_sync(kFull, rv_i, at);
       edge |= key0[u] + kP8Page > min_lim;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int nb = 0; nb < NB; ++nb) {
+        float y4[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = e & 1;  // row 2 t + i, token g + 8 (e / 2)
           const float y = fmaf(s[u][nb][e], qs[nb][i], qb[nb][i]);
           // one rounding either way, so that the output does not depend on the weights' being kept
           s[u][nb][e] = fmaf(y, ks, lv[u]);
-          if constexpr (MASS)
-            if (lim[nb][i] > 0 && (u == 0 || j + u < count))
-              sp[(nb * 8 + i) * Lp + key0[u] + 8 * (e >> 1)] = y * ks;
+          if constexpr (MASS) y4[e] = y * ks;
         }
+        if constexpr (MASS)
+          if (lim[nb][0] > 0 && (u == 0 || j + u < count)) {
+            float* to = sp + static_cast<int64_t>(key0[u]) * p.RS + nb * 8;
+            *reinterpret_cast<float2*>(to) = make_float2(y4[0], y4[1]);
+            *reinterpret_cast<float2*>(to + 8 * p.RS) = make_float2(y4[2], y4[3]);
+          }
+      }
     }
     if (edge) {
 #pragma unroll
@@ -626,8 +643,8 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
       __syncthreads();
       for (int j = threadIdx.x; j < si.kv; j += kWarps * 32) {
         const int64_t at = mass_at(p, table, h, j);
-        p.mass_out[at] = p.mass_in[at] + weight_of(p.ws_s + item * R * Lp + j, Lp,
-                                                   max(0, j - start) * p.G, rows, s_qs);
+        p.mass_out[at] = p.mass_in[at] + weight_of<R>(p.ws_s + (item * Lp + j) * p.RS, 0,
+                                                      max(0, j - start) * p.G, rows, s_qs);
       }
     }
   }
@@ -750,8 +767,9 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < kTokens / 256; ++i) {
       const int j = j0 + i * 256 + threadIdx.x;
       if (j < si.kv)
-        p.mass_out[at[i]] = before[i] + weight_of(p.ws_s + item0 * R * Lp + j, Lp,
-                                                  max(0, j - start) * p.G, si.rows, s_lse);
+        p.mass_out[at[i]] = before[i] + weight_of<R>(p.ws_s + (item0 * Lp + j) * p.RS,
+                                                     Lp * p.RS, max(0, j - start) * p.G, si.rows,
+                                                     s_lse);
     }
   }
 }
@@ -879,7 +897,8 @@ P8AttnPlan p8_attn_plan(const P8Cache& c, const P8Seqs& s, int group, int max_q_
   pl.splits = (s.max_pages + pl.chunk - 1) / pl.chunk;
   if (pl.splits > 1) pl.n_o = items * pl.splits * R * c.D;
   if (pl.splits > 1 || mass) pl.n_lse = items * pl.splits * R;
-  if (mass) pl.n_s = items * R * s.max_pages * kP8Page;
+  pl.score_rows = rows <= 4 ? 4 : R;
+  if (mass) pl.n_s = items * pl.score_rows * s.max_pages * kP8Page;
   return pl;
 }
 
@@ -907,6 +926,7 @@ int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, const P8Att
   p.ws_o = ws;
   p.ws_lse = p.ws_o + plan.n_o;
   p.ws_s = p.ws_lse + plan.n_lse;
+  p.RS = plan.score_rows;
   p.mass_in = a.mass_in;
   p.mass_out = a.mass_out;
   p.err = err;
