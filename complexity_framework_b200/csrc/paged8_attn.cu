@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
 // order of its pages.  `wpr` warps share a row (eight where there are many chunks).  With
 // mass, further CTAs of kTokens tokens of a (sequence, KV head) add the weights.  Launched so
 // that its start overlaps the end of p8_attn_kernel, which it waits for.
-constexpr int kTokens = 512;
+constexpr int kTokens = 1024;
 template <typename T, int D, int NB, bool MASS>
 __global__ void __launch_bounds__(256)
     p8_finish_kernel(const AttnParams p, int join_ctas, int wpr) {
