@@ -84,11 +84,11 @@ template <int FMT>
 __device__ __forceinline__ uint32_t p8_from_float(const float* f) {
   if constexpr (FMT == kP8Int8) {
     constexpr float kRound = 12582912.f;
-    const uint32_t a = __float_as_uint(__fadd_rn(f[0], kRound));
-    const uint32_t b = __float_as_uint(__fadd_rn(f[1], kRound));
-    const uint32_t c = __float_as_uint(__fadd_rn(f[2], kRound));
-    const uint32_t d = __float_as_uint(__fadd_rn(f[3], kRound));
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    const float2 ab = add2(make_float2(f[0], f[1]), make_float2(kRound, kRound));
+    const float2 cd = add2(make_float2(f[2], f[3]), make_float2(kRound, kRound));
+    return __byte_perm(
+        __byte_perm(__float_as_uint(ab.x), __float_as_uint(ab.y), 0x0040),
+        __byte_perm(__float_as_uint(cd.x), __float_as_uint(cd.y), 0x0040), 0x5410);
   } else {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE,
                                                  __NV_E4M3);

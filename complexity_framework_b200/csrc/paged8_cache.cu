@@ -16,8 +16,9 @@ constexpr unsigned kFull = 0xffffffffu;
 //   become round(code * s0 / s).
 // One warp owns a (block, head, K or V): the block's maximum is one warp reduction and
 // nothing is shared between warps.  A lane holds 8 values (16 bytes) of each of D / 16
-// loads, all issued before the reduction.  max|x| is taken on the bit patterns, which
-// order as the magnitudes do and let a NaN through to the scale.
+// loads, all issued before the reduction.  max|x| is taken on the 16-bit patterns, which
+// order as the magnitudes do and let a NaN through to the scale.  Long chunks are bound by
+// instructions as much as by bytes, hence the packed maxima.
 //
 // Blocks are enumerated without reading lengths on the host: sequence i either has a row of
 // the grid, as long as the blocks a chunk of max_q_len can touch, or, when chunks are uneven,
@@ -86,38 +87,43 @@ __global__ void __launch_bounds__(256, 3)
   float* scale = c.scales + ph;
   uint8_t* codes = c.codes + ph * (kP8Page * D);
   const float s0 = lo > 0 ? *scale : 0.f;
-  uint32_t top = 0;
+  // magnitudes as pairs of 16-bit patterns: three instructions for four values
+  uint32_t top2 = 0;
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const uint32_t w[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = P8Io<T>::unpack(w[e]);
-      top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-    }
+    top2 = __vimax3_u16x2(top2, in[i].x & 0x7fff7fffu, in[i].y & 0x7fff7fffu);
+    top2 = __vimax3_u16x2(top2, in[i].z & 0x7fff7fffu, in[i].w & 0x7fff7fffu);
   }
-  top = __reduce_max_sync(kFull, top);
-  const float sn = __fdiv_rn(__uint_as_float(top), p8_levels<FMT>());
+  const uint32_t top = __reduce_max_sync(kFull, max(top2 & 0xffffu, top2 >> 16));
+  const float sn = __fdiv_rn(P8Io<T>::unpack(top).x, p8_levels<FMT>());
   const float sc = (sn > s0 || sn != sn) ? sn : s0;
   const bool fine = sc <= 3.402823466e38f;
   const float inv = fine && sc > 0.f ? __fdiv_rn(1.f, sc) : 0.f;
-  const bool tiny = isinf(inv);  // a subnormal scale: divide instead
+  auto store = [&](auto scaled) {
 #pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const int t = i * RPL + r;
-    if (t < lo || t >= hi) continue;
-    const uint32_t w[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
-    float f[8];
+    for (int i = 0; i < NL; ++i) {
+      const int t = i * RPL + r;
+      if (t < lo || t >= hi) continue;
+      const uint32_t w[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+      float f[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 p = P8Io<T>::unpack(w[e]);
-      f[2 * e] = tiny ? __fdiv_rn(p.x, sc) : p.x * inv;
-      f[2 * e + 1] = tiny ? __fdiv_rn(p.y, sc) : p.y * inv;
+      for (int e = 0; e < 4; ++e) {
+        const float2 q = scaled(P8Io<T>::unpack(w[e]));
+        f[2 * e] = q.x;
+        f[2 * e + 1] = q.y;
+      }
+      *reinterpret_cast<uint2*>(codes + t * D + col) =
+          make_uint2(p8_from_float<FMT>(f), p8_from_float<FMT>(f + 4));
     }
-    uint2 w2 = make_uint2(p8_from_float<FMT>(f), p8_from_float<FMT>(f + 4));
-    if (!fine) w2 = make_uint2(0, 0);
-    *reinterpret_cast<uint2*>(codes + t * D + col) = w2;
-  }
+  };
+  if (!fine)
+    store([](float2) { return make_float2(0.f, 0.f); });
+  else if (isinf(inv))  // a subnormal scale
+    store([&](float2 x) { return make_float2(__fdiv_rn(x.x, sc), __fdiv_rn(x.y, sc)); });
+  else
+    // scalar products: a packed one would be fused with the adder's rounding, and codes would
+    // differ from the formula's at ties
+    store([&](float2 x) { return make_float2(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv)); });
   if (lo > 0 && sc != s0) {  // the scale grew: the older codes follow it
     const float ratio = fine && sc > 0.f ? __fdiv_rn(s0, sc) : 0.f;
 #pragma unroll
@@ -130,7 +136,7 @@ __global__ void __launch_bounds__(256, 3)
       p8_to_float<FMT>(old.x, f);
       p8_to_float<FMT>(old.y, f + 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= ratio;
+      for (int e = 0; e < 8; ++e) f[e] = __fmul_rn(f[e], ratio);
       *at = make_uint2(p8_from_float<FMT>(f), p8_from_float<FMT>(f + 4));
     }
   }
@@ -392,7 +398,7 @@ __global__ void __launch_bounds__(256)
         float f[4];
         p8_to_float<FMT>(q[j], f);
 #pragma unroll
-        for (int z = 0; z < 4; ++z) f[z] *= ratio[i];
+        for (int z = 0; z < 4; ++z) f[z] = __fmul_rn(f[z], ratio[i]);
         q[j] = p8_from_float<FMT>(f);
       }
     }
