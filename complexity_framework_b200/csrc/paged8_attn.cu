@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
   constexpr int PB = Cfg::PAGE_BYTES;
   constexpr int HALF = kP8Page / 2 * D;  // bytes of eight tokens
   constexpr bool kInt8 = FMT == kP8Int8;
-  constexpr int U = NB <= 2 ? 2 : 1;     // pages of an iteration: two hide each other's latency
+  constexpr int U = NB <= 3 ? 2 : 1;     // pages of an iteration: two hide each other's latency
   constexpr int AHEAD = kStages / U - 1; // groups of pages in flight beyond the current one
   extern __shared__ __align__(128) uint8_t smem[];
   float* s_o = reinterpret_cast<float*>(smem);                        // [kWarps][R][D]

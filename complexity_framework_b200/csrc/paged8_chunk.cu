@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CT
   const int row0 = __ldg(p.cu_q + seq), q_len = __ldg(p.cu_q + seq + 1) - row0;
   if (row0 < 0 || q_len < 0 || static_cast<int64_t>(row0) + q_len > p.N) {
     if (threadIdx.x == 0) report_error(p.err, kErrBounds, 82);
+    p8_grid_wait();  // no CTA ends before the kernels it follows
     return;
   }
   const int kv = p8_len(p.kv_lens, seq, p.max_pages, p.err, 83);
@@ -273,7 +274,10 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CT
   const int tok0 = rc * NQ * TT;
   if (rc == p.row_ctas - 1 && q_len > tok0 + NQ * TT && threadIdx.x == 0)
     report_error(p.err, kErrBounds, 84);   // a chunk longer than max_q_len
-  if (tok0 >= q_len) return;
+  if (tok0 >= q_len) {
+    p8_grid_wait();
+    return;
+  }
   const int start = kv - q_len;
   // key tiles of row tile x, and this split's share of them
   auto tiles_of = [&](int x) {
@@ -665,10 +669,14 @@ __global__ void __launch_bounds__(MassCfg<D>::THREADS, 1)
   const int row0 = __ldg(p.cu_q + seq), q_len = __ldg(p.cu_q + seq + 1) - row0;
   if (row0 < 0 || q_len < 0 || static_cast<int64_t>(row0) + q_len > p.N) {
     if (threadIdx.x == 0) report_error(p.err, kErrBounds, 91);
+    p8_grid_wait();
     return;
   }
   const int kv = p8_len(p.kv_lens, seq, p.max_pages, p.err, 92);
-  if (k0 >= kv) return;
+  if (k0 >= kv) {
+    p8_grid_wait();
+    return;
+  }
   const int start = kv - q_len, TT = kT / p.G;
   // this CTA's row tiles: part, part + parts, .. of those that see the keys
   const int i0 = max(0, k0 - start) / TT + part;
