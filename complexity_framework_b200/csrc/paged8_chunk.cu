@@ -12,8 +12,8 @@
 //
 // p8_chunk_kernel: one CTA per (NQ x 128 rows, KV head, sequence, KV split).  A row tile
 // packs floor(128 / G) tokens x G heads, so all the heads of a group share each K/V tile.
-//   warps 0 .. 4 NQ - 1  softmax, one row per thread: S from TMEM, running maximum with a
-//                        lazy rescale (only when it grows by more than 2^8), P back to TMEM
+//   warps 0 .. 4 NQ - 1  softmax, one row per thread: S from TMEM, P against a bound that
+//                        moves only when f16 would overflow, P back to TMEM
 //   next warp            TMA producer: Q once, then K and V tiles through rings of their own
 //   last warp            MMA issuer: S_x = Q_x K^T of the next tile, then O_x += P_x V
 // Key tiles are 64 wide so that TMEM (512 columns) holds two S of each row tile beside O:
@@ -38,7 +38,7 @@ namespace {
 
 constexpr int kT = 128;               // rows of a tile
 constexpr int kKeys = 64;             // keys of a tile of the forward kernel
-constexpr float kRescaleLog2 = 8.f;
+constexpr float kMostSum = 8192.f;    // of a row's P in a key tile: no P overflows f16
 constexpr float kTinyScale = 7.888609e-31f;  // 2^-100: blocks below it count as zeros
 
 __device__ __forceinline__ float ex2c(float x) {
@@ -474,82 +474,102 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CT
       const uint32_t t_s = tmem + (2 * x + (j & 1)) * kKeys + lane_off;
       const int kmax = lim - (j0 + j) * kKeys;  // keys of the tile that this row sees
       const bool edge = __any_sync(0xffffffffu, kmax < kKeys);
-      // One pass over S computes P against the bound in use and the row's maximum; only
-      // where the maximum turns out too far above the bound is the bound moved and the pass
-      // repeated (always in a row's first tile, seldom later).
+      // One pass over S computes P against the bound in use.  Its sum tells whether the bound
+      // still holds (f16 takes P up to 65504): only where it does not, or before a row's first
+      // key, is the row's maximum looked for, the bound moved and the pass repeated.
       uint32_t pk[kKeys / 2];
-      float sum;
+      float sum = 0.f, raw = 0.f;
       bool nan_row = false;
-      auto pass = [&](auto masked, float msub) {
-        float mx = -INFINITY;
-        float2 l2 = make_float2(0.f, 0.f);
-        uint32_t buf[kKeys / 32][32];
+      auto scores = [&](uint32_t (&buf)[kKeys / 32][32]) {
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) tmem_ld32_async(t_s + c * 32, buf[c]);
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) tmem_ready32(buf[c]);
+      };
+      auto row_max = [&](float msub) {  // relative to msub
+        uint32_t buf[kKeys / 32][32];
+        scores(buf);
+        float mx = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) {
-          uint32_t(&cur)[32] = buf[c];
+        for (int b = 0; b < BL; ++b) {
+          const float4 f = s_par[b];
+          if (f.x != f.x) continue;
+          float m = -INFINITY;
 #pragma unroll
-          for (int b = 2 * c; b < 2 * c + 2; ++b) {
-            const float4 f = s_par[b];
-            float kf = f.x, nm = f.y - msub;
-            if (kf != kf) {  // NaN for the rows that see the block, nothing for the others
-              nan_row |= b * 16 < kmax;
-              kf = 1.f;
-              nm = -INFINITY;
-            }
-            float2 rs = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const int u = (b & 1) * 16 + i;
-              float2 sv = make_float2(__uint_as_float(cur[u]), __uint_as_float(cur[u + 1]));
-              if constexpr (decltype(masked)::value) {
-                if (b * 16 + i >= kmax) sv.x = -INFINITY;
-                if (b * 16 + i + 1 >= kmax) sv.y = -INFINITY;
-              }
-              const float2 xv = fma2(sv, make_float2(kf, kf), make_float2(nm, nm));
-              mx = max3(mx, xv.x, xv.y);
-              const float2 pv = make_float2(ex2c(xv.x), ex2c(xv.y));
-              rs = add2(rs, pv);
-              pk[b * 8 + i / 2] = P8Io<__half>::pack(pv.x, pv.y);
-            }
-            l2 = fma2(rs, make_float2(f.z, f.z), l2);
-          }
+          for (int i = 0; i < 16; ++i)
+            if (b * 16 + i < kmax)
+              m = fmaxf(m, __uint_as_float(buf[b >> 1][(b & 1) * 16 + i]));
+          mx = fmaxf(mx, fmaf(m, f.x, f.y - msub));
         }
-        sum = l2.x + l2.y;
         return mx;
       };
-      for (int tries = 0; tries < 4; ++tries) {  // two are enough for finite scores
-        const float msub = m_used == -INFINITY ? 0.f : m_used;
-        // the maximum, relative to the bound
-        const float mx = edge ? pass(std::true_type{}, msub) : pass(std::false_type{}, msub);
-        const bool grow = m_used == -INFINITY ? mx > -INFINITY : mx > kRescaleLog2;
-        if (!__any_sync(0xffffffffu, grow)) break;
-        const bool had = m_used != -INFINITY;
-        const float alpha = grow && had ? ex2c(-mx) : 1.f;
-        if (grow) m_used = msub + mx;
-        l *= alpha;
-        if (__any_sync(0xffffffffu, grow && had)) {
-          // O_x holds the earlier tiles' P V, once the last of them is done
-          if (!wait_warp(&bars->o_full[x][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, p.err,
-                         kErrTimeoutTmem, 78)) {
-            ok = false;
-            break;
+      auto pass = [&](auto masked, float msub) {
+        uint32_t buf[kKeys / 32][32];
+        scores(buf);
+        float2 l2 = make_float2(0.f, 0.f), r2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int b = 0; b < BL; ++b) {
+          const float4 f = s_par[b];
+          float kf = f.x, nm = f.y - msub;
+          if (kf != kf) {  // NaN for the rows that see the block, nothing for the others
+            nan_row |= b * 16 < kmax;
+            kf = 1.f;
+            nm = -INFINITY;
           }
-          tc_fence_after();
+          float2 rs = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int c = 0; c < D; c += 16) {
-            uint32_t o[16];
-            tmem_ld16_async(t_o + c, o);
-            tmem_wait16(o);
+          for (int i = 0; i < 16; i += 2) {
+            const int u = (b & 1) * 16 + i;
+            float2 sv = make_float2(__uint_as_float(buf[b >> 1][u]),
+                                    __uint_as_float(buf[b >> 1][u + 1]));
+            if constexpr (decltype(masked)::value) {
+              if (b * 16 + i >= kmax) sv.x = -INFINITY;
+              if (b * 16 + i + 1 >= kmax) sv.y = -INFINITY;
+            }
+            const float2 xv = fma2(sv, make_float2(kf, kf), make_float2(nm, nm));
+            const float2 pv = make_float2(ex2c(xv.x), ex2c(xv.y));
+            rs = add2(rs, pv);
+            pk[b * 8 + i / 2] = P8Io<__half>::pack(pv.x, pv.y);
+          }
+          r2 = add2(r2, rs);
+          l2 = fma2(rs, make_float2(f.z, f.z), l2);
+        }
+        sum = l2.x + l2.y;
+        raw = r2.x + r2.y;
+      };
+      bool move = m_used == -INFINITY && kmax > 0;
+      for (int tries = 0; tries < 4; ++tries) {  // two are enough for finite scores
+        if (__any_sync(0xffffffffu, move)) {
+          const float mx = row_max(m_used == -INFINITY ? 0.f : m_used);
+          const bool had = m_used != -INFINITY, grow = move && mx > (had ? 0.f : -INFINITY);
+          const float alpha = grow && had ? ex2c(-mx) : 1.f;
+          if (grow) m_used = (had ? m_used : 0.f) + mx;
+          l *= alpha;
+          if (__any_sync(0xffffffffu, grow && had)) {
+            // O_x holds the earlier tiles' P V, once the last of them is done
+            if (!wait_warp(&bars->o_full[x][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, p.err,
+                           kErrTimeoutTmem, 78)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st16(t_o + c, o);
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16_async(t_o + c, o);
+              tmem_wait16(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(t_o + c, o);
+            }
           }
         }
+        const float msub = m_used == -INFINITY ? 0.f : m_used;
+        if (edge) pass(std::true_type{}, msub);
+        else pass(std::false_type{}, msub);
+        move = raw > kMostSum;
+        if (!__any_sync(0xffffffffu, move)) break;
       }
       if (!ok) break;
       l += nan_row ? __uint_as_float(0x7fc00000u) : sum;
