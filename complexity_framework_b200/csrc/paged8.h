@@ -79,8 +79,9 @@ P8AttnPlan p8_attn_plan(const P8Cache& c, const P8Seqs& s, int group, int max_q_
 int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, const P8AttnPlan& plan,
                  float* ws, int* err, cudaStream_t stream);
 
-// Long chunks.  Joins the splits: out, and each row's total, from ws_o and ws_lse.
-int p8_combine(const P8Attn& a, int D, cudaStream_t stream);
+// Long chunks.  Joins the splits of the sequences' rows: out, and each row's total, from ws_o
+// and ws_lse.
+int p8_combine(const P8Seqs& s, const P8Attn& a, int D, cudaStream_t stream);
 int p8_chunk_blocks(const P8Seqs& s);
 // Whether a call's chunks go to the tcgen05 kernels.
 bool p8_is_chunk(int max_q_len, int group);

@@ -783,17 +783,23 @@ __global__ void __launch_bounds__(256)
 
 // Joins the splits of a long chunk's rows: out = sum 2^(lse_s - L) o_s with
 // L = log2 sum 2^lse_s, which goes to `total` where the weights need it.  A thread has four
-// dims of a row; all it reads is on its way before it is looked at.
+// dims of a row; all it reads is on its way before it is looked at.  Rows outside
+// [cu_q[0], cu_q[S]) are other calls': their part of the workspace was never written, and
+// their outputs stay.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
     p8_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_lse,
-                      float* __restrict__ total, T* __restrict__ out, int64_t rows, int splits) {
+                      float* __restrict__ total, T* __restrict__ out, P8Seqs seqs, int Hq,
+                      int64_t rows, int splits) {
   constexpr int kMost = 4;  // splits read ahead
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = at / (D / 4);
   const int d = static_cast<int>(at % (D / 4)) * 4;
+  // inputs, complete before the chunk kernel began
+  const int64_t begin = static_cast<int64_t>(__ldg(seqs.cu_q)) * Hq;
+  const int64_t end = static_cast<int64_t>(__ldg(seqs.cu_q + seqs.num_seqs)) * Hq;
   p8_grid_wait();
-  if (row >= rows) return;
+  if (row >= rows || row < begin || row >= end) return;
   const float* lse = ws_lse + row * splits;
   const float* o = ws_o + row * splits * D + d;
   float ls[kMost];
@@ -868,14 +874,14 @@ int launch_attn(const AttnParams& p, int nb, cudaStream_t st) {
 
 }  // namespace
 
-int p8_combine(const P8Attn& a, int D, cudaStream_t st) {
+int p8_combine(const P8Seqs& s, const P8Attn& a, int D, cudaStream_t st) {
   const int64_t n = a.N * a.Hq;
   const int64_t grid = (n * (D / 4) + 255) / 256;
   if (grid > 0x7fffffff) return -3;
   const dim3 g(static_cast<unsigned>(grid));
 #define CFB_COMBINE(T, DD)                                                                  \
   return p8_launch(p8_combine_kernel<T, DD>, g, 256, 0, st, a.ws_o, a.ws_lse, a.ws_total,   \
-                   static_cast<T*>(a.out), n, a.splits)
+                   static_cast<T*>(a.out), s, a.Hq, n, a.splits)
   if (a.type == kP8Bf16) {
     if (D == 128) CFB_COMBINE(__nv_bfloat16, 128);
     CFB_COMBINE(__nv_bfloat16, 64);

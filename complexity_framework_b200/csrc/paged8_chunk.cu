@@ -955,7 +955,7 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
                        : launch_fwd<T, D, 1>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st);
   if (rc) return rc;
   if (p.splits > 1) {
-    rc = p8_combine(a, c.D, st);
+    rc = p8_combine(s, a, c.D, st);
     if (rc) return rc;
   }
   if (mass) {
