@@ -457,7 +457,9 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
           if constexpr (MASS) y4[e] = y * ks;
         }
         if constexpr (MASS)
-          if (lim[nb][0] > 0 && (u == 0 || j + u < count)) {
+          // either row may see no key: the first of them lies before the sequence's first token
+          // or the second past the last row
+          if (max(lim[nb][0], lim[nb][1]) > 0 && (u == 0 || j + u < count)) {
             float* to = sp + static_cast<int64_t>(key0[u]) * p.RS + nb * 8;
             *reinterpret_cast<float2*>(to) = make_float2(y4[0], y4[1]);
             *reinterpret_cast<float2*>(to + 8 * p.RS) = make_float2(y4[2], y4[3]);

@@ -173,3 +173,12 @@ def test_engine_prompt_joins_a_running_request():
     # the same sums in 32 bits; the matrix products of 1 and 301 rows round to bf16 apart
     for a, b in zip(*seen):
         assert (a - b).abs().max() <= 2.0 ** -5 * a.abs().max()
+
+
+# ----------------------------------------------------------- rows before a sequence's first token
+@pytest.mark.parametrize("lens,new,hq,hkv", [([1], [2], 2, 2), ([3], [4], 2, 2), ([3], [4], 14, 2),
+                                             ([3, 40], [4, 5], 14, 2), ([1030, 2], [1, 5], 3, 3)])
+def test_weights_with_rows_before_the_first_token(lens, new, hq, hkv):
+    """An odd group and an odd number of such rows: of two neighbouring rows one sees keys."""
+    L = Layer(lens, hkv, 64, INT8, "cuda", seed=3)
+    check(L, new, hq, torch.bfloat16, mass=True)
