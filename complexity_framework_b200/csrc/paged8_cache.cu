@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(256, 3)
     }
     seq = lo;
     j -= __ldg(s.cu_q + seq) / kP8Page + 2 * static_cast<int64_t>(seq);
+    if (j < 0) return;  // rows before cu_q[0] are not this call's
   }
   const int row0 = __ldg(s.cu_q + seq);
   const int q_len = __ldg(s.cu_q + seq + 1) - row0;

@@ -182,3 +182,30 @@ def test_weights_with_rows_before_the_first_token(lens, new, hq, hkv):
     """An odd group and an odd number of such rows: of two neighbouring rows one sees keys."""
     L = Layer(lens, hkv, 64, INT8, "cuda", seed=3)
     check(L, new, hq, torch.bfloat16, mass=True)
+
+
+# -------------------------------------------------------------------- append of part of a batch
+@pytest.mark.parametrize("dtype", [INT8, FP8])
+@pytest.mark.parametrize("part", [(1, 4), (2, 5), (3, 4), (4, 5)])
+def test_append_of_part_of_a_batch(dtype, part):
+    """Uneven chunks of a call that begins past row 16: the same cache as on the CPU."""
+    from complexity_framework_b200.ops import paged8
+
+    new = [70, 1, 90, 300, 2]
+    a, e = part
+    cu = offsets(new)
+    g = torch.Generator().manual_seed(2)
+    k, v = torch.randn(2, cu[-1], 2, 64, generator=g).bfloat16()
+    caches = []
+    for device in ("cuda", "cpu"):
+        L = Layer([100, 40, 90, 307, 50], 2, 64, dtype, device, seed=3)
+        # a first block that is not finite: codes of 0 where tokens are added, else as it was
+        L.scales[int(L.table[a, 0])] = float("nan")
+        mass = torch.ones(L.num_pages, 2, PAGE, device=device)
+        paged8.paged8_append(k.to(device), v.to(device), L.codes, L.scales, L.table[a:e],
+                             torch.tensor(cu[a:e + 1], dtype=torch.int32, device=device),
+                             L.kv_lens[a:e], max_q_len=max(new[a:e]), mass=mass)
+        caches.append((f64(L.codes), f64(L.scales), mass.cpu()))
+    clean()
+    for x, y in zip(*caches):
+        assert torch.allclose(x, y, rtol=2.0 ** -22, atol=0, equal_nan=True)
