@@ -69,6 +69,7 @@ struct AttnParams {
   int64_t N;
   int Hq, G;
   int row_tiles;               // of the longest chunk of new tokens
+  int max_rows;                // its rows: the workspace has no room for more
   int chunk, splits;           // pages of a CTA, CTAs of the longest item
   float scale_log2;
   float* ws_o;                 // [items, splits, R, D] partial outputs (splits > 1)
@@ -160,7 +161,6 @@ struct SeqInfo {
   int row0, q_len, kv, rows;  // rows of a KV head: tokens x G
 };
 
-template <int R>
 __device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int seq) {
   SeqInfo i;
   i.row0 = __ldg(p.s.cu_q + seq);
@@ -170,9 +170,9 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int seq) {
     report_error(p.err, kErrBounds, 70);
     i.q_len = 0;
   }
-  if (static_cast<int64_t>(i.q_len) * p.G > p.row_tiles * R) {  // longer than max_q_len
+  if (static_cast<int64_t>(i.q_len) * p.G > p.max_rows) {  // longer than max_q_len
     report_error(p.err, kErrBounds, 71);
-    i.rows = p.row_tiles * R;
+    i.rows = p.max_rows;
   } else {
     i.rows = i.q_len * p.G;
   }
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kWarps * 32, (AttnCfg<D, NB>::MIN_CTAS))
   const int page = split * p.chunk, first = page + warp;
   const int entry = first + kWarps * lane;
   int id = entry < p.s.max_pages ? __ldg(table + entry) : 0;
-  const SeqInfo si = seq_info<R>(p, seq);
+  const SeqInfo si = seq_info(p, seq);
   const int rows = si.rows, first_row = rt * R;
   // row r is token r / G and head r % G; it sees the keys [0, start + token + 1)
   const int start = si.kv - si.q_len;
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(256)
   __shared__ float s_lse[kMaxRows];
   __shared__ float s_acc[8][D];
   const int seq = blockIdx.y / p.c.Hkv, h = blockIdx.y % p.c.Hkv;
-  const SeqInfo si = seq_info<R>(p, seq);  // inputs, complete before p8_attn_kernel began
+  const SeqInfo si = seq_info(p, seq);  // inputs, complete before p8_attn_kernel began
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int start = si.kv - si.q_len;
   const int64_t item0 = static_cast<int64_t>(blockIdx.y) * p.row_tiles;
@@ -937,6 +937,7 @@ int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, const P8Att
   p.Hq = a.Hq;
   p.G = a.Hq / c.Hkv;
   p.row_tiles = plan.row_tiles;
+  p.max_rows = a.max_q_len * p.G;
   p.chunk = plan.chunk;
   p.splits = plan.splits;
   p.scale_log2 = a.scale * 1.4426950408889634f;

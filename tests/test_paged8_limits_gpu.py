@@ -209,3 +209,20 @@ def test_append_of_part_of_a_batch(dtype, part):
     clean()
     for x, y in zip(*caches):
         assert torch.allclose(x, y, rtol=2.0 ** -22, atol=0, equal_nan=True)
+
+
+# ---------------------------------------------------------------- chunks longer than max_q_len
+@pytest.mark.parametrize("mass", [False, True])
+@pytest.mark.parametrize("new,max_q_len,hq", [([2, 0], 1, 8), ([0, 2], 1, 8), ([7, 1], 6, 10)])
+def test_short_chunk_longer_than_max_q_len_is_reported(new, max_q_len, hq, mass):
+    """Also where the kernels' rows, a multiple of eight, would hold it; the tables are full."""
+    from complexity_framework_b200.ops import check_errors
+
+    L = Layer([48, 48], 2, 64, INT8, "cuda", seed=3)
+    q = torch.randn(sum(new), hq, 64, device="cuda").bfloat16()
+    m = torch.zeros(L.num_pages, 2, PAGE, device="cuda") if mass else None
+    ops().paged8_attention(q, L.codes, L.scales, L.table, ints(offsets(new)), L.kv_lens,
+                           scale=0.1, max_q_len=max_q_len, mass=m)
+    with pytest.raises(RuntimeError, match="code=4 site=71"):
+        check_errors(0)
+    clean()
