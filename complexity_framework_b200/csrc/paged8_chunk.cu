@@ -196,7 +196,7 @@ struct ChunkParams {
   float* lse;                  // [N * Hq, splits], log2 units (splits > 1, or for the weights)
   float* ws_o;                 // [N * Hq, splits, D] (splits > 1)
   int64_t N;
-  int Hq, Hkv, G, splits, row_ctas, num_seqs;
+  int Hq, Hkv, G, splits, row_ctas, num_seqs, max_q_len;
   int* err;
 };
 
@@ -275,8 +275,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, NQ>::THREADS, (ChunkCfg<D, NQ>::CT
   const int kv = p8_len(p.kv_lens, seq, p.max_pages, p.err, 83);
   const int TT = kT / p.G;                 // tokens of a row tile
   const int tok0 = rc * NQ * TT;
-  if (rc == p.row_ctas - 1 && q_len > tok0 + NQ * TT && threadIdx.x == 0)
-    report_error(p.err, kErrBounds, 84);   // a chunk longer than max_q_len
+  if (q_len > p.max_q_len && threadIdx.x == 0) report_error(p.err, kErrBounds, 84);
   if (tok0 >= q_len) {
     p8_grid_wait();
     return;
@@ -902,6 +901,7 @@ int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
   constexpr auto kern = p8_chunk_kernel<T, D, NQ>;
   const int per_cta = NQ * (kT / p.G);
   p.row_ctas = (max_q_len + per_cta - 1) / per_cta;
+  p.max_q_len = max_q_len;
   p.num_seqs = num_seqs;
   const int64_t gx = static_cast<int64_t>(p.row_ctas) * p.splits * p.Hkv * num_seqs;
   if (gx > 0x7fffffff) return -3;
@@ -948,7 +948,7 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
   p.Hkv = c.Hkv;
   p.G = G;
   p.splits = a.splits;
-  p.row_ctas = 0;
+  p.row_ctas = p.max_q_len = 0;  // set at the launch
   p.err = err;
   const bool mass = a.mass_out != nullptr;
   rc = a.chunk_nq == 2 ? launch_fwd<T, D, 2>(tq, tk, tv, p, a.max_q_len, s.num_seqs, st)

@@ -226,3 +226,19 @@ def test_short_chunk_longer_than_max_q_len_is_reported(new, max_q_len, hq, mass)
     with pytest.raises(RuntimeError, match="code=4 site=71"):
         check_errors(0)
     clean()
+
+
+@pytest.mark.parametrize("mass", [False, True])
+@pytest.mark.parametrize("new,max_q_len", [([20, 1], 19), ([1, 70], 69), ([70, 70], 33)])
+def test_long_chunk_longer_than_max_q_len_is_reported(new, max_q_len, mass):
+    """Also within the last tile of rows."""
+    from complexity_framework_b200.ops import check_errors
+
+    L = Layer([100, 80], 2, 64, INT8, "cuda", seed=3)
+    q = torch.randn(sum(new), 16, 64, device="cuda").bfloat16()
+    m = torch.zeros(L.num_pages, 2, PAGE, device="cuda") if mass else None
+    ops().paged8_attention(q, L.codes, L.scales, L.table, ints(offsets(new)), L.kv_lens,
+                           scale=0.1, max_q_len=max_q_len, mass=m)
+    with pytest.raises(RuntimeError, match="code=4 site=84"):
+        check_errors(0)
+    clean()
