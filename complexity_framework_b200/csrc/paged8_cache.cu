@@ -32,7 +32,7 @@ template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(256, 3)
     p8_append_kernel(P8Cache c, P8Seqs s, const T* __restrict__ k, int64_t k_stride,
                      const T* __restrict__ v, int64_t v_stride, int64_t N, unsigned units,
-                     int per_seq, float* __restrict__ mass, int* err) {
+                     int per_seq, int max_q_len, float* __restrict__ mass, int* err) {
   constexpr int CH = D / 8;        // lanes of a row
   constexpr int RPL = 32 / CH;     // rows of one load
   constexpr int NL = kP8Page / RPL;
@@ -61,9 +61,7 @@ __global__ void __launch_bounds__(256, 3)
   const int first = max(start, 0);
   const int64_t blk = first / kP8Page + j;
   if (q_len <= 0 || blk * kP8Page >= kv) return;
-  if (per_seq > 0 && j == per_seq - 1 && (blk + 1) * kP8Page < kv) {
-    if (lane == 0) report_error(err, kErrBounds, 59);  // the chunk is longer than max_q_len
-  }
+  if (q_len > max_q_len && lane == 0) report_error(err, kErrBounds, 59);
   if (row0 < 0 || static_cast<int64_t>(row0) + q_len > N) {
     if (lane == 0) report_error(err, kErrBounds, 61);
     return;
@@ -414,12 +412,12 @@ __global__ void __launch_bounds__(256)
 
 template <typename T, int FMT, int D>
 int launch_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t ks, const void* v,
-                  int64_t vs, int64_t N, unsigned units, int per_seq, float* mass, int* err,
-                  cudaStream_t st) {
+                  int64_t vs, int64_t N, unsigned units, int per_seq, int max_q_len, float* mass,
+                  int* err, cudaStream_t st) {
   return p8_launch(p8_append_kernel<T, FMT, D>,
                    dim3((units + 7) / 8, per_seq > 0 ? s.num_seqs : 1), 256, 0, st, c, s,
                    static_cast<const T*>(k), ks, static_cast<const T*>(v), vs, N, units, per_seq,
-                   mass, err);
+                   max_q_len, mass, err);
 }
 
 }  // namespace
@@ -453,7 +451,7 @@ int p8_append(const P8Cache& c, const P8Seqs& s, const void* k, int64_t k_stride
   int rc = 0;
 #define CFB_CALL(T, F, DD)                                                                       \
   rc = launch_append<T, F, DD>(c, s, k, k_stride, v, v_stride, N, static_cast<unsigned>(units), ps, \
-                               mass, err, stream)
+                               max_q_len, mass, err, stream)
   CFB_P8_TYPES(CFB_CALL);
 #undef CFB_CALL
   return rc ? rc : static_cast<int>(cudaGetLastError());

@@ -242,3 +242,17 @@ def test_long_chunk_longer_than_max_q_len_is_reported(new, max_q_len, mass):
     with pytest.raises(RuntimeError, match="code=4 site=84"):
         check_errors(0)
     clean()
+
+
+@pytest.mark.parametrize("new,max_q_len", [([2, 1], 1), ([1, 33], 32), ([100, 1, 1, 1], 99)])
+def test_append_longer_than_max_q_len_is_reported(new, max_q_len):
+    """Whether or not its blocks fit what the launch covers, in both enumerations."""
+    from complexity_framework_b200.ops import check_errors
+
+    L = Layer([100] * len(new), 2, 64, INT8, "cuda", seed=3)
+    k = torch.randn(sum(new), 2, 64, device="cuda").bfloat16()
+    ops().paged8_append(k, k, L.codes, L.scales, L.table, ints(offsets(new)), L.kv_lens,
+                        max_q_len=max_q_len)
+    with pytest.raises(RuntimeError, match="code=4 site=59"):
+        check_errors(0)
+    clean()
