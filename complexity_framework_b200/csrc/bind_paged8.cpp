@@ -194,7 +194,11 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
   a.Hq = static_cast<int>(Hq);
   a.max_q_len = static_cast<int>(max_q_len);
   a.scale = static_cast<float>(scale);
-  if (N == 0 || s.num_seqs == 0) return out;
+  if (s.num_seqs == 0 || (N == 0 && a.mass_out == a.mass_in)) return out;
+  if (N == 0) {  // no rows, but the cached tokens' weights go on to mass_out
+    a.Hq = c.Hkv;
+    a.max_q_len = 1;
+  }
   const int sms = cfb_num_sms(codes.get_device()), group = a.Hq / c.Hkv;
   int* err = cfb_err_ptr(codes.get_device());
   const auto stream = at::cuda::getCurrentCUDAStream();

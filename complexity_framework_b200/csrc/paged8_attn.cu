@@ -921,7 +921,7 @@ P8AttnPlan p8_attn_plan(const P8Cache& c, const P8Seqs& s, int group, int max_q_
 
 int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, const P8AttnPlan& plan,
                  float* ws, int* err, cudaStream_t stream) {
-  if (a.N <= 0 || s.num_seqs <= 0) return 0;
+  if (s.num_seqs <= 0) return 0;
   const int64_t heads = static_cast<int64_t>(s.num_seqs) * c.Hkv;
   if (heads > 65535 || c.num_pages * c.Hkv > 0x7fffffff ||
       static_cast<int64_t>(plan.splits) * plan.row_tiles > 0x7fffffff ||

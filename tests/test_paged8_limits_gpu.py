@@ -256,3 +256,23 @@ def test_append_longer_than_max_q_len_is_reported(new, max_q_len):
     with pytest.raises(RuntimeError, match="code=4 site=59"):
         check_errors(0)
     clean()
+
+
+# ------------------------------------------------------------------------------- no new tokens
+@pytest.mark.parametrize("hq", [1, 100])
+@pytest.mark.parametrize("width", [4, 80])
+def test_weights_pass_through_a_call_without_new_tokens(hq, width):
+    L = Layer([40, 0, 17], 1, 64, INT8, "cuda", seed=3, width=width)
+    q = torch.empty(0, hq, 64, dtype=torch.bfloat16, device="cuda")
+    m_in = torch.rand(L.num_pages, 1, PAGE, device="cuda")
+    m_out = torch.full_like(m_in, -7.0)
+    out = ops().paged8_attention(q, L.codes, L.scales, L.table, ints([0] * 4), L.kv_lens,
+                                 scale=1.0, max_q_len=9, mass=m_in, mass_out=m_out)
+    clean()
+    assert out.shape == q.shape
+    want = torch.full_like(m_in, -7.0)
+    for i, n in enumerate(L.lens):
+        for j in range(n):
+            at = int(L.table[i, j // PAGE]), 0, j % PAGE
+            want[at] = m_in[at]
+    assert torch.equal(m_out, want)
