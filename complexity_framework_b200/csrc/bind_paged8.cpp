@@ -208,12 +208,25 @@ Tensor paged8_attention(const Tensor& q_in, const Tensor& codes, const Tensor& s
                   c.num_pages * c.Hkv <= 0x7fffffff,
               "too many sequences or pages");
   if (!cfb::p8_is_chunk(a.max_q_len, group)) {
-    const cfb::P8AttnPlan plan = cfb::p8_attn_plan(c, s, group, a.max_q_len, mass, sms);
+    // sequences at a time, within the workspace limit: kept scores are as long as the table is wide
+    cfb::P8Seqs part = s;
+    cfb::P8AttnPlan plan = cfb::p8_attn_plan(c, part, group, a.max_q_len, mass, sms);
+    while (part.num_seqs > 1 && plan.floats() > workspace_bytes / 4) {
+      part.num_seqs = (part.num_seqs + 1) / 2;
+      plan = cfb::p8_attn_plan(c, part, group, a.max_q_len, mass, sms);
+    }
+    const int seqs_each = part.num_seqs;
     Tensor ws;
     if (plan.floats() > 0) ws = empty({plan.floats()}, torch::kFloat32, codes);
-    check_rc(cfb::p8_attention(c, s, a, plan, plan.floats() > 0 ? ws.data_ptr<float>() : nullptr,
-                               err, stream),
-             "paged8_attention");
+    for (int64_t i = 0; i < s.num_seqs; i += seqs_each) {
+      part.table = s.table + i * s.max_pages;
+      part.cu_q = s.cu_q + i;
+      part.kv_lens = s.kv_lens + i;
+      part.num_seqs = static_cast<int>(std::min<int64_t>(seqs_each, s.num_seqs - i));
+      check_rc(cfb::p8_attention(c, part, a, plan,
+                                 plan.floats() > 0 ? ws.data_ptr<float>() : nullptr, err, stream),
+               "paged8_attention");
+    }
     return out;
   }
   const int64_t blocks = cfb::p8_chunk_blocks(s);

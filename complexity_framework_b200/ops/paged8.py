@@ -136,8 +136,9 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
 
     With ``mass`` the softmax weights every cached token receives from this call are added to
     it: in place, or into ``mass_out`` (which takes the tokens of this call's sequences only).
-    Long chunks expand keys and values to 16 bits first, in a workspace of at most
-    ``workspace_bytes`` (or one sequence's, where that is more).
+    Long chunks expand keys and values to 16 bits first, and short ones with ``mass`` keep their
+    scores, both as long as the page table is wide: in a workspace of about ``workspace_bytes``
+    at most (or one sequence's, where that is more), with the sequences taken in parts.
     """
     if not 0.0 < scale < float("inf"):
         raise ValueError("scale must be positive and finite")

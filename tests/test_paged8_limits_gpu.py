@@ -276,3 +276,29 @@ def test_weights_pass_through_a_call_without_new_tokens(hq, width):
             at = int(L.table[i, j // PAGE]), 0, j % PAGE
             want[at] = m_in[at]
     assert torch.equal(m_out, want)
+
+
+# ------------------------------------------------------------------------------------ workspaces
+@pytest.mark.parametrize("new,limit", [(1, 8 << 20), (8, 24 << 20)])
+def test_kept_scores_stay_within_the_workspace(new, limit):
+    """Weights of short chunks over a table far wider than the sequences."""
+    seqs = 12
+    lens = [20 + 30 * i for i in range(seqs)]
+    L = Layer(lens, 2, 64, INT8, "cuda", seed=3, width=4096)
+    q = torch.randn(seqs * new, 8, 64, device="cuda").bfloat16()
+    cu = ints(offsets([new] * seqs))
+    m = torch.zeros(2, L.num_pages, 2, PAGE, device="cuda")
+    outs, peak = [], []
+    for i, ws in enumerate((4 << 30, limit)):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        outs.append(ops().paged8_attention(q, L.codes, L.scales, L.table, cu, L.kv_lens,
+                                           scale=0.125, max_q_len=new, mass=m[i],
+                                           workspace_bytes=ws))
+        peak.append(torch.cuda.max_memory_allocated() - held)
+    clean()
+    assert peak[0] > 2 * limit and peak[1] <= limit + (1 << 20), peak   # beside the output
+    # other chunks of the cache, the same sums
+    assert (outs[0].float() - outs[1].float()).abs().max() < 2.0 ** -6
+    assert torch.allclose(m[0], m[1], rtol=1e-4, atol=1e-6)
