@@ -87,8 +87,9 @@ int type_of(torch::ScalarType t, const char* name) {
   return t == torch::kBFloat16 ? cfb::kP8Bf16 : cfb::kP8Half;
 }
 
-// [N, H, D] whose rows of H * D elements are dense, 16-byte aligned and any distance apart
-// (a slice of a fused projection is one); other layouts are copied.
+// [N, H, D] whose rows of H * D elements are dense, 16-byte aligned and any distance apart that
+// keeps them disjoint (a slice of a fused projection is one; TMA takes no expanded rows); other
+// layouts are copied.
 Tensor rows_of(const Tensor& t, const Tensor& codes, int64_t D, const char* name) {
   same_device(t, codes, name);
   TORCH_CHECK(t.dim() == 3 && t.size(2) == D, name, " must be [tokens, heads, ", D, "]");
@@ -96,7 +97,7 @@ Tensor rows_of(const Tensor& t, const Tensor& codes, int64_t D, const char* name
   TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()),
               "the 8-bit KV cache operators have no gradient; call them under torch.no_grad()");
   const bool dense = t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == D) &&
-                     (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= 0)) &&
+                     (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) * D)) &&
                      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   return dense ? t : t.clone(at::MemoryFormat::Contiguous);
 }

@@ -302,3 +302,11 @@ def test_kept_scores_stay_within_the_workspace(new, limit):
     # other chunks of the cache, the same sums
     assert (outs[0].float() - outs[1].float()).abs().max() < 2.0 ** -6
     assert torch.allclose(m[0], m[1], rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("new", [[1, 3], [60, 20]])
+def test_expanded_q(new):
+    """One row for all tokens: strides that no TMA map may have."""
+    L = Layer([200, 70], 2, 64, INT8, "cuda", seed=3)
+    q = torch.randn(1, 14, 64, device="cuda").bfloat16().expand(sum(new), 14, 64)
+    check(L, new, 14, torch.bfloat16, q=q)
