@@ -304,6 +304,42 @@ def test_kept_scores_stay_within_the_workspace(new, limit):
     assert torch.allclose(m[0], m[1], rtol=1e-4, atol=1e-6)
 
 
+# ------------------------------------------------------------------------- layouts and ranges of q
+@pytest.mark.parametrize("new", [[1, 3], [60, 20]])
+def test_q_of_a_fused_projection(new):
+    hq, hkv, d = 14, 2, 64
+    L = Layer([200, 70], hkv, d, INT8, "cuda", seed=3)
+    n = sum(new)
+    kqv = torch.randn(n, (2 * hkv + hq) * d, device="cuda").bfloat16()
+    check(L, new, hq, torch.bfloat16, q=kqv[:, hkv * d:(hkv + hq) * d].view(n, hq, d))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_zero_and_uneven_value_scales(new):
+    """V blocks of zeros, and blocks whose scales lie far apart, in both attention kernels."""
+    L = Layer([200, 100], 2, 64, INT8, "cuda", seed=9)
+    L.scales[::3, :, 1] = 0
+    L.scales[1::3, :, 1] *= 1e-4
+    L.codes[::3, :, 1] = 0
+    check(L, [new, new], 8, torch.bfloat16, mass=True)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_q_elements_far_apart(new):
+    """Short chunks hold q in f16 scaled by the row's largest element: elements more than 2^17
+    below it lose bits, at most 2^-25 of the largest each; small codes beside the offset of
+    128 that int8 codes carry through the score's sum."""
+    L = Layer([150, 70], 2, 64, INT8, "cuda", seed=9)
+    L.codes[..., 0, :, :] //= 32
+    q = torch.randn(2 * new, 8, 64) * 2.0 ** -21
+    q[..., 5] = 1.0
+    k = torch.cat([L.values(i)[0].reshape(-1, 64) for i in range(2)])
+    lost = 2.0 ** -25 * k.abs().sum(-1).max().item() / 8
+    offset = 128 * L.scales.max().item() * q.abs().sum(-1).max().item() / 8
+    check(L, [new, new], 8, torch.bfloat16, q=q.bfloat16().cuda(), mass=True,
+          q_err=lost + math.log(2) * score_error(offset))
+
+
 @pytest.mark.parametrize("new", [[1, 3], [60, 20]])
 def test_expanded_q(new):
     """One row for all tokens: strides that no TMA map may have."""
