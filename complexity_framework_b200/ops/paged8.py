@@ -171,7 +171,12 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
         seen = torch.arange(n) <= (n - rows + torch.arange(rows))[:, None]
         s = s.masked_fill(~seen, float("-inf"))
         p = torch.where(seen.any(-1, keepdim=True), torch.softmax(s, -1), torch.zeros_like(s))
-        o = torch.matmul(p, x[1][:, None])
+        # what is not finite reaches the rows that see it only, not the others as 0 * NaN
+        bad = ~torch.isfinite(x[1])
+        o = torch.matmul(p, x[1].masked_fill(bad, 0.0)[:, None])
+        if bad.any():
+            hit = torch.matmul(seen.float(), bad.float()) > 0                 # [H, rows, D]
+            o = o.masked_fill(hit[:, None], float("nan"))
         out[cu[i]:cu[i + 1]] = o.permute(2, 0, 1, 3).reshape(rows, H * G, D).to(out.dtype)
         if mass is not None:
             w = torch.zeros(H, blocks * PAGE)

@@ -1,0 +1,34 @@
+"""The 8-bit paged KV cache on the CPU where values are not finite and sequences change hands."""
+import pytest
+import torch
+
+from paged8_oracle import PAGE, Layer, attention, f64
+
+from complexity_framework_b200.ops import paged8
+
+INT8, FP8 = torch.int8, torch.float8_e4m3fn
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("dtype", [INT8, FP8])
+def test_a_later_block_that_is_not_finite_is_masked(dtype):
+    """Rows before the block see and weigh the tokens before it as if it were not there."""
+    L = Layer([64], 1, 16, dtype, "cpu", seed=2)
+    q = torch.randn(20, 2, 16)
+    m = torch.zeros(2, L.num_pages, 1, PAGE)
+    outs = []
+    for i in range(2):
+        outs.append(paged8.paged8_attention(q, L.codes, L.scales, L.table, ints([0, 20]), L.kv_lens,
+                                            scale=0.25, max_q_len=20, mass=m[i]))
+        L.scales[int(L.table[0, 3])] = float("nan")
+        L.codes[int(L.table[0, 3])] = 0
+    assert torch.equal(outs[0][:4], outs[1][:4])         # positions 44 .. 47 see blocks 0 .. 2
+    assert torch.isnan(outs[1][4:]).all()
+    # the first rows alone: their weights are numbers
+    m[0] = 0
+    paged8.paged8_attention(q[:4], L.codes, L.scales, L.table, ints([0, 4]), ints([48]), scale=0.25,
+                            max_q_len=4, mass=m[0])
+    assert torch.isfinite(m[0]).all() and abs(m[0].sum().item() - 8) < 1e-4
