@@ -170,7 +170,8 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
         s = torch.matmul(qs, x[0][:, None].transpose(-1, -2)) * scale     # [H, G, rows, n]
         seen = torch.arange(n) <= (n - rows + torch.arange(rows))[:, None]
         s = s.masked_fill(~seen, float("-inf"))
-        p = torch.where(seen.any(-1, keepdim=True), torch.softmax(s, -1), torch.zeros_like(s))
+        # 0 at hidden tokens also where the row is NaN, and for rows that see nothing
+        p = torch.where(seen, torch.softmax(s, -1), torch.zeros_like(s))
         # what is not finite reaches the rows that see it only, not the others as 0 * NaN
         bad = ~torch.isfinite(x[1])
         o = torch.matmul(p, x[1].masked_fill(bad, 0.0)[:, None])

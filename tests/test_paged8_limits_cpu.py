@@ -32,3 +32,18 @@ def test_a_later_block_that_is_not_finite_is_masked(dtype):
     paged8.paged8_attention(q[:4], L.codes, L.scales, L.table, ints([0, 4]), ints([48]), scale=0.25,
                             max_q_len=4, mass=m[0])
     assert torch.isfinite(m[0]).all() and abs(m[0].sum().item() - 8) < 1e-4
+
+
+def test_weights_of_hidden_tokens_are_not_touched_by_nan_rows():
+    """A row that is not a number weighs the tokens it sees only."""
+    L = Layer([40], 1, 16, INT8, "cpu", seed=2)
+    q = torch.randn(20, 2, 16)
+    q[3] = float("nan")                                     # at position 23
+    m = torch.zeros(L.num_pages, 1, PAGE)
+    paged8.paged8_attention(q, L.codes, L.scales, L.table, ints([0, 20]), L.kv_lens, scale=0.25,
+                            max_q_len=20, mass=m)
+    q[3] = 0
+    weights = attention(L, q, [0, 20], 0.25)[2][0]
+    got = m[L.table[0].long(), 0].reshape(-1)[:40]
+    assert torch.isnan(got[:24]).all()
+    assert (f64(got[24:]) - weights[0, 24:]).abs().max() < 1e-5

@@ -346,3 +346,21 @@ def test_expanded_q(new):
     L = Layer([200, 70], 2, 64, INT8, "cuda", seed=3)
     q = torch.randn(1, 14, 64, device="cuda").bfloat16().expand(sum(new), 14, 64)
     check(L, new, 14, torch.bfloat16, q=q)
+
+
+@pytest.mark.parametrize("heads", [1, 8])
+def test_nan_rows_weigh_the_tokens_they_see_only(heads):
+    """In both attention kernels."""
+    L = Layer([40], 1, 64, INT8, "cuda", seed=2)
+    q = torch.randn(20, heads, 64, device="cuda").bfloat16()
+    m = torch.zeros(2, L.num_pages, 1, PAGE, device="cuda")
+    outs = []
+    for i in range(2):
+        outs.append(ops().paged8_attention(q, L.codes, L.scales, L.table, ints([0, 20]), L.kv_lens,
+                                           scale=0.125, max_q_len=20, mass=m[i]))
+        q[3] = float("nan")                                 # at position 23
+    clean()
+    rows = torch.tensor([t != 3 for t in range(20)], device="cuda")
+    assert torch.equal(outs[0][rows], outs[1][rows]) and torch.isnan(outs[1][3]).all()
+    clear, nan = (x[L.table[0].long(), 0].reshape(-1)[:40] for x in m)
+    assert torch.isnan(nan[:24]).all() and torch.equal(clear[24:], nan[24:])
