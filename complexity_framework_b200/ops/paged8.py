@@ -223,9 +223,11 @@ def paged8_evict(codes: torch.Tensor, scales: torch.Tensor, mass: torch.Tensor,
                 raise ValueError("dst_table has too few pages")
             pages = page_table[i, :blocks].long()
             m = ms[lay, pages].transpose(0, 1).reshape(H, -1)[:, :n]
-            rank = m.clone()
-            rank[:, n - (recent if n > budget else n):] = float("inf")
-            idx = rank.sort(dim=-1, descending=True, stable=True).indices[:, :kept].sort(-1).values
+            # the recent tokens apart: no older mass, infinite or NaN, may take their place
+            older = n - recent if n > budget else 0
+            idx = m[:, :older].sort(dim=-1, descending=True, stable=True).indices
+            idx = torch.cat((idx[:, :kept - (n - older)].sort(-1).values,
+                             torch.arange(older, n).expand(H, -1)), -1)
             ks[lay, i, :, :kept] = idx.int()
             page, slot, head = pages[idx // PAGE], idx % PAGE, torch.arange(H)[:, None]
             old = ss[lay, page, head]                                   # [H, kept, 2]

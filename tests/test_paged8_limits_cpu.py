@@ -47,3 +47,15 @@ def test_weights_of_hidden_tokens_are_not_touched_by_nan_rows():
     got = m[L.table[0].long(), 0].reshape(-1)[:40]
     assert torch.isnan(got[:24]).all()
     assert (f64(got[24:]) - weights[0, 24:]).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize("top", [float("inf"), float("nan")])
+def test_recent_tokens_stay_beside_masses_that_are_not_finite(top):
+    """The last tokens are kept whatever the older ones' masses are."""
+    L = Layer([40], 1, 8, INT8, "cpu", extra_pages=3)
+    mass = torch.rand(L.num_pages, 1, PAGE)
+    for j in range(2, 30):
+        mass[int(L.table[0, j // PAGE]), 0, j % PAGE] = top
+    keep = paged8.paged8_evict(L.codes, L.scales, mass, L.table, L.kv_lens, ints([L.spare[:1]]),
+                               budget=12, recent=5)
+    assert keep[0, 0].tolist() == list(range(2, 9)) + list(range(35, 40))
