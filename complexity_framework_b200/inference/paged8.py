@@ -14,6 +14,7 @@ position in their rotation, so slots need not follow positions).
 """
 from __future__ import annotations
 
+import itertools
 from typing import Dict, List, Sequence, Tuple
 
 import torch
@@ -52,17 +53,25 @@ class Paged8Pool(PagePool):
         self.pages: Dict[int, List[int]] = {}
         self.lengths: Dict[int, int] = {}
         self.dropped: Dict[int, int] = {}
-        self.moves: Dict[int, int] = {}  # how often a sequence's pages were replaced
+        # a number of its own for each time a sequence's pages were replaced
+        self.moves: Dict[int, int] = {}
+        self._move = itertools.count()
 
     def allocate_sequence(self, seq_id: int) -> None:
         super().allocate_sequence(seq_id)
         self.dropped[seq_id] = 0
-        self.moves[seq_id] = 0
+        self.moves[seq_id] = next(self._move)
 
     def free_sequence(self, seq_id: int) -> None:
         super().free_sequence(seq_id)
         self.dropped.pop(seq_id, None)
         self.moves.pop(seq_id, None)
+
+    def truncate_sequence(self, seq_id: int, length: int) -> None:
+        held = len(self.pages[seq_id])
+        super().truncate_sequence(seq_id, length)
+        if len(self.pages[seq_id]) < held:
+            self.moves[seq_id] = next(self._move)
 
     def fork_sequence(self, src: int, dst: int) -> None:
         if dst in self.pages:
@@ -126,7 +135,7 @@ class Paged8Pool(PagePool):
             self.pages[s] = pages
             self.dropped[s] += self.lengths[s] - budget
             self.lengths[s] = budget
-            self.moves[s] += 1
+            self.moves[s] = next(self._move)
 
     def batch(self, chunks: Sequence[SeqChunk]) -> "Paged8Batch":
         return Paged8Batch(self, chunks)
@@ -233,7 +242,7 @@ class StaticDecode8Batch(_Attend8, StaticDecodeBatch):
         self.rows = torch.arange(B, device=dev)
         self.positions = torch.zeros(B, dtype=torch.long, device=dev)
         self.ids = torch.zeros(B, dtype=torch.long, device=dev)
-        self._row_seq = [None] * B   # (sequence, its moves) of each row
+        self._row_seq = [None] * B   # (sequence, its last move) of each row
         self._row_pages = [0] * B    # pages of that sequence already in the table row
         self._live = []
 

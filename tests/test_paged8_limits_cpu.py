@@ -59,3 +59,39 @@ def test_recent_tokens_stay_beside_masses_that_are_not_finite(top):
     keep = paged8.paged8_evict(L.codes, L.scales, mass, L.table, L.kv_lens, ints([L.spare[:1]]),
                                budget=12, recent=5)
     assert keep[0, 0].tolist() == list(range(2, 9)) + list(range(35, 40))
+
+
+def test_static_batch_follows_a_sequence_whose_pages_change(monkeypatch):
+    """A row's page table after its sequence was freed and allocated anew under the same id,
+    forked into, or cut and grown again, with its old pages in other hands."""
+    from complexity_framework_b200.inference import Paged8Pool
+
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
+    pool = Paged8Pool(1, 1, 8, 20, dtype=torch.float32)
+    batch = pool.static_batch(2, 8, 127)
+
+    def step(seq, position):
+        batch.fill([(seq, 1, position)])
+        batch.commit()
+        n = len(pool.pages[seq])
+        assert batch.page_table[0, :n].tolist() == pool.pages[seq]
+
+    def grow(seq, tokens):
+        if seq not in pool.pages:
+            pool.allocate_sequence(seq)
+        pool.reserve(seq, tokens - pool.lengths[seq])
+        pool.lengths[seq] = tokens
+
+    grow(0, 40)
+    step(0, 40)
+    pool.free_sequence(0)
+    grow(1, 20)
+    grow(0, 30)
+    step(0, 30)
+    pool.truncate_sequence(0, 10)
+    grow(1, 40)
+    grow(0, 33)
+    step(0, 33)
+    pool.fork_sequence(1, 0)
+    grow(2, 20)
+    step(0, 40)
