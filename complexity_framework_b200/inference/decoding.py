@@ -18,7 +18,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 import torch.nn as nn
 
-from .paged import PagedBatch, PagePool, SeqChunk
+from .paged import PagePool, SeqChunk
 
 
 def _pool_for(model, num_seqs: int, max_len: int, page_size: int = 16) -> PagePool:
@@ -36,7 +36,7 @@ def paged_logits(model, pool: PagePool, chunks: Sequence[SeqChunk], toks: Sequen
     every token ``[len, V]`` with ``all_positions``)."""
     from .engine import forward_paged
 
-    batch = PagedBatch(pool, chunks)
+    batch = pool.batch(chunks)
     dev = pool.device
     hidden = forward_paged(model, torch.tensor(list(toks), dtype=torch.long, device=dev), batch)
     batch.commit()

@@ -95,3 +95,36 @@ def test_static_batch_follows_a_sequence_whose_pages_change(monkeypatch):
     pool.fork_sequence(1, 0)
     grow(2, 20)
     step(0, 40)
+
+
+def small_model():
+    from complexity_framework_b200 import ComplexityModel, ModelConfig
+
+    torch.manual_seed(0)
+    return ComplexityModel(ModelConfig(
+        hidden_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+        vocab_size=256, intermediate_size=64, shared_intermediate_size=64, num_experts=2, top_k=1,
+        max_position_embeddings=512)).eval()
+
+
+def test_paged_logits_over_an_8_bit_pool():
+    """A prompt, then four drafted tokens at once: the logits of the same tokens one by one."""
+    from complexity_framework_b200.inference import Paged8Pool, SeqChunk, paged_logits
+
+    m = small_model()
+    toks = torch.randint(0, 256, (24,), generator=torch.Generator().manual_seed(1)).tolist()
+    logits = []
+    for steps in ((20, 4), (20, 1, 1, 1, 1)):
+        pool = Paged8Pool(2, 2, 16, 4, dtype=torch.float32)
+        pool.allocate_sequence(0)
+        at, rows = 0, []
+        for n in steps:
+            rows += paged_logits(m, pool, [SeqChunk(0, at, n)], toks[at:at + n],
+                                 all_positions=True)[0]
+            at += n
+        logits.append(torch.stack(rows))
+    assert logits[0].shape == (24, 256)
+    # the prompt's chunk is the same call; a block's older codes may be rounded once more when
+    # tokens arrive one by one, half a step of 1/127 of the largest value
+    assert torch.equal(logits[0][:20], logits[1][:20])
+    assert (logits[0] - logits[1]).abs().max() <= logits[0].abs().max() / 16
