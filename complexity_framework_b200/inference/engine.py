@@ -23,7 +23,7 @@ from typing import Dict, Iterator, List, Optional, Sequence, Union
 
 import torch
 
-from .paged import OutOfPages, PagedBatch, PagePool, SeqChunk
+from .paged import PagedBatch, PagePool, SeqChunk
 from .paged8 import Paged8Pool
 
 
@@ -79,7 +79,8 @@ class InferenceConfig:
     kv_cache_dtype: Optional[str] = None
     # with an 8-bit cache: cut a sequence that holds ``kv_evict_slack`` tokens more than
     # ``kv_evict_budget`` to that budget, keeping the last ``kv_evict_recent`` tokens and
-    # those that received the most attention; 0: keep everything
+    # those that received the most attention; 0: keep everything.  The pool has the pages of
+    # one budget beside ``num_pages``, to move kept tokens to when all others are taken
     kv_evict_budget: int = 0
     kv_evict_recent: int = 64
     kv_evict_slack: int = 256
@@ -177,7 +178,8 @@ class InferenceEngine:
             self.pool = Paged8Pool(mc.num_hidden_layers, kv_heads, mc.head_dim, pages,
                                    cfg.page_size, dtype=self.dtype, device=self.device,
                                    kv_dtype=cfg.kv_cache_dtype,
-                                   track_mass=cfg.kv_evict_budget > 0)
+                                   track_mass=cfg.kv_evict_budget > 0,
+                                   evict_pages=-(-cfg.kv_evict_budget // cfg.page_size))
         self._ids = itertools.count()
         self._graphs: Dict[int, tuple] = {}
         self.requests: Dict[int, _Req] = {}
@@ -298,19 +300,17 @@ class InferenceEngine:
         return finished
 
     def _evict(self) -> None:
-        """Cut the sequences that outgrew the cache budget.  Where no pages are free to move
-        the kept tokens to, they stay whole until some are."""
+        """Cut the sequences that outgrew the cache budget, as many at a time as there are free
+        pages to move the kept tokens to (the pool holds back enough for one)."""
         cfg = self.config
+        each = -(-cfg.kv_evict_budget // cfg.page_size)
         over = [s for s, n in self.pool.lengths.items()
                 if n >= cfg.kv_evict_budget + cfg.kv_evict_slack]
         while over:
-            try:
-                self.pool.evict(over, cfg.kv_evict_budget, cfg.kv_evict_recent)
-            except OutOfPages:
-                over = over[:len(over) // 2]  # fewer at a time: the old pages come back
-                continue
-            self.stats["evictions"] = self.stats.get("evictions", 0) + len(over)
-            break
+            some = over[:max(1, len(self.pool.free) // each)]
+            self.pool.evict(some, cfg.kv_evict_budget, cfg.kv_evict_recent)
+            self.stats["evictions"] = self.stats.get("evictions", 0) + len(some)
+            over = over[len(some):]
 
     @torch.no_grad()
     def step(self) -> List[int]:

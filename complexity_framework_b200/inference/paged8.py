@@ -29,9 +29,12 @@ SHORT_ROWS = 64
 
 
 class Paged8Pool(PagePool):
+    """``num_pages`` pages for sequences, and ``evict_pages`` more that only ``evict`` takes: with
+    a budget's worth of them one sequence at a time can be cut however full the pool is."""
+
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int,
                  page_size: int = ops.PAGE, dtype=torch.bfloat16, device="cpu",
-                 kv_dtype: str = "int8", track_mass: bool = False):
+                 kv_dtype: str = "int8", track_mass: bool = False, evict_pages: int = 0):
         if kv_dtype not in CODE_TYPES:
             raise ValueError(f"kv_dtype must be one of {sorted(CODE_TYPES)}, got {kv_dtype!r}")
         if page_size != ops.PAGE:
@@ -43,7 +46,9 @@ class Paged8Pool(PagePool):
             if dtype not in (torch.bfloat16, torch.float16):
                 raise ValueError(f"the 8-bit cache kernels take bf16 or fp16 models, got {dtype}")
         self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim
+        num_pages += evict_pages
         self.num_pages, self.page_size, self.dtype, self.kv_dtype = num_pages, page_size, dtype, kv_dtype
+        self.evict_pages = evict_pages
         shape = (num_layers, num_pages, num_kv_heads)
         self.codes = torch.zeros(*shape, 2, page_size, head_dim, dtype=CODE_TYPES[kv_dtype],
                                  device=self.device)
@@ -66,6 +71,16 @@ class Paged8Pool(PagePool):
         super().free_sequence(seq_id)
         self.dropped.pop(seq_id, None)
         self.moves.pop(seq_id, None)
+
+    def reserve(self, seq_id: int, new_tokens: int) -> None:
+        if not self.can_reserve(seq_id, self.lengths[seq_id] + new_tokens):
+            raise OutOfPages("KV page pool exhausted")
+        super().reserve(seq_id, new_tokens)
+
+    def can_reserve(self, seq_id, length_after: int, current: int = 0) -> bool:
+        have = len(self.pages.get(seq_id, [])) if seq_id is not None else 0
+        need = -(-length_after // self.page_size) - have
+        return need <= max(0, len(self.free) - self.evict_pages)
 
     def truncate_sequence(self, seq_id: int, length: int) -> None:
         held = len(self.pages[seq_id])
@@ -113,8 +128,8 @@ class Paged8Pool(PagePool):
     def evict(self, seq_ids: Sequence[int], budget: int, recent: int) -> None:
         """Cut each sequence that holds more than ``budget`` tokens to ``budget``: its last
         ``recent`` tokens and the older ones of largest mass, by layer and KV head.  Takes the
-        new pages from the free list (``OutOfPages`` when they do not suffice) and returns the
-        old ones."""
+        new pages from all that are free (``OutOfPages`` when they do not suffice) and returns
+        the old ones, which are as many or more."""
         if self.mass is None:
             raise RuntimeError("eviction needs a pool with track_mass=True")
         if budget < 1 or not 0 <= recent <= budget:

@@ -128,3 +128,43 @@ def test_paged_logits_over_an_8_bit_pool():
     # tokens arrive one by one, half a step of 1/127 of the largest value
     assert torch.equal(logits[0][:20], logits[1][:20])
     assert (logits[0] - logits[1]).abs().max() <= logits[0].abs().max() / 16
+
+
+@pytest.mark.parametrize("lens,num_pages", [((100,), 8), ((70, 60, 50), 14)])
+def test_engine_evicts_with_no_page_free(lens, num_pages):
+    """Requests that fill the pool are cut to the budget, not refused the next token's page."""
+    from complexity_framework_b200.inference import (GenerationConfig, InferenceConfig,
+                                                     InferenceEngine)
+
+    eng = InferenceEngine(small_model(), InferenceConfig(
+        max_cache_length=512, max_batch_size=4, num_pages=num_pages, kv_cache_dtype="int8",
+        kv_evict_budget=40, kv_evict_recent=16, kv_evict_slack=16, prefill_chunk_size=128))
+    g = torch.Generator().manual_seed(1)
+    rids = [eng.add_request(torch.randint(0, 256, (n,), generator=g).tolist(),
+                            GenerationConfig(max_new_tokens=90)) for n in lens]
+    while eng.has_pending():
+        eng.step()
+    assert [len(eng.requests[r].output) for r in rids] == [90] * len(lens)
+    assert eng.stats["evictions"] >= 2 * len(lens)
+    assert len(eng.pool.free) == eng.pool.num_pages
+
+
+def test_pages_held_for_evictions():
+    """No sequence takes them; an eviction does, and gives back as many."""
+    from complexity_framework_b200.inference import OutOfPages, Paged8Pool
+
+    pool = Paged8Pool(1, 1, 8, 4, dtype=torch.float32, track_mass=True, evict_pages=2)
+    assert len(pool.free) == pool.num_pages == 6
+    pool.allocate_sequence(0)
+    pool.allocate_sequence(1)
+    assert pool.can_reserve(0, 64) and not pool.can_reserve(0, 65)
+    pool.reserve(0, 64)
+    pool.lengths[0] = 64
+    pool.reserve(0, 0)
+    with pytest.raises(OutOfPages):
+        pool.reserve(1, 1)
+    pool.evict([0], budget=32, recent=8)
+    assert len(pool.free) == 4 and pool.lengths[0] == 32
+    pool.reserve(1, 32)
+    with pytest.raises(OutOfPages):
+        pool.fork_sequence(0, 2)
