@@ -75,7 +75,8 @@ def cmd_train(argv: List[str]) -> None:
 def _engine_config(a):
     from ..inference.engine import InferenceConfig
 
-    return InferenceConfig(kv_cache_dtype=a.kv_cache_dtype, kv_evict_budget=a.kv_evict_budget)
+    return InferenceConfig(kv_cache_dtype=a.kv_cache_dtype, kv_evict_budget=a.kv_evict_budget,
+                           kv_evict_recent=a.kv_evict_recent, kv_evict_slack=a.kv_evict_slack)
 
 
 def cmd_generate(a) -> None:
@@ -343,6 +344,10 @@ def build_parser() -> argparse.ArgumentParser:
                        help="hold the KV cache in 8 bits")
         p.add_argument("--kv-evict-budget", type=int, default=0,
                        help="cached tokens kept for a sequence (8-bit cache; 0: all)")
+        p.add_argument("--kv-evict-recent", type=int, default=None,
+                       help="of these, the last ones (default: 64, or half of a smaller budget)")
+        p.add_argument("--kv-evict-slack", type=int, default=256,
+                       help="tokens past the budget at which a sequence is cut to it")
 
     g = sub.add_parser("generate")
     model_args(g)

@@ -57,6 +57,8 @@ class BatchConfig:
     timeout_seconds: float = 60.0
     kv_cache_dtype: Optional[str] = None   # see InferenceConfig
     kv_evict_budget: int = 0
+    kv_evict_recent: Optional[int] = None
+    kv_evict_slack: int = 256
 
 
 class ContinuousBatcher:
@@ -67,7 +69,9 @@ class ContinuousBatcher:
                                max_tokens_per_step=self.config.max_tokens_per_batch or 8192,
                                prefill_chunk_size=self.config.prefill_chunk_size,
                                kv_cache_dtype=self.config.kv_cache_dtype,
-                               kv_evict_budget=self.config.kv_evict_budget)
+                               kv_evict_budget=self.config.kv_evict_budget,
+                               kv_evict_recent=self.config.kv_evict_recent,
+                               kv_evict_slack=self.config.kv_evict_slack)
         self.engine = InferenceEngine(model, icfg)
         self.requests: Dict[str, Request] = {}
         self._eng_ids: Dict[int, str] = {}

@@ -82,7 +82,7 @@ class InferenceConfig:
     # those that received the most attention; 0: keep everything.  The pool has the pages of
     # one budget beside ``num_pages``, to move kept tokens to when all others are taken
     kv_evict_budget: int = 0
-    kv_evict_recent: int = 64
+    kv_evict_recent: Optional[int] = None    # default: 64, or half of a budget below 64
     kv_evict_slack: int = 256
 
 
@@ -168,8 +168,11 @@ class InferenceEngine:
         cfg = self.config
         if cfg.kv_evict_budget and cfg.kv_cache_dtype is None:
             raise ValueError("kv_evict_budget needs an 8-bit cache (kv_cache_dtype)")
+        self.kv_evict_recent = cfg.kv_evict_recent
+        if self.kv_evict_recent is None:
+            self.kv_evict_recent = 64 if cfg.kv_evict_budget >= 64 else cfg.kv_evict_budget // 2
         if cfg.kv_evict_budget < 0 or (cfg.kv_evict_budget and not (
-                0 <= cfg.kv_evict_recent <= cfg.kv_evict_budget and cfg.kv_evict_slack >= 1)):
+                0 <= self.kv_evict_recent <= cfg.kv_evict_budget and cfg.kv_evict_slack >= 1)):
             raise ValueError("need 0 <= kv_evict_recent <= kv_evict_budget and a positive slack")
         if cfg.kv_cache_dtype is None:
             self.pool = PagePool(mc.num_hidden_layers, kv_heads, mc.head_dim, pages,
@@ -308,7 +311,7 @@ class InferenceEngine:
                 if n >= cfg.kv_evict_budget + cfg.kv_evict_slack]
         while over:
             some = over[:max(1, len(self.pool.free) // each)]
-            self.pool.evict(some, cfg.kv_evict_budget, cfg.kv_evict_recent)
+            self.pool.evict(some, cfg.kv_evict_budget, self.kv_evict_recent)
             self.stats["evictions"] = self.stats.get("evictions", 0) + len(some)
             over = over[len(some):]
 

@@ -168,3 +168,31 @@ def test_pages_held_for_evictions():
     pool.reserve(1, 32)
     with pytest.raises(OutOfPages):
         pool.fork_sequence(0, 2)
+
+
+def test_small_budgets_and_the_recent_tokens_option():
+    """A budget below 64 needs no further option; batcher and command line can set the rest."""
+    from complexity_framework_b200.cli.app import _engine_config, build_parser
+    from complexity_framework_b200.inference import (BatchConfig, ContinuousBatcher,
+                                                     InferenceConfig, InferenceEngine)
+
+    m = small_model()
+    for budget, want in ((1, 0), (48, 24), (64, 64), (1024, 64)):
+        eng = InferenceEngine(m, InferenceConfig(max_cache_length=64, max_batch_size=1,
+                                                 kv_cache_dtype="int8", kv_evict_budget=budget))
+        assert eng.kv_evict_recent == want
+    b = ContinuousBatcher(m, BatchConfig(max_batch_size=1, max_sequence_length=64,
+                                         kv_cache_dtype="fp8", kv_evict_budget=48,
+                                         kv_evict_recent=8, kv_evict_slack=5))
+    got = b.engine.config
+    assert (got.kv_evict_budget, got.kv_evict_recent, got.kv_evict_slack) == (48, 8, 5)
+    base = ["bench-infer", "--model", "x", "--kv-cache-dtype", "int8", "--kv-evict-budget", "48"]
+    for more, recent, slack in (([], None, 256),
+                                (["--kv-evict-recent", "7", "--kv-evict-slack", "9"], 7, 9)):
+        c = _engine_config(build_parser().parse_args(base + more))
+        assert (c.kv_evict_budget, c.kv_evict_recent, c.kv_evict_slack) == (48, recent, slack)
+        InferenceEngine(m, c)
+    with pytest.raises(ValueError):
+        InferenceEngine(m, InferenceConfig(max_cache_length=64, max_batch_size=1,
+                                           kv_cache_dtype="int8", kv_evict_budget=48,
+                                           kv_evict_recent=49))
