@@ -78,8 +78,8 @@ __device__ __forceinline__ void p8_to_float(uint32_t w, float* f) {
 }
 
 // Four scaled values, finite and |f| <= levels up to rounding, to codes: to nearest, ties to
-// even.  int8 rounds in the adder: f + 1.5 * 2^23 has the integer in its low byte.  (The
-// conversion instruction runs at an eighth of the adder's rate, and an append would wait on it.)
+// even.  int8 rounds in the adder: f + 1.5 * 2^23 has the integer in its low byte: no
+// conversion, and byte permutations gather the codes.
 template <int FMT>
 __device__ __forceinline__ uint32_t p8_from_float(const float* f) {
   if constexpr (FMT == kP8Int8) {

@@ -14,6 +14,8 @@
 namespace cfb {
 
 constexpr int kP8Page = 16;  // tokens of a page, and of a scale block
+// Rows (new tokens x query heads of a KV head) up to which a chunk takes the decode kernel.
+constexpr int kP8ShortRows = 64;
 
 enum P8Fmt : int { kP8Int8 = 0, kP8E4m3 = 1 };
 enum P8Type : int { kP8Bf16 = 0, kP8Half = 1 };

@@ -21,12 +21,17 @@
 // subnormal (c + 128) 2^-24, which is its byte with the sign bit flipped and needs one byte
 // permutation for two codes.  The offset comes out again exactly where it went in: 128 sum(q)
 // is subtracted from the score, 128 sum(P) (an MMA against ones, so of the rounded P) from the
-// output.  q is scaled by a power of two per row into f16 range, where a bf16 q is exact too.
+// output; the score's 32-bit sum carries 128 sum|q| in place of sum|q c| on the way.
+// q is scaled by a power of two per row into f16 range.  A bf16 element is exact there down to
+// 2^-17 of the row's largest; below it loses at most 2^-25 of the largest, as much as the 32-bit
+// sum may.  (The long chunks' products take a bf16 q as it is.)
 // Scores, maxima, sums and the output accumulate in fp32; the probabilities are rounded to
 // f16 (11 bits, against 8 of bf16).
 // V's block scale cannot be taken out of the sum over blocks, so it goes into the exponent:
 // with w_j = s_j + log2 vs[b(j)] and M a running bound of w,
 //   P_j = 2^(w_j - M),  O = sum P_j cV_j,  l = sum P_j / vs[b(j)],  o = O / l.
+// What P loses to f16's subnormals, where a block's vs lies 2^14 or more below the largest
+// product's, is at most 2^-25 of that product.
 // M moves only when some w exceeds it by more than 2^8 (then by a warp-wide maximum), which
 // leaves one vote per page in the usual case.
 //
@@ -54,7 +59,6 @@ constexpr int kWarps = 4;
 constexpr int kStages = 4;                   // pages of a warp's ring: two used, two in flight
 constexpr int kWholePages = 32;              // up to here an item is one CTA's
 constexpr int kMinPages = 32, kMaxPages = 64;  // chunk of a CTA otherwise
-constexpr int kMaxRows = 64;                 // rows of a KV head (longer chunks: paged8_chunk.cu)
 constexpr float kGrow = 8.f;                 // log2 of how far P may exceed 1
 constexpr float kNone = -1e30f;              // M before any visible key
 constexpr float kTinyScale = 7.888609e-31f;  // 2^-100: V blocks below it count as zeros
@@ -669,7 +673,7 @@ __global__ void __launch_bounds__(256)
     p8_finish_kernel(const AttnParams p, int join_ctas, int wpr) {
   constexpr int R = 8 * NB;
   constexpr int VL = D / 32;  // dims of a lane
-  __shared__ float s_lse[kMaxRows];
+  __shared__ float s_lse[kP8ShortRows];
   __shared__ float s_acc[8][D];
   const int seq = blockIdx.y / p.c.Hkv, h = blockIdx.y % p.c.Hkv;
   const SeqInfo si = seq_info(p, seq);  // inputs, complete before p8_attn_kernel began
@@ -925,7 +929,7 @@ int p8_attention(const P8Cache& c, const P8Seqs& s, const P8Attn& a, const P8Att
   const int64_t heads = static_cast<int64_t>(s.num_seqs) * c.Hkv;
   if (heads > 65535 || c.num_pages * c.Hkv > 0x7fffffff ||
       static_cast<int64_t>(plan.splits) * plan.row_tiles > 0x7fffffff ||
-      plan.chunk > 32 * kWarps || static_cast<int64_t>(a.max_q_len) * (a.Hq / c.Hkv) > kMaxRows)
+      plan.chunk > 32 * kWarps || static_cast<int64_t>(a.max_q_len) * (a.Hq / c.Hkv) > kP8ShortRows)
     return -3;
   AttnParams p;
   p.c = c;

@@ -68,12 +68,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code, site));
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 // 16 columns of TMEM into registers, and the wait that makes them readable: the registers
 // pass through the wait, so no use of them can move before it.
 __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
@@ -1013,7 +1007,7 @@ int launch_chunk(const P8Cache& c, const P8Seqs& s, const P8Attn& a, int* err, c
 // one of 2048 16.4 and 17.0,
 // one of 32768 72.2 and 71.4, 8 of 16384 187 and 231; at 32 rows 16 of 2048 take 42 and 61.
 bool p8_is_chunk(int max_q_len, int group) {
-  return static_cast<int64_t>(max_q_len) * group > 64;
+  return static_cast<int64_t>(max_q_len) * group > kP8ShortRows;
 }
 
 void p8_chunk_plan(const P8Seqs& s, int Hkv, int group, int max_q_len, int num_sms, int* nq,

@@ -25,6 +25,7 @@ from .paged import OutOfPages, PagedBatch, PagePool, SeqChunk, StaticDecodeBatch
 CODE_TYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 
 #: rows (new tokens x query heads of a KV head) up to which a sequence takes the decode kernel
+#: (``kP8ShortRows`` of the kernels)
 SHORT_ROWS = 64
 
 
