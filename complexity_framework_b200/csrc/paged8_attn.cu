@@ -44,7 +44,7 @@
 // slower (39.0 us against 36.3, with weights 60.8 against 49.7, at the time): it needs all its
 // CTAs' slots at once.
 //
-// Measured (D 128, int8, GQA 32/8, whole calls): 64 requests of 129 to 2304 tokens 34.2 us, 4.3
+// Measured (D 128, int8, GQA 32/8, whole calls): 64 requests of 129 to 2304 tokens 34.1 us, 4.3
 // TB/s, bound by start, last wave and join; 256 of 1000 tokens 86.2 us, 6.1 TB/s (0.95 of a copy).
 // 311 warp instructions for a page of one head, 42% of the issue slots.
 #include <algorithm>

@@ -22,8 +22,8 @@
 // keys of two row tiles, of which their exponentials need 2100).  A cubic on the FMA pipe for
 // a share of the exponentials was not worth its code (140.9 us with a quarter of them, 142.8
 // without, before later changes).
-// Measured: 2 x 1024 tokens over 3077 and 5120, GQA 32/8, D 128: 147 us with the expansion (12),
-// 819 TFLOP/s, tensor pipe 45% and exponential unit 46% busy; neither is the limit, likely the
+// Measured: 2 x 1024 tokens over 3077 and 5120, GQA 32/8, D 128: 146 us with the expansion (12),
+// 825 TFLOP/s, tensor pipe 45% and exponential unit 46% busy; neither is the limit, likely the
 // softmax warps' waits.  Half a row a thread (twice the warps) was slower: 159 us against 144.
 // p8_chunk_mass_kernel: weights summed over the rows need each row's final log-sum-exp, so
 // they are recomputed: one CTA per (128 keys, KV head, sequence) walks the row tiles with

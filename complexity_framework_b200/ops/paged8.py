@@ -56,8 +56,8 @@ def paged8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales:
     A block's scale is the largest magnitude among its new tokens over the largest code, or
     its present scale where that is larger and the block holds older tokens; the older codes
     are rounded anew when the scale grows.  ``kv_lens`` counts the new tokens; ``max_q_len``
-    bounds the new tokens of a sequence; the new tokens' ``mass`` starts at 0.  A block with a value that is not finite reads as NaN
-    or infinity throughout.
+    bounds the new tokens of a sequence; the new tokens' ``mass`` starts at 0.  A block with a
+    value that is not finite reads as NaN or infinity throughout.
     """
     if codes.is_cuda:
         require().paged8_append(k, v, codes, scales, page_table, cu_q, kv_lens, max_q_len, mass)
@@ -136,6 +136,8 @@ def paged8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
 
     With ``mass`` the softmax weights every cached token receives from this call are added to
     it: in place, or into ``mass_out`` (which takes the tokens of this call's sequences only).
+    Rows of ``out`` before ``cu_q[0]`` or from ``cu_q[-1]`` on, which are other calls', stay as
+    they are.
     Long chunks expand keys and values to 16 bits first, and short ones with ``mass`` keep their
     scores, both as long as the page table is wide: in a workspace of about ``workspace_bytes``
     at most (or one sequence's, where that is more), with the sequences taken in parts.
