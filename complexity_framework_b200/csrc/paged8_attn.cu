@@ -23,8 +23,8 @@
 // is subtracted from the score, 128 sum(P) (an MMA against ones, so of the rounded P) from the
 // output; the score's 32-bit sum carries 128 sum|q| in place of sum|q c| on the way.
 // q is scaled by a power of two per row into f16 range.  A bf16 element is exact there down to
-// 2^-17 of the row's largest; below it loses at most 2^-25 of the largest, as much as the 32-bit
-// sum may.  (The long chunks' products take a bf16 q as it is.)
+// 2^-17 of the row's largest; below it loses at most 2^-25 of the largest.  (The long chunks'
+// products take a bf16 q as it is.)
 // Scores, maxima, sums and the output accumulate in fp32; the probabilities are rounded to
 // f16 (11 bits, against 8 of bf16).
 // V's block scale cannot be taken out of the sum over blocks, so it goes into the exponent:
