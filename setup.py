@@ -23,6 +23,8 @@ SOURCES = [
     "paged8_cache.cu",
     "paged8_attn.cu",
     "paged8_chunk.cu",
+    "bind_stream.cpp",
+    "residual.cu",
     "dist_fused.cu",
     "noalloc.cu",
     "tp_fused.cu",
