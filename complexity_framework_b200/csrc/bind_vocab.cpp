@@ -1,0 +1,162 @@
+// Python bindings of the cross-entropy over the vocabulary (vocab_loss.cu).
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <cmath>
+
+#include "vocab_loss.h"
+
+int* cfb_err_ptr(int device);
+int cfb_num_sms(int device);
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+Tensor empty(at::IntArrayRef sizes, torch::ScalarType dtype, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
+}
+
+// A bf16 matrix of contiguous, 16-byte-aligned rows; other layouts are copied.
+Tensor matrix(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK_TYPE(t.scalar_type() == torch::kBFloat16, name, " must be bfloat16, got ",
+                   t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == 2, name, " must be 2-D");
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 != 0 ? c.clone() : c;
+}
+__nv_bfloat16* bf(const Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
+
+void check_rc(int rc) {
+  TORCH_CHECK(rc == 0, "vocab_loss failed with code ", rc, " ",
+              rc > 0 && rc < 1000 ? cudaGetErrorString(static_cast<cudaError_t>(rc)) : "");
+}
+
+cfb::VlCall call_of(int64_t T, const Tensor& w, double scale, double smooth, double z,
+                    int64_t ignore) {
+  TORCH_CHECK_VALUE(T <= 0x7fffff00 && w.size(0) >= 1 && w.size(0) <= 0x7fffff00,
+                    "too many rows or words");
+  TORCH_CHECK_VALUE(w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(1) <= (1 << 20),
+                    "the hidden size must be a multiple of 8, got ", w.size(1));
+  TORCH_CHECK_VALUE(std::isfinite(scale), "logit_scale must be finite");
+  TORCH_CHECK_VALUE(smooth >= 0.0 && smooth <= 1.0, "label_smoothing must be between 0 and 1");
+  TORCH_CHECK_VALUE(z >= 0.0 && std::isfinite(z), "z_loss must not be negative");
+  cfb::VlCall c;
+  c.T = T;
+  c.V = static_cast<int>(w.size(0));
+  c.H = static_cast<int>(w.size(1));
+  c.scale = static_cast<float>(scale);
+  c.smooth = static_cast<float>(smooth);
+  c.z = static_cast<float>(z);
+  c.ignore = ignore;
+  c.w = bf(w);
+  c.num_sms = cfb_num_sms(w.get_device());
+  c.err = cfb_err_ptr(w.get_device());
+  return c;
+}
+
+// ints: cnt [2] (and two spare) | target [R] | src [R] | pos [T];  floats: lse2 [R] | ginv [1]
+void bind_saved(cfb::VlCall& c, const Tensor& hc, const Tensor& ints, const Tensor& floats) {
+  const int64_t R = cfb::vl_rows(c.T);
+  TORCH_CHECK(hc.numel() == R * c.H && ints.numel() == 4 + 2 * R + c.T && floats.numel() == R + 1,
+              "saved tensors do not match");
+  int* p = ints.data_ptr<int>();
+  c.cnt = p;
+  c.target = p + 4;
+  c.src = p + 4 + R;
+  c.pos = p + 4 + 2 * R;
+  c.hc = bf(hc);
+  c.lse2 = floats.data_ptr<float>();
+  c.ginv = c.lse2 + R;
+}
+
+// reduction: 0 none (the row losses), 1 mean over the counted rows, 2 sum.  Returns the loss and
+// what the backward pass needs: compact rows, index and row tensors, the weight as it was read.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> vocab_loss_fwd(
+    const Tensor& h_in, const Tensor& w_in, const Tensor& y_in, int64_t ignore, double smooth,
+    double z, double scale, int64_t reduction) {
+  TORCH_CHECK(w_in.is_cuda(), "weight must be a CUDA tensor");
+  const c10::cuda::CUDAGuard guard(w_in.device());
+  const Tensor h = matrix(h_in, "hidden"), w = matrix(w_in, "weight");
+  TORCH_CHECK(h.get_device() == w.get_device() && y_in.is_cuda() &&
+                  y_in.get_device() == w.get_device(),
+              "hidden, weight and targets must be on one CUDA device");
+  TORCH_CHECK_VALUE(h.size(1) == w.size(1), "hidden and weight must have one hidden size");
+  TORCH_CHECK_TYPE(y_in.scalar_type() == torch::kInt64, "targets must be int64");
+  TORCH_CHECK_VALUE(y_in.dim() == 1 && y_in.size(0) == h.size(0), "targets must be [rows]");
+  TORCH_CHECK(reduction >= 0 && reduction <= 2, "bad reduction");
+  const Tensor y = y_in.contiguous();
+  const int64_t T = h.size(0), R = cfb::vl_rows(T);
+  cfb::VlCall c = call_of(T, w, scale, smooth, z, ignore);
+  Tensor hc = empty({R, c.H}, torch::kBFloat16, w);
+  Tensor ints = empty({4 + 2 * R + T}, torch::kInt32, w);
+  Tensor floats = empty({R + 1}, torch::kFloat32, w);
+  bind_saved(c, hc, ints, floats);
+  Tensor rows = empty({T}, torch::kFloat32, w), total;
+  cfb::VlForward f;
+  f.h = bf(h);
+  f.targets = y.data_ptr<int64_t>();
+  f.rows = rows.data_ptr<float>();
+  f.mean = reduction == 1;
+  if (reduction != 0) {
+    total = empty({}, torch::kFloat32, w);
+    f.total = total.data_ptr<float>();
+  }
+  if (T == 0) {
+    if (reduction != 0) total.zero_();
+    return {reduction == 0 ? rows : total, hc, ints, floats, w};
+  }
+  const Tensor ws = empty({cfb::vl_forward_floats(c)}, torch::kFloat32, w);
+  f.ws = ws.data_ptr<float>();
+  check_rc(cfb::vl_forward(c, f, at::cuda::getCurrentCUDAStream()));
+  return {reduction == 0 ? rows : total, hc, ints, floats, w};
+}
+
+// (dhidden [T, H], dweight [V, H]), each where it is needed.
+std::tuple<OptTensor, OptTensor> vocab_loss_bwd(const Tensor& gout_in, const Tensor& hc,
+                                                const Tensor& ints, const Tensor& floats,
+                                                const Tensor& w, int64_t T, double smooth, double z,
+                                                double scale, bool per_row, bool need_h,
+                                                bool need_w, int64_t workspace_bytes) {
+  const c10::cuda::CUDAGuard guard(w.device());
+  cfb::VlCall c = call_of(T, w, scale, smooth, z, 0);
+  bind_saved(c, hc, ints, floats);
+  OptTensor dh, dw;
+  if (need_h) dh = empty({T, c.H}, torch::kBFloat16, w);
+  if (need_w) dw = empty({c.V, c.H}, torch::kBFloat16, w);
+  if (T == 0 || !(need_h || need_w)) {
+    if (dw.has_value()) dw->zero_();
+    return {dh, dw};
+  }
+  TORCH_CHECK(gout_in.is_cuda() && gout_in.get_device() == w.get_device() &&
+                  gout_in.scalar_type() == torch::kFloat32 &&
+                  gout_in.numel() == (per_row ? T : 1),
+              "bad gradient of the loss");
+  const Tensor gout = gout_in.contiguous();
+  cfb::VlBackward b;
+  b.gout = gout.data_ptr<float>();
+  b.per_row = per_row;
+  cfb::vl_backward_plan(c, workspace_bytes, &b);
+  const Tensor dl = empty({cfb::vl_rows(T), b.piece}, torch::kBFloat16, w);
+  b.dl = bf(dl);
+  Tensor acc;
+  if (need_h) {
+    acc = empty({cfb::vl_acc_floats(c, b)}, torch::kFloat32, w);
+    b.acc = acc.data_ptr<float>();
+    b.dh = bf(*dh);
+  }
+  if (need_w) b.dw = bf(*dw);
+  check_rc(cfb::vl_backward(c, b, at::cuda::getCurrentCUDAStream()));
+  return {dh, dw};
+}
+
+}  // namespace
+
+void register_vocab(pybind11::module& m) {
+  m.def("vocab_loss_fwd", &vocab_loss_fwd);
+  m.def("vocab_loss_bwd", &vocab_loss_bwd);
+}

@@ -695,6 +695,7 @@ int64_t gemm_choose_bn(int64_t M, int64_t N, int64_t device) {
 void register_elementwise(pybind11::module& m);
 void register_paged8(pybind11::module& m);
 void register_stream(pybind11::module& m);
+void register_vocab(pybind11::module& m);
 
 int* cfb_err_ptr(int device) { return err_ptr(device); }
 int cfb_num_sms(int device) { return num_sms(device); }
@@ -747,4 +748,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_elementwise(m);
   register_paged8(m);
   register_stream(m);
+  register_vocab(m);
 }

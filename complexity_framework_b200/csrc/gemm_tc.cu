@@ -45,7 +45,8 @@ constexpr int kBK = 64;
 // output of a column chunk in flight while the next chunk is converted.
 __host__ __device__ constexpr int epi_slots(int epi) {
   return epi == EPI_SWIGLU_FWD ? 3
-         : (epi == EPI_STORE || epi == EPI_RESID || epi == EPI_CE_STATS) ? 2 : 0;
+         : (epi == EPI_STORE || epi == EPI_RESID || epi == EPI_CE_STATS || epi == EPI_CE_GRAD)
+             ? 2 : 0;
 }
 // Epilogue operands read by TMA (32x32 bf16 boxes per column chunk): the
 // residual for EPI_RESID, the saved gate and up pre-activations for
@@ -230,9 +231,25 @@ struct SegMaps {
 // K blocks [kb0, kb1), group g.  Every role decodes the same units, so a unit
 // without work is skipped by all of them (no loads, MMAs or epilogue hand-off).
 struct Unit {
-  int t, kb0, kb1, g;
+  int t, kb0, kb1, g, s;
   bool skip;
 };
+
+// Row and column tile of schedule position t: row by row, or in groups of group_m row tiles
+// whose column tiles come one after the other (a wide B is then read once a group, not once a
+// row tile).
+__device__ __forceinline__ void tile_at(int t, int num_m, int num_n, int group_m, int* m, int* n) {
+  if (group_m <= 0) {
+    *m = t / num_n;
+    *n = t % num_n;
+    return;
+  }
+  const int g = t / (group_m * num_n), first = g * group_m;
+  const int rows = num_m - first < group_m ? num_m - first : group_m;
+  const int in = t - first * num_n;
+  *n = in / rows;
+  *m = first + in % rows;
+}
 
 __device__ __forceinline__ Unit decode_unit(int u, int num_tiles, int num_n, int num_m,
                                             int m_shift, int ksplit, int nk, const GemmGroups& gr) {
@@ -242,7 +259,7 @@ __device__ __forceinline__ Unit decode_unit(int u, int num_tiles, int num_n, int
     r.g = u / per_group;
     const int rem = u % per_group;
     r.t = rem / ksplit;
-    const int s = rem % ksplit;
+    const int s = r.s = rem % ksplit;
     const int g0 = __ldg(gr.k_start + r.g) / 64, g1 = __ldg(gr.k_start + r.g + 1) / 64;
     r.kb0 = g0 + s * (g1 - g0) / ksplit;
     r.kb1 = g0 + (s + 1) * (g1 - g0) / ksplit;
@@ -250,8 +267,9 @@ __device__ __forceinline__ Unit decode_unit(int u, int num_tiles, int num_n, int
     return r;
   }
   r.t = u / ksplit;
-  r.kb0 = (u % ksplit) * nk / ksplit;
-  r.kb1 = ((u % ksplit) + 1) * nk / ksplit;
+  r.s = u % ksplit;
+  r.kb0 = static_cast<int>(static_cast<int64_t>(r.s) * nk / ksplit);
+  r.kb1 = static_cast<int>(static_cast<int64_t>(r.s + 1) * nk / ksplit);
   r.g = 0;
   r.skip = false;
   if (gr.mode == 1) {
@@ -266,7 +284,7 @@ __global__ void __launch_bounds__(384, 1)
     gemm_tc_kernel(const __grid_constant__ SegMaps<NA> tmA,
                    const __grid_constant__ SegMaps<NB> tmB,
                    const __grid_constant__ CUtensorMap tmC0,
-                   const __grid_constant__ CUtensorMap tmC1, int M, int N, int K, int ksplit,
+                   const __grid_constant__ CUtensorMap tmC1, int M_max, int N, int K_max, int ksplit,
                    GemmEpi ep, int* err) {
   constexpr int SLOTS = epi_slots(EPI);
   constexpr int LOADS = epi_loads(EPI);
@@ -295,6 +313,8 @@ __global__ void __launch_bounds__(384, 1)
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
+  const int M = ep.m_dev != nullptr ? min(M_max, __ldg(ep.m_dev)) : M_max;
+  const int K = ep.k_dev != nullptr ? min(K_max, __ldg(ep.k_dev)) : K_max;
   const int num_m = (M + Cfg::TILE_M - 1) / Cfg::TILE_M;
   // with the fused all-gather, this rank's own row tiles come first
   const int m_shift = ep.ag.active ? (ep.sync.rank * ep.ag.rows) / Cfg::TILE_M : 0;
@@ -357,9 +377,11 @@ __global__ void __launch_bounds__(384, 1)
       for (int u = unit; u < total && ok; u += units) {
         const Unit un = decode_unit(u, num_tiles, num_n, num_m, m_shift, ksplit, nk, ep.grp);
         if (un.skip) continue;
-        const int t = un.t, kb0 = un.kb0, kb1 = un.kb1;
-        const int m0 = ((t / num_n + m_shift) % num_m) * Cfg::TILE_M + static_cast<int>(rank) * kBM;
-        const int n0 = (t % num_n) * BN;
+        const int kb0 = un.kb0, kb1 = un.kb1;
+        int m_blk, n_blk;
+        tile_at(un.t, num_m, num_n, ep.group_m, &m_blk, &n_blk);
+        const int m0 = ((m_blk + m_shift) % num_m) * Cfg::TILE_M + static_cast<int>(rank) * kBM;
+        const int n0 = n_blk * BN;
         // row-grouped: this group's B rows (K-major B) or K rows (MN-major B)
         const int b_off = ep.grp.mode == 1 ? static_cast<int>(un.g * ep.grp.b_stride) : 0;
         if (ep.ag.active) {
@@ -455,7 +477,9 @@ __global__ void __launch_bounds__(384, 1)
       for (int u = unit; u < total && ok; u += units) {
         const Unit un = decode_unit(u, num_tiles, num_n, num_m, m_shift, ksplit, nk, ep.grp);
         if (un.skip) continue;
-        const int t = un.t, kb0 = un.kb0, kb1 = un.kb1;
+        const int kb0 = un.kb0, kb1 = un.kb1;
+        int m_blk, n_blk;
+        tile_at(un.t, num_m, num_n, ep.group_m, &m_blk, &n_blk);
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, abort_flag, err, kErrTimeoutTmem, 11)) {
           ok = false;
           break;
@@ -463,7 +487,7 @@ __global__ void __launch_bounds__(384, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         // the last column tile may be narrower than BN: issue a narrower MMA
-        const int n_rem = N - (t % num_n) * BN;
+        const int n_rem = N - n_blk * BN;
         const uint32_t idesc = idesc_bf16(Cfg::TILE_M, n_rem < BN ? n_rem : BN, A_MN, B_MN);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, abort_flag, err, kErrTimeoutFull, 12)) {
@@ -567,11 +591,11 @@ __global__ void __launch_bounds__(384, 1)
     for (int u = unit; u < total; u += units) {
       const Unit un = decode_unit(u, num_tiles, num_n, num_m, m_shift, ksplit, nk, ep.grp);
       if (un.skip) continue;
-      const int t = un.t;
       // K-grouped weight gradients: this group's output rows
       const int64_t c_row0 = ep.grp.mode == 2 ? un.g * ep.grp.c_stride : 0;
-      const int m_blk = (t / num_n + m_shift) % num_m;
-      const int n_blk = t % num_n;
+      int m_blk, n_blk;
+      tile_at(un.t, num_m, num_n, ep.group_m, &m_blk, &n_blk);
+      m_blk = (m_blk + m_shift) % num_m;
       const int m0 = m_blk * Cfg::TILE_M + static_cast<int>(rank) * kBM;
       const int n0 = n_blk * BN;
       // operand boxes of the warp's first column chunk load while the MMA runs
@@ -718,6 +742,92 @@ __global__ void __launch_bounds__(384, 1)
           // one (max, sumexp) pair per half tile (BN/2 columns)
           st[static_cast<int64_t>(row) * num_n * 2 + n_blk * 2 + wg] = make_float2(mx, se);
         }
+      } else if constexpr (EPI == EPI_CE_FWD) {
+        // Softmax statistics of the half tile in units of log 2; columns from n_valid on are
+        // padding.  A half tile of -inf alone has the maximum -inf and the sum 0.
+        const int half = 2 * n_blk + wg;
+        const int64_t at = static_cast<int64_t>(row) * 2 * num_n + half;
+        const int tgt = row_ok ? ep.ce.target[row] : -1;
+        float mx = -INFINITY, se = 0.0f, zs = 0.0f;
+#pragma unroll 1
+        for (int c = wg * BN / 2; c < (wg + 1) * BN / 2; c += 32) {
+          const int left = ep.ce.n_valid - (n0 + c);
+          if (left <= 0) break;  // warp-uniform
+          float v[32];
+          tmem_ld32(tbase + c, v);
+          tmem_wait_ld();
+          const int ti = tgt - (n0 + c);
+          if (ti >= 0 && ti < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i == ti) ep.ce.zt[row] = v[i] * ep.ce.scale;
+          }
+          if (ep.ce.zsum != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) zs += v[i];  // padding columns are 0
+          }
+          float lm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (left >= 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              v[i] *= ep.ce.k2;
+              lm[i & 3] = fmaxf(lm[i & 3], v[i]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              v[i] = i < left ? v[i] * ep.ce.k2 : -INFINITY;
+              lm[i & 3] = fmaxf(lm[i & 3], v[i]);
+            }
+          }
+          const float nm = fmaxf(fmaxf(fmaxf(lm[0], lm[1]), fmaxf(lm[2], lm[3])), mx);
+          const float base = nm == -INFINITY ? 0.0f : nm;
+          float s[4] = {se * exp2_approx(mx - base), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i & 3] += exp2_approx(v[i] - base);
+          se = (s[0] + s[1]) + (s[2] + s[3]);
+          mx = nm;
+        }
+        if (row_ok) {
+          ep.ce.stats[at] = make_float2(mx, se);
+          if (ep.ce.zsum != nullptr) ep.ce.zsum[at] = zs * ep.ce.scale;
+        }
+      } else if constexpr (EPI == EPI_CE_GRAD) {
+        // d(logits) = ga p - gc, less gb at the target; rows past the last one give 0, which the
+        // weight gradient's last K block reads.
+        float lse2 = 0.0f, ga = 0.0f, gb = 0.0f, gc = 0.0f;
+        int tgt = -1;
+        const int src = row_ok ? ep.ce.src[row] : -1;
+        if (src >= 0) {
+          float g = ep.ce.gout[ep.ce.per_row ? src : 0] * ep.ce.scale;
+          if (ep.ce.ginv != nullptr) g *= *ep.ce.ginv;
+          lse2 = ep.ce.lse2[row];
+          ga = g * (1.0f + ep.ce.z2 * (lse2 * 0.693147180559945f));
+          gb = g * (1.0f - ep.ce.smooth);
+          gc = g * ep.ce.smooth_v;
+          tgt = ep.ce.target[row] - ep.ce.col0;
+        }
+#pragma unroll 1
+        for (int c = wg * BN / 2; c < (wg + 1) * BN / 2; c += 32) {
+          if (n0 + c >= N) break;  // warp-uniform
+          float v[32];
+          tmem_ld32(tbase + c, v);
+          tmem_wait_ld();
+          const int ti = tgt - (n0 + c);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] = fmaf(ga, exp2_approx(fmaf(v[i], ep.ce.k2, -lse2)), -gc);
+          if (ti >= 0 && ti < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i == ti) v[i] -= gb;
+          }
+          if (src < 0) {  // also where the row held something that is not finite
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+          }
+          ring.put(&tmC0, v, 1.0f, n0 + c, m0 + wq * 32);
+        }
       } else {
 #pragma unroll 1
         for (int c = wg * BN / 2; c < (wg + 1) * BN / 2; c += 32) {
@@ -764,6 +874,7 @@ __global__ void __launch_bounds__(384, 1)
                            v[4 * q + 2] * ep.alpha, v[4 * q + 3] * ep.alpha);
             } else if constexpr (EPI == EPI_F32 || EPI == EPI_F32_ACC) {
               float4* out = reinterpret_cast<float4*>(reinterpret_cast<float*>(ep.c) +
+                                                      un.s * ep.split_stride +
                                                       static_cast<int64_t>(row) * ep.ldc + n0 + c);
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
@@ -962,8 +1073,9 @@ static int launch_impl(const SegMaps<NA>& ta, const SegMaps<NB>& tb, const CUten
 template <int BN, bool A_MN, bool B_MN, int EPI>
 static int launch_pair_or_single(const SegMaps<1>& ta, const SegMaps<1>& tb, const CUtensorMap* tc,
                                  int M, int N, int K, const GemmEpi& ep, int sms, cudaStream_t s,
-                                 int* err) {
-  const int ks = EPI == EPI_F32_ATOMIC ? 0 : 1;  // 0 = choose
+                                 int* err, int ksplit = 1) {
+  // 0 = choose
+  const int ks = EPI == EPI_F32_ATOMIC ? 0 : EPI == EPI_F32 || EPI == EPI_F32_ACC ? ksplit : 1;
   // 256-row tiles over an SM pair halve each SM's operand traffic per FLOP;
   // a single 128-row tile is used only when M itself fits in one.
   // (keep in sync with the B tensor-map box chosen in gemm_tc_launch)
@@ -974,14 +1086,14 @@ static int launch_pair_or_single(const SegMaps<1>& ta, const SegMaps<1>& tb, con
 template <int BN, int EPI>
 static int dispatch_major(bool a_mn, bool b_mn, const SegMaps<1>& ta, const SegMaps<1>& tb,
                           const CUtensorMap* tc, int M, int N, int K, const GemmEpi& ep, int sms,
-                          cudaStream_t s, int* err) {
+                          cudaStream_t s, int* err, int ksplit) {
   if (!a_mn && !b_mn)
-    return launch_pair_or_single<BN, false, false, EPI>(ta, tb, tc, M, N, K, ep, sms, s, err);
+    return launch_pair_or_single<BN, false, false, EPI>(ta, tb, tc, M, N, K, ep, sms, s, err, ksplit);
   if (!a_mn && b_mn)
-    return launch_pair_or_single<BN, false, true, EPI>(ta, tb, tc, M, N, K, ep, sms, s, err);
+    return launch_pair_or_single<BN, false, true, EPI>(ta, tb, tc, M, N, K, ep, sms, s, err, ksplit);
   if (a_mn && !b_mn)
-    return launch_pair_or_single<BN, true, false, EPI>(ta, tb, tc, M, N, K, ep, sms, s, err);
-  return launch_pair_or_single<BN, true, true, EPI>(ta, tb, tc, M, N, K, ep, sms, s, err);
+    return launch_pair_or_single<BN, true, false, EPI>(ta, tb, tc, M, N, K, ep, sms, s, err, ksplit);
+  return launch_pair_or_single<BN, true, true, EPI>(ta, tb, tc, M, N, K, ep, sms, s, err, ksplit);
 }
 
 int choose_bn(int M, int N, int num_sms) {
@@ -997,6 +1109,8 @@ static int make_operand_map(CUtensorMap* map, const void* base, bool mn, int64_t
             : make_tmap_2d(map, base, rows, cols, ld, kBK, box_rows_kmajor);
 }
 
+static int64_t columns(const GemmArgs& g) { return g.n_valid > 0 ? g.n_valid : g.N; }
+
 static int epilogue_maps(const GemmArgs& g, const GemmEpi& ep, CUtensorMap* tc) {
   // epilogue store maps (bf16 outputs written by TMA from staging boxes)
   memset(tc, 0, 2 * sizeof(CUtensorMap));
@@ -1004,7 +1118,8 @@ static int epilogue_maps(const GemmArgs& g, const GemmEpi& ep, CUtensorMap* tc) 
   switch (g.epi) {
     case EPI_STORE:
     case EPI_CE_STATS:
-      rc = make_tmap_2d_store(&tc[0], ep.c, g.M, g.N, ep.ldc);
+    case EPI_CE_GRAD:
+      rc = make_tmap_2d_store(&tc[0], ep.c, g.M, columns(g), ep.ldc);
       break;
     case EPI_RESID:
       rc = make_tmap_2d_store(&tc[0], ep.c, g.M, g.N, ep.ldc);
@@ -1123,6 +1238,8 @@ int gemm_tc_launch(const GemmArgs& g, const GemmEpi& ep, cudaStream_t stream, in
     if (g.epi == EPI_F32_ATOMIC && g.N % 256 != 0 && g.N % 128 == 0) bn = 128;
   }
   if (bn != 128 && bn != 256) return -3;
+  if (g.n_valid > 0 && (g.n_valid + 31) / 32 * 32 != g.N) return -10;
+  if (g.ksplit < 1 || g.ksplit > (g.K + kBK - 1) / kBK) return -10;
   SegMaps<1> ta, tb;
   ta.seg_rows = tb.seg_rows = 0;
   ta.nseg = tb.nseg = 1;
@@ -1138,8 +1255,9 @@ int gemm_tc_launch(const GemmArgs& g, const GemmEpi& ep, cudaStream_t stream, in
   // row-grouped: B holds every group's rows
   const int64_t b_rows = ep.grp.mode == 1 ? ep.grp.ngroups * ep.grp.b_stride : -1;
   // pair mode: each CTA loads half of a K-major B tile
-  rc = g.b_mn ? make_operand_map(&tb.m[0], g.B, true, b_rows > 0 ? b_rows : g.K, g.N, g.ldb, bn)
-              : make_operand_map(&tb.m[0], g.B, false, b_rows > 0 ? b_rows : g.N, g.K, g.ldb,
+  rc = g.b_mn ? make_operand_map(&tb.m[0], g.B, true, b_rows > 0 ? b_rows : g.K, columns(g), g.ldb,
+                                 bn)
+              : make_operand_map(&tb.m[0], g.B, false, b_rows > 0 ? b_rows : columns(g), g.K, g.ldb,
                                  g.M > kBM ? bn / 2 : bn);
   if (rc) return rc;
   CUtensorMap tc[2];
@@ -1149,9 +1267,9 @@ int gemm_tc_launch(const GemmArgs& g, const GemmEpi& ep, cudaStream_t stream, in
 #define CFB_EPI_CASE(E)                                                                          \
   case E:                                                                                        \
     return bn == 256 ? dispatch_major<256, E>(g.a_mn, g.b_mn, ta, tb, tc, g.M, g.N, g.K, ep,      \
-                                              g.num_sms, stream, err)                            \
+                                              g.num_sms, stream, err, g.ksplit)                  \
                      : dispatch_major<128, E>(g.a_mn, g.b_mn, ta, tb, tc, g.M, g.N, g.K, ep,      \
-                                              g.num_sms, stream, err);
+                                              g.num_sms, stream, err, g.ksplit);
   switch (g.epi) {
     CFB_EPI_CASE(EPI_STORE)
     CFB_EPI_CASE(EPI_RESID)
@@ -1159,6 +1277,14 @@ int gemm_tc_launch(const GemmArgs& g, const GemmEpi& ep, cudaStream_t stream, in
     CFB_EPI_CASE(EPI_F32_ACC)
     CFB_EPI_CASE(EPI_F32_ATOMIC)
     CFB_EPI_CASE(EPI_CE_STATS)
+    case EPI_CE_FWD:
+    case EPI_CE_GRAD:
+      if (g.a_mn || g.b_mn || bn != 256 || g.n_valid <= 0) return -4;
+      return g.epi == EPI_CE_FWD
+                 ? launch_pair_or_single<256, false, false, EPI_CE_FWD>(
+                       ta, tb, tc, g.M, g.N, g.K, ep, g.num_sms, stream, err)
+                 : launch_pair_or_single<256, false, false, EPI_CE_GRAD>(
+                       ta, tb, tc, g.M, g.N, g.K, ep, g.num_sms, stream, err);
     case EPI_SWIGLU_FWD:
       if (g.a_mn || g.b_mn) return -4;
       return launch_pair_or_single<256, false, false, EPI_SWIGLU_FWD>(ta, tb, tc, g.M, g.N, g.K, ep,

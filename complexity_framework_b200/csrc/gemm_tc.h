@@ -18,6 +18,9 @@ enum GemmEpilogue : int {
   EPI_CE_STATS = 6,    // C(bf16) logits = alpha*acc; stats[row, N/128] = (max, sumexp); BN=256
   EPI_PEER_STORE = 8,  // reduce-scatter partials: owner = row / peer_rows; fp32 tile stored
                        // over NVLink into peer_c[owner][sync.rank][row % peer_rows][col]
+  EPI_CE_FWD = 9,      // nothing of C is stored: per (row, 128 columns) softmax statistics and
+                       // the target's logit; BN=256 (see GemmCe)
+  EPI_CE_GRAD = 10,    // C(bf16) = d(loss)/d(logits) of the columns' part of the vocabulary
 };
 
 constexpr int kMaxSeg = 8;
@@ -76,6 +79,30 @@ struct GemmGroups {
   int64_t c_stride = 0;
 };
 
+// Cross-entropy epilogues: acc is h . w of a row and a word, its logit z = scale * acc and
+// t = k2 * acc the same in units of log 2.
+struct GemmCe {
+  float k2 = 0.f;     // scale * log2(e)
+  float scale = 1.f;  // logit scale
+  const int* target = nullptr;  // [M] word of each row, < 0: none
+  // forward: (max t, sum 2^(t - max)) of a half tile, scale * acc of the target, and (where
+  // wanted) the sum of scale * acc over a half tile
+  float2* stats = nullptr;  // [M][2 * ceil(N / 256)]
+  float* zt = nullptr;      // [M]
+  float* zsum = nullptr;    // [M][2 * ceil(N / 256)]
+  // gradient: g (p (1 + 2 lambda lse) - (1 - eps) [target] - eps / V) * scale, g = gout * ginv
+  const float* lse2 = nullptr;  // [M] log-sum-exp in units of log 2
+  const float* gout = nullptr;  // one value, or one for each row of the call's own order
+  const int* src = nullptr;     // [M] that order's row of each row here, < 0: none
+  const float* ginv = nullptr;  // one value, or null
+  int per_row = 0;
+  float z2 = 0.f;        // 2 lambda
+  float smooth = 0.f;    // eps
+  float smooth_v = 0.f;  // eps / V
+  int col0 = 0;          // first word of this call's columns
+  int n_valid = 0;       // columns that are words (the others pad N to 32)
+};
+
 struct GemmEpi {
   void* c = nullptr;
   int64_t ldc = 0;
@@ -97,6 +124,13 @@ struct GemmEpi {
   DistSync sync;
   AgCopy ag;
   GemmGroups grp;
+  GemmCe ce;
+  // sizes that the host does not know: fewer rows of C (m_dev) or of K (k_dev) than M or K
+  const int* m_dev = nullptr;
+  const int* k_dev = nullptr;
+  int64_t split_stride = 0;  // EPI_F32 / EPI_F32_ACC: K slices write their own C, this far apart
+  int group_m = 0;           // > 0: the schedule takes the row tiles in groups of this many, every
+                             // column tile of a group before the next group
 };
 
 struct GemmArgs {
@@ -110,6 +144,8 @@ struct GemmArgs {
   int epi = EPI_STORE;
   int bn = 0;  // 0 = choose
   int num_sms = 148;
+  int n_valid = 0;  // > 0: B and C have this many columns only; N is it rounded up to 32
+  int ksplit = 1;   // EPI_F32 / EPI_F32_ACC: K slices (at most one a 64-wide K block)
   // Operand segments (all-gather fused into the GEMM): when a_nseg > 0 the A
   // matrix is the concatenation, along its storage rows (M for K-major, K for
   // MN-major), of a_nseg matrices of a_seg_rows rows each, at A_seg[i] (peer

@@ -1,0 +1,351 @@
+// Softmax cross-entropy over a large vocabulary, and its gradients, without keeping the logits.
+//
+// With z_v = scale * h . w_v, lse = log sum_v exp(z_v) and p_v = exp(z_v - lse), a counted row
+// with the word y has
+//
+//   loss = lse - (1 - eps) z_y - eps / V sum_v z_v + lambda lse^2
+//   d loss / d z_v = p_v (1 + 2 lambda lse) - (1 - eps) [v = y] - eps / V
+//
+// Forward: one product h W^T whose epilogue leaves, of each row's 128 words, their maximum, the
+// sum of exponentials and (for smoothing) the sum, and the target's logit: 1/16 of a bf16 logit
+// matrix's bytes.  Backward: for a piece of the vocabulary at a time, the product again with an
+// epilogue that writes d loss / d z in bf16, then dh += dz W and dW = dz^T h.  That is four
+// products of 2 T V H operations where three would do with the logits kept; all run on the
+// tensor cores from fp32 accumulators, and the logits are never rounded to bf16.
+//
+// Rows that do not count (ignored targets) are left out before the first product: the others are
+// gathered in their order, and the products take their number from device memory.  A batch with
+// half of its tokens ignored costs half, and what an ignored row holds reaches nothing.
+//
+// dz is rounded to bf16 (2^-9 of its size, as the tensor cores' operand); its sums are fp32.  No
+// sum depends on the order of atomics: equal calls give equal bits.
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "gemm_tc.h"
+#include "vocab_loss.h"
+
+namespace cfb {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The counted rows in their order: every block of `per` rows counts the rows before its own
+// (T targets are far fewer bytes than T rows), so one launch does, without atomics.
+__global__ void __launch_bounds__(256) vl_gather_k(const VlCall c, const VlForward f, int per) {
+  __shared__ int warp_n[8];
+  __shared__ int dest[256];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per;
+  const auto counts = [&](int64_t y) { return y != c.ignore && y >= 0 && y < c.V; };
+  int before = 0;
+  for (int64_t i = tid; i < first; i += 256) before += counts(f.targets[i]) ? 1 : 0;
+  before = __reduce_add_sync(0xffffffffu, before);
+  if (lane == 0) warp_n[warp] = before;
+  __syncthreads();
+  before = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) before += warp_n[k];
+  __syncthreads();
+  const int64_t row = first + tid;
+  const bool mine = tid < per && row < c.T;
+  const int64_t y = mine ? f.targets[row] : c.ignore;
+  const bool on = mine && counts(y);
+  const uint32_t ballot = __ballot_sync(0xffffffffu, on);
+  if (lane == 0) warp_n[warp] = __popc(ballot);
+  __syncthreads();
+  int at = before, end = before;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (k < warp) at += warp_n[k];
+    end += warp_n[k];
+  }
+  at += __popc(ballot & ((1u << lane) - 1u));
+  if (mine) {
+    dest[tid] = on ? at : -1;
+    c.pos[row] = on ? at : -1;
+    if (on) {
+      c.target[at] = static_cast<int>(y);
+      c.src[at] = static_cast<int>(row);
+    } else {
+      // a target that is neither a word nor ignored: reported, and a loss of NaN
+      if (y != c.ignore) report_error(c.err, kErrBounds, 60);
+      f.rows[row] = y == c.ignore ? 0.f : NAN;
+    }
+  }
+  __syncthreads();
+  const int nv = c.H >> 3;
+  for (int r = warp; r < per && first + r < c.T; r += 8) {
+    if (dest[r] < 0) continue;
+    const uint4* in = reinterpret_cast<const uint4*>(f.h + (first + r) * c.H);
+    uint4* out = reinterpret_cast<uint4*>(c.hc + static_cast<int64_t>(dest[r]) * c.H);
+    for (int i = lane; i < nv; i += 32) out[i] = in[i];
+  }
+  if (blockIdx.x + 1 < gridDim.x) return;
+  // the last block knows the count; rows up to the next whole block of 64 become 0
+  const int64_t stop = end <= 64 ? 64 : (static_cast<int64_t>(end) + 63) / 64 * 64;
+  for (int64_t r = end + warp; r < stop; r += 8) {
+    uint4* out = reinterpret_cast<uint4*>(c.hc + r * c.H);
+    for (int i = lane; i < nv; i += 32) out[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (lane == 0) {
+      c.target[r] = -1;
+      c.src[r] = -1;
+    }
+  }
+  if (tid == 0) {
+    c.cnt[0] = end;
+    c.cnt[1] = end > 0 ? end : 1;
+    *c.ginv = f.mean ? 1.f / static_cast<float>(end > 0 ? end : 1) : 1.f;
+  }
+}
+
+// Joins the half tiles' statistics of rows [first, first + n), a warp a row.
+__global__ void __launch_bounds__(256) vl_rows_k(const VlCall c, const VlForward f,
+                                                 const float2* __restrict__ stats,
+                                                 const float* __restrict__ zt,
+                                                 const float* __restrict__ zsum, int halves) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= c.cnt[1]) return;
+  const float2* st = stats + row * halves;
+  float mx = -INFINITY;
+  for (int i = lane; i < halves; i += 32) mx = fmaxf(mx, st[i].x);
+  mx = warp_max(mx);
+  float se = 0.f, zs = 0.f;
+  for (int i = lane; i < halves; i += 32) {
+    const float2 v = st[i];
+    se += v.y * exp2_approx(v.x - mx);
+    if (zsum != nullptr) zs += zsum[row * halves + i];
+  }
+  se = warp_sum(se);
+  if (zsum != nullptr) zs = warp_sum(zs);
+  if (lane != 0) return;
+  const float lse2 = mx + log2f(se);
+  c.lse2[row] = lse2;
+  const int src = c.src[row];
+  if (src < 0) return;
+  const float lse = lse2 * kLn2;
+  float loss = lse - zt[row];
+  if (c.smooth > 0.f) loss += c.smooth * (zt[row] - zs / static_cast<float>(c.V));
+  f.rows[src] = loss + c.z * lse * lse;
+}
+
+__global__ void __launch_bounds__(1024) vl_total_k(const VlCall c, const VlForward f) {
+  __shared__ float part[32];
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < c.T; i += 1024) s += f.rows[i];
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warp_sum(part[threadIdx.x]);
+    if (threadIdx.x == 0) *f.total = s * *c.ginv;
+  }
+}
+
+// dh in the call's order: the K slices' sum of a counted row, 0 of the others.
+__global__ void __launch_bounds__(256) vl_scatter_k(const VlCall c, const float* __restrict__ acc,
+                                                    int ldc, int64_t slice, int slices,
+                                                    __nv_bfloat16* __restrict__ dh) {
+  const int lane = threadIdx.x & 31, nv = c.H >> 3;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < c.T;
+       row += static_cast<int64_t>(gridDim.x) * 8) {
+    const int at = c.pos[row];
+    uint4* out = reinterpret_cast<uint4*>(dh + row * c.H);
+    for (int i = lane; i < nv; i += 32) {
+      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      if (at >= 0) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        const float* p = acc + static_cast<int64_t>(at) * ldc + i * 8;
+        for (int k = 0; k < slices; ++k) {
+          const float4 x = *reinterpret_cast<const float4*>(p + k * slice);
+          const float4 y = *reinterpret_cast<const float4*>(p + k * slice + 4);
+          a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+          b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+        }
+        u = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y),
+                       pack_bf16x2(b.z, b.w));
+      }
+      out[i] = u;
+    }
+  }
+}
+
+int pad32(int n) { return (n + 31) / 32 * 32; }
+int halves_of(const VlCall& c) { return 2 * ((c.V + 255) / 256); }
+
+GemmEpi epi_of(const VlCall& c) {
+  GemmEpi ep;
+  ep.ce.k2 = c.scale * kLog2e;
+  ep.ce.scale = c.scale;
+  ep.ce.target = c.target;
+  ep.ce.n_valid = 0;
+  ep.m_dev = c.cnt + 1;
+  return ep;
+}
+
+}  // namespace
+
+int64_t vl_forward_floats(const VlCall& c) {
+  const int64_t R = vl_rows(c.T), h = halves_of(c);
+  return R * h * (c.smooth > 0.f ? 3 : 2) + R;
+}
+
+int vl_forward(const VlCall& c, const VlForward& f, cudaStream_t s) {
+  const int64_t R = vl_rows(c.T);
+  const int halves = halves_of(c);
+  // rows a block: enough blocks to copy with every SM, few enough that the counting stays small
+  int per = static_cast<int>((c.T + 2 * c.num_sms - 1) / (2 * c.num_sms));
+  per = per < 8 ? 8 : per > 256 ? 256 : per;
+  vl_gather_k<<<static_cast<unsigned>((c.T + per - 1) / per), 256, 0, s>>>(c, f, per);
+  float2* stats = reinterpret_cast<float2*>(f.ws);
+  float* zsum = c.smooth > 0.f ? f.ws + 2 * R * halves : nullptr;
+  float* zt = f.ws + R * halves * (c.smooth > 0.f ? 3 : 2);
+  GemmArgs g;
+  g.A = c.hc;
+  g.lda = c.H;
+  g.B = c.w;
+  g.ldb = c.H;
+  g.M = static_cast<int>(R);
+  g.N = pad32(c.V);
+  g.n_valid = c.V;
+  g.K = c.H;
+  g.epi = EPI_CE_FWD;
+  g.bn = 256;
+  g.num_sms = c.num_sms;
+  GemmEpi ep = epi_of(c);
+  ep.ce.stats = stats;
+  ep.ce.zt = zt;
+  ep.ce.zsum = zsum;
+  ep.ce.n_valid = c.V;
+  ep.group_m = 8;
+  const int rc = gemm_tc_launch(g, ep, s, c.err);
+  if (rc) return rc;
+  vl_rows_k<<<static_cast<unsigned>((R + 7) / 8), 256, 0, s>>>(c, f, stats, zt, zsum, halves);
+  if (f.total != nullptr) vl_total_k<<<1, 1024, 0, s>>>(c, f);
+  return static_cast<int>(cudaGetLastError());
+}
+
+void vl_backward_plan(const VlCall& c, int64_t workspace_bytes, VlBackward* b) {
+  const int64_t R = vl_rows(c.T);
+  int64_t most = workspace_bytes / (2 * R) / 256 * 256;
+  if (most < 256) most = 256;
+  const int64_t pieces = (c.V + most - 1) / most;
+  b->piece = static_cast<int>(((c.V + pieces - 1) / pieces + 255) / 256 * 256);
+  // few rows: the hidden gradient's K, the words, over several CTAs
+  const bool pair = R > 128;
+  const int64_t tiles = ((R + 255) / 256) * ((c.H + 255) / 256);
+  const int64_t units = pair ? c.num_sms / 2 : c.num_sms;
+  const int64_t blocks = (std::min<int64_t>(b->piece, c.V) + 63) / 64;
+  // words of the last piece, which every slice needs some of
+  const int64_t last = (c.V - (pieces - 1) * b->piece + 63) / 64;
+  int64_t ks = units / tiles;
+  if (ks > blocks / 4) ks = blocks / 4;
+  if (ks > last) ks = last;
+  b->ksplit = ks < 1 ? 1 : static_cast<int>(ks);
+}
+
+int64_t vl_acc_floats(const VlCall& c, const VlBackward& b) {
+  return static_cast<int64_t>(b.ksplit) * vl_rows(c.T) * pad32(c.H);
+}
+
+int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
+  const int64_t R = vl_rows(c.T);
+  const int ldh = pad32(c.H);
+  for (int v0 = 0; v0 < c.V; v0 += b.piece) {
+    const int n = c.V - v0 < b.piece ? c.V - v0 : b.piece;
+    const __nv_bfloat16* w = c.w + static_cast<int64_t>(v0) * c.H;
+    GemmArgs g;
+    g.num_sms = c.num_sms;
+    // dz of the piece
+    g.A = c.hc;
+    g.lda = c.H;
+    g.B = w;
+    g.ldb = c.H;
+    g.M = static_cast<int>(R);
+    g.N = pad32(n);
+    g.n_valid = n;
+    g.K = c.H;
+    g.epi = EPI_CE_GRAD;
+    g.bn = 256;
+    GemmEpi ep = epi_of(c);
+    ep.c = b.dl;
+    ep.ldc = b.piece;
+    ep.ce.lse2 = c.lse2;
+    ep.ce.gout = b.gout;
+    ep.ce.per_row = b.per_row ? 1 : 0;
+    ep.ce.ginv = b.per_row ? nullptr : c.ginv;
+    ep.ce.src = c.src;
+    ep.ce.z2 = 2.f * c.z;
+    ep.ce.smooth = c.smooth;
+    ep.ce.smooth_v = c.smooth / static_cast<float>(c.V);
+    ep.ce.col0 = v0;
+    ep.ce.n_valid = n;
+    ep.group_m = 8;
+    int rc = gemm_tc_launch(g, ep, s, c.err);
+    if (rc) return rc;
+    if (b.dh != nullptr) {  // dh (+)= dz W
+      GemmArgs d;
+      d.num_sms = c.num_sms;
+      d.A = b.dl;
+      d.lda = b.piece;
+      d.B = w;
+      d.ldb = c.H;
+      d.b_mn = true;
+      d.M = static_cast<int>(R);
+      d.N = ldh;
+      d.n_valid = c.H;
+      d.K = n;
+      d.ksplit = b.ksplit;
+      d.epi = v0 == 0 ? EPI_F32 : EPI_F32_ACC;
+      GemmEpi e;
+      e.m_dev = c.cnt + 1;
+      e.c = b.acc;
+      e.ldc = ldh;
+      e.split_stride = R * ldh;
+      rc = gemm_tc_launch(d, e, s, c.err);
+      if (rc) return rc;
+    }
+    if (b.dw != nullptr) {  // dW of the piece = dz^T h
+      GemmArgs d;
+      d.num_sms = c.num_sms;
+      d.A = b.dl;
+      d.lda = b.piece;
+      d.a_mn = true;
+      d.B = c.hc;
+      d.ldb = c.H;
+      d.b_mn = true;
+      d.M = n;
+      d.N = ldh;
+      d.n_valid = c.H;
+      d.K = static_cast<int>(R);
+      d.epi = EPI_STORE;
+      GemmEpi e;
+      e.k_dev = c.cnt + 1;
+      e.c = b.dw + static_cast<int64_t>(v0) * c.H;
+      e.ldc = c.H;
+      rc = gemm_tc_launch(d, e, s, c.err);
+      if (rc) return rc;
+    }
+  }
+  if (b.dh != nullptr) {
+    const int64_t want = (c.T + 7) / 8, most = static_cast<int64_t>(c.num_sms) * 8;
+    vl_scatter_k<<<static_cast<unsigned>(want < most ? want : most), 256, 0, s>>>(
+        c, b.acc, ldh, R * ldh, b.ksplit, b.dh);
+  }
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace cfb

@@ -25,6 +25,8 @@ SOURCES = [
     "paged8_chunk.cu",
     "bind_stream.cpp",
     "residual.cu",
+    "bind_vocab.cpp",
+    "vocab_loss.cu",
     "dist_fused.cu",
     "noalloc.cu",
     "tp_fused.cu",
