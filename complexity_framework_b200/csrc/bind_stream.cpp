@@ -40,12 +40,10 @@ void like(const Tensor& t, const Tensor& x, const char* name) {
                    x.scalar_type(), ", got ", t.scalar_type());
 }
 
-// Contiguous; and copied where it starts off a 16-byte boundary although its rows are in 16-byte
-// units, so that only odd widths take the kernels' element-wise accesses.
+// Contiguous and 16-byte aligned; other layouts are copied.
 Tensor dense(const Tensor& t) {
   const Tensor c = t.contiguous();
-  const bool units = t.dim() > 0 && t.size(-1) * t.element_size() % 16 == 0;
-  return units && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 != 0 ? c.clone() : c;
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 != 0 ? c.clone() : c;
 }
 
 Tensor rows(const Tensor& t, const Tensor& x, const char* name) {
@@ -95,8 +93,7 @@ cfb::JoinArgs args_of(const Tensor& x, const OptTensor& w1, const OptTensor& gat
   TORCH_CHECK_VALUE(x.size(-1) <= 0x7fffffff, "rows are too wide");
   a.H = static_cast<int>(x.size(-1));
   a.T = x.numel() / a.H;
-  TORCH_CHECK_VALUE(cfb::join_width_ok(a.H, a.type), "rows of ", a.H,
-                    " channels are too wide");
+  TORCH_CHECK_VALUE(cfb::join_width_ok(a.H), "rows of ", a.H, " channels are too wide");
   TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
   TORCH_CHECK_VALUE(eps >= 0.0 && std::isfinite(eps), "eps must not be negative");
   a.w1 = ptr(w1);
@@ -194,11 +191,11 @@ Tensor dropout(const Tensor& x_in, double p, const OptTensor& seed, int64_t seed
                int64_t stream) {
   const int type = type_of(x_in, "x");
   const c10::cuda::CUDAGuard guard(x_in.device());
-  const Tensor x = x_in.contiguous();
+  const Tensor x = dense(x_in);
   const cfb::DropArgs d = drop_of(p, seed, seed_value, stream, x);
   Tensor y = empty(x.sizes(), x.scalar_type(), x);
   check_rc(cfb::dropout_run(x.data_ptr(), y.data_ptr(), x.numel(), type, d,
-                            cfb_num_sms(x.get_device()), at::cuda::getCurrentCUDAStream()),
+                            at::cuda::getCurrentCUDAStream()),
            "dropout");
   return y;
 }

@@ -43,43 +43,60 @@ __device__ __forceinline__ __half from_f(float v) { return __float2half(v); }
 template <>
 __device__ __forceinline__ float from_f(float v) { return v; }
 
-// VEC elements: one 16-byte access, or one element where rows are not in 16-byte units.
-template <typename T, int VEC>
-struct Vec {
-  uint4 raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void load_once(const T* p) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(raw.x), "=r"(raw.y), "=r"(raw.z), "=r"(raw.w)
-                 : "l"(p));
-  }
-  __device__ __forceinline__ void get(float* v) const {
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = to_f<T>(e[j]);
-  }
-  static __device__ __forceinline__ void store(T* p, const float* v) {
-    uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) e[j] = from_f<T>(v[j]);
-    *reinterpret_cast<uint4*>(p) = u;
-  }
-};
+// Eight elements, a block of the dropout generator, in 16-byte accesses.
 template <typename T>
-struct Vec<T, 1> {
-  T raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *p; }
-  __device__ __forceinline__ void load_once(const T* p) { raw = *p; }
-  __device__ __forceinline__ void get(float* v) const { v[0] = to_f<T>(raw); }
-  static __device__ __forceinline__ void store(T* p, const float* v) { *p = from_f<T>(v[0]); }
+struct Oct {
+  uint4 raw[sizeof(T) / 2];
+  __device__ __forceinline__ void load_once(const T* p) {
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q)
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(raw[q].x), "=r"(raw[q].y), "=r"(raw[q].z), "=r"(raw[q].w)
+                   : "l"(reinterpret_cast<const uint4*>(p) + q));
+  }
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q)
+      raw[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
+  }
+  __device__ __forceinline__ void get(float2* v) const {
+    const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = make_float2(to_f<T>(e[2 * j]), to_f<T>(e[2 * j + 1]));
+  }
+  static __device__ __forceinline__ void store(T* p, const float2* v) {
+    uint4 u[sizeof(T) / 2];
+    T* e = reinterpret_cast<T*>(u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      e[2 * j] = from_f<T>(v[j].x);
+      e[2 * j + 1] = from_f<T>(v[j].y);
+    }
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q)
+      reinterpret_cast<uint4*>(p)[q] = u[q];
+  }
 };
+template <>
+__device__ __forceinline__ void Oct<__nv_bfloat16>::get(float2* v) const {
+  const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ void Oct<__nv_bfloat16>::store(__nv_bfloat16* p, const float2* v) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[1].x, v[1].y),
+                 pack_bf16x2(v[2].x, v[2].y), pack_bf16x2(v[3].x, v[3].y));
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
 
 // Sum over the RT threads of a row.  `red` holds RT / 32 floats of this row's group; the caller
 // alternates between two of them, so one barrier a sum is enough.
@@ -96,294 +113,350 @@ __device__ __forceinline__ float row_sum(float v, float* red, int group, int tid
   return v;
 }
 
-// Dropout factors of VEC elements from element e on (a multiple of VEC).
-template <int VEC>
-__device__ __forceinline__ void drop_factors(const DropArgs& d, uint64_t seed, float factor,
-                                             int64_t e, float* m) {
-  const uint4 r = philox_block(static_cast<uint64_t>(e) >> 3, d.stream, seed);
-  if constexpr (VEC == 8) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = philox_lane(r, j) >= d.threshold ? factor : 0.f;
-  } else if constexpr (VEC == 4) {
-    const bool high = (e & 4) != 0;
-    const uint4 h = make_uint4(high ? r.z : r.x, high ? r.w : r.y, 0u, 0u);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = philox_lane(h, j) >= d.threshold ? factor : 0.f;
-  } else {
-    const int j = static_cast<int>(e & 7);
-    const uint32_t w = j < 4 ? (j < 2 ? r.x : r.y) : (j < 6 ? r.z : r.w);
-    const int u = static_cast<int>((j & 1) ? w >> 16 : w & 0xffffu);
-    m[0] = u >= d.threshold ? factor : 0.f;
+// Which of the eight elements of block `block` are kept.  limit = (threshold << 16) - 1: 16 bits
+// u are >= threshold where (u << 16) > limit; the bits below do not matter for the upper half of
+// a word, which is compared as it is.
+struct Keep {
+  uint32_t w[4];
+  uint32_t limit;
+  __device__ __forceinline__ void draw(const DropArgs& d, uint64_t seed, uint64_t block) {
+    const uint4 r = philox_block(block, d.stream, seed);
+    w[0] = r.x;
+    w[1] = r.y;
+    w[2] = r.z;
+    w[3] = r.w;
+    limit = (static_cast<uint32_t>(d.threshold) << 16) - 1u;
   }
+  // zero, not a product, where dropped: what is there need not be finite
+  __device__ __forceinline__ void apply(float2* v) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j].x = (w[j] << 16) > limit ? v[j].x : 0.f;
+      v[j].y = w[j] > limit ? v[j].y : 0.f;
+    }
+  }
+};
+__device__ __forceinline__ uint64_t seed_of(const DropArgs& d) {
+  return d.seed_ptr != nullptr ? static_cast<uint64_t>(*d.seed_ptr) : d.seed;
 }
 
-// A dropped element is 0 whatever it was (not 0 * NaN).
-__device__ __forceinline__ float masked(float v, float m) { return m == 0.f ? 0.f : v * m; }
+// The columns of a thread.  Every thread takes NV blocks of eight elements that begin on
+// multiples of eight of the tensor's flat index.  Where the width is not a multiple of eight (ODD)
+// a row starts `shift` elements into its first block, and blocks at a row's ends are partial; a
+// group's rows are eight apart (or a multiple), so its shift and its threads' columns stay.
+template <typename T, int NV, int RT, bool ODD>
+struct Cols {
+  int H, tid, shift;
+  int64_t total;
+  __device__ __forceinline__ Cols(const JoinArgs& a, int tid_, int64_t row0)
+      : H(a.H), tid(tid_), shift(ODD ? static_cast<int>((row0 * a.H) & 7) : 0), total(a.T * a.H) {}
+  __device__ __forceinline__ int col(int k) const { return (tid + k * RT) * 8 - shift; }
+  __device__ __forceinline__ bool on(int k) const { return col(k) < H; }
+  __device__ __forceinline__ bool whole(int k) const {
+    return !ODD || (col(k) >= 0 && col(k) + 8 <= H);
+  }
+  __device__ __forceinline__ void load(Oct<T>& o, const T* p, int64_t base, int k) const {
+    const int64_t at = base + col(k);
+    if (!ODD || at + 8 <= total) {
+      o.load_once(p + at);
+    } else {  // the tensor's end
+      T* e = reinterpret_cast<T*>(o.raw);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = at + j < total ? p[at + j] : from_f<T>(0.f);
+    }
+  }
+  // 0 in the neighbouring rows' elements
+  __device__ __forceinline__ void get(const Oct<T>& o, float2* v, int k) const {
+    o.get(v);
+    if (ODD && !whole(k)) {
+      const int c = col(k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (c + 2 * j < 0 || c + 2 * j >= H) v[j].x = 0.f;
+        if (c + 2 * j + 1 < 0 || c + 2 * j + 1 >= H) v[j].y = 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int64_t base, int k, const float2* v) const {
+    if (whole(k)) {
+      Oct<T>::store(p + base + col(k), v);
+    } else {
+      const int c = col(k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (c + 2 * j >= 0 && c + 2 * j < H) p[base + c + 2 * j] = from_f<T>(v[j].x);
+        if (c + 2 * j + 1 >= 0 && c + 2 * j + 1 < H) p[base + c + 2 * j + 1] = from_f<T>(v[j].y);
+      }
+    }
+  }
+  // a weight's columns, times v
+  __device__ __forceinline__ void times(const T* w, int k, float2* v) const {
+    if (!ODD) {
+      Oct<T> o;
+      float2 u[4];
+      o.load(w + col(k));
+      o.get(u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], u[j]);
+    } else {
+      const int c = col(k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (c + 2 * j >= 0 && c + 2 * j < H) v[j].x *= to_f<T>(w[c + 2 * j]);
+        if (c + 2 * j + 1 >= 0 && c + 2 * j + 1 < H) v[j].y *= to_f<T>(w[c + 2 * j + 1]);
+      }
+    }
+  }
+  // f * w1 * gate, the branch's factors (null: 1)
+  __device__ __forceinline__ void factors(const JoinArgs& a, float f, int k, float2* v) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = splat(f);
+    if (a.w1 != nullptr) times(static_cast<const T*>(a.w1), k, v);
+    if (a.gate != nullptr) times(static_cast<const T*>(a.gate), k, v);
+  }
+};
 
-template <typename T, int VEC, int NV, int RT, bool DROP>
+// Two blocks a thread at most keep their columns' weights in registers for all rows; wider rows
+// read them again from L1.
+template <int NV>
+constexpr bool hold = NV <= 2;
+
+template <typename T, int NV, int RT, bool ODD, bool DROP>
 __global__ void __launch_bounds__(RT > 256 ? RT : 256)
     join_fwd_k(const JoinArgs a, float factor) {
   __shared__ float red_all[2][32];
   const int group = threadIdx.x / RT, tid = threadIdx.x % RT, groups = blockDim.x / RT;
   float* red0 = red_all[0] + group * (RT / 32);
   float* red1 = red_all[1] + group * (RT / 32);
-  const int nv = a.H / VEC;
   const T* x = static_cast<const T*>(a.x);
   const T* b = static_cast<const T*>(a.b);
-  const T* w1 = static_cast<const T*>(a.w1);
-  const T* gate = static_cast<const T*>(a.gate);
   const T* w2 = static_cast<const T*>(a.w2);
-  uint64_t seed = 0;
-  if constexpr (DROP)
-    seed = a.drop.seed_ptr != nullptr ? static_cast<uint64_t>(*a.drop.seed_ptr) : a.drop.seed;
-  const float inv_h = 1.f / a.H;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * groups + group; row < a.T;
-       row += static_cast<int64_t>(gridDim.x) * groups) {
-    const int64_t base = row * a.H;
-    Vec<T, VEC> bv[NV], xv[NV];
+  const uint64_t seed = DROP ? seed_of(a.drop) : 0;
+  const float inv_h = 1.f / a.H, f = a.scale * factor;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups + group;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
+  const Cols<T, NV, RT, ODD> cols(a, tid, row0);
+  float2 c[NV][4], v2[NV][4];
+  if constexpr (hold<NV>) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = tid + k * RT;
-      if (i < nv) {
-        bv[k].load_once(b + base + static_cast<int64_t>(i) * VEC);
-        xv[k].load_once(x + base + static_cast<int64_t>(i) * VEC);
+    for (int k = 0; k < NV; ++k)
+      if (cols.on(k)) {
+        cols.factors(a, f, k, c[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v2[k][j] = splat(1.f);
+        if (w2 != nullptr) cols.times(w2, k, v2[k]);
       }
-    }
+  }
+  for (int64_t row = row0; row < a.T; row += step) {
+    const int64_t base = row * a.H;
+    Oct<T> bv[NV], xv[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (cols.on(k)) {
+        cols.load(bv[k], b, base, k);
+        cols.load(xv[k], x, base, k);
+      }
     float r1 = 1.f;
-    if (w1 != nullptr) {
-      float ss = 0.f;
+    if (a.w1 != nullptr) {
+      float2 ss = splat(0.f);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (tid + k * RT < nv) {
-          float v[VEC];
-          bv[k].get(v);
+        if (cols.on(k)) {
+          float2 v[4];
+          cols.get(bv[k], v, k);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) ss += v[j] * v[j];
+          for (int j = 0; j < 4; ++j) ss = fma2(v[j], v[j], ss);
         }
-      r1 = rsqrtf(row_sum<RT>(ss, red0, group, tid) * inv_h + a.eps);
+      r1 = rsqrtf(row_sum<RT>(ss.x + ss.y, red0, group, tid) * inv_h + a.eps);
       if (a.r1 != nullptr && tid == 0) a.r1[row] = r1;
     }
-    float nx[NV][VEC];
-    float ss = 0.f;
+    float2 nx[NV][4];
+    float2 ss = splat(0.f);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = tid + k * RT;
-      if (i < nv) {
-        float u[VEC], v[VEC];
-        bv[k].get(u);
-        if (w1 != nullptr) {
-          Vec<T, VEC> wv;
-          wv.load(w1 + i * VEC);
-          wv.get(v);
+    for (int k = 0; k < NV; ++k)
+      if (cols.on(k)) {
+        float2 u[4];
+        cols.get(bv[k], u, k);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) u[j] *= r1 * v[j];
-        }
-        if (gate != nullptr) {
-          Vec<T, VEC> gv;
-          gv.load(gate + i * VEC);
-          gv.get(v);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) u[j] *= v[j];
-        }
+        for (int j = 0; j < 4; ++j) u[j] = mul2(u[j], splat(r1));
         if constexpr (DROP) {
-          drop_factors<VEC>(a.drop, seed, factor, base + static_cast<int64_t>(i) * VEC, v);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) u[j] = masked(u[j], v[j]);
+          Keep m;
+          m.draw(a.drop, seed, static_cast<uint64_t>(base + cols.col(k)) >> 3);
+          m.apply(u);
         }
-        xv[k].get(v);
+        cols.get(xv[k], nx[k], k);
+        float2 t[4];
+        if constexpr (!hold<NV>) cols.factors(a, f, k, t);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          nx[k][j] = v[j] + a.scale * u[j];
-          ss += nx[k][j] * nx[k][j];
+        for (int j = 0; j < 4; ++j) {
+          nx[k][j] = fma2(u[j], hold<NV> ? c[k][j] : t[j], nx[k][j]);
+          ss = fma2(nx[k][j], nx[k][j], ss);
         }
-        Vec<T, VEC>::store(static_cast<T*>(a.xnew) + base + static_cast<int64_t>(i) * VEC, nx[k]);
+        cols.store(static_cast<T*>(a.xnew), base, k, nx[k]);
       }
-    }
     if (w2 != nullptr) {
       // from x' in 32 bits: y carries one rounding, its own
-      const float r2 = rsqrtf(row_sum<RT>(ss, red1, group, tid) * inv_h + a.eps);
+      const float r2 = rsqrtf(row_sum<RT>(ss.x + ss.y, red1, group, tid) * inv_h + a.eps);
       if (a.r2 != nullptr && tid == 0) a.r2[row] = r2;
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int i = tid + k * RT;
-        if (i < nv) {
-          Vec<T, VEC> wv;
-          float v[VEC];
-          wv.load(w2 + i * VEC);
-          wv.get(v);
+      for (int k = 0; k < NV; ++k)
+        if (cols.on(k)) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) v[j] *= nx[k][j] * r2;
-          Vec<T, VEC>::store(static_cast<T*>(a.y) + base + static_cast<int64_t>(i) * VEC, v);
+          for (int j = 0; j < 4; ++j) {
+            nx[k][j] = mul2(nx[k][j], splat(r2));
+            if constexpr (hold<NV>) nx[k][j] = mul2(nx[k][j], v2[k][j]);
+          }
+          if constexpr (!hold<NV>) cols.times(w2, k, nx[k]);
+          cols.store(static_cast<T*>(a.y), base, k, nx[k]);
         }
-      }
     }
-    // without one of the two sums a group's slots are written again after one barrier only
-    if (RT > 32 && ((w1 != nullptr) != (w2 != nullptr))) named_bar_sync(1 + group, RT);
+    // with one of the two sums alone a group's slots are written again after one barrier
+    if (RT > 32 && ((a.w1 != nullptr) != (w2 != nullptr))) named_bar_sync(1 + group, RT);
   }
 }
 
-template <typename T, int VEC, int NV, int RT, bool DROP>
+template <typename T, int NV, int RT, bool ODD, bool DROP>
 __global__ void __launch_bounds__(RT > 256 ? RT : 256)
     join_bwd_k(const JoinArgs a, float factor) {
   __shared__ float red_all[2][32];
   const int group = threadIdx.x / RT, tid = threadIdx.x % RT, groups = blockDim.x / RT;
   float* red0 = red_all[0] + group * (RT / 32);
   float* red1 = red_all[1] + group * (RT / 32);
-  const int nv = a.H / VEC;
   const T* xn = static_cast<const T*>(a.xnew);
   const T* b = static_cast<const T*>(a.b);
-  const T* w1 = static_cast<const T*>(a.w1);
-  const T* gate = static_cast<const T*>(a.gate);
   const T* w2 = static_cast<const T*>(a.w2);
   const T* dxn = static_cast<const T*>(a.dxnew);
   const T* dy = static_cast<const T*>(a.dy);
-  uint64_t seed = 0;
-  if constexpr (DROP)
-    seed = a.drop.seed_ptr != nullptr ? static_cast<uint64_t>(*a.drop.seed_ptr) : a.drop.seed;
-  const float inv_h = 1.f / a.H;
-  const bool need_b = w1 != nullptr || a.dgate != nullptr;  // b itself enters the gradients
+  const uint64_t seed = DROP ? seed_of(a.drop) : 0;
+  const float inv_h = 1.f / a.H, f = a.scale * factor;
+  const bool post = a.w1 != nullptr;
   const bool branch = a.db != nullptr || a.dgate != nullptr || a.dw1 != nullptr;
-  float s1[NV][VEC], s2[NV][VEC];  // columns' sums of t bh and dy xh
+  const bool need_b = branch && (post || a.dgate != nullptr);  // b itself enters the gradients
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups + group;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
+  const Cols<T, NV, RT, ODD> cols(a, tid, row0);
+  float2 s1[NV][4], s2[NV][4];  // columns' sums of g m bh and dy xh
+  float2 c[NV][4], v2[NV][4];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+  for (int k = 0; k < NV; ++k) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) s1[k][j] = s2[k][j] = 0.f;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * groups + group; row < a.T;
-       row += static_cast<int64_t>(gridDim.x) * groups) {
+    for (int j = 0; j < 4; ++j) s1[k][j] = s2[k][j] = splat(0.f);
+    if constexpr (hold<NV>) {
+      if (cols.on(k)) {
+        cols.factors(a, f, k, c[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v2[k][j] = splat(1.f);
+        if (w2 != nullptr) cols.times(w2, k, v2[k]);
+      }
+    }
+  }
+  for (int64_t row = row0; row < a.T; row += step) {
     const int64_t base = row * a.H;
-    Vec<T, VEC> bv[NV], xv[NV], yv[NV], gv[NV];
+    Oct<T> bv[NV], xv[NV], yv[NV], gv[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = tid + k * RT;
-      const int64_t at = base + static_cast<int64_t>(i) * VEC;
-      if (i < nv) {
+    for (int k = 0; k < NV; ++k)
+      if (cols.on(k)) {
         if (dy != nullptr) {
-          yv[k].load_once(dy + at);
-          xv[k].load_once(xn + at);
+          cols.load(yv[k], dy, base, k);
+          cols.load(xv[k], xn, base, k);
         }
-        if (dxn != nullptr) gv[k].load_once(dxn + at);
-        if (branch && need_b) bv[k].load_once(b + at);
+        if (dxn != nullptr) cols.load(gv[k], dxn, base, k);
+        if (need_b) cols.load(bv[k], b, base, k);
       }
-    }
-    float g[NV][VEC];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if (dxn != nullptr && tid + k * RT < nv) {
-        gv[k].get(g[k]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) g[k][j] = 0.f;
-      }
-    }
+    float r2 = 0.f, mean = 0.f;
     if (dy != nullptr) {
-      const float r2 = a.r2[row];
-      float dot = 0.f;
+      r2 = a.r2[row];
+      float2 dot = splat(0.f);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int i = tid + k * RT;
-        if (i < nv) {
-          float d[VEC], v[VEC], w[VEC];
-          Vec<T, VEC> wv;
-          wv.load(w2 + i * VEC);
-          yv[k].get(d);
-          xv[k].get(v);
-          wv.get(w);
+      for (int k = 0; k < NV; ++k)
+        if (cols.on(k)) {
+          float2 d[4], v[4], w[4];
+          cols.get(yv[k], d, k);
+          cols.get(xv[k], v, k);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float dxh = d[j] * (v[j] * r2);
-            s2[k][j] += dxh;
-            dot += dxh * w[j];
+          for (int j = 0; j < 4; ++j) {
+            d[j] = mul2(d[j], mul2(v[j], splat(r2)));
+            s2[k][j] = add2(s2[k][j], d[j]);
+          }
+          if constexpr (!hold<NV>) cols.times(w2, k, d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            dot = hold<NV> ? fma2(d[j], v2[k][j], dot) : add2(d[j], dot);
+        }
+      mean = row_sum<RT>(dot.x + dot.y, red0, group, tid) * inv_h;
+    }
+    const float r1 = post && branch ? a.r1[row] : 1.f;
+    float2 g[NV][4];
+    float2 dot = splat(0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (cols.on(k)) {
+        if (dxn != nullptr) {
+          cols.get(gv[k], g[k], k);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) g[k][j] = splat(0.f);
+        }
+        if (dy != nullptr) {
+          float2 d[4], v[4];
+          cols.get(yv[k], d, k);
+          cols.get(xv[k], v, k);
+          if constexpr (!hold<NV>) cols.times(w2, k, d);
+          const float2 sub = splat(-r2 * r2 * mean);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (hold<NV>) d[j] = mul2(d[j], v2[k][j]);
+            g[k][j] = fma2(d[j], splat(r2), g[k][j]);
+            g[k][j] = fma2(v[j], sub, g[k][j]);
           }
         }
-      }
-      const float mean = row_sum<RT>(dot, red0, group, tid) * inv_h;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int i = tid + k * RT;
-        if (i < nv) {
-          float d[VEC], v[VEC], w[VEC];
-          Vec<T, VEC> wv;
-          wv.load(w2 + i * VEC);
-          yv[k].get(d);
-          xv[k].get(v);
-          wv.get(w);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) g[k][j] += r2 * (d[j] * w[j] - v[j] * r2 * mean);
-        }
-      }
-    }
-    if (a.dx != nullptr) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int i = tid + k * RT;
-        if (i < nv)
-          Vec<T, VEC>::store(static_cast<T*>(a.dx) + base + static_cast<int64_t>(i) * VEC, g[k]);
-      }
-    }
-    if (branch) {
-      const float r1 = w1 != nullptr ? a.r1[row] : 1.f;
-      float dot = 0.f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int i = tid + k * RT;
-        if (i < nv) {
-          float v[VEC];
+        if (a.dx != nullptr) cols.store(static_cast<T*>(a.dx), base, k, g[k]);
+        if (branch) {
+          float2 bh[4];
+          Keep m;
           if constexpr (DROP) {
-            drop_factors<VEC>(a.drop, seed, factor, base + static_cast<int64_t>(i) * VEC, v);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) g[k][j] = masked(g[k][j], v[j]);
+            m.draw(a.drop, seed, static_cast<uint64_t>(base + cols.col(k)) >> 3);
+            m.apply(g[k]);
           }
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) g[k][j] *= a.scale;
-          float bh[VEC];
           if (need_b) {
-            bv[k].get(bh);
+            cols.get(bv[k], bh, k);
+            if constexpr (DROP) m.apply(bh);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              bh[j] *= r1;
-              s1[k][j] += DROP && v[j] == 0.f ? 0.f : g[k][j] * bh[j];
+            for (int j = 0; j < 4; ++j) {
+              bh[j] = mul2(bh[j], splat(r1));
+              s1[k][j] = fma2(g[k][j], bh[j], s1[k][j]);
             }
           }
-          if (gate != nullptr) {
-            Vec<T, VEC> wv;
-            wv.load(gate + i * VEC);
-            wv.get(v);
+          float2 t[4];
+          if constexpr (!hold<NV>) cols.factors(a, f, k, t);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) g[k][j] *= v[j];
-          }
-          if (w1 != nullptr) {
-            Vec<T, VEC> wv;
-            wv.load(w1 + i * VEC);
-            wv.get(v);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              g[k][j] *= v[j];
-              dot += g[k][j] * bh[j];
-            }
+          for (int j = 0; j < 4; ++j) {
+            g[k][j] = mul2(g[k][j], hold<NV> ? c[k][j] : t[j]);
+            if (post) dot = fma2(g[k][j], bh[j], dot);  // 0 where dropped
           }
         }
       }
-      if (w1 != nullptr) {
-        const float mean = row_sum<RT>(dot, red1, group, tid) * inv_h;
+    if (branch) {
+      if (post) {
+        const float2 sub =
+            splat(-r1 * r1 * (row_sum<RT>(dot.x + dot.y, red1, group, tid) * inv_h));
 #pragma unroll
         for (int k = 0; k < NV; ++k)
-          if (tid + k * RT < nv) {
-            float bh[VEC];
-            bv[k].get(bh);
+          if (cols.on(k)) {
+            float2 v[4];
+            cols.get(bv[k], v, k);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) g[k][j] = r1 * (g[k][j] - bh[j] * r1 * mean);
+            for (int j = 0; j < 4; ++j)
+              g[k][j] = fma2(v[j], sub, mul2(g[k][j], splat(r1)));
           }
       }
       if (a.db != nullptr) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int i = tid + k * RT;
-          if (i < nv)
-            Vec<T, VEC>::store(static_cast<T*>(a.db) + base + static_cast<int64_t>(i) * VEC, g[k]);
-        }
+        for (int k = 0; k < NV; ++k)
+          if (cols.on(k)) cols.store(static_cast<T*>(a.db), base, k, g[k]);
       }
     }
-    if (RT > 32 && ((branch && w1 != nullptr) != (dy != nullptr))) named_bar_sync(1 + group, RT);
+    if (RT > 32 && ((branch && post) != (dy != nullptr))) named_bar_sync(1 + group, RT);
   }
   if (a.partials == nullptr) return;
   // the groups of the CTA one after the other, through this CTA's part of the workspace
@@ -392,15 +465,16 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
     if (q == group) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int i = tid + k * RT;
-        if (i < nv) {
+        const int c0 = cols.col(k);
+        const float* u1 = reinterpret_cast<const float*>(s1[k]);
+        const float* u2 = reinterpret_cast<const float*>(s2[k]);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            float* at = p + i * VEC + j;
-            at[0] = (q == 0 ? 0.f : at[0]) + s1[k][j];
-            at[a.H] = (q == 0 ? 0.f : at[a.H]) + s2[k][j];
+        for (int j = 0; j < 8; ++j)
+          if (c0 + j >= 0 && c0 + j < a.H) {
+            float* at = p + c0 + j;
+            at[0] = (q == 0 ? 0.f : at[0]) + u1[j];
+            at[a.H] = (q == 0 ? 0.f : at[a.H]) + u2[j];
           }
-        }
       }
     }
     __syncthreads();
@@ -409,7 +483,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
 
 // The CTAs' column sums, 32 columns a block, 32 threads a column, in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(1024) join_cols_k(const JoinArgs a, int blocks) {
+__global__ void __launch_bounds__(1024) join_cols_k(const JoinArgs a, int blocks, float f) {
   __shared__ float t1[32][33], t2[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + tx;
@@ -425,7 +499,7 @@ __global__ void __launch_bounds__(1024) join_cols_k(const JoinArgs a, int blocks
   t1[ty][tx] = s1;
   t2[ty][tx] = s2;
   __syncthreads();
-  s1 = warp_sum(t1[tx][ty]);
+  s1 = f * warp_sum(t1[tx][ty]);
   s2 = warp_sum(t2[tx][ty]);
   const int col = blockIdx.x * 32 + ty;
   if (tx != 0 || col >= a.H) return;
@@ -438,70 +512,61 @@ __global__ void __launch_bounds__(1024) join_cols_k(const JoinArgs a, int blocks
     static_cast<T*>(a.dw1)[col] = from_f<T>(gate != nullptr ? s1 * to_f<T>(gate[col]) : s1);
 }
 
-// y = m * x, eight elements (one block of the generator) a thread and turn.
-template <typename T, bool ALIGNED>
+// y = m * x / kept share: kDropVecs blocks of eight elements a thread, loaded before the generator
+// runs for them.
+constexpr int kDropVecs = 4;
+
+template <typename T>
 __global__ void __launch_bounds__(256) dropout_k(const T* __restrict__ x, T* __restrict__ y,
                                                  int64_t n, const DropArgs d, float factor) {
-  constexpr int VEC = 16 / sizeof(T);
-  const uint64_t seed =
-      d.seed_ptr != nullptr ? static_cast<uint64_t>(*d.seed_ptr) : d.seed;
-  const int64_t blocks = (n + 7) / 8;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < blocks;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t e = i * 8;
-    float v[8], m[8];
-    if (ALIGNED && e + 8 <= n) {
-      Vec<T, VEC> in[8 / VEC];
+  const uint64_t seed = seed_of(d);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 * kDropVecs + threadIdx.x;
+  Oct<T> in[kDropVecs];
 #pragma unroll
-      for (int q = 0; q < 8 / VEC; ++q) in[q].load_once(x + e + q * VEC);
-      drop_factors<8>(d, seed, factor, e, m);
+  for (int k = 0; k < kDropVecs; ++k) {
+    const int64_t e = (first + k * 256) * 8;
+    if (e + 8 <= n) in[k].load_once(x + e);
+  }
 #pragma unroll
-      for (int q = 0; q < 8 / VEC; ++q) {
-        in[q].get(v + q * VEC);
+  for (int k = 0; k < kDropVecs; ++k) {
+    const int64_t e = (first + k * 256) * 8;
+    if (e >= n) break;
+    Keep m;
+    float2 v[4];
+    m.draw(d, seed, static_cast<uint64_t>(e) >> 3);
+    if (e + 8 <= n) {
+      in[k].get(v);
+      m.apply(v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[q * VEC + j] = masked(v[q * VEC + j], m[q * VEC + j]);
-        Vec<T, VEC>::store(y + e + q * VEC, v + q * VEC);
-      }
+      for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], splat(factor));
+      Oct<T>::store(y + e, v);
     } else {
-      drop_factors<8>(d, seed, factor, e, m);
+      float* s = reinterpret_cast<float*>(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = e + j < n ? to_f<T>(x[e + j]) : 0.f;
+      m.apply(v);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (e + j < n) y[e + j] = from_f<T>(masked(to_f<T>(x[e + j]), m[j]));
+        if (e + j < n) y[e + j] = from_f<T>(s[j] * factor);
     }
   }
 }
 
 // ---------------------------------------------------------------- host side
-int elem_bytes(int type) { return type == kStreamFloat ? 4 : 2; }
-bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-bool join_aligned(const JoinArgs& a) {
-  return a.H % (16 / elem_bytes(a.type)) == 0 && al16(a.x) && al16(a.b) && al16(a.w1) &&
-         al16(a.gate) && al16(a.w2) && al16(a.xnew) && al16(a.y) && al16(a.dxnew) && al16(a.dy) &&
-         al16(a.dx) && al16(a.db);
-}
-
-// Calls f with the (VEC, NV, RT) of a row: the fewest threads that hold it in a few vectors.
-template <typename T, typename F>
+// Calls f with the (NV, RT, ODD) of a row: the fewest threads that hold it.
+template <typename F>
 int with_shape(const JoinArgs& a, F f) {
-  constexpr int V = 16 / sizeof(T);
-  if (join_aligned(a)) {
-    const int n = a.H / V;
-    if (n <= 32) return f(std::integral_constant<int, V>(), std::integral_constant<int, 1>(),
-                          std::integral_constant<int, 32>());
-    if (n <= 128) return f(std::integral_constant<int, V>(), std::integral_constant<int, 1>(),
-                           std::integral_constant<int, 128>());
-    if (n <= 512) return f(std::integral_constant<int, V>(), std::integral_constant<int, 2>(),
-                           std::integral_constant<int, 256>());
-    if (n <= kJoinMaxVecs)
-      return f(std::integral_constant<int, V>(), std::integral_constant<int, 4>(),
-               std::integral_constant<int, 512>());
-    return -2;
-  }
-  if (a.H <= 1024) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 4>(),
-                            std::integral_constant<int, 256>());
-  if (a.H <= kJoinMaxOdd)
-    return f(std::integral_constant<int, 1>(), std::integral_constant<int, 16>(),
-             std::integral_constant<int, 512>());
+  const int n = a.H % 8 == 0 ? a.H / 8 : (a.H + 14) / 8;
+  const auto go = [&](auto nv, auto rt) {
+    return a.H % 8 == 0 ? f(nv, rt, std::false_type()) : f(nv, rt, std::true_type());
+  };
+  using std::integral_constant;
+  if (n <= 32) return go(integral_constant<int, 1>(), integral_constant<int, 32>());
+  if (n <= 128) return go(integral_constant<int, 1>(), integral_constant<int, 128>());
+  if (n <= 256) return go(integral_constant<int, 1>(), integral_constant<int, 256>());
+  if (n <= 512) return go(integral_constant<int, 2>(), integral_constant<int, 256>());
+  if (n <= 1024) return go(integral_constant<int, 2>(), integral_constant<int, 512>());
+  if (n <= 2048) return go(integral_constant<int, 4>(), integral_constant<int, 512>());
   return -2;
 }
 
@@ -519,38 +584,42 @@ int groups_of(int rt, int64_t rows, int num_sms) {
   return g;
 }
 
-// CTAs of a persistent launch: one for each `groups` rows, at most what is resident at once.
+// CTAs of a persistent launch: one for each `groups` rows, at most what is resident at once; a
+// group's rows are a multiple of eight apart where the width is not a multiple of eight.
 template <typename K>
-int grid_of(K kern, int threads, int64_t rows, int groups, int num_sms) {
-  const int64_t want = rows > 0 ? (rows + groups - 1) / groups : 1;
-  if (want <= num_sms) return static_cast<int>(want);
-  int n = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1)
-    n = 1;
-  const int64_t most = static_cast<int64_t>(num_sms) * n;
-  return static_cast<int>(want < most ? want : most);
+int grid_of(K kern, int threads, const JoinArgs& a, int groups, int num_sms) {
+  const int64_t want = a.T > 0 ? (a.T + groups - 1) / groups : 1;
+  int64_t grid = want;
+  if (want > num_sms) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess ||
+        n < 1)
+      n = 1;
+    const int64_t most = static_cast<int64_t>(num_sms) * n;
+    if (most < grid) grid = most;
+  }
+  if (a.H % 8 != 0) grid = (grid + 7) / 8 * 8;
+  return static_cast<int>(grid);
 }
 
 }  // namespace
 
-bool join_width_ok(int H, int type) {
-  const int v = 16 / elem_bytes(type);
-  return H % v == 0 ? H / v <= kJoinMaxVecs : H <= kJoinMaxOdd;
-}
+bool join_width_ok(int H) { return H <= (H % 8 == 0 ? kJoinMaxWidth : kJoinMaxOdd); }
 
 int join_fwd(const JoinArgs& a, int num_sms, cudaStream_t s) {
   if (a.T == 0) return 0;
   return with_type(a.type, [&](auto t) {
     using T = decltype(t);
-    return with_shape<T>(a, [&](auto vec, auto nv, auto rt) {
-      constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, RT = decltype(rt)::value;
+    return with_shape(a, [&](auto nv, auto rt, auto odd) {
+      constexpr int NV = decltype(nv)::value, RT = decltype(rt)::value;
+      constexpr bool ODD = decltype(odd)::value;
       const int groups = groups_of(RT, a.T, num_sms), threads = RT * groups;
       const auto go = [&](auto kern) {
-        kern<<<grid_of(kern, threads, a.T, groups, num_sms), threads, 0, s>>>(a, a.drop.factor());
+        kern<<<grid_of(kern, threads, a, groups, num_sms), threads, 0, s>>>(a, a.drop.factor());
         return static_cast<int>(cudaGetLastError());
       };
-      return a.drop.threshold > 0 ? go(join_fwd_k<T, VEC, NV, RT, true>)
-                                  : go(join_fwd_k<T, VEC, NV, RT, false>);
+      return a.drop.threshold > 0 ? go(join_fwd_k<T, NV, RT, ODD, true>)
+                                  : go(join_fwd_k<T, NV, RT, ODD, false>);
     });
   });
 }
@@ -559,10 +628,11 @@ template <typename F>
 static int bwd_shape(const JoinArgs& a, F f) {
   return with_type(a.type, [&](auto t) {
     using T = decltype(t);
-    return with_shape<T>(a, [&](auto vec, auto nv, auto rt) {
-      constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, RT = decltype(rt)::value;
-      return a.drop.threshold > 0 ? f(t, join_bwd_k<T, VEC, NV, RT, true>, RT)
-                                  : f(t, join_bwd_k<T, VEC, NV, RT, false>, RT);
+    return with_shape(a, [&](auto nv, auto rt, auto odd) {
+      constexpr int NV = decltype(nv)::value, RT = decltype(rt)::value;
+      constexpr bool ODD = decltype(odd)::value;
+      return a.drop.threshold > 0 ? f(t, join_bwd_k<T, NV, RT, ODD, true>, RT)
+                                  : f(t, join_bwd_k<T, NV, RT, ODD, false>, RT);
     });
   });
 }
@@ -570,7 +640,7 @@ static int bwd_shape(const JoinArgs& a, F f) {
 int join_bwd_blocks(const JoinArgs& a, int num_sms) {
   return bwd_shape(a, [&](auto, auto kern, int rt) {
     const int groups = groups_of(rt, a.T, num_sms);
-    return grid_of(kern, rt * groups, a.T, groups, num_sms);
+    return grid_of(kern, rt * groups, a, groups, num_sms);
   });
 }
 
@@ -580,24 +650,22 @@ int join_bwd(const JoinArgs& a, int blocks, int num_sms, cudaStream_t s) {
     const int groups = groups_of(rt, a.T, num_sms);
     kern<<<blocks, rt * groups, 0, s>>>(a, a.drop.factor());
     if (a.partials != nullptr)
-      join_cols_k<T><<<(a.H + 31) / 32, 1024, 0, s>>>(a, blocks);
+      join_cols_k<T><<<(a.H + 31) / 32, 1024, 0, s>>>(a, blocks, a.scale * a.drop.factor());
     return static_cast<int>(cudaGetLastError());
   });
 }
 
-int dropout_run(const void* x, void* y, int64_t n, int type, const DropArgs& d, int num_sms,
-                cudaStream_t s) {
+int dropout_run(const void* x, void* y, int64_t n, int type, const DropArgs& d, cudaStream_t s) {
   if (n == 0) return 0;
-  const int64_t want = ((n + 7) / 8 + 255) / 256, most = static_cast<int64_t>(num_sms) * 8;
-  const unsigned grid = static_cast<unsigned>(want < most ? want : most);
+  const int64_t each = static_cast<int64_t>(256) * 8 * kDropVecs;
+  if ((n + each - 1) / each > 0x7fffffff) return -2;
+  const unsigned grid = static_cast<unsigned>((n + each - 1) / each);
   return with_type(type, [&](auto t) {
     using T = decltype(t);
-    if (al16(x) && al16(y))
-      dropout_k<T, true><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), n, d,
-                                              d.factor());
-    else
-      dropout_k<T, false><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), n, d,
-                                               d.factor());
+    if (d.threshold == 0)
+      return static_cast<int>(cudaMemcpyAsync(y, x, n * sizeof(T), cudaMemcpyDeviceToDevice, s));
+    dropout_k<T><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), n, d,
+                                      d.factor());
     return static_cast<int>(cudaGetLastError());
   });
 }

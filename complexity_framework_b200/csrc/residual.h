@@ -33,15 +33,13 @@ struct JoinArgs {
   int type = kStreamBf16;
 };
 
-// Widest rows: in 16-byte vectors, or in elements where a row is not a whole number of those.
-constexpr int kJoinMaxVecs = 2048;
-constexpr int kJoinMaxOdd = 8192;
+// Widest rows: 2048 blocks of eight elements, of which the ends of odd rows take one more.
+constexpr int kJoinMaxWidth = 16384, kJoinMaxOdd = 16370;
 
-bool join_width_ok(int H, int type);
+bool join_width_ok(int H);
 int join_fwd(const JoinArgs& a, int num_sms, cudaStream_t s);
 int join_bwd_blocks(const JoinArgs& a, int num_sms);
 int join_bwd(const JoinArgs& a, int blocks, int num_sms, cudaStream_t s);
-int dropout_run(const void* x, void* y, int64_t n, int type, const DropArgs& d, int num_sms,
-                cudaStream_t s);
+int dropout_run(const void* x, void* y, int64_t n, int type, const DropArgs& d, cudaStream_t s);
 
 }  // namespace cfb

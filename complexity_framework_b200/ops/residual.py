@@ -22,8 +22,8 @@ graph reads anew at every replay (``new_seed`` draws one from PyTorch's generato
 too); an int is part of the capture.
 
 On CUDA the operators run the sm_100a kernels on the current stream: bfloat16, float16 or
-float32, weights and gate in the activations' type, rows of up to 2048 16-byte units (odd
-widths: 8192 elements).  Sums and statistics are held in fp32 and each result is rounded once.
+float32, weights and gate in the activations' type, rows of up to 16384 channels (16370 where
+their number is no multiple of 8).  Sums and statistics are held in fp32 and each result is rounded once.
 On the CPU the same formulas run in PyTorch.
 """
 from __future__ import annotations

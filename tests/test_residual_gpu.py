@@ -111,7 +111,7 @@ def check(got, want, tol, dt):
 
 
 SHAPES = [(1, 8), (3, 24), (65, 72), (7, 256), (130, 896), (300, 1024), (5, 1111), (33, 2056),
-          (9, 4096), (2, 8192), (1, 1), (4, 3), (3, 8191)]
+          (9, 4096), (2, 8192), (1, 1), (4, 3), (3, 8191), (29, 903), (17, 4095), (2, 6001)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
@@ -133,12 +133,17 @@ def test_join_parts(post, gate, p, norm, H):
     check(call(t, 1.0, p, 5 if p else None, 0), want, tol, torch.bfloat16)
 
 
-def test_join_widest():
-    t = make(3, 16384, torch.bfloat16, True, True, True)
-    want, tol = oracle(t, 1.0, 0.0, 0, 0)
-    check(call(t, 1.0, 0.0, None, 0), want, tol, torch.bfloat16)
-    for H, dt in ((16392, torch.bfloat16), (8196, torch.float32), (8193, torch.bfloat16)):
-        z = torch.zeros(1, H, device="cuda", dtype=dt)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("H", [16384, 16370, 12345])
+def test_join_widest(H, dtype):
+    t = make(11, H, DT[dtype], True, True, True)
+    want, tol = oracle(t, 1.0, 0.1, 8, 0)
+    check(call(t, 1.0, 0.1, 8, 0), want, tol, DT[dtype])
+
+
+def test_join_too_wide():
+    for H in (16392, 16371):
+        z = torch.zeros(1, H, device="cuda", dtype=torch.bfloat16)
         with pytest.raises(ValueError, match="too wide"):
             R.residual_norm(z, z)
 
