@@ -100,6 +100,7 @@ cfb::JoinArgs args_of(const Tensor& x, const OptTensor& w1, const OptTensor& gat
   a.gate = ptr(gate);
   a.w2 = ptr(w2);
   a.drop = drop;
+  a.err = cfb_err_ptr(x.get_device());
   a.scale = static_cast<float>(scale);
   a.eps = static_cast<float>(eps);
   return a;
@@ -183,7 +184,7 @@ std::vector<OptTensor> residual_norm_bwd(const OptTensor& dxnew_in, const OptTen
     ws = empty({static_cast<int64_t>(blocks) * 2 * a.H}, torch::kFloat32, xnew);
     a.partials = ws.data_ptr<float>();
   }
-  check_rc(cfb::join_bwd(a, blocks, sms, at::cuda::getCurrentCUDAStream()), "residual_norm");
+  check_rc(cfb::join_bwd(a, sms, at::cuda::getCurrentCUDAStream()), "residual_norm");
   return out;
 }
 

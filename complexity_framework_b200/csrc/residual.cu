@@ -43,6 +43,8 @@ __device__ __forceinline__ __half from_f(float v) { return __float2half(v); }
 template <>
 __device__ __forceinline__ float from_f(float v) { return v; }
 
+constexpr int kMaxStages = 4;
+
 // Eight elements, a block of the dropout generator, in 16-byte accesses.
 template <typename T>
 struct Oct {
@@ -98,8 +100,8 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
 
-// Sum over the RT threads of a row.  `red` holds RT / 32 floats of this row's group; the caller
-// alternates between two of them, so one barrier a sum is enough.
+// Sum over the RT threads of a row.  `red` holds RT / 32 floats of this row's group; a row's two
+// sums have their own, and a barrier ends the row, so one barrier a sum is enough.
 template <int RT>
 __device__ __forceinline__ float row_sum(float v, float* red, int group, int tid) {
   v = warp_sum(v);
@@ -216,26 +218,138 @@ struct Cols {
   }
 };
 
+// The input rows of a group.  With RING they come through shared memory: one thread keeps
+// `stages` rows of bulk copies in flight, whatever the threads compute meanwhile, and nothing of a
+// row has to stay in registers from one of its sums to the next.  Without, a row is loaded into
+// registers (odd widths, whose rows do not start on 16-byte boundaries, and rows so wide that two
+// do not fit).  A wait that runs out is reported and the rows that follow are computed from what
+// is there.
+template <typename T, int NV, int RT, int NT, bool ODD, bool RING>
+struct Feed {
+  const T* p[NT];  // null: not read
+  Oct<T> reg[RING ? 1 : NT][RING ? 1 : NV];
+  const Cols<T, NV, RT, ODD>& cols;
+  uint8_t* ring;
+  uint64_t* bar;
+  volatile int* abort_flag;
+  int* err;
+  int stages, stage, row_bytes, group;
+  uint32_t phase;
+  int64_t step, T_rows, issued;
+
+  __device__ __forceinline__ Feed(const JoinArgs& a, const Cols<T, NV, RT, ODD>& c, uint8_t* smem,
+                                  uint64_t* bars, int* flag, int stages_, int group_, int64_t step_)
+      : cols(c), ring(smem), bar(bars), abort_flag(flag), err(a.err), stages(stages_), stage(0),
+        row_bytes(a.H * static_cast<int>(sizeof(T))), group(group_), phase(0), step(step_),
+        T_rows(a.T), issued(0) {}
+  __device__ __forceinline__ uint8_t* at(int s, int i) const {
+    return ring + (static_cast<int64_t>(s) * NT + i) * row_bytes;
+  }
+  __device__ __forceinline__ void issue(int s, int64_t row) {
+    ++issued;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) n += p[i] != nullptr ? 1 : 0;
+    mbar_arrive_expect_tx(&bar[s], static_cast<uint32_t>(n * row_bytes));
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      if (p[i] != nullptr) bulk_load(at(s, i), p[i] + row * cols.H, row_bytes, &bar[s]);
+  }
+  __device__ __forceinline__ void start(int64_t row0) {
+    if constexpr (RING) {
+      if (cols.tid == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(&bar[s], 1);
+        fence_barrier_init();
+        fence_proxy_async_shared();
+        for (int s = 0; s < stages; ++s)
+          if (row0 + s * step < T_rows) issue(s, row0 + s * step);
+      }
+      sync();
+    }
+  }
+  __device__ __forceinline__ void sync() const {
+    if constexpr (RT > 32)
+      named_bar_sync(1 + group, RT);
+    else
+      __syncwarp();
+  }
+  __device__ __forceinline__ void begin(int64_t row) {
+    if constexpr (RING) {
+      mbar_wait(&bar[stage], phase, abort_flag, err, kErrTimeoutFull, 61);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (cols.on(k)) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            if (p[i] != nullptr) cols.load(reg[i][k], p[i], row * cols.H, k);
+        }
+    }
+  }
+  __device__ __forceinline__ void get(int i, int k, float2* v) const {
+    if constexpr (RING) {
+      Oct<T> o;
+      const uint4* q = reinterpret_cast<const uint4*>(at(stage, i)) +
+                       (cols.tid + k * RT) * static_cast<int>(sizeof(T) / 2);
+#pragma unroll
+      for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) o.raw[j] = q[j];
+      o.get(v);
+    } else {
+      cols.get(reg[i][k], v, k);
+    }
+  }
+  // every thread is done with the row; its stage takes the row `stages` further on
+  __device__ __forceinline__ void end(int64_t row) {
+    if (RT > 32 || RING) sync();
+    if constexpr (RING) {
+      if (cols.tid == 0 && row + stages * step < T_rows && *abort_flag == 0)
+        issue(stage, row + stages * step);
+      if (++stage == stages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+  }
+  // after a wait that ran out: a bounded wait for the copies that are still under way
+  __device__ __forceinline__ void drain() {
+    if constexpr (RING) {
+      if (*abort_flag != 0 && cols.tid == 0)
+        for (int s = 0; s < stages && s < issued; ++s)
+          mbar_wait(&bar[s], static_cast<uint32_t>(((issued - 1 - s) / stages) & 1), nullptr, err,
+                    kErrTimeoutFull, 62);
+    }
+  }
+};
+
 // Two blocks a thread at most keep their columns' weights in registers for all rows; wider rows
 // read them again from L1.
 template <int NV>
 constexpr bool hold = NV <= 2;
 
-template <typename T, int NV, int RT, bool ODD, bool DROP>
+template <typename T, int NV, int RT, bool ODD, bool DROP, bool RING>
 __global__ void __launch_bounds__(RT > 256 ? RT : 256)
-    join_fwd_k(const JoinArgs a, float factor) {
+    join_fwd_k(const JoinArgs a, float factor, int stages) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t bars[8][kMaxStages];
+  __shared__ int abort_flag;
   __shared__ float red_all[2][32];
   const int group = threadIdx.x / RT, tid = threadIdx.x % RT, groups = blockDim.x / RT;
   float* red0 = red_all[0] + group * (RT / 32);
   float* red1 = red_all[1] + group * (RT / 32);
-  const T* x = static_cast<const T*>(a.x);
-  const T* b = static_cast<const T*>(a.b);
   const T* w2 = static_cast<const T*>(a.w2);
   const uint64_t seed = DROP ? seed_of(a.drop) : 0;
   const float inv_h = 1.f / a.H, f = a.scale * factor;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups + group;
   const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
   const Cols<T, NV, RT, ODD> cols(a, tid, row0);
+  if (threadIdx.x == 0) abort_flag = 0;
+  __syncthreads();
+  Feed<T, NV, RT, 2, ODD, RING> in(a, cols, ring + static_cast<int64_t>(group) * stages * 2 * a.H *
+                                              static_cast<int>(sizeof(T)),
+                                   bars[group], &abort_flag, stages, group, step);
+  in.p[0] = static_cast<const T*>(a.x);
+  in.p[1] = static_cast<const T*>(a.b);
+  in.start(row0);
   float2 c[NV][4], v2[NV][4];
   if constexpr (hold<NV>) {
 #pragma unroll
@@ -249,13 +363,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
   }
   for (int64_t row = row0; row < a.T; row += step) {
     const int64_t base = row * a.H;
-    Oct<T> bv[NV], xv[NV];
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (cols.on(k)) {
-        cols.load(bv[k], b, base, k);
-        cols.load(xv[k], x, base, k);
-      }
+    in.begin(row);
     float r1 = 1.f;
     if (a.w1 != nullptr) {
       float2 ss = splat(0.f);
@@ -263,7 +371,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
       for (int k = 0; k < NV; ++k)
         if (cols.on(k)) {
           float2 v[4];
-          cols.get(bv[k], v, k);
+          in.get(1, k, v);
 #pragma unroll
           for (int j = 0; j < 4; ++j) ss = fma2(v[j], v[j], ss);
         }
@@ -276,7 +384,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
     for (int k = 0; k < NV; ++k)
       if (cols.on(k)) {
         float2 u[4];
-        cols.get(bv[k], u, k);
+        in.get(1, k, u);
 #pragma unroll
         for (int j = 0; j < 4; ++j) u[j] = mul2(u[j], splat(r1));
         if constexpr (DROP) {
@@ -284,7 +392,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
           m.draw(a.drop, seed, static_cast<uint64_t>(base + cols.col(k)) >> 3);
           m.apply(u);
         }
-        cols.get(xv[k], nx[k], k);
+        in.get(0, k, nx[k]);
         float2 t[4];
         if constexpr (!hold<NV>) cols.factors(a, f, k, t);
 #pragma unroll
@@ -310,20 +418,21 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
           cols.store(static_cast<T*>(a.y), base, k, nx[k]);
         }
     }
-    // with one of the two sums alone a group's slots are written again after one barrier
-    if (RT > 32 && ((a.w1 != nullptr) != (w2 != nullptr))) named_bar_sync(1 + group, RT);
+    in.end(row);
   }
+  in.drain();
 }
 
-template <typename T, int NV, int RT, bool ODD, bool DROP>
+template <typename T, int NV, int RT, bool ODD, bool DROP, bool RING>
 __global__ void __launch_bounds__(RT > 256 ? RT : 256)
-    join_bwd_k(const JoinArgs a, float factor) {
+    join_bwd_k(const JoinArgs a, float factor, int stages) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t bars[8][kMaxStages];
+  __shared__ int abort_flag;
   __shared__ float red_all[2][32];
   const int group = threadIdx.x / RT, tid = threadIdx.x % RT, groups = blockDim.x / RT;
   float* red0 = red_all[0] + group * (RT / 32);
   float* red1 = red_all[1] + group * (RT / 32);
-  const T* xn = static_cast<const T*>(a.xnew);
-  const T* b = static_cast<const T*>(a.b);
   const T* w2 = static_cast<const T*>(a.w2);
   const T* dxn = static_cast<const T*>(a.dxnew);
   const T* dy = static_cast<const T*>(a.dy);
@@ -335,6 +444,16 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups + group;
   const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
   const Cols<T, NV, RT, ODD> cols(a, tid, row0);
+  if (threadIdx.x == 0) abort_flag = 0;
+  __syncthreads();
+  Feed<T, NV, RT, 4, ODD, RING> in(a, cols, ring + static_cast<int64_t>(group) * stages * 4 * a.H *
+                                              static_cast<int>(sizeof(T)),
+                                   bars[group], &abort_flag, stages, group, step);
+  in.p[0] = dy;
+  in.p[1] = dy != nullptr ? static_cast<const T*>(a.xnew) : nullptr;
+  in.p[2] = dxn;
+  in.p[3] = need_b ? static_cast<const T*>(a.b) : nullptr;
+  in.start(row0);
   float2 s1[NV][4], s2[NV][4];  // columns' sums of g m bh and dy xh
   float2 c[NV][4], v2[NV][4];
 #pragma unroll
@@ -352,17 +471,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
   }
   for (int64_t row = row0; row < a.T; row += step) {
     const int64_t base = row * a.H;
-    Oct<T> bv[NV], xv[NV], yv[NV], gv[NV];
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (cols.on(k)) {
-        if (dy != nullptr) {
-          cols.load(yv[k], dy, base, k);
-          cols.load(xv[k], xn, base, k);
-        }
-        if (dxn != nullptr) cols.load(gv[k], dxn, base, k);
-        if (need_b) cols.load(bv[k], b, base, k);
-      }
+    in.begin(row);
     float r2 = 0.f, mean = 0.f;
     if (dy != nullptr) {
       r2 = a.r2[row];
@@ -370,9 +479,9 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
 #pragma unroll
       for (int k = 0; k < NV; ++k)
         if (cols.on(k)) {
-          float2 d[4], v[4], w[4];
-          cols.get(yv[k], d, k);
-          cols.get(xv[k], v, k);
+          float2 d[4], v[4];
+          in.get(0, k, d);
+          in.get(1, k, v);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             d[j] = mul2(d[j], mul2(v[j], splat(r2)));
@@ -392,15 +501,15 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
     for (int k = 0; k < NV; ++k)
       if (cols.on(k)) {
         if (dxn != nullptr) {
-          cols.get(gv[k], g[k], k);
+          in.get(2, k, g[k]);
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) g[k][j] = splat(0.f);
         }
         if (dy != nullptr) {
           float2 d[4], v[4];
-          cols.get(yv[k], d, k);
-          cols.get(xv[k], v, k);
+          in.get(0, k, d);
+          in.get(1, k, v);
           if constexpr (!hold<NV>) cols.times(w2, k, d);
           const float2 sub = splat(-r2 * r2 * mean);
 #pragma unroll
@@ -419,7 +528,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
             m.apply(g[k]);
           }
           if (need_b) {
-            cols.get(bv[k], bh, k);
+            in.get(3, k, bh);
             if constexpr (DROP) m.apply(bh);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -444,7 +553,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
         for (int k = 0; k < NV; ++k)
           if (cols.on(k)) {
             float2 v[4];
-            cols.get(bv[k], v, k);
+            in.get(3, k, v);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               g[k][j] = fma2(v[j], sub, mul2(g[k][j], splat(r1)));
@@ -456,8 +565,9 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
           if (cols.on(k)) cols.store(static_cast<T*>(a.db), base, k, g[k]);
       }
     }
-    if (RT > 32 && ((branch && post) != (dy != nullptr))) named_bar_sync(1 + group, RT);
+    in.end(row);
   }
+  in.drain();
   if (a.partials == nullptr) return;
   // the groups of the CTA one after the other, through this CTA's part of the workspace
   float* p = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * a.H;
@@ -584,16 +694,34 @@ int groups_of(int rt, int64_t rows, int num_sms) {
   return g;
 }
 
-// CTAs of a persistent launch: one for each `groups` rows, at most what is resident at once; a
-// group's rows are a multiple of eight apart where the width is not a multiple of eight.
+// A launch: shared memory of the rings and the CTAs of the persistent grid.
+struct JoinLaunch {
+  int groups = 1, threads = 0, stages = 0, smem = 0, grid = 1;
+};
+
+// Stages of a group's ring: the CTA's share of an SM's shared memory where the SM holds 768
+// threads (512 with two blocks a thread, which take more registers); all of it where the share is
+// less than two rows; 0, no ring, where that is too.
+int ring_stages(const JoinArgs& a, int tensors, int groups, int rt, int nv) {
+  if (a.H % 8 != 0) return 0;
+  const int64_t row =
+      static_cast<int64_t>(a.H) * (a.type == kStreamFloat ? 4 : 2) * tensors * groups;
+  const int64_t whole = 220 * 1024, share = whole * (rt * groups) / (nv == 1 ? 768 : 512);
+  int64_t n = share / row;
+  if (n < 2) n = whole / row;
+  return n < 2 ? 0 : n > kMaxStages ? kMaxStages : static_cast<int>(n);
+}
+
+// One CTA for each `groups` rows, at most what is resident at once; a group's rows are a multiple
+// of eight apart where the width is not a multiple of eight.
 template <typename K>
-int grid_of(K kern, int threads, const JoinArgs& a, int groups, int num_sms) {
-  const int64_t want = a.T > 0 ? (a.T + groups - 1) / groups : 1;
+int grid_of(K kern, const JoinLaunch& l, const JoinArgs& a, int num_sms) {
+  const int64_t want = a.T > 0 ? (a.T + l.groups - 1) / l.groups : 1;
   int64_t grid = want;
   if (want > num_sms) {
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess ||
-        n < 1)
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, l.threads, l.smem) !=
+            cudaSuccess || n < 1)
       n = 1;
     const int64_t most = static_cast<int64_t>(num_sms) * n;
     if (most < grid) grid = most;
@@ -606,51 +734,69 @@ int grid_of(K kern, int threads, const JoinArgs& a, int groups, int num_sms) {
 
 bool join_width_ok(int H) { return H <= (H % 8 == 0 ? kJoinMaxWidth : kJoinMaxOdd); }
 
-int join_fwd(const JoinArgs& a, int num_sms, cudaStream_t s) {
-  if (a.T == 0) return 0;
+// Calls f(element, kernel, launch) with the kernel of a call's type, width and dropout.
+template <bool BWD, typename F>
+static int with_kernel(const JoinArgs& a, int num_sms, F f) {
   return with_type(a.type, [&](auto t) {
     using T = decltype(t);
     return with_shape(a, [&](auto nv, auto rt, auto odd) {
       constexpr int NV = decltype(nv)::value, RT = decltype(rt)::value;
       constexpr bool ODD = decltype(odd)::value;
-      const int groups = groups_of(RT, a.T, num_sms), threads = RT * groups;
+      JoinLaunch l;
+      l.groups = groups_of(RT, a.T, num_sms);
+      l.threads = RT * l.groups;
+      constexpr int tensors = BWD ? 4 : 2;
+      l.stages = ring_stages(a, tensors, l.groups, RT, NV);
+      l.smem = l.stages * l.groups * tensors * a.H * static_cast<int>(sizeof(T));
       const auto go = [&](auto kern) {
-        kern<<<grid_of(kern, threads, a, groups, num_sms), threads, 0, s>>>(a, a.drop.factor());
-        return static_cast<int>(cudaGetLastError());
+        if (l.smem > 48 * 1024) {
+          const cudaError_t e = cudaFuncSetAttribute(
+              kern, cudaFuncAttributeMaxDynamicSharedMemorySize, l.smem);
+          if (e != cudaSuccess) return static_cast<int>(e);
+        }
+        l.grid = grid_of(kern, l, a, num_sms);
+        return f(t, kern, l);
       };
-      return a.drop.threshold > 0 ? go(join_fwd_k<T, NV, RT, ODD, true>)
-                                  : go(join_fwd_k<T, NV, RT, ODD, false>);
+      const auto pick = [&](auto drop, auto ring) {
+        constexpr bool D = decltype(drop)::value, R = decltype(ring)::value;
+        if constexpr (BWD)
+          return go(join_bwd_k<T, NV, RT, ODD, D, R>);
+        else
+          return go(join_fwd_k<T, NV, RT, ODD, D, R>);
+      };
+      if constexpr (!ODD)
+        if (l.stages > 0)
+          return a.drop.threshold > 0 ? pick(std::true_type(), std::true_type())
+                                      : pick(std::false_type(), std::true_type());
+      return a.drop.threshold > 0 ? pick(std::true_type(), std::false_type())
+                                  : pick(std::false_type(), std::false_type());
     });
   });
 }
 
-template <typename F>
-static int bwd_shape(const JoinArgs& a, F f) {
-  return with_type(a.type, [&](auto t) {
-    using T = decltype(t);
-    return with_shape(a, [&](auto nv, auto rt, auto odd) {
-      constexpr int NV = decltype(nv)::value, RT = decltype(rt)::value;
-      constexpr bool ODD = decltype(odd)::value;
-      return a.drop.threshold > 0 ? f(t, join_bwd_k<T, NV, RT, ODD, true>, RT)
-                                  : f(t, join_bwd_k<T, NV, RT, ODD, false>, RT);
-    });
+int join_fwd(const JoinArgs& a, int num_sms, cudaStream_t s) {
+  if (a.T == 0) return 0;
+  return with_kernel<false>(a, num_sms, [&](auto, auto kern, const JoinLaunch& l) {
+    kern<<<l.grid, l.threads, l.smem, s>>>(a, a.drop.factor(), l.stages);
+    return static_cast<int>(cudaGetLastError());
   });
 }
 
 int join_bwd_blocks(const JoinArgs& a, int num_sms) {
-  return bwd_shape(a, [&](auto, auto kern, int rt) {
-    const int groups = groups_of(rt, a.T, num_sms);
-    return grid_of(kern, rt * groups, a, groups, num_sms);
+  int blocks = -1;
+  const int rc = with_kernel<true>(a, num_sms, [&](auto, auto, const JoinLaunch& l) {
+    blocks = l.grid;
+    return 0;
   });
+  return rc != 0 ? -1 : blocks;
 }
 
-int join_bwd(const JoinArgs& a, int blocks, int num_sms, cudaStream_t s) {
-  return bwd_shape(a, [&](auto t, auto kern, int rt) {
+int join_bwd(const JoinArgs& a, int num_sms, cudaStream_t s) {
+  return with_kernel<true>(a, num_sms, [&](auto t, auto kern, const JoinLaunch& l) {
     using T = decltype(t);
-    const int groups = groups_of(rt, a.T, num_sms);
-    kern<<<blocks, rt * groups, 0, s>>>(a, a.drop.factor());
+    kern<<<l.grid, l.threads, l.smem, s>>>(a, a.drop.factor(), l.stages);
     if (a.partials != nullptr)
-      join_cols_k<T><<<(a.H + 31) / 32, 1024, 0, s>>>(a, blocks, a.scale * a.drop.factor());
+      join_cols_k<T><<<(a.H + 31) / 32, 1024, 0, s>>>(a, l.grid, a.scale * a.drop.factor());
     return static_cast<int>(cudaGetLastError());
   });
 }

@@ -31,6 +31,7 @@ struct JoinArgs {
   int64_t T = 0;
   int H = 0;
   int type = kStreamBf16;
+  int* err = nullptr;                                // device error word
 };
 
 // Widest rows: 2048 blocks of eight elements, of which the ends of odd rows take one more.
@@ -39,7 +40,7 @@ constexpr int kJoinMaxWidth = 16384, kJoinMaxOdd = 16370;
 bool join_width_ok(int H);
 int join_fwd(const JoinArgs& a, int num_sms, cudaStream_t s);
 int join_bwd_blocks(const JoinArgs& a, int num_sms);
-int join_bwd(const JoinArgs& a, int blocks, int num_sms, cudaStream_t s);
+int join_bwd(const JoinArgs& a, int num_sms, cudaStream_t s);
 int dropout_run(const void* x, void* y, int64_t n, int type, const DropArgs& d, cudaStream_t s);
 
 }  // namespace cfb
