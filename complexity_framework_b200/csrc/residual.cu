@@ -101,7 +101,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
 
 // Sum over the RT threads of a row.  `red` holds RT / 32 floats of this row's group; a row's two
-// sums have their own, and a barrier ends the row, so one barrier a sum is enough.
+// sums have their own, so that one barrier a sum is enough (see Feed::end).
 template <int RT>
 __device__ __forceinline__ float row_sum(float v, float* red, int group, int tid) {
   v = warp_sum(v);
@@ -157,26 +157,23 @@ struct Cols {
   __device__ __forceinline__ bool whole(int k) const {
     return !ODD || (col(k) >= 0 && col(k) + 8 <= H);
   }
+  // 0 in the elements of a partial block that are the neighbouring rows'
+  __device__ __forceinline__ void clear(Oct<T>& o, int k) const {
+    const int c = col(k);
+    T* e = reinterpret_cast<T*>(o.raw);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < 0 || c + j >= H) e[j] = from_f<T>(0.f);
+  }
   __device__ __forceinline__ void load(Oct<T>& o, const T* p, int64_t base, int k) const {
-    const int64_t at = base + col(k);
-    if (!ODD || at + 8 <= total) {
-      o.load_once(p + at);
-    } else {  // the tensor's end
+    if (whole(k)) {
+      o.load_once(p + base + col(k));
+    } else {
+      const int c = col(k);
       T* e = reinterpret_cast<T*>(o.raw);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = at + j < total ? p[at + j] : from_f<T>(0.f);
-    }
-  }
-  // 0 in the neighbouring rows' elements
-  __device__ __forceinline__ void get(const Oct<T>& o, float2* v, int k) const {
-    o.get(v);
-    if (ODD && !whole(k)) {
-      const int c = col(k);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (c + 2 * j < 0 || c + 2 * j >= H) v[j].x = 0.f;
-        if (c + 2 * j + 1 < 0 || c + 2 * j + 1 >= H) v[j].y = 0.f;
-      }
+      for (int j = 0; j < 8; ++j)
+        e[j] = c + j >= 0 && c + j < H ? p[base + c + j] : from_f<T>(0.f);
     }
   }
   __device__ __forceinline__ void store(T* p, int64_t base, int k, const float2* v) const {
@@ -221,9 +218,10 @@ struct Cols {
 // The input rows of a group.  With RING they come through shared memory: one thread keeps
 // `stages` rows of bulk copies in flight, whatever the threads compute meanwhile, and nothing of a
 // row has to stay in registers from one of its sums to the next.  Without, a row is loaded into
-// registers (odd widths, whose rows do not start on 16-byte boundaries, and rows so wide that two
-// do not fit).  A wait that runs out is reported and the rows that follow are computed from what
-// is there.
+// registers (rows so wide that two do not fit).  A copy takes the row's whole blocks, which start
+// on 16-byte boundaries also where the row does not (the tensor's last block, where it is not
+// whole, is left out); a row's partial blocks are put right by the threads that read them.  A wait that runs out is reported and the rows that follow are
+// computed from what is there.
 template <typename T, int NV, int RT, int NT, bool ODD, bool RING>
 struct Feed {
   const T* p[NT];  // null: not read
@@ -235,13 +233,14 @@ struct Feed {
   int* err;
   int stages, stage, row_bytes, group;
   uint32_t phase;
-  int64_t step, T_rows, issued;
+  int64_t step, T_rows, issued, base;
 
   __device__ __forceinline__ Feed(const JoinArgs& a, const Cols<T, NV, RT, ODD>& c, uint8_t* smem,
                                   uint64_t* bars, int* flag, int stages_, int group_, int64_t step_)
       : cols(c), ring(smem), bar(bars), abort_flag(flag), err(a.err), stages(stages_), stage(0),
-        row_bytes(a.H * static_cast<int>(sizeof(T))), group(group_), phase(0), step(step_),
-        T_rows(a.T), issued(0) {}
+        row_bytes(pitch(a.H) * static_cast<int>(sizeof(T))), group(group_), phase(0), step(step_),
+        T_rows(a.T), issued(0), base(0) {}
+  static __host__ __device__ constexpr int pitch(int H) { return ODD ? (H + 14) / 8 * 8 : H; }
   __device__ __forceinline__ uint8_t* at(int s, int i) const {
     return ring + (static_cast<int64_t>(s) * NT + i) * row_bytes;
   }
@@ -250,10 +249,19 @@ struct Feed {
     int n = 0;
 #pragma unroll
     for (int i = 0; i < NT; ++i) n += p[i] != nullptr ? 1 : 0;
-    mbar_arrive_expect_tx(&bar[s], static_cast<uint32_t>(n * row_bytes));
+    const int64_t first = row * cols.H - cols.shift;
+    uint32_t bytes = static_cast<uint32_t>(row_bytes);
+    if constexpr (ODD) {
+      int64_t blocks = (cols.H + cols.shift + 7) / 8;
+      const int64_t most = (cols.total - first) / 8;
+      if (blocks > most) blocks = most;
+      bytes = static_cast<uint32_t>(blocks * 8 * static_cast<int>(sizeof(T)));
+    }
+    mbar_arrive_expect_tx(&bar[s], n * bytes);
+    if (bytes == 0) return;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
-      if (p[i] != nullptr) bulk_load(at(s, i), p[i] + row * cols.H, row_bytes, &bar[s]);
+      if (p[i] != nullptr) bulk_load(at(s, i), p[i] + first, bytes, &bar[s]);
   }
   __device__ __forceinline__ void start(int64_t row0) {
     if constexpr (RING) {
@@ -274,8 +282,33 @@ struct Feed {
       __syncwarp();
   }
   __device__ __forceinline__ void begin(int64_t row) {
+    base = row * cols.H;
     if constexpr (RING) {
       mbar_wait(&bar[stage], phase, abort_flag, err, kErrTimeoutFull, 61);
+      if constexpr (ODD) {  // blocks at the row's ends, each read by this thread alone
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+          if (cols.on(k) && !cols.whole(k)) {
+            const bool copied = base + cols.col(k) + 8 <= cols.total;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+              if (p[i] != nullptr) {
+                uint4* q = reinterpret_cast<uint4*>(at(stage, i)) +
+                           (cols.tid + k * RT) * static_cast<int>(sizeof(T) / 2);
+                Oct<T> o;
+                if (copied) {
+#pragma unroll
+                  for (int w = 0; w < static_cast<int>(sizeof(T) / 2); ++w) o.raw[w] = q[w];
+                  cols.clear(o, k);
+                } else {
+                  cols.load(o, p[i], base, k);
+                }
+#pragma unroll
+                for (int w = 0; w < static_cast<int>(sizeof(T) / 2); ++w) q[w] = o.raw[w];
+              }
+            fence_proxy_async_shared();  // before the stage's next copy
+          }
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -295,12 +328,14 @@ struct Feed {
       for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) o.raw[j] = q[j];
       o.get(v);
     } else {
-      cols.get(reg[i][k], v, k);
+      reg[i][k].get(v);
     }
   }
-  // every thread is done with the row; its stage takes the row `stages` further on
+  // Every thread is done with the row (the barrier also keeps a sum's slots of two rows apart); its
+  // stage takes the row `stages` further on.  Refilling it only after the next row's first sum
+  // would save the barrier, and measured slower (backward of 32768 x 896: 92 -> 103 us).
   __device__ __forceinline__ void end(int64_t row) {
-    if (RT > 32 || RING) sync();
+    sync();
     if constexpr (RING) {
       if (cols.tid == 0 && row + stages * step < T_rows && *abort_flag == 0)
         issue(stage, row + stages * step);
@@ -321,10 +356,89 @@ struct Feed {
   }
 };
 
-// Two blocks a thread at most keep their columns' weights in registers for all rows; wider rows
-// read them again from L1.
-template <int NV>
-constexpr bool hold = NV <= 2;
+// The branch's factors f * w1 * gate and the norm's weights w2 (1 where there are none) of a
+// thread's columns: in registers for all rows (up to two blocks a thread), in shared memory as
+// fp32 (a warp a row: its four blocks would take 64 registers), or read again from L1 for every
+// row (four blocks of the widest rows).
+enum Hold { kInRegs, kInShared, kAgain };
+__host__ __device__ constexpr Hold hold_of(int nv, int rt) {
+  return nv <= 2 ? kInRegs : rt == 32 ? kInShared : kAgain;
+}
+
+template <typename T, int NV, int RT, bool ODD>
+struct Weights {
+  static constexpr Hold how = hold_of(NV, RT);
+  const JoinArgs& a;
+  const Cols<T, NV, RT, ODD>& cols;
+  const float f;
+  float2 c[how == kInRegs ? NV : 1][4], v2[how == kInRegs ? NV : 1][4];
+  float4* shared;  // [4][H / 8]: lower and upper halves of the factors, of w2
+
+  __device__ __forceinline__ Weights(const JoinArgs& a_, const Cols<T, NV, RT, ODD>& cols_, float f_,
+                                     void* smem)
+      : a(a_), cols(cols_), f(f_), shared(static_cast<float4*>(smem)) {
+    if constexpr (how == kInRegs) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (cols.on(k)) {
+          cols.factors(a, f, k, c[k]);
+          norm_from(k, v2[k]);
+        }
+    } else if constexpr (how == kInShared) {
+      const int n8 = a.H / 8;
+      for (int i = threadIdx.x; i < 4 * n8; i += blockDim.x) {
+        float* out = reinterpret_cast<float*>(shared + i);
+        const int o = i % n8, c0 = o * 8 + (i / n8 & 1) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v = 1.f;
+          if (i / n8 < 2) {
+            v = f;
+            if (a.w1 != nullptr) v *= to_f<T>(static_cast<const T*>(a.w1)[c0 + j]);
+            if (a.gate != nullptr) v *= to_f<T>(static_cast<const T*>(a.gate)[c0 + j]);
+          } else if (a.w2 != nullptr) {
+            v = to_f<T>(static_cast<const T*>(a.w2)[c0 + j]);
+          }
+          out[j] = v;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ void norm_from(int k, float2* t) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = splat(1.f);
+    if (a.w2 != nullptr) cols.times(static_cast<const T*>(a.w2), k, t);
+  }
+  __device__ __forceinline__ void from_shared(int which, int k, float2* t) const {
+    const int n8 = a.H / 8, o = cols.tid + k * RT;
+    const float4 lo = shared[2 * which * n8 + o], hi = shared[(2 * which + 1) * n8 + o];
+    t[0] = make_float2(lo.x, lo.y);
+    t[1] = make_float2(lo.z, lo.w);
+    t[2] = make_float2(hi.x, hi.y);
+    t[3] = make_float2(hi.z, hi.w);
+  }
+  __device__ __forceinline__ void branch(int k, float2* t) const {
+    if constexpr (how == kInRegs) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = c[k][j];
+    } else if constexpr (how == kInShared) {
+      from_shared(0, k, t);
+    } else {
+      cols.factors(a, f, k, t);
+    }
+  }
+  __device__ __forceinline__ void norm(int k, float2* t) const {
+    if constexpr (how == kInRegs) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = v2[k][j];
+    } else if constexpr (how == kInShared) {
+      from_shared(1, k, t);
+    } else {
+      norm_from(k, t);
+    }
+  }
+};
 
 template <typename T, int NV, int RT, bool ODD, bool DROP, bool RING>
 __global__ void __launch_bounds__(RT > 256 ? RT : 256)
@@ -344,23 +458,13 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
   const Cols<T, NV, RT, ODD> cols(a, tid, row0);
   if (threadIdx.x == 0) abort_flag = 0;
   __syncthreads();
-  Feed<T, NV, RT, 2, ODD, RING> in(a, cols, ring + static_cast<int64_t>(group) * stages * 2 * a.H *
-                                              static_cast<int>(sizeof(T)),
-                                   bars[group], &abort_flag, stages, group, step);
+  using In = Feed<T, NV, RT, 2, ODD, RING>;
+  const int ring_bytes = stages * 2 * In::pitch(a.H) * static_cast<int>(sizeof(T));  // of a group
+  In in(a, cols, ring + group * ring_bytes, bars[group], &abort_flag, stages, group, step);
   in.p[0] = static_cast<const T*>(a.x);
   in.p[1] = static_cast<const T*>(a.b);
   in.start(row0);
-  float2 c[NV][4], v2[NV][4];
-  if constexpr (hold<NV>) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (cols.on(k)) {
-        cols.factors(a, f, k, c[k]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v2[k][j] = splat(1.f);
-        if (w2 != nullptr) cols.times(w2, k, v2[k]);
-      }
-  }
+  const Weights<T, NV, RT, ODD> weights(a, cols, f, ring + groups * ring_bytes);
   for (int64_t row = row0; row < a.T; row += step) {
     const int64_t base = row * a.H;
     in.begin(row);
@@ -394,10 +498,10 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
         }
         in.get(0, k, nx[k]);
         float2 t[4];
-        if constexpr (!hold<NV>) cols.factors(a, f, k, t);
+        weights.branch(k, t);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          nx[k][j] = fma2(u[j], hold<NV> ? c[k][j] : t[j], nx[k][j]);
+          nx[k][j] = fma2(u[j], t[j], nx[k][j]);
           ss = fma2(nx[k][j], nx[k][j], ss);
         }
         cols.store(static_cast<T*>(a.xnew), base, k, nx[k]);
@@ -409,12 +513,10 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
 #pragma unroll
       for (int k = 0; k < NV; ++k)
         if (cols.on(k)) {
+          float2 t[4];
+          weights.norm(k, t);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            nx[k][j] = mul2(nx[k][j], splat(r2));
-            if constexpr (hold<NV>) nx[k][j] = mul2(nx[k][j], v2[k][j]);
-          }
-          if constexpr (!hold<NV>) cols.times(w2, k, nx[k]);
+          for (int j = 0; j < 4; ++j) nx[k][j] = mul2(mul2(nx[k][j], splat(r2)), t[j]);
           cols.store(static_cast<T*>(a.y), base, k, nx[k]);
         }
     }
@@ -433,7 +535,6 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
   const int group = threadIdx.x / RT, tid = threadIdx.x % RT, groups = blockDim.x / RT;
   float* red0 = red_all[0] + group * (RT / 32);
   float* red1 = red_all[1] + group * (RT / 32);
-  const T* w2 = static_cast<const T*>(a.w2);
   const T* dxn = static_cast<const T*>(a.dxnew);
   const T* dy = static_cast<const T*>(a.dy);
   const uint64_t seed = DROP ? seed_of(a.drop) : 0;
@@ -446,35 +547,36 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
   const Cols<T, NV, RT, ODD> cols(a, tid, row0);
   if (threadIdx.x == 0) abort_flag = 0;
   __syncthreads();
-  Feed<T, NV, RT, 4, ODD, RING> in(a, cols, ring + static_cast<int64_t>(group) * stages * 4 * a.H *
-                                              static_cast<int>(sizeof(T)),
-                                   bars[group], &abort_flag, stages, group, step);
+  using In = Feed<T, NV, RT, 4, ODD, RING>;
+  const int ring_bytes = stages * 4 * In::pitch(a.H) * static_cast<int>(sizeof(T));  // of a group
+  In in(a, cols, ring + group * ring_bytes, bars[group], &abort_flag, stages, group, step);
   in.p[0] = dy;
   in.p[1] = dy != nullptr ? static_cast<const T*>(a.xnew) : nullptr;
   in.p[2] = dxn;
   in.p[3] = need_b ? static_cast<const T*>(a.b) : nullptr;
   in.start(row0);
+  const Weights<T, NV, RT, ODD> weights(a, cols, f, ring + groups * ring_bytes);
   float2 s1[NV][4], s2[NV][4];  // columns' sums of g m bh and dy xh
-  float2 c[NV][4], v2[NV][4];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
+  for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int j = 0; j < 4; ++j) s1[k][j] = s2[k][j] = splat(0.f);
-    if constexpr (hold<NV>) {
-      if (cols.on(k)) {
-        cols.factors(a, f, k, c[k]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v2[k][j] = splat(1.f);
-        if (w2 != nullptr) cols.times(w2, k, v2[k]);
-      }
-    }
+  float r1_next = 1.f, r2_next = 0.f;
+  if (row0 < a.T) {
+    if (a.r1 != nullptr) r1_next = a.r1[row0];
+    if (dy != nullptr) r2_next = a.r2[row0];
   }
   for (int64_t row = row0; row < a.T; row += step) {
     const int64_t base = row * a.H;
     in.begin(row);
-    float r2 = 0.f, mean = 0.f;
+    // the next row's statistics are on their way while this one is computed
+    const float r1 = r1_next, r2 = r2_next;
+    if (row + step < a.T) {
+      if (a.r1 != nullptr) r1_next = a.r1[row + step];
+      if (dy != nullptr) r2_next = a.r2[row + step];
+    }
+    float mean = 0.f;
     if (dy != nullptr) {
-      r2 = a.r2[row];
       float2 dot = splat(0.f);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -487,14 +589,12 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
             d[j] = mul2(d[j], mul2(v[j], splat(r2)));
             s2[k][j] = add2(s2[k][j], d[j]);
           }
-          if constexpr (!hold<NV>) cols.times(w2, k, d);
+          weights.norm(k, v);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            dot = hold<NV> ? fma2(d[j], v2[k][j], dot) : add2(d[j], dot);
+          for (int j = 0; j < 4; ++j) dot = fma2(d[j], v[j], dot);
         }
       mean = row_sum<RT>(dot.x + dot.y, red0, group, tid) * inv_h;
     }
-    const float r1 = post && branch ? a.r1[row] : 1.f;
     float2 g[NV][4];
     float2 dot = splat(0.f);
 #pragma unroll
@@ -507,21 +607,20 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
           for (int j = 0; j < 4; ++j) g[k][j] = splat(0.f);
         }
         if (dy != nullptr) {
-          float2 d[4], v[4];
+          float2 d[4], v[4], t[4];
           in.get(0, k, d);
           in.get(1, k, v);
-          if constexpr (!hold<NV>) cols.times(w2, k, d);
+          weights.norm(k, t);
           const float2 sub = splat(-r2 * r2 * mean);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if constexpr (hold<NV>) d[j] = mul2(d[j], v2[k][j]);
-            g[k][j] = fma2(d[j], splat(r2), g[k][j]);
+            g[k][j] = fma2(mul2(d[j], t[j]), splat(r2), g[k][j]);
             g[k][j] = fma2(v[j], sub, g[k][j]);
           }
         }
         if (a.dx != nullptr) cols.store(static_cast<T*>(a.dx), base, k, g[k]);
         if (branch) {
-          float2 bh[4];
+          float2 bh[4], t[4];
           Keep m;
           if constexpr (DROP) {
             m.draw(a.drop, seed, static_cast<uint64_t>(base + cols.col(k)) >> 3);
@@ -529,19 +628,19 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
           }
           if (need_b) {
             in.get(3, k, bh);
-            if constexpr (DROP) m.apply(bh);
+            // with its norm a branch that is not finite makes the whole row so
+            if (DROP && !post) m.apply(bh);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               bh[j] = mul2(bh[j], splat(r1));
               s1[k][j] = fma2(g[k][j], bh[j], s1[k][j]);
             }
           }
-          float2 t[4];
-          if constexpr (!hold<NV>) cols.factors(a, f, k, t);
+          weights.branch(k, t);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            g[k][j] = mul2(g[k][j], hold<NV> ? c[k][j] : t[j]);
-            if (post) dot = fma2(g[k][j], bh[j], dot);  // 0 where dropped
+            g[k][j] = mul2(g[k][j], t[j]);
+            if (post) dot = fma2(g[k][j], bh[j], dot);
           }
         }
       }
@@ -663,15 +762,28 @@ __global__ void __launch_bounds__(256) dropout_k(const T* __restrict__ x, T* __r
 }
 
 // ---------------------------------------------------------------- host side
-// Calls f with the (NV, RT, ODD) of a row: the fewest threads that hold it.
-template <typename F>
-int with_shape(const JoinArgs& a, F f) {
-  const int n = a.H % 8 == 0 ? a.H / 8 : (a.H + 14) / 8;
+// Calls f with the (NV, RT, ODD) of a row: the fewest threads that hold it.  Up to 128 blocks of a
+// 16-bit type, with rows for every warp of the machine, take fewer threads with more blocks each:
+// a row's fixed work (its sums and barriers) is then one or two warps' instead of four's.  32768 x
+// 896 with dropout, us: forward 60 with four warps a row, 51 with one; backward 123 with four, 114
+// with two (one: 153, its columns' sums leave 8 warps an SM).
+template <typename T, bool BWD, typename F>
+int with_shape(const JoinArgs& a, int num_sms, F f) {
+  const bool odd = a.H % 8 != 0;
+  const int n = odd ? (a.H + 14) / 8 : a.H / 8;
   const auto go = [&](auto nv, auto rt) {
-    return a.H % 8 == 0 ? f(nv, rt, std::false_type()) : f(nv, rt, std::true_type());
+    return odd ? f(nv, rt, std::true_type()) : f(nv, rt, std::false_type());
   };
   using std::integral_constant;
   if (n <= 32) return go(integral_constant<int, 1>(), integral_constant<int, 32>());
+  if constexpr (sizeof(T) == 2) {
+    if (n <= 128 && a.T >= 16 * num_sms) {
+      if constexpr (!BWD)
+        if (!odd)
+          return f(integral_constant<int, 4>(), integral_constant<int, 32>(), std::false_type());
+      return go(integral_constant<int, 2>(), integral_constant<int, 64>());
+    }
+  }
   if (n <= 128) return go(integral_constant<int, 1>(), integral_constant<int, 128>());
   if (n <= 256) return go(integral_constant<int, 1>(), integral_constant<int, 256>());
   if (n <= 512) return go(integral_constant<int, 2>(), integral_constant<int, 256>());
@@ -703,9 +815,8 @@ struct JoinLaunch {
 // threads (512 with two blocks a thread, which take more registers); all of it where the share is
 // less than two rows; 0, no ring, where that is too.
 int ring_stages(const JoinArgs& a, int tensors, int groups, int rt, int nv) {
-  if (a.H % 8 != 0) return 0;
-  const int64_t row =
-      static_cast<int64_t>(a.H) * (a.type == kStreamFloat ? 4 : 2) * tensors * groups;
+  const int64_t row = static_cast<int64_t>(a.H % 8 == 0 ? a.H : (a.H + 14) / 8 * 8) *
+                      (a.type == kStreamFloat ? 4 : 2) * tensors * groups;
   const int64_t whole = 220 * 1024, share = whole * (rt * groups) / (nv == 1 ? 768 : 512);
   int64_t n = share / row;
   if (n < 2) n = whole / row;
@@ -726,7 +837,7 @@ int grid_of(K kern, const JoinLaunch& l, const JoinArgs& a, int num_sms) {
     const int64_t most = static_cast<int64_t>(num_sms) * n;
     if (most < grid) grid = most;
   }
-  if (a.H % 8 != 0) grid = (grid + 7) / 8 * 8;
+  if (a.H % 8 != 0) grid = grid < 8 ? 8 : grid / 8 * 8;
   return static_cast<int>(grid);
 }
 
@@ -739,7 +850,7 @@ template <bool BWD, typename F>
 static int with_kernel(const JoinArgs& a, int num_sms, F f) {
   return with_type(a.type, [&](auto t) {
     using T = decltype(t);
-    return with_shape(a, [&](auto nv, auto rt, auto odd) {
+    return with_shape<T, BWD>(a, num_sms, [&](auto nv, auto rt, auto odd) {
       constexpr int NV = decltype(nv)::value, RT = decltype(rt)::value;
       constexpr bool ODD = decltype(odd)::value;
       JoinLaunch l;
@@ -747,7 +858,9 @@ static int with_kernel(const JoinArgs& a, int num_sms, F f) {
       l.threads = RT * l.groups;
       constexpr int tensors = BWD ? 4 : 2;
       l.stages = ring_stages(a, tensors, l.groups, RT, NV);
-      l.smem = l.stages * l.groups * tensors * a.H * static_cast<int>(sizeof(T));
+      l.smem = l.stages * l.groups * tensors *
+               Feed<T, NV, RT, tensors, ODD, true>::pitch(a.H) * static_cast<int>(sizeof(T));
+      if (hold_of(NV, RT) == kInShared) l.smem += 8 * a.H;
       const auto go = [&](auto kern) {
         if (l.smem > 48 * 1024) {
           const cudaError_t e = cudaFuncSetAttribute(
@@ -764,10 +877,9 @@ static int with_kernel(const JoinArgs& a, int num_sms, F f) {
         else
           return go(join_fwd_k<T, NV, RT, ODD, D, R>);
       };
-      if constexpr (!ODD)
-        if (l.stages > 0)
-          return a.drop.threshold > 0 ? pick(std::true_type(), std::true_type())
-                                      : pick(std::false_type(), std::true_type());
+      if (l.stages > 0)
+        return a.drop.threshold > 0 ? pick(std::true_type(), std::true_type())
+                                    : pick(std::false_type(), std::true_type());
       return a.drop.threshold > 0 ? pick(std::true_type(), std::false_type())
                                   : pick(std::false_type(), std::false_type());
     });
