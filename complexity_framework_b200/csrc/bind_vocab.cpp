@@ -59,26 +59,34 @@ cfb::VlCall call_of(int64_t T, const Tensor& w, double scale, double smooth, dou
   return c;
 }
 
-// ints: cnt [2] (and two spare) | target [R] | src [R] | pos [T];  floats: lse2 [R] | ginv [1]
-void bind_saved(cfb::VlCall& c, const Tensor& hc, const Tensor& ints, const Tensor& floats) {
-  const int64_t R = cfb::vl_rows(c.T);
-  TORCH_CHECK(hc.numel() == R * c.H && ints.numel() == 4 + 2 * R + c.T && floats.numel() == R + 1,
-              "saved tensors do not match");
-  int* p = ints.data_ptr<int>();
-  c.cnt = p;
-  c.target = p + 4;
-  c.src = p + 4 + R;
-  c.pos = p + 4 + 2 * R;
-  c.hc = bf(hc);
-  c.lse2 = floats.data_ptr<float>();
-  c.ginv = c.lse2 + R;
+int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// What the backward pass needs, in one buffer: compact rows | lse2 [R] | ginv [1] | cnt [2] |
+// target [R] | src [R] | pos [T].  With `base` null, its size in bytes.
+int64_t place_saved(cfb::VlCall* c, char* base) {
+  const int64_t R = cfb::vl_rows(c->T);
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    char* p = base == nullptr ? nullptr : base + at;
+    at += up16(bytes);
+    return p;
+  };
+  c->hc = reinterpret_cast<__nv_bfloat16*>(take(R * c->H * 2));
+  c->lse2 = reinterpret_cast<float*>(take(4 * R));
+  c->ginv = reinterpret_cast<float*>(take(4));
+  c->cnt = reinterpret_cast<int*>(take(8));
+  c->target = reinterpret_cast<int*>(take(4 * R));
+  c->src = reinterpret_cast<int*>(take(4 * R));
+  c->pos = reinterpret_cast<int*>(take(4 * c->T));
+  return at;
 }
 
-// reduction: 0 none (the row losses), 1 mean over the counted rows, 2 sum.  Returns the loss and
-// what the backward pass needs: compact rows, index and row tensors, the weight as it was read.
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> vocab_loss_fwd(
-    const Tensor& h_in, const Tensor& w_in, const Tensor& y_in, int64_t ignore, double smooth,
-    double z, double scale, int64_t reduction) {
+// reduction: 0 none (the row losses, times sign), 1 mean over the counted rows, 2 sum.  Returns
+// the loss, what the backward pass needs, and the weight as it was read.
+std::tuple<Tensor, Tensor, Tensor> vocab_loss_fwd(const Tensor& h_in, const Tensor& w_in,
+                                                  const Tensor& y_in, int64_t ignore,
+                                                  double smooth, double z, double scale,
+                                                  int64_t reduction, double sign, bool save) {
   TORCH_CHECK(w_in.is_cuda(), "weight must be a CUDA tensor");
   const c10::cuda::CUDAGuard guard(w_in.device());
   const Tensor h = matrix(h_in, "hidden"), w = matrix(w_in, "weight");
@@ -90,41 +98,50 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> vocab_loss_fwd(
   TORCH_CHECK_VALUE(y_in.dim() == 1 && y_in.size(0) == h.size(0), "targets must be [rows]");
   TORCH_CHECK(reduction >= 0 && reduction <= 2, "bad reduction");
   const Tensor y = y_in.contiguous();
-  const int64_t T = h.size(0), R = cfb::vl_rows(T);
+  const int64_t T = h.size(0);
   cfb::VlCall c = call_of(T, w, scale, smooth, z, ignore);
-  Tensor hc = empty({R, c.H}, torch::kBFloat16, w);
-  Tensor ints = empty({4 + 2 * R + T}, torch::kInt32, w);
-  Tensor floats = empty({R + 1}, torch::kFloat32, w);
-  bind_saved(c, hc, ints, floats);
-  Tensor rows = empty({T}, torch::kFloat32, w), total;
+  c.sign = static_cast<float>(sign);
+  Tensor out = reduction == 0 ? empty({T}, torch::kFloat32, w) : empty({}, torch::kFloat32, w);
+  const int64_t saved_bytes = place_saved(&c, nullptr);
+  if (T == 0) {
+    if (reduction != 0) out.zero_();
+    return {out, empty({saved_bytes}, torch::kUInt8, w), w};
+  }
+  // without a backward pass what it would need is workspace like the rest
+  const int64_t ws_bytes =
+      up16(4 * cfb::vl_forward_floats(c)) + (reduction != 0 ? up16(4 * T) : 0);
+  Tensor saved = empty({saved_bytes + (save ? 0 : ws_bytes)}, torch::kUInt8, w), ws;
+  char* at = static_cast<char*>(saved.data_ptr());
+  place_saved(&c, at);
+  if (save) {
+    ws = empty({ws_bytes}, torch::kUInt8, w);
+    at = static_cast<char*>(ws.data_ptr());
+  } else {
+    at += saved_bytes;
+  }
   cfb::VlForward f;
   f.h = bf(h);
   f.targets = y.data_ptr<int64_t>();
-  f.rows = rows.data_ptr<float>();
   f.mean = reduction == 1;
-  if (reduction != 0) {
-    total = empty({}, torch::kFloat32, w);
-    f.total = total.data_ptr<float>();
-  }
-  if (T == 0) {
-    if (reduction != 0) total.zero_();
-    return {reduction == 0 ? rows : total, hc, ints, floats, w};
-  }
-  const Tensor ws = empty({cfb::vl_forward_floats(c)}, torch::kFloat32, w);
-  f.ws = ws.data_ptr<float>();
+  f.ws = reinterpret_cast<float*>(at);
+  f.rows = reduction == 0 ? out.data_ptr<float>()
+                          : reinterpret_cast<float*>(at + up16(4 * cfb::vl_forward_floats(c)));
+  if (reduction != 0) f.total = out.data_ptr<float>();
   check_rc(cfb::vl_forward(c, f, at::cuda::getCurrentCUDAStream()));
-  return {reduction == 0 ? rows : total, hc, ints, floats, w};
+  return {out, saved, w};
 }
 
 // (dhidden [T, H], dweight [V, H]), each where it is needed.
-std::tuple<OptTensor, OptTensor> vocab_loss_bwd(const Tensor& gout_in, const Tensor& hc,
-                                                const Tensor& ints, const Tensor& floats,
+std::tuple<OptTensor, OptTensor> vocab_loss_bwd(const Tensor& gout_in, const Tensor& saved,
                                                 const Tensor& w, int64_t T, double smooth, double z,
-                                                double scale, bool per_row, bool need_h,
-                                                bool need_w, int64_t workspace_bytes) {
+                                                double scale, bool per_row, double sign,
+                                                bool need_h, bool need_w,
+                                                int64_t workspace_bytes) {
   const c10::cuda::CUDAGuard guard(w.device());
   cfb::VlCall c = call_of(T, w, scale, smooth, z, 0);
-  bind_saved(c, hc, ints, floats);
+  c.sign = static_cast<float>(sign);
+  TORCH_CHECK(saved.numel() == place_saved(&c, nullptr), "saved tensors do not match");
+  place_saved(&c, static_cast<char*>(saved.data_ptr()));
   OptTensor dh, dw;
   if (need_h) dh = empty({T, c.H}, torch::kBFloat16, w);
   if (need_w) dw = empty({c.V, c.H}, torch::kBFloat16, w);
@@ -141,12 +158,15 @@ std::tuple<OptTensor, OptTensor> vocab_loss_bwd(const Tensor& gout_in, const Ten
   b.gout = gout.data_ptr<float>();
   b.per_row = per_row;
   cfb::vl_backward_plan(c, workspace_bytes, &b);
-  const Tensor dl = empty({cfb::vl_rows(T), b.piece}, torch::kBFloat16, w);
-  b.dl = bf(dl);
-  Tensor acc;
+  const int64_t R = cfb::vl_rows(T);
+  const int64_t dl_bytes = up16(2 * R * b.piece), resid_bytes = up16(4 * R);
+  const Tensor ws = empty({dl_bytes + resid_bytes + (need_h ? 4 * cfb::vl_acc_floats(c, b) : 0)},
+                          torch::kUInt8, w);
+  char* at = static_cast<char*>(ws.data_ptr());
+  b.dl = reinterpret_cast<__nv_bfloat16*>(at);
+  b.resid = reinterpret_cast<float*>(at + dl_bytes);
   if (need_h) {
-    acc = empty({cfb::vl_acc_floats(c, b)}, torch::kFloat32, w);
-    b.acc = acc.data_ptr<float>();
+    b.acc = reinterpret_cast<float*>(at + dl_bytes + resid_bytes);
     b.dh = bf(*dh);
   }
   if (need_w) b.dw = bf(*dw);

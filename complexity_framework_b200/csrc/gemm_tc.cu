@@ -799,7 +799,7 @@ __global__ void __launch_bounds__(384, 1)
         int tgt = -1;
         const int src = row_ok ? ep.ce.src[row] : -1;
         if (src >= 0) {
-          float g = ep.ce.gout[ep.ce.per_row ? src : 0] * ep.ce.scale;
+          float g = ep.ce.gout[ep.ce.per_row ? src : 0] * (ep.ce.scale * ep.ce.gsign);
           if (ep.ce.ginv != nullptr) g *= *ep.ce.ginv;
           lse2 = ep.ce.lse2[row];
           ga = g * (1.0f + ep.ce.z2 * (lse2 * 0.693147180559945f));
@@ -820,7 +820,10 @@ __global__ void __launch_bounds__(384, 1)
           if (ti >= 0 && ti < 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (i == ti) v[i] -= gb;
+              if (i == ti) {
+                v[i] -= gb;
+                ep.ce.resid[row] = v[i] - __bfloat162float(__float2bfloat16(v[i]));
+              }
           }
           if (src < 0) {  // also where the row held something that is not finite
 #pragma unroll

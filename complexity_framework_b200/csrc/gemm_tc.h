@@ -96,9 +96,11 @@ struct GemmCe {
   const int* src = nullptr;     // [M] that order's row of each row here, < 0: none
   const float* ginv = nullptr;  // one value, or null
   int per_row = 0;
+  float gsign = 1.f;     // of gout
   float z2 = 0.f;        // 2 lambda
   float smooth = 0.f;    // eps
   float smooth_v = 0.f;  // eps / V
+  float* resid = nullptr;  // [M] the target's gradient less its rounded value
   int col0 = 0;          // first word of this call's columns
   int n_valid = 0;       // columns that are words (the others pad N to 32)
 };

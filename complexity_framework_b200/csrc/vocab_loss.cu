@@ -51,7 +51,15 @@ __global__ void __launch_bounds__(256) vl_gather_k(const VlCall c, const VlForwa
   const int64_t first = static_cast<int64_t>(blockIdx.x) * per;
   const auto counts = [&](int64_t y) { return y != c.ignore && y >= 0 && y < c.V; };
   int before = 0;
-  for (int64_t i = tid; i < first; i += 256) before += counts(f.targets[i]) ? 1 : 0;
+  int64_t i0 = tid;
+  for (; i0 + 7 * 256 < first; i0 += 8 * 256) {  // eight loads under way
+    int64_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = f.targets[i0 + k * 256];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) before += counts(v[k]) ? 1 : 0;
+  }
+  for (; i0 < first; i0 += 256) before += counts(f.targets[i0]) ? 1 : 0;
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) warp_n[warp] = before;
   __syncthreads();
@@ -87,11 +95,27 @@ __global__ void __launch_bounds__(256) vl_gather_k(const VlCall c, const VlForwa
   }
   __syncthreads();
   const int nv = c.H >> 3;
-  for (int r = warp; r < per && first + r < c.T; r += 8) {
-    if (dest[r] < 0) continue;
-    const uint4* in = reinterpret_cast<const uint4*>(f.h + (first + r) * c.H);
-    uint4* out = reinterpret_cast<uint4*>(c.hc + static_cast<int64_t>(dest[r]) * c.H);
-    for (int i = lane; i < nv; i += 32) out[i] = in[i];
+  for (int r0 = warp; r0 < per && first + r0 < c.T; r0 += 4 * 8) {  // four rows at a time
+    const uint4* in[4];
+    uint4* out[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + k * 8;
+      const int to = r < per && first + r < c.T ? dest[r] : -1;
+      in[k] = to < 0 ? nullptr : reinterpret_cast<const uint4*>(f.h + (first + r) * c.H);
+      out[k] = to < 0 ? nullptr
+                      : reinterpret_cast<uint4*>(c.hc + static_cast<int64_t>(to) * c.H);
+    }
+#pragma unroll 2
+    for (int i = lane; i < nv; i += 32) {
+      uint4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (in[k] != nullptr) v[k] = in[k][i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (in[k] != nullptr) out[k][i] = v[k];
+    }
   }
   if (blockIdx.x + 1 < gridDim.x) return;
   // the last block knows the count; rows up to the next whole block of 64 become 0
@@ -139,12 +163,13 @@ __global__ void __launch_bounds__(256) vl_rows_k(const VlCall c, const VlForward
   const float lse = lse2 * kLn2;
   float loss = lse - zt[row];
   if (c.smooth > 0.f) loss += c.smooth * (zt[row] - zs / static_cast<float>(c.V));
-  f.rows[src] = loss + c.z * lse * lse;
+  f.rows[src] = c.sign * (loss + c.z * lse * lse);
 }
 
 __global__ void __launch_bounds__(1024) vl_total_k(const VlCall c, const VlForward f) {
   __shared__ float part[32];
   float s = 0.f;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < c.T; i += 1024) s += f.rows[i];
   s = warp_sum(s);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
@@ -155,19 +180,30 @@ __global__ void __launch_bounds__(1024) vl_total_k(const VlCall c, const VlForwa
   }
 }
 
-// dh in the call's order: the K slices' sum of a counted row, 0 of the others.
+// dh in the call's order: the K slices' sum of a counted row, 0 of the others.  The target's
+// gradient, about -1 beside words' of some 1 / V, is most of a row's: what rounding it to bf16
+// took (resid) is added back as resid w_target, so that its error is not dh's.
 __global__ void __launch_bounds__(256) vl_scatter_k(const VlCall c, const float* __restrict__ acc,
                                                     int ldc, int64_t slice, int slices,
+                                                    const float* __restrict__ resid,
                                                     __nv_bfloat16* __restrict__ dh) {
   const int lane = threadIdx.x & 31, nv = c.H >> 3;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < c.T;
        row += static_cast<int64_t>(gridDim.x) * 8) {
     const int at = c.pos[row];
     uint4* out = reinterpret_cast<uint4*>(dh + row * c.H);
+    const float r = at >= 0 ? resid[at] : 0.f;
+    const uint4* w =
+        reinterpret_cast<const uint4*>(c.w + static_cast<int64_t>(at >= 0 ? c.target[at] : 0) * c.H);
+#pragma unroll 2
     for (int i = lane; i < nv; i += 32) {
       uint4 u = make_uint4(0u, 0u, 0u, 0u);
       if (at >= 0) {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        const uint4 t = w[i];
+        const float2 t0 = unpack_bf16x2(t.x), t1 = unpack_bf16x2(t.y), t2 = unpack_bf16x2(t.z),
+                     t3 = unpack_bf16x2(t.w);
+        float4 a = make_float4(r * t0.x, r * t0.y, r * t1.x, r * t1.y);
+        float4 b = make_float4(r * t2.x, r * t2.y, r * t3.x, r * t3.y);
         const float* p = acc + static_cast<int64_t>(at) * ldc + i * 8;
         for (int k = 0; k < slices; ++k) {
           const float4 x = *reinterpret_cast<const float4*>(p + k * slice);
@@ -190,6 +226,7 @@ GemmEpi epi_of(const VlCall& c) {
   GemmEpi ep;
   ep.ce.k2 = c.scale * kLog2e;
   ep.ce.scale = c.scale;
+  ep.ce.gsign = c.sign;
   ep.ce.target = c.target;
   ep.ce.n_valid = 0;
   ep.m_dev = c.cnt + 1;
@@ -238,23 +275,58 @@ int vl_forward(const VlCall& c, const VlForward& f, cudaStream_t s) {
   return static_cast<int>(cudaGetLastError());
 }
 
+// The pieces of the vocabulary and the K slices of the hidden gradient.
+//
+// A product's tiles (256 x 256, one CTA pair each) come in waves of all pairs, and the last wave
+// may be nearly empty: dW of 8192 words x 896 is 128 tiles, 1.7 waves, and its second costs as
+// much as the first.  So, within the workspace, the piece whose dW waves over the vocabulary and
+// per-piece costs (dh read and written once more, launches) come out least.  And dh, whose tiles
+// are few (4 x 12 at 3000 x 1024: 48 of 74 pairs), is cut along the words into the slices that
+// fill the waves best; as the counted rows may be any part of all, the rule takes the mean over
+// all, three quarters and half of them.
 void vl_backward_plan(const VlCall& c, int64_t workspace_bytes, VlBackward* b) {
   const int64_t R = vl_rows(c.T);
-  int64_t most = workspace_bytes / (2 * R) / 256 * 256;
-  if (most < 256) most = 256;
-  const int64_t pieces = (c.V + most - 1) / most;
-  b->piece = static_cast<int>(((c.V + pieces - 1) / pieces + 255) / 256 * 256);
-  // few rows: the hidden gradient's K, the words, over several CTAs
-  const bool pair = R > 128;
-  const int64_t tiles = ((R + 255) / 256) * ((c.H + 255) / 256);
-  const int64_t units = pair ? c.num_sms / 2 : c.num_sms;
-  const int64_t blocks = (std::min<int64_t>(b->piece, c.V) + 63) / 64;
-  // words of the last piece, which every slice needs some of
-  const int64_t last = (c.V - (pieces - 1) * b->piece + 63) / 64;
-  int64_t ks = units / tiles;
-  if (ks > blocks / 4) ks = blocks / 4;
-  if (ks > last) ks = last;
-  b->ksplit = ks < 1 ? 1 : static_cast<int>(ks);
+  const double rate = 1.4e9, hbm = 6.5e6;  // operations and bytes a us
+  const int64_t cols = (c.H + 255) / 256;
+  const auto waves = [&](int64_t tiles, int64_t rows) {
+    const int64_t units = rows > 128 ? c.num_sms / 2 : c.num_sms;
+    return static_cast<double>((tiles + units - 1) / units) * units;
+  };
+  int64_t most = workspace_bytes / (2 * R) / 256;  // in 256 words
+  const int64_t all = (static_cast<int64_t>(c.V) + 255) / 256;
+  most = std::max<int64_t>(1, std::min(most, all));
+  const double tile_us = 2.0 * 256 * 256 * static_cast<double>(R) / rate;
+  const double piece_us = 10 + 8.0 * static_cast<double>(R) * pad32(c.H) / hbm;
+  double best = 0;
+  for (int64_t p = most; p >= std::max<int64_t>(1, most / 3); --p) {
+    const int64_t full = all / p, rest = all % p;
+    double us = (full * waves(p * cols, 256) + (rest ? waves(rest * cols, 256) : 0.0)) * tile_us +
+                static_cast<double>(full + (rest ? 1 : 0)) * piece_us;
+    if (best == 0 || us < best) {
+      best = us;
+      b->piece = static_cast<int>(p * 256);
+    }
+  }
+  // slices of at least eight K blocks, and some of the last piece's for each
+  const int64_t words = std::min<int64_t>(b->piece, c.V);
+  const int64_t last = (c.V - (c.V - 1) / b->piece * b->piece + 63) / 64;
+  const int64_t top = std::min<int64_t>(std::min<int64_t>(words / 512, last), 64);
+  best = 0;
+  b->ksplit = 1;
+  for (int64_t ks = 1; ks <= std::max<int64_t>(1, top); ++ks) {
+    double us = 0;
+    for (int part = 2; part <= 4; ++part) {
+      const int64_t rows = std::max<int64_t>(1, R * part / 4);
+      const int64_t tiles = (R > 128 ? (rows + 255) / 256 : 1) * cols * ks;
+      const double tile = 2.0 * (R > 128 ? 256 : 128) * 256 * static_cast<double>(words) / ks;
+      us += waves(tiles, R) * tile / rate +
+            static_cast<double>(ks) * rows * pad32(c.H) * 8 / hbm;
+    }
+    if (best == 0 || us < 0.97 * best) {
+      best = us;
+      b->ksplit = static_cast<int>(ks);
+    }
+  }
 }
 
 int64_t vl_acc_floats(const VlCall& c, const VlBackward& b) {
@@ -292,6 +364,7 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
     ep.ce.smooth = c.smooth;
     ep.ce.smooth_v = c.smooth / static_cast<float>(c.V);
     ep.ce.col0 = v0;
+    ep.ce.resid = b.resid;
     ep.ce.n_valid = n;
     ep.group_m = 8;
     int rc = gemm_tc_launch(g, ep, s, c.err);
@@ -343,7 +416,7 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
   if (b.dh != nullptr) {
     const int64_t want = (c.T + 7) / 8, most = static_cast<int64_t>(c.num_sms) * 8;
     vl_scatter_k<<<static_cast<unsigned>(want < most ? want : most), 256, 0, s>>>(
-        c, b.acc, ldh, R * ldh, b.ksplit, b.dh);
+        c, b.acc, ldh, R * ldh, b.ksplit, b.resid, b.dh);
   }
   return static_cast<int>(cudaGetLastError());
 }

@@ -18,6 +18,7 @@ struct VlCall {
   int64_t T = 0;
   int V = 0, H = 0;
   float scale = 1.f, smooth = 0.f, z = 0.f;
+  float sign = 1.f;                  // of the row losses (-1: log-probabilities)
   int64_t ignore = -100;
   const __nv_bfloat16* w = nullptr;  // [V, H]
   __nv_bfloat16* hc = nullptr;       // [R, H] compact rows
@@ -48,6 +49,7 @@ struct VlBackward {
   int piece = 0, ksplit = 1;
   __nv_bfloat16* dl = nullptr;       // [R, piece]
   float* acc = nullptr;              // vl_acc_floats
+  float* resid = nullptr;            // [R] what rounding took from each row's target
 };
 void vl_backward_plan(const VlCall& c, int64_t workspace_bytes, VlBackward* b);
 int64_t vl_acc_floats(const VlCall& c, const VlBackward& b);

@@ -32,24 +32,23 @@ WORKSPACE_BYTES = 512 << 20
 
 class _VocabLossFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, smooth, z, scale, reduction, ws):
-        loss, hc, ints, floats, w = require().vocab_loss_fwd(hidden, weight, targets, ignore_index,
-                                                             smooth, z, scale, reduction)
+    def forward(ctx, hidden, weight, targets, ignore_index, smooth, z, scale, reduction, sign, ws):
+        loss, saved, w = require().vocab_loss_fwd(hidden, weight, targets, ignore_index, smooth, z,
+                                                  scale, reduction, sign, True)
         # the caller's weight itself where it was read in place, so that a change to it before
         # the backward pass is noticed
-        ctx.save_for_backward(hc, ints, floats,
-                              weight if w.data_ptr() == weight.data_ptr() else w)
-        ctx.meta = (hidden.shape[0], smooth, z, scale, reduction == 0)
+        ctx.save_for_backward(saved, weight if w.data_ptr() == weight.data_ptr() else w)
+        ctx.meta = (hidden.shape[0], smooth, z, scale, reduction == 0, sign)
         ctx.ws = ws
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        hc, ints, floats, w = ctx.saved_tensors
-        dh, dw = require().vocab_loss_bwd(gout, hc, ints, floats, w, *ctx.meta,
-                                          ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.ws)
-        return dh, dw, None, None, None, None, None, None, None
+        saved, w = ctx.saved_tensors
+        dh, dw = require().vocab_loss_bwd(gout, saved, w, *ctx.meta, ctx.needs_input_grad[0],
+                                          ctx.needs_input_grad[1], ctx.ws)
+        return dh, dw, None, None, None, None, None, None, None, None
 
 
 def _rows_torch(h, w, y, ignore_index, smooth, z, scale):
@@ -79,6 +78,12 @@ def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: tor
     sum, or, with ``reduction="none"``, every row's, shaped like ``targets``."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {list(_REDUCTIONS)}")
+    return _loss(hidden, weight, targets, ignore_index, label_smoothing, z_loss, logit_scale,
+                 reduction, 1.0, workspace_bytes)
+
+
+def _loss(hidden, weight, targets, ignore_index, label_smoothing, z_loss, logit_scale, reduction,
+          sign, workspace_bytes):
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError("label_smoothing must be between 0 and 1")
     if not 0.0 <= z_loss < float("inf"):
@@ -94,13 +99,13 @@ def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: tor
     h, y = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1)
     if h.is_cuda:
         args = (h, weight, y, ignore_index, label_smoothing, z_loss, logit_scale,
-                _REDUCTIONS[reduction])
+                _REDUCTIONS[reduction], sign)
         if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
             loss = _VocabLossFn.apply(*args, workspace_bytes)
         else:
-            loss = require().vocab_loss_fwd(*args)[0]
+            loss = require().vocab_loss_fwd(*args, False)[0]
         return loss.view(targets.shape) if reduction == "none" else loss
-    rows = _rows_torch(h, weight, y, ignore_index, label_smoothing, z_loss, logit_scale)
+    rows = sign * _rows_torch(h, weight, y, ignore_index, label_smoothing, z_loss, logit_scale)
     if reduction == "none":
         return rows.view(targets.shape)
     if reduction == "sum":
@@ -113,6 +118,5 @@ def token_logprobs(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
                    workspace_bytes: int = WORKSPACE_BYTES) -> torch.Tensor:
     """Log-probability of every target under ``softmax(logit_scale * hidden @ weight.T)``, fp32,
     shaped like ``targets``; 0 where the target is ``ignore_index``."""
-    return -vocab_cross_entropy(hidden, weight, targets, ignore_index=ignore_index,
-                                logit_scale=logit_scale, reduction="none",
-                                workspace_bytes=workspace_bytes)
+    return _loss(hidden, weight, targets, ignore_index, 0.0, 0.0, logit_scale, "none", -1.0,
+                 workspace_bytes)
