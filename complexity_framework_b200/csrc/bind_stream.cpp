@@ -2,6 +2,8 @@
 // checked here; every entry allocates its outputs and launches on the current stream of its
 // tensors' device.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -12,6 +14,22 @@
 
 int* cfb_err_ptr(int device);
 int cfb_num_sms(int device);
+
+// Gradients under create_graph: they have no gradient themselves, and say so when asked.
+torch::autograd::variable_list cfb_once_differentiable(torch::autograd::variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list defined;
+  for (const auto& g : grads)
+    if (g.defined()) defined.push_back(g.detach().requires_grad_());
+  if (defined.empty()) return grads;
+  const auto node = std::make_shared<torch::autograd::DelayedError>(
+      "these gradients cannot be differentiated twice", static_cast<int64_t>(defined.size()));
+  const torch::autograd::variable_list out = (*node)(std::move(defined));
+  size_t k = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = out[k++];
+  return grads;
+}
 
 namespace {
 
@@ -201,10 +219,93 @@ Tensor dropout(const Tensor& x_in, double p, const OptTensor& seed, int64_t seed
   return y;
 }
 
+// ------------------------------------------------------------------ autograd
+// The nodes are C++ ones: a Python node's backward takes the interpreter's lock on the engine's
+// thread, which is more time than the kernels of a small call take.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+struct DropoutNode : torch::autograd::Function<DropoutNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& seed, double p,
+                        int64_t seed_value, int64_t stream) {
+    ctx->save_for_backward({or_none(seed)});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed_value;
+    ctx->saved_data["stream"] = stream;
+    return dropout(x, p, seed, seed_value, stream);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor dx = dropout(dy[0], ctx->saved_data["p"].toDouble(), opt(saved[0]),
+                        ctx->saved_data["seed"].toInt(), ctx->saved_data["stream"].toInt());
+    return cfb_once_differentiable({dx, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+Tensor dropout_grad(const Tensor& x, double p, const OptTensor& seed, int64_t seed_value,
+                    int64_t stream) {
+  return DropoutNode::apply(x, seed, p, seed_value, stream);
+}
+
+struct ResidualNormNode : torch::autograd::Function<ResidualNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& b,
+                               const OptTensor& w1, const OptTensor& gate, const OptTensor& w2,
+                               const OptTensor& seed, double scale, double p, int64_t seed_value,
+                               int64_t stream, double eps) {
+    ctx->set_materialize_grads(false);
+    auto [xnew, y, r1, r2] = residual_norm_fwd(x, b, w1, gate, w2, scale, p, seed, seed_value,
+                                               stream, eps, true);
+    ctx->save_for_backward({xnew, b, or_none(w1), or_none(gate), or_none(w2), or_none(r1),
+                            or_none(r2), or_none(seed)});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed_value;
+    ctx->saved_data["stream"] = stream;
+    variable_list out = {xnew};
+    if (y.has_value()) out.push_back(*y);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(11);
+    const auto v = ctx->get_saved_variables();
+    const bool dy = g.size() > 1 && g[1].defined();
+    std::vector<bool> need(5);
+    for (int i = 0, k = 0; i < 5; ++i) {
+      // the graph's edges are the defined inputs' only
+      const bool given = i < 2 || v[i].defined();
+      need[i] = given && ctx->needs_input_grad(k);
+      if (given) ++k;
+    }
+    need[4] = need[4] && dy;
+    if ((!g[0].defined() && !dy) || !(need[0] || need[1] || need[2] || need[3] || need[4]))
+      return out;
+    const auto grads = residual_norm_bwd(
+        opt(g[0]), dy ? OptTensor(g[1]) : OptTensor(), v[0], v[1], opt(v[2]), opt(v[3]), opt(v[4]),
+        opt(v[5]), opt(v[6]), ctx->saved_data["scale"].toDouble(), ctx->saved_data["p"].toDouble(),
+        opt(v[7]), ctx->saved_data["seed"].toInt(), ctx->saved_data["stream"].toInt(), need);
+    for (int i = 0; i < 5; ++i) out[i] = or_none(grads[i]);
+    return cfb_once_differentiable(std::move(out));
+  }
+};
+
+std::tuple<Tensor, OptTensor> residual_norm_grad(const Tensor& x, const Tensor& b,
+                                                 const OptTensor& w1, const OptTensor& gate,
+                                                 const OptTensor& w2, double scale, double p,
+                                                 const OptTensor& seed, int64_t seed_value,
+                                                 int64_t stream, double eps) {
+  const auto out = ResidualNormNode::apply(x, b, w1, gate, w2, seed, scale, p, seed_value, stream,
+                                           eps);
+  return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
+}
+
 }  // namespace
 
 void register_stream(pybind11::module& m) {
   m.def("residual_norm_fwd", &residual_norm_fwd);
-  m.def("residual_norm_bwd", &residual_norm_bwd);
   m.def("dropout", &dropout);
+  m.def("residual_norm_grad", &residual_norm_grad);
+  m.def("dropout_grad", &dropout_grad);
 }

@@ -1,5 +1,6 @@
 // Python bindings of the cross-entropy over the vocabulary (vocab_loss.cu).
 #include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -10,6 +11,7 @@
 
 int* cfb_err_ptr(int device);
 int cfb_num_sms(int device);
+torch::autograd::variable_list cfb_once_differentiable(torch::autograd::variable_list grads);
 
 namespace {
 
@@ -174,9 +176,51 @@ std::tuple<OptTensor, OptTensor> vocab_loss_bwd(const Tensor& gout_in, const Ten
   return {dh, dw};
 }
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct VocabLossNode : torch::autograd::Function<VocabLossNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& y,
+                        int64_t ignore, double smooth, double z, double scale, int64_t reduction,
+                        double sign, int64_t workspace_bytes) {
+    auto [loss, saved, read] = vocab_loss_fwd(h, w, y, ignore, smooth, z, scale, reduction, sign,
+                                              true);
+    // the caller's weight itself where it was read in place, so that a change to it before the
+    // backward pass is noticed
+    ctx->save_for_backward({saved, read.data_ptr() == w.data_ptr() ? w : read});
+    ctx->saved_data["rows"] = h.size(0);
+    ctx->saved_data["smooth"] = smooth;
+    ctx->saved_data["z"] = z;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["per_row"] = reduction == 0;
+    ctx->saved_data["sign"] = sign;
+    ctx->saved_data["workspace"] = workspace_bytes;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    const auto saved = ctx->get_saved_variables();
+    const auto num = [&](const char* key) { return ctx->saved_data[key].toDouble(); };
+    const auto grads = vocab_loss_bwd(
+        gout[0].detach(), saved[0], saved[1].detach(), ctx->saved_data["rows"].toInt(),
+        num("smooth"), num("z"), num("scale"), ctx->saved_data["per_row"].toBool(), num("sign"),
+        ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->saved_data["workspace"].toInt());
+    variable_list out(10);
+    if (std::get<0>(grads).has_value()) out[0] = *std::get<0>(grads);
+    if (std::get<1>(grads).has_value()) out[1] = *std::get<1>(grads);
+    return cfb_once_differentiable(std::move(out));
+  }
+};
+
+// The loss alone, with its gradient where `grad` asks for it.
+Tensor vocab_loss(const Tensor& h, const Tensor& w, const Tensor& y, int64_t ignore, double smooth,
+                  double z, double scale, int64_t reduction, double sign, int64_t workspace_bytes,
+                  bool grad) {
+  if (grad)
+    return VocabLossNode::apply(h, w, y, ignore, smooth, z, scale, reduction, sign,
+                                workspace_bytes);
+  return std::get<0>(vocab_loss_fwd(h, w, y, ignore, smooth, z, scale, reduction, sign, false));
+}
+
 }  // namespace
 
-void register_vocab(pybind11::module& m) {
-  m.def("vocab_loss_fwd", &vocab_loss_fwd);
-  m.def("vocab_loss_bwd", &vocab_loss_bwd);
-}
+void register_vocab(pybind11::module& m) { m.def("vocab_loss", &vocab_loss); }

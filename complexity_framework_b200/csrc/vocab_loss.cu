@@ -277,41 +277,30 @@ int vl_forward(const VlCall& c, const VlForward& f, cudaStream_t s) {
 
 // The pieces of the vocabulary and the K slices of the hidden gradient.
 //
-// A product's tiles (256 x 256, one CTA pair each) come in waves of all pairs, and the last wave
-// may be nearly empty: dW of 8192 words x 896 is 128 tiles, 1.7 waves, and its second costs as
-// much as the first.  So, within the workspace, the piece whose dW waves over the vocabulary and
-// per-piece costs (dh read and written once more, launches) come out least.  And dh, whose tiles
-// are few (4 x 12 at 3000 x 1024: 48 of 74 pairs), is cut along the words into the slices that
-// fill the waves best; as the counted rows may be any part of all, the rule takes the mean over
-// all, three quarters and half of them.
+// One piece where the workspace holds all of dz; else about 256 MB of it, but at least 4096 words:
+// two L2 caches' worth, of which the next product still finds half, while every piece costs a
+// launch of three products and dh read and written once more.  32768 x 32000 x 896 in 128, 256,
+// 512, 2048 MB: 9.8, 6.4, 6.5, 6.9 ms (on a card at its power limit the last three are 6.4, 7.0,
+// 6.9); 4096 x 100000 x 4096 in 64, 192, 256, 512 MB: 11.0, 10.1, 10.1, 10.5 ms; one piece against
+// two of 3001 x 50021 x 1024: 0.93, 1.01 ms.
+//
+// dh has few tiles (256 x 256, one CTA pair each): 48 at 3000 x 1024 for 74 pairs.  It is cut along
+// the words into the slices that fill the waves of pairs best; as the counted rows may be any part
+// of all, the rule takes the mean over all, three quarters and half of them.
 void vl_backward_plan(const VlCall& c, int64_t workspace_bytes, VlBackward* b) {
   const int64_t R = vl_rows(c.T);
+  int64_t words = std::max<int64_t>(workspace_bytes / (2 * R) / 256 * 256, 256);
+  if (words < c.V) words = std::min(words, std::max<int64_t>((128 << 20) / R / 256 * 256, 4096));
+  const int64_t pieces = (c.V + words - 1) / words;
+  b->piece = static_cast<int>(((c.V + pieces - 1) / pieces + 255) / 256 * 256);
   const double rate = 1.4e9, hbm = 6.5e6;  // operations and bytes a us
   const int64_t cols = (c.H + 255) / 256;
-  const auto waves = [&](int64_t tiles, int64_t rows) {
-    const int64_t units = rows > 128 ? c.num_sms / 2 : c.num_sms;
-    return static_cast<double>((tiles + units - 1) / units) * units;
-  };
-  int64_t most = workspace_bytes / (2 * R) / 256;  // in 256 words
-  const int64_t all = (static_cast<int64_t>(c.V) + 255) / 256;
-  most = std::max<int64_t>(1, std::min(most, all));
-  const double tile_us = 2.0 * 256 * 256 * static_cast<double>(R) / rate;
-  const double piece_us = 10 + 8.0 * static_cast<double>(R) * pad32(c.H) / hbm;
-  double best = 0;
-  for (int64_t p = most; p >= std::max<int64_t>(1, most / 3); --p) {
-    const int64_t full = all / p, rest = all % p;
-    double us = (full * waves(p * cols, 256) + (rest ? waves(rest * cols, 256) : 0.0)) * tile_us +
-                static_cast<double>(full + (rest ? 1 : 0)) * piece_us;
-    if (best == 0 || us < best) {
-      best = us;
-      b->piece = static_cast<int>(p * 256);
-    }
-  }
+  const int64_t units = R > 128 ? c.num_sms / 2 : c.num_sms;
   // slices of at least eight K blocks, and some of the last piece's for each
-  const int64_t words = std::min<int64_t>(b->piece, c.V);
+  words = std::min<int64_t>(b->piece, c.V);
   const int64_t last = (c.V - (c.V - 1) / b->piece * b->piece + 63) / 64;
   const int64_t top = std::min<int64_t>(std::min<int64_t>(words / 512, last), 64);
-  best = 0;
+  double best = 0;
   b->ksplit = 1;
   for (int64_t ks = 1; ks <= std::max<int64_t>(1, top); ++ks) {
     double us = 0;
@@ -319,7 +308,7 @@ void vl_backward_plan(const VlCall& c, int64_t workspace_bytes, VlBackward* b) {
       const int64_t rows = std::max<int64_t>(1, R * part / 4);
       const int64_t tiles = (R > 128 ? (rows + 255) / 256 : 1) * cols * ks;
       const double tile = 2.0 * (R > 128 ? 256 : 128) * 256 * static_cast<double>(words) / ks;
-      us += waves(tiles, R) * tile / rate +
+      us += static_cast<double>((tiles + units - 1) / units * units) * tile / rate +
             static_cast<double>(ks) * rows * pad32(c.H) * 8 / hbm;
     }
     if (best == 0 || us < 0.97 * best) {

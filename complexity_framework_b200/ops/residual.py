@@ -31,8 +31,6 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
-
 from ._ext import require
 
 Seed = Union[int, torch.Tensor]
@@ -109,21 +107,6 @@ def dropout_factors(shape, p: float, seed: Seed, *, stream: int = 0,
 
 
 # ------------------------------------------------------------------- dropout
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, seed, seed_value, stream):
-        ctx.save_for_backward(seed)
-        ctx.meta = (p, seed_value, stream)
-        return require().dropout(x, p, seed, seed_value, stream)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        (seed,) = ctx.saved_tensors
-        p, seed_value, stream = ctx.meta
-        return require().dropout(dy, p, seed, seed_value, stream), None, None, None, None
-
-
 def dropout(x: torch.Tensor, p: float, seed: Seed, *, stream: int = 0) -> torch.Tensor:
     """``x`` with a share ``p`` of its elements set to 0 and the others divided by the kept
     share, by the counter-based generator (see the module)."""
@@ -137,37 +120,11 @@ def dropout(x: torch.Tensor, p: float, seed: Seed, *, stream: int = 0) -> torch.
         wide = x if x.dtype == torch.float64 else x.float()
         return torch.where(f == 0, 0.0, wide * f).to(x.dtype)
     if torch.is_grad_enabled() and x.requires_grad:
-        return _DropoutFn.apply(x, p, tensor, value, stream)
+        return require().dropout_grad(x, p, tensor, value, stream)
     return require().dropout(x, p, tensor, value, stream)
 
 
 # -------------------------------------------------------------- residual join
-class _ResidualNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, branch, w1, gate, w2, seed, scale, p, seed_value, stream, eps):
-        ctx.set_materialize_grads(False)
-        new, y, r1, r2 = require().residual_norm_fwd(x, branch, w1, gate, w2, scale, p, seed,
-                                                     seed_value, stream, eps, True)
-        # x' is needed for its norm only, but its shape and type always
-        ctx.save_for_backward(new, branch, w1, gate, w2, r1, r2, seed)
-        ctx.meta = (scale, p, seed_value, stream)
-        return new, y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dnew, dy):
-        new, branch, w1, gate, w2, r1, r2, seed = ctx.saved_tensors
-        scale, p, seed_value, stream = ctx.meta
-        need = list(ctx.needs_input_grad[:5])
-        if (dnew is None and dy is None) or not any(need):
-            return (None,) * 11
-        if dy is None:
-            need[4] = False
-        grads = require().residual_norm_bwd(dnew, dy, new, branch, w1, gate, w2, r1, r2, scale, p,
-                                            seed, seed_value, stream, need)
-        return (*grads, None, None, None, None, None, None)
-
-
 def _residual_norm_torch(x, branch, w1, gate, w2, scale, factors, eps):
     """The formulas in PyTorch, in fp32 (fp64 for fp64 tensors), rounded at the ends."""
     dt = x.dtype
@@ -222,5 +179,5 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, *,
         return _residual_norm_torch(x, branch, branch_weight, gate, norm_weight, scale, f, eps)
     ts = (x, branch, branch_weight, gate, norm_weight)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        return _ResidualNormFn.apply(*ts, tensor, scale, p, value, stream, eps)
+        return require().residual_norm_grad(*ts, scale, p, tensor, value, stream, eps)
     return require().residual_norm_fwd(*ts, scale, p, tensor, value, stream, eps, False)[:2]

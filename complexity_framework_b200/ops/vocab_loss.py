@@ -22,33 +22,11 @@ CPU the same formulas run in PyTorch, any floating-point type.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._ext import require
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 WORKSPACE_BYTES = 512 << 20
-
-
-class _VocabLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, smooth, z, scale, reduction, sign, ws):
-        loss, saved, w = require().vocab_loss_fwd(hidden, weight, targets, ignore_index, smooth, z,
-                                                  scale, reduction, sign, True)
-        # the caller's weight itself where it was read in place, so that a change to it before
-        # the backward pass is noticed
-        ctx.save_for_backward(saved, weight if w.data_ptr() == weight.data_ptr() else w)
-        ctx.meta = (hidden.shape[0], smooth, z, scale, reduction == 0, sign)
-        ctx.ws = ws
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gout):
-        saved, w = ctx.saved_tensors
-        dh, dw = require().vocab_loss_bwd(gout, saved, w, *ctx.meta, ctx.needs_input_grad[0],
-                                          ctx.needs_input_grad[1], ctx.ws)
-        return dh, dw, None, None, None, None, None, None, None, None
 
 
 def _rows_torch(h, w, y, ignore_index, smooth, z, scale):
@@ -98,12 +76,9 @@ def _loss(hidden, weight, targets, ignore_index, label_smoothing, z_loss, logit_
         raise TypeError("targets must be int64")
     h, y = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1)
     if h.is_cuda:
-        args = (h, weight, y, ignore_index, label_smoothing, z_loss, logit_scale,
-                _REDUCTIONS[reduction], sign)
-        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-            loss = _VocabLossFn.apply(*args, workspace_bytes)
-        else:
-            loss = require().vocab_loss_fwd(*args, False)[0]
+        grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+        loss = require().vocab_loss(h, weight, y, ignore_index, label_smoothing, z_loss, logit_scale,
+                                    _REDUCTIONS[reduction], sign, workspace_bytes, grad)
         return loss.view(targets.shape) if reduction == "none" else loss
     rows = sign * _rows_torch(h, weight, y, ignore_index, label_smoothing, z_loss, logit_scale)
     if reduction == "none":
