@@ -161,12 +161,13 @@ std::tuple<OptTensor, OptTensor> vocab_loss_bwd(const Tensor& gout_in, const Ten
   b.per_row = per_row;
   cfb::vl_backward_plan(c, workspace_bytes, &b);
   const int64_t R = cfb::vl_rows(T);
-  const int64_t dl_bytes = up16(2 * R * b.piece), resid_bytes = up16(4 * R);
+  const int64_t dl_bytes = up16(2 * R * b.piece), resid_bytes = up16(4 * R + 4);
   const Tensor ws = empty({dl_bytes + resid_bytes + (need_h ? 4 * cfb::vl_acc_floats(c, b) : 0)},
                           torch::kUInt8, w);
   char* at = static_cast<char*>(ws.data_ptr());
   b.dl = reinterpret_cast<__nv_bfloat16*>(at);
   b.resid = reinterpret_cast<float*>(at + dl_bytes);
+  b.alpha = b.resid + R;
   if (need_h) {
     b.acc = reinterpret_cast<float*>(at + dl_bytes + resid_bytes);
     b.dh = bf(*dh);

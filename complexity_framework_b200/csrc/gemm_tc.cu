@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(384, 1)
                                               load_bar + kMaxLoadDepth * (warp - 4), 0u,
                                       0u, lane};
     bool ep_ok = true;
+    const float alpha = ep.alpha_dev != nullptr ? ep.alpha * __ldg(ep.alpha_dev) : ep.alpha;
     for (int u = unit; u < total; u += units) {
       const Unit un = decode_unit(u, num_tiles, num_n, num_m, m_shift, ksplit, nk, ep.grp);
       if (un.skip) continue;
@@ -799,8 +800,7 @@ __global__ void __launch_bounds__(384, 1)
         int tgt = -1;
         const int src = row_ok ? ep.ce.src[row] : -1;
         if (src >= 0) {
-          float g = ep.ce.gout[ep.ce.per_row ? src : 0] * (ep.ce.scale * ep.ce.gsign);
-          if (ep.ce.ginv != nullptr) g *= *ep.ce.ginv;
+          const float g = (ep.ce.gout != nullptr ? ep.ce.gout[src] : 1.0f) * ep.ce.inv_unit;
           lse2 = ep.ce.lse2[row];
           ga = g * (1.0f + ep.ce.z2 * (lse2 * 0.693147180559945f));
           gb = g * (1.0f - ep.ce.smooth);
@@ -846,7 +846,7 @@ __global__ void __launch_bounds__(384, 1)
           tmem_ld32(tbase + c, v);
           tmem_wait_ld();
           if constexpr (EPI == EPI_STORE) {
-            if (n0 + c < N) ring.put(&tmC0, v, ep.alpha, n0 + c, m0 + wq * 32);
+            if (n0 + c < N) ring.put(&tmC0, v, alpha, n0 + c, m0 + wq * 32);
           } else if constexpr (EPI == EPI_RESID) {
             if (!lring.wait(abort_flag, err)) {
               ep_ok = false;
@@ -881,8 +881,8 @@ __global__ void __launch_bounds__(384, 1)
                                                       static_cast<int64_t>(row) * ep.ldc + n0 + c);
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
-                float4 w = make_float4(v[4 * q] * ep.alpha, v[4 * q + 1] * ep.alpha,
-                                       v[4 * q + 2] * ep.alpha, v[4 * q + 3] * ep.alpha);
+                float4 w = make_float4(v[4 * q] * alpha, v[4 * q + 1] * alpha,
+                                       v[4 * q + 2] * alpha, v[4 * q + 3] * alpha);
                 if constexpr (EPI == EPI_F32_ACC) {
                   float4 o = out[q];
                   w.x += o.x; w.y += o.y; w.z += o.z; w.w += o.w;

@@ -90,13 +90,13 @@ struct GemmCe {
   float2* stats = nullptr;  // [M][2 * ceil(N / 256)]
   float* zt = nullptr;      // [M]
   float* zsum = nullptr;    // [M][2 * ceil(N / 256)]
-  // gradient: g (p (1 + 2 lambda lse) - (1 - eps) [target] - eps / V) * scale, g = gout * ginv
+  // gradient: g_t (p (1 + 2 lambda lse) - eps / V - (1 - eps) [target]) / unit, where g_t is the
+  // row's own factor (per_row) or 1, and unit is 1 - eps (1 where that is 0): the target's term of
+  // a row without a factor is then -1, which bf16 holds exactly
   const float* lse2 = nullptr;  // [M] log-sum-exp in units of log 2
-  const float* gout = nullptr;  // one value, or one for each row of the call's own order
+  const float* gout = nullptr;  // null, or one factor for each row of the call's own order
   const int* src = nullptr;     // [M] that order's row of each row here, < 0: none
-  const float* ginv = nullptr;  // one value, or null
-  int per_row = 0;
-  float gsign = 1.f;     // of gout
+  float inv_unit = 1.f;
   float z2 = 0.f;        // 2 lambda
   float smooth = 0.f;    // eps
   float smooth_v = 0.f;  // eps / V
@@ -131,6 +131,7 @@ struct GemmEpi {
   const int* m_dev = nullptr;
   const int* k_dev = nullptr;
   int64_t split_stride = 0;  // EPI_F32 / EPI_F32_ACC: K slices write their own C, this far apart
+  const float* alpha_dev = nullptr;  // EPI_STORE, EPI_F32, EPI_F32_ACC: a further factor of acc
   int group_m = 0;           // > 0: the schedule takes the row tiles in groups of this many, every
                              // column tile of a group before the next group
 };

@@ -862,7 +862,7 @@ static int with_kernel(const JoinArgs& a, int num_sms, F f) {
                Feed<T, NV, RT, tensors, ODD, true>::pitch(a.H) * static_cast<int>(sizeof(T));
       if (hold_of(NV, RT) == kInShared) l.smem += 8 * a.H;
       const auto go = [&](auto kern) {
-        if (l.smem > 48 * 1024) {
+        if (l.smem > 40 * 1024) {  // 48 KB with the static part need no consent
           const cudaError_t e = cudaFuncSetAttribute(
               kern, cudaFuncAttributeMaxDynamicSharedMemorySize, l.smem);
           if (e != cudaSuccess) return static_cast<int>(e);

@@ -17,8 +17,10 @@
 // gathered in their order, and the products take their number from device memory.  A batch with
 // half of its tokens ignored costs half, and what an ignored row holds reaches nothing.
 //
-// dz is rounded to bf16 (2^-9 of its size, as the tensor cores' operand); its sums are fp32.  No
-// sum depends on the order of atomics: equal calls give equal bits.
+// dz is rounded to bf16, as the tensor cores' operand; its sums are fp32.  The factors that all
+// rows share (1 / counted rows, the incoming gradient, scale, 1 - eps) are left to the products'
+// epilogues, so that a target's term is p - 1 and the -1 is exact: scaled first, every target's
+// term would be off by the same part of up to 2^-9.  No sum depends on the order of atomics: equal calls give equal bits.
 #include <algorithm>
 #include <cmath>
 
@@ -186,13 +188,14 @@ __global__ void __launch_bounds__(1024) vl_total_k(const VlCall c, const VlForwa
 __global__ void __launch_bounds__(256) vl_scatter_k(const VlCall c, const float* __restrict__ acc,
                                                     int ldc, int64_t slice, int slices,
                                                     const float* __restrict__ resid,
+                                                    const float* __restrict__ alpha,
                                                     __nv_bfloat16* __restrict__ dh) {
   const int lane = threadIdx.x & 31, nv = c.H >> 3;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < c.T;
        row += static_cast<int64_t>(gridDim.x) * 8) {
     const int at = c.pos[row];
     uint4* out = reinterpret_cast<uint4*>(dh + row * c.H);
-    const float r = at >= 0 ? resid[at] : 0.f;
+    const float r = at >= 0 ? resid[at] * *alpha : 0.f;
     const uint4* w =
         reinterpret_cast<const uint4*>(c.w + static_cast<int64_t>(at >= 0 ? c.target[at] : 0) * c.H);
 #pragma unroll 2
@@ -219,6 +222,14 @@ __global__ void __launch_bounds__(256) vl_scatter_k(const VlCall c, const float*
   }
 }
 
+// What the rows' gradients of the logits leave out: scale, sign and unit, and the loss's own factor
+// where the rows share it.
+__global__ void vl_alpha_k(const VlCall c, const float* gout, bool per_row, float unit,
+                           float* alpha) {
+  *alpha = c.scale * c.sign * unit * (per_row ? 1.f : *gout * *c.ginv);
+}
+float unit_of(const VlCall& c) { return c.smooth < 1.f ? 1.f - c.smooth : 1.f; }
+
 int pad32(int n) { return (n + 31) / 32 * 32; }
 int halves_of(const VlCall& c) { return 2 * ((c.V + 255) / 256); }
 
@@ -226,7 +237,6 @@ GemmEpi epi_of(const VlCall& c) {
   GemmEpi ep;
   ep.ce.k2 = c.scale * kLog2e;
   ep.ce.scale = c.scale;
-  ep.ce.gsign = c.sign;
   ep.ce.target = c.target;
   ep.ce.n_valid = 0;
   ep.m_dev = c.cnt + 1;
@@ -278,11 +288,11 @@ int vl_forward(const VlCall& c, const VlForward& f, cudaStream_t s) {
 // The pieces of the vocabulary and the K slices of the hidden gradient.
 //
 // One piece where the workspace holds all of dz; else about 256 MB of it, but at least 4096 words:
-// two L2 caches' worth, of which the next product still finds half, while every piece costs a
-// launch of three products and dh read and written once more.  32768 x 32000 x 896 in 128, 256,
-// 512, 2048 MB: 9.8, 6.4, 6.5, 6.9 ms (on a card at its power limit the last three are 6.4, 7.0,
-// 6.9); 4096 x 100000 x 4096 in 64, 192, 256, 512 MB: 11.0, 10.1, 10.1, 10.5 ms; one piece against
-// two of 3001 x 50021 x 1024: 0.93, 1.01 ms.
+// of two L2 caches' worth the next product still finds some, while every piece costs three launches
+// and dh read and written once more.  32768 x 32000 x 896 in 128, 256, 512, 2048 MB: 9.8, 6.4, 6.5,
+// 6.9 ms; 4096 x 100000 x 4096 in 64, 192, 256, 512 MB: 11.0, 10.1, 10.1, 10.5 ms; one piece against
+// two of 3001 x 50021 x 1024: 0.93, 1.01 ms.  (Back to back for a second, a card at its power limit
+// takes 6.7 to 6.9 ms for the first whatever the piece.)
 //
 // dh has few tiles (256 x 256, one CTA pair each): 48 at 3000 x 1024 for 74 pairs.  It is cut along
 // the words into the slices that fill the waves of pairs best; as the counted rows may be any part
@@ -325,6 +335,7 @@ int64_t vl_acc_floats(const VlCall& c, const VlBackward& b) {
 int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
   const int64_t R = vl_rows(c.T);
   const int ldh = pad32(c.H);
+  vl_alpha_k<<<1, 1, 0, s>>>(c, b.gout, b.per_row, unit_of(c), b.alpha);
   for (int v0 = 0; v0 < c.V; v0 += b.piece) {
     const int n = c.V - v0 < b.piece ? c.V - v0 : b.piece;
     const __nv_bfloat16* w = c.w + static_cast<int64_t>(v0) * c.H;
@@ -345,9 +356,8 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
     ep.c = b.dl;
     ep.ldc = b.piece;
     ep.ce.lse2 = c.lse2;
-    ep.ce.gout = b.gout;
-    ep.ce.per_row = b.per_row ? 1 : 0;
-    ep.ce.ginv = b.per_row ? nullptr : c.ginv;
+    ep.ce.gout = b.per_row ? b.gout : nullptr;
+    ep.ce.inv_unit = 1.f / unit_of(c);
     ep.ce.src = c.src;
     ep.ce.z2 = 2.f * c.z;
     ep.ce.smooth = c.smooth;
@@ -377,6 +387,7 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
       e.c = b.acc;
       e.ldc = ldh;
       e.split_stride = R * ldh;
+      e.alpha_dev = b.alpha;
       rc = gemm_tc_launch(d, e, s, c.err);
       if (rc) return rc;
     }
@@ -396,6 +407,7 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
       d.epi = EPI_STORE;
       GemmEpi e;
       e.k_dev = c.cnt + 1;
+      e.alpha_dev = b.alpha;
       e.c = b.dw + static_cast<int64_t>(v0) * c.H;
       e.ldc = c.H;
       rc = gemm_tc_launch(d, e, s, c.err);
@@ -405,7 +417,7 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
   if (b.dh != nullptr) {
     const int64_t want = (c.T + 7) / 8, most = static_cast<int64_t>(c.num_sms) * 8;
     vl_scatter_k<<<static_cast<unsigned>(want < most ? want : most), 256, 0, s>>>(
-        c, b.acc, ldh, R * ldh, b.ksplit, b.resid, b.dh);
+        c, b.acc, ldh, R * ldh, b.ksplit, b.resid, b.alpha, b.dh);
   }
   return static_cast<int>(cudaGetLastError());
 }

@@ -50,6 +50,7 @@ struct VlBackward {
   __nv_bfloat16* dl = nullptr;       // [R, piece]
   float* acc = nullptr;              // vl_acc_floats
   float* resid = nullptr;            // [R] what rounding took from each row's target
+  float* alpha = nullptr;            // [1] workspace: the factor that all rows share
 };
 void vl_backward_plan(const VlCall& c, int64_t workspace_bytes, VlBackward* b);
 int64_t vl_acc_floats(const VlCall& c, const VlBackward& b);
