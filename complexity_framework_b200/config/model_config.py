@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import dataclasses
 import json
+import math
 from dataclasses import dataclass, field
 from typing import Any, Dict, Optional
 
@@ -146,6 +147,13 @@ class ModelConfig:
     # normalisation
     norm_type: str = "rmsnorm"
     norm_eps: float = 1e-6
+    # residual stream: "sandwich" also normalises what a branch adds; a learned gate of each
+    # channel (from this value), a factor and dropout of the branches, dropout of the embedding
+    norm_placement: str = "pre"
+    residual_gate_init: Optional[float] = None
+    residual_scale: float = 1.0
+    residual_dropout: float = 0.0
+    embedding_dropout: float = 0.0
     # embeddings
     tie_word_embeddings: bool = True
     # runtime
@@ -217,6 +225,11 @@ class ModelConfig:
             need(self.num_key_value_heads == self.num_attention_heads,
                  "TR-MHA requires one K/V head per query head")
         need(0.0 <= self.attention_dropout < 1.0, "attention_dropout must be in [0, 1)")
+        need(self.norm_placement in ("pre", "sandwich"),
+             "norm_placement must be 'pre' or 'sandwich'")
+        need(0.0 <= self.residual_dropout < 1.0, "residual_dropout must be in [0, 1)")
+        need(0.0 <= self.embedding_dropout < 1.0, "embedding_dropout must be in [0, 1)")
+        need(math.isfinite(self.residual_scale), "residual_scale must be finite")
         need(0.0 < self.rope_fraction <= 1.0, "rope_fraction must be in (0, 1]")
         need(self.sliding_window is None or self.sliding_window > 0,
              "sliding_window must be positive when set")
@@ -260,6 +273,12 @@ class ModelConfig:
                  "token_frequencies length must match vocab_size")
 
     # -------------------------------------------------------------- properties
+    @property
+    def joined_residual(self) -> bool:
+        """Whether a branch is more than added to the residual stream."""
+        return (self.norm_placement != "pre" or self.residual_gate_init is not None
+                or self.residual_scale != 1.0 or self.residual_dropout > 0.0)
+
     @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_attention_heads

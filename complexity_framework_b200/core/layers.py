@@ -5,11 +5,13 @@ on CUDA bf16 it runs the fused kernel.  RotaryEmbedding keeps the persistent
 ``inv_freq`` buffer of the checkpoint format and rotate-half RoPE with
 cos/sin of ``cat(freqs, freqs)`` (complexity/core/position/rotary.py:17-72);
 the fused kernels read the half-width fp32 tables returned by ``tables``.
+ResidualJoin is the residual add of blocks whose branches are normalised, gated, scaled or
+dropped out.
 """
 from __future__ import annotations
 
 import math
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -66,6 +68,41 @@ class IdentityNorm(nn.Module):
 
     def forward(self, x):
         return x
+
+
+class ResidualJoin(nn.Module):
+    """``x + scale * dropout(gate * rmsnorm(branch))`` and, of the sum, the next block's norm.
+
+    ``norm``: the branch is normalised, with a learned weight; ``gate_init``: a learned gate of
+    each channel starts there; ``p``: dropout in training, from a seed drawn for each call from
+    PyTorch's generator.  One ``ops.residual.residual_norm`` on any device.
+    """
+
+    def __init__(self, hidden_size: int, *, norm: bool = True, gate_init: Optional[float] = None,
+                 scale: float = 1.0, p: float = 0.0, eps: float = 1e-6):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(hidden_size)) if norm else None
+        self.gate = (None if gate_init is None
+                     else nn.Parameter(torch.full((hidden_size,), float(gate_init))))
+        self.scale, self.p, self.eps = scale, p, eps
+
+    def forward(self, x: torch.Tensor, branch: torch.Tensor, next_norm: Optional[nn.Module] = None):
+        """``(x', next_norm(x'))``; the second is None without ``next_norm``."""
+        from ..ops.residual import new_seed, residual_norm
+
+        fused = (isinstance(next_norm, RMSNorm) and next_norm.eps == self.eps
+                 and next_norm.weight.dtype == x.dtype)
+        p = self.p if self.training else 0.0
+        new, y = residual_norm(x, branch.to(x.dtype), branch_weight=self.weight, gate=self.gate,
+                               norm_weight=next_norm.weight if fused else None, scale=self.scale,
+                               p=p, seed=new_seed(x.device) if p > 0 else None, eps=self.eps)
+        if next_norm is not None and not fused:
+            y = next_norm(new)
+        return new, y
+
+    def extra_repr(self) -> str:
+        return (f"norm={self.weight is not None}, gate={self.gate is not None}, "
+                f"scale={self.scale}, p={self.p}")
 
 
 def rotate_half(x: torch.Tensor) -> torch.Tensor:

@@ -16,6 +16,8 @@ from typing import Any, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..core.losses import model_token_logprobs
+
 
 @dataclass
 class BenchmarkResult:
@@ -37,14 +39,12 @@ def choice_logprobs(model, tokenizer, context: str, choices: Sequence[str],
     ids = torch.full((len(seqs), L), pad, dtype=torch.long)
     for i, s in enumerate(seqs):
         ids[i, :len(s)] = torch.tensor(s)
-    logp = torch.log_softmax(model(ids.to(dev))["logits"].float(), -1).cpu()
-    out = []
+    targets = torch.full((len(seqs), L), -100, dtype=torch.long)
     for i, s in enumerate(seqs):
-        n = len(s) - len(ctx)
-        tgt = torch.tensor(s[len(ctx):])
-        lp = logp[i, len(ctx) - 1:len(s) - 1].gather(-1, tgt[:, None]).sum()
-        out.append(float(lp) / (n if normalize and n else 1))
-    return out
+        targets[i, len(ctx) - 1:len(s) - 1] = torch.tensor(s[len(ctx):], dtype=torch.long)
+    sums = model_token_logprobs(model, ids.to(dev), targets.to(dev)).sum(-1).tolist()
+    return [v / (len(s) - len(ctx) if normalize and len(s) > len(ctx) else 1)
+            for v, s in zip(sums, seqs)]
 
 
 class Benchmark:

@@ -4,6 +4,10 @@ Module names (``input_layernorm``, ``self_attn``, ``post_attention_layernorm``,
 ``mlp``) and the per-layer interpolation of the shared/routed output scales
 follow complexity/models/block.py:20-280.  On the fused path both residual
 adds happen inside GEMM epilogues (o_proj and MLP down projection).
+
+With ``norm_placement="sandwich"``, a residual gate, scale or dropout, a branch joins the stream
+through ``attn_join`` / ``mlp_join`` instead: ``x += scale * dropout(gate * norm(branch))``, one
+kernel with the norm that follows (``core.layers.ResidualJoin``).
 """
 from __future__ import annotations
 
@@ -14,6 +18,7 @@ import torch.nn as nn
 
 from ..config.model_config import ModelConfig
 from ..core.attention import AttentionConfig
+from ..core.layers import ResidualJoin
 from ..core.mlp import MLPConfig
 from ..core.registry import ATTENTION_REGISTRY, MLP_REGISTRY, NORMALIZATION_REGISTRY
 
@@ -86,6 +91,13 @@ class TransformerBlock(nn.Module):
             micro_expert_gate_init=config.micro_expert_gate_init)
         from ..core import dense_mlp, lexical_mlp  # noqa: F401  (registers MLP types)
         self.mlp = MLP_REGISTRY.build(config.mlp_type, mlp_cfg)
+        self.joined = config.joined_residual
+        if self.joined:
+            join = dict(norm=config.norm_placement == "sandwich",
+                        gate_init=config.residual_gate_init, scale=config.residual_scale,
+                        p=config.residual_dropout, eps=config.norm_eps)
+            self.attn_join = ResidualJoin(config.hidden_size, **join)
+            self.mlp_join = ResidualJoin(config.hidden_size, **join)
 
     def forward(self, hidden_states: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                 past_key_value: Optional[Any] = None, use_cache: bool = False,
@@ -101,6 +113,11 @@ class TransformerBlock(nn.Module):
         h, hidden_states = self._norm_skip(self.input_layernorm, hidden_states)
         if token_ids is not None and hasattr(self.self_attn, "set_token_ids"):
             self.self_attn.set_token_ids(token_ids)
+        if self.joined:
+            a, new_kv = self.self_attn(h, attention_mask=attention_mask,
+                                       past_key_value=past_key_value, use_cache=use_cache)
+            x, h = self.attn_join(hidden_states, a, self.post_attention_layernorm)
+            return self.mlp_join(x, self.mlp(h, token_ids=token_ids))[0], new_kv, None
         x, new_kv = self.self_attn(h, attention_mask=attention_mask,
                                    past_key_value=past_key_value, use_cache=use_cache,
                                    residual=hidden_states)
@@ -110,6 +127,9 @@ class TransformerBlock(nn.Module):
 
     def forward_sp(self, x_shard: torch.Tensor, token_ids: torch.Tensor, B: int, S: int, ws):
         """Fused sequence-parallel block on a [T/P, H] token shard."""
+        if self.joined:
+            raise NotImplementedError("the fused sequence-parallel block adds its branches in GEMM "
+                                      "epilogues: no sandwich norms, residual gate, scale or dropout")
         name = f"layer{self.layer_idx}"
         h, x = self._norm_skip(self.input_layernorm, x_shard)
         x = self.self_attn.forward_sp(h, x, B, S, ws, name + ".attn")
@@ -128,6 +148,13 @@ class TransformerBlock(nn.Module):
         h = self.input_layernorm(hidden_states)
         if hasattr(self.self_attn, "set_token_ids"):
             self.self_attn.set_token_ids(token_ids)
+        if self.joined:
+            if getattr(self.self_attn, "tp_group", None) is not None:
+                raise NotImplementedError("tensor-parallel decoding adds its branches while it "
+                                          "reduces them: no sandwich norms, residual gate or scale")
+            a = self.self_attn.forward_paged(h, cache, self.layer_idx)
+            x, h = self.attn_join(hidden_states, a, self.post_attention_layernorm)
+            return self.mlp_join(x, self.mlp(h, token_ids=token_ids))[0]
         x = self.self_attn.forward_paged(h, cache, self.layer_idx, residual=hidden_states)
         h = self.post_attention_layernorm(x)
         return self.mlp(h, token_ids=token_ids, residual=x)

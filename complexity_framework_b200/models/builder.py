@@ -199,6 +199,10 @@ class ComplexityModel(nn.Module):
             if past_key_values is not None and past_key_values[0] is not None:
                 past_len = past_key_values[0][0].shape[2]
             hidden = self.embed_positions(hidden, offset=past_len)
+        if self.training and self.config.embedding_dropout > 0:
+            from ..ops.residual import dropout, new_seed
+
+            hidden = dropout(hidden, self.config.embedding_dropout, new_seed(hidden.device))
         token_ids = routing_ids if routing_ids is not None else input_ids
         if token_ids is None:
             token_ids = torch.zeros(B, S, dtype=torch.long, device=hidden.device)
@@ -239,8 +243,16 @@ class ComplexityModel(nn.Module):
                 logits = logits / mult
         return logits
 
+    @property
+    def logit_scale(self) -> float:
+        """Factor of the logits (muP's output multiplier)."""
+        if not self.config.use_mup_output_mult:
+            return 1.0
+        return 1.0 / max(1.0, self.config.hidden_size / self.config.mup_base_width)
+
     def loss(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
-             ignore_index: int = -100) -> torch.Tensor:
+             ignore_index: int = -100, label_smoothing: float = 0.0,
+             z_loss_coef: float = 0.0) -> torch.Tensor:
         """Mean next-token cross-entropy; the LM head is fused with the loss on CUDA.
 
         ``labels`` default to ``input_ids`` shifted left by one with the last
@@ -250,19 +262,19 @@ class ComplexityModel(nn.Module):
         from ..core.losses import causal_lm_loss_from_hidden
 
         if getattr(self, "sp_ws", None) is not None and input_ids.is_cuda:
-            return self._loss_sp(input_ids, labels, ignore_index)
+            return self._loss_sp(input_ids, labels, ignore_index, label_smoothing, z_loss_coef)
         hidden = self(input_ids, return_logits=False)["last_hidden_state"]
         if labels is None:
             labels = torch.roll(input_ids, -1, dims=1)
             labels[:, -1] = ignore_index
-        scale = 1.0
-        if self.config.use_mup_output_mult:
-            scale = 1.0 / max(1.0, self.config.hidden_size / self.config.mup_base_width)
         return causal_lm_loss_from_hidden(hidden, self.output_weight(), labels,
-                                          ignore_index=ignore_index, logit_scale=scale)
+                                          ignore_index=ignore_index, logit_scale=self.logit_scale,
+                                          label_smoothing=label_smoothing,
+                                          z_loss_coef=z_loss_coef)
 
     def _loss_sp(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor],
-                 ignore_index: int) -> torch.Tensor:
+                 ignore_index: int, label_smoothing: float = 0.0,
+                 z_loss_coef: float = 0.0) -> torch.Tensor:
         """Fused sequence-parallel TP loss: this rank embeds, normalises and scores
         its T/P token rows; attention / MLP communicate inside their GEMMs.
         Returns this rank's share of the global mean loss (shares sum to the
@@ -289,7 +301,9 @@ class ComplexityModel(nn.Module):
         n_local = (lab != ignore_index).sum()
         n_total = (labels != ignore_index).sum().clamp_min(1)
         loss = causal_lm_loss_from_hidden(x.view(1, rows, -1), self.output_weight(),
-                                          lab.view(1, rows), ignore_index=ignore_index)
+                                          lab.view(1, rows), ignore_index=ignore_index,
+                                          label_smoothing=label_smoothing,
+                                          z_loss_coef=z_loss_coef)
         return loss * (n_local / n_total)
 
     # ------------------------------------------------------------ generation

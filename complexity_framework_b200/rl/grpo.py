@@ -19,6 +19,8 @@ from typing import Callable, Dict, List, Optional, Sequence
 import torch
 import torch.nn.functional as F
 
+from ..core.losses import model_token_logprobs
+
 
 @dataclass
 class GRPOConfig:
@@ -52,18 +54,19 @@ def sequence_log_probs(model, prompt_ids: Sequence[Sequence[int]],
     ids = torch.full((len(seqs), L), pad_id, dtype=torch.long)
     for i, s in enumerate(seqs):
         ids[i, :len(s)] = torch.tensor(s)
-    ids = ids.to(dev)
-    logits = model(ids)["logits"].float()
-    lp = torch.log_softmax(logits, -1)
+    targets = torch.full((len(seqs), L), -100, dtype=torch.long)
+    for i, (p, c) in enumerate(zip(prompt_ids, completion_ids)):
+        c = list(c)[not p:]  # the first token of a sequence follows nothing
+        start = max(len(p) - 1, 0)
+        targets[i, start:start + len(c)] = torch.tensor(c, dtype=torch.long)
+    lp = model_token_logprobs(model, ids.to(dev), targets.to(dev))
     out = torch.zeros(len(seqs), Lc, device=dev)
     mask = torch.zeros(len(seqs), Lc, device=dev)
     for i, (p, c) in enumerate(zip(prompt_ids, completion_ids)):
-        if not c:
-            continue
-        pos = torch.arange(len(p) - 1, len(p) - 1 + len(c), device=dev)
-        tgt = torch.tensor(list(c), device=dev)
-        out[i, :len(c)] = lp[i, pos, tgt]
-        mask[i, :len(c)] = 1.0
+        first, start = int(not p), max(len(p) - 1, 0)
+        n = max(len(c) - first, 0)
+        out[i, first:first + n] = lp[i, start:start + n]
+        mask[i, first:first + n] = 1.0
     return out, mask
 
 

@@ -26,6 +26,9 @@ class TrainingConfig:
     wsd_decay_ratio: float = 0.2
     precision: str = "bf16"
     grad_clip: float = 1.0
+    # of the training loss only; evaluation reports the plain cross-entropy
+    label_smoothing: float = 0.0
+    z_loss_coef: float = 0.0
     skip_param_update_check: bool = False
     # capture forward + backward + optimizer of a step in one CUDA graph after
     # `cuda_graph_warmup` eager steps (single GPU, fused AdamW); replays skip
@@ -59,6 +62,8 @@ class TrainingConfig:
             (0.0 <= self.wsd_decay_ratio <= 1.0, "wsd_decay_ratio must be in [0, 1]"),
             (self.precision in ("fp32", "fp16", "bf16"), "precision must be one of: fp32, fp16, bf16"),
             (self.grad_clip >= 0, "grad_clip must be non-negative"),
+            (0.0 <= self.label_smoothing <= 1.0, "label_smoothing must be in [0, 1]"),
+            (self.z_loss_coef >= 0, "z_loss_coef must be non-negative"),
             (self.save_steps > 0, "save_steps must be positive"),
             (self.log_steps > 0, "log_steps must be positive"),
             (self.eval_steps >= 0, "eval_steps must be non-negative"),

@@ -100,6 +100,9 @@ class TrainRunner:
                                 "sophia", "adam8bit", "came", "adalomo", "musgd"])
         p.add_argument("--weight-decay", type=float, default=0.1)
         p.add_argument("--grad-clip", type=float, default=1.0)
+        p.add_argument("--label-smoothing", type=float, default=0.0)
+        p.add_argument("--z-loss", type=float, default=0.0,
+                       help="weight of the mean squared log-sum-exp of the logits")
         p.add_argument("--top-k", type=int, default=None)
         p.add_argument("--use-custom-kernels", default="auto", choices=["auto", "true", "false"])
         p.add_argument("--seed", type=int, default=42)
@@ -211,6 +214,7 @@ class TrainRunner:
                               learning_rate=args.lr, weight_decay=args.weight_decay,
                               warmup_steps=warmup, lr_scheduler=args.lr_scheduler,
                               precision=args.precision, grad_clip=args.grad_clip,
+                              label_smoothing=args.label_smoothing, z_loss_coef=args.z_loss,
                               checkpoint_dir=args.checkpoint_dir, save_steps=save_steps,
                               log_steps=args.log_steps, eval_steps=args.eval_steps,
                               num_workers=args.num_workers,

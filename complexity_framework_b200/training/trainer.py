@@ -152,6 +152,10 @@ class Trainer:
     def compute_loss(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None):
         if self._compute_loss is not None:
             return self._compute_loss(self.model, input_ids, labels)
+        c = self.config
+        if self.model.training and (c.label_smoothing > 0 or c.z_loss_coef > 0):
+            return self.model.loss(input_ids, labels, label_smoothing=c.label_smoothing,
+                                   z_loss_coef=c.z_loss_coef)
         return self.model.loss(input_ids, labels)
 
     def train_step(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None, *,
