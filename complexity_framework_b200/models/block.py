@@ -114,6 +114,10 @@ class TransformerBlock(nn.Module):
         if token_ids is not None and hasattr(self.self_attn, "set_token_ids"):
             self.self_attn.set_token_ids(token_ids)
         if self.joined:
+            if (self.training and self.attn_join.p > 0
+                    and getattr(self.self_attn, "tp_group", None) is not None):
+                raise NotImplementedError("residual_dropout under tensor parallelism: the ranks "
+                                          "of a group would draw different masks")
             a, new_kv = self.self_attn(h, attention_mask=attention_mask,
                                        past_key_value=past_key_value, use_cache=use_cache)
             x, h = self.attn_join(hidden_states, a, self.post_attention_layernorm)

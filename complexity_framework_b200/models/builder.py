@@ -290,6 +290,8 @@ class ComplexityModel(nn.Module):
         if labels is None:
             labels = torch.roll(input_ids, -1, dims=1)
             labels[:, -1] = ignore_index
+        if self.training and self.config.embedding_dropout > 0:
+            raise NotImplementedError("embedding_dropout under the fused sequence-parallel loss")
         if self.training and torch.is_grad_enabled():
             ws.begin_step()
         flat = input_ids.reshape(-1)

@@ -300,9 +300,11 @@ def save_to_huggingface(model, save_path: str, model_type: str = "llama", config
     are left out)."""
     from safetensors.torch import save_file
 
+    cfg = config or model.config
+    if cfg.joined_residual:
+        raise ValueError("the Llama layout has no norms, gates or factors of the branches")
     out = Path(save_path)
     out.mkdir(parents=True, exist_ok=True)
-    cfg = config or model.config
     sd = {k: v.detach().contiguous().cpu() for k, v in
           convert_to_hf_state_dict(model.state_dict(), model_type).items()
           if not any(k.endswith(s) for s in ROUTE_BUFFER_SUFFIXES + EXPERT_PARAM_SUFFIXES)

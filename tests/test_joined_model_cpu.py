@@ -112,6 +112,16 @@ def test_config_round_trip_and_refusals(tmp_path):
         TrainingConfig(label_smoothing=2.0)
     with pytest.raises(NotImplementedError):
         m.layers[0].forward_sp(None, None, 1, 1, None)
+    from complexity_framework_b200.quantization.gguf import export_gguf
+    from complexity_framework_b200.utils.conversion import save_to_huggingface
+
+    for export in (export_gguf, save_to_huggingface):
+        with pytest.raises(ValueError, match="branches"):
+            export(m, str(tmp_path / "x"))
+    m.train()
+    m.layers[0].self_attn.tp_group = object()
+    with pytest.raises(NotImplementedError, match="tensor parallelism"):
+        m.layers[0](torch.zeros(1, 2, 64), token_ids=torch.zeros(1, 2, dtype=torch.long))
 
 
 def test_join_with_another_norm():
