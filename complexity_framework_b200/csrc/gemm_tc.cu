@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(384, 1)
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
-  const int M = ep.m_dev != nullptr ? min(M_max, __ldg(ep.m_dev)) : M_max;
+  const int M = ep.m_dev != nullptr ? max(0, min(M_max, __ldg(ep.m_dev) - ep.m_off)) : M_max;
   const int K = ep.k_dev != nullptr ? min(K_max, __ldg(ep.k_dev)) : K_max;
   const int num_m = (M + Cfg::TILE_M - 1) / Cfg::TILE_M;
   // with the fused all-gather, this rank's own row tiles come first

@@ -129,6 +129,7 @@ struct GemmEpi {
   GemmCe ce;
   // sizes that the host does not know: fewer rows of C (m_dev) or of K (k_dev) than M or K
   const int* m_dev = nullptr;
+  int m_off = 0;             // rows of m_dev before this launch's first
   const int* k_dev = nullptr;
   int64_t split_stride = 0;  // EPI_F32 / EPI_F32_ACC: K slices write their own C, this far apart
   const float* alpha_dev = nullptr;  // EPI_STORE, EPI_F32, EPI_F32_ACC: a further factor of acc

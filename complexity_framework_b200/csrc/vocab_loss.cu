@@ -141,11 +141,13 @@ __global__ void __launch_bounds__(256) vl_gather_k(const VlCall c, const VlForwa
 __global__ void __launch_bounds__(256) vl_rows_k(const VlCall c, const VlForward f,
                                                  const float2* __restrict__ stats,
                                                  const float* __restrict__ zt,
-                                                 const float* __restrict__ zsum, int halves) {
+                                                 const float* __restrict__ zsum, int halves,
+                                                 int64_t first, int64_t n) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= c.cnt[1]) return;
-  const float2* st = stats + row * halves;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t row = first + at;
+  if (at >= n || row >= c.cnt[1]) return;
+  const float2* st = stats + at * halves;
   float mx = -INFINITY;
   for (int i = lane; i < halves; i += 32) mx = fmaxf(mx, st[i].x);
   mx = warp_max(mx);
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(256) vl_rows_k(const VlCall c, const VlForward
   for (int i = lane; i < halves; i += 32) {
     const float2 v = st[i];
     se += v.y * exp2_approx(v.x - mx);
-    if (zsum != nullptr) zs += zsum[row * halves + i];
+    if (zsum != nullptr) zs += zsum[at * halves + i];
   }
   se = warp_sum(se);
   if (zsum != nullptr) zs = warp_sum(zs);
@@ -163,8 +165,8 @@ __global__ void __launch_bounds__(256) vl_rows_k(const VlCall c, const VlForward
   const int src = c.src[row];
   if (src < 0) return;
   const float lse = lse2 * kLn2;
-  float loss = lse - zt[row];
-  if (c.smooth > 0.f) loss += c.smooth * (zt[row] - zs / static_cast<float>(c.V));
+  float loss = lse - zt[at];
+  if (c.smooth > 0.f) loss += c.smooth * (zt[at] - zs / static_cast<float>(c.V));
   f.rows[src] = c.sign * (loss + c.z * lse * lse);
 }
 
@@ -245,42 +247,54 @@ GemmEpi epi_of(const VlCall& c) {
 
 }  // namespace
 
+// Rows whose statistics are held at a time: about 256 MB of them, whole row tiles.
+static int64_t rows_each(const VlCall& c) {
+  const int64_t R = vl_rows(c.T), row = static_cast<int64_t>(halves_of(c)) * 12;
+  const int64_t n = std::max<int64_t>(1, (256 << 20) / row / 256) * 256;
+  return std::min(R, n);
+}
+
 int64_t vl_forward_floats(const VlCall& c) {
-  const int64_t R = vl_rows(c.T), h = halves_of(c);
-  return R * h * (c.smooth > 0.f ? 3 : 2) + R;
+  return rows_each(c) * (static_cast<int64_t>(halves_of(c)) * (c.smooth > 0.f ? 3 : 2) + 1);
 }
 
 int vl_forward(const VlCall& c, const VlForward& f, cudaStream_t s) {
-  const int64_t R = vl_rows(c.T);
+  const int64_t R = vl_rows(c.T), each = rows_each(c);
   const int halves = halves_of(c);
   // rows a block: enough blocks to copy with every SM, few enough that the counting stays small
   int per = static_cast<int>((c.T + 2 * c.num_sms - 1) / (2 * c.num_sms));
   per = per < 8 ? 8 : per > 256 ? 256 : per;
   vl_gather_k<<<static_cast<unsigned>((c.T + per - 1) / per), 256, 0, s>>>(c, f, per);
   float2* stats = reinterpret_cast<float2*>(f.ws);
-  float* zsum = c.smooth > 0.f ? f.ws + 2 * R * halves : nullptr;
-  float* zt = f.ws + R * halves * (c.smooth > 0.f ? 3 : 2);
-  GemmArgs g;
-  g.A = c.hc;
-  g.lda = c.H;
-  g.B = c.w;
-  g.ldb = c.H;
-  g.M = static_cast<int>(R);
-  g.N = pad32(c.V);
-  g.n_valid = c.V;
-  g.K = c.H;
-  g.epi = EPI_CE_FWD;
-  g.bn = 256;
-  g.num_sms = c.num_sms;
-  GemmEpi ep = epi_of(c);
-  ep.ce.stats = stats;
-  ep.ce.zt = zt;
-  ep.ce.zsum = zsum;
-  ep.ce.n_valid = c.V;
-  ep.group_m = 8;
-  const int rc = gemm_tc_launch(g, ep, s, c.err);
-  if (rc) return rc;
-  vl_rows_k<<<static_cast<unsigned>((R + 7) / 8), 256, 0, s>>>(c, f, stats, zt, zsum, halves);
+  float* zsum = c.smooth > 0.f ? f.ws + 2 * each * halves : nullptr;
+  float* zt = f.ws + each * halves * (c.smooth > 0.f ? 3 : 2);
+  for (int64_t r0 = 0; r0 < R; r0 += each) {
+    const int64_t n = std::min(each, R - r0);
+    GemmArgs g;
+    g.A = c.hc + r0 * c.H;
+    g.lda = c.H;
+    g.B = c.w;
+    g.ldb = c.H;
+    g.M = static_cast<int>(n);
+    g.N = pad32(c.V);
+    g.n_valid = c.V;
+    g.K = c.H;
+    g.epi = EPI_CE_FWD;
+    g.bn = 256;
+    g.num_sms = c.num_sms;
+    GemmEpi ep = epi_of(c);
+    ep.m_off = static_cast<int>(r0);
+    ep.ce.target = c.target + r0;
+    ep.ce.stats = stats;
+    ep.ce.zt = zt;
+    ep.ce.zsum = zsum;
+    ep.ce.n_valid = c.V;
+    ep.group_m = 8;
+    const int rc = gemm_tc_launch(g, ep, s, c.err);
+    if (rc) return rc;
+    vl_rows_k<<<static_cast<unsigned>((n + 7) / 8), 256, 0, s>>>(c, f, stats, zt, zsum, halves, r0,
+                                                                 n);
+  }
   if (f.total != nullptr) vl_total_k<<<1, 1024, 0, s>>>(c, f);
   return static_cast<int>(cudaGetLastError());
 }

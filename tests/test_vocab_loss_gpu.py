@@ -52,6 +52,21 @@ def oracle(h, w, y, up, smooth=0.0, z=0.0, scale=1.0):
     return loss, loss_tol, dh, dh_tol, dw, dw_tol
 
 
+def oracle_loss(h, w, y):
+    """Losses and their bounds alone (see ``oracle``), a few rows at a time."""
+    out = []
+    for a in range(0, h.shape[0], 32):
+        hh, yy = h[a:a + 32].double(), y[a:a + 32]
+        zl = hh @ w.double().t()
+        lse = torch.logsumexp(zl, -1)
+        loss = torch.where(yy != -100, lse - zl.gather(1, yy.clamp_min(0)[:, None])[:, 0], 0.0)
+        ez = (h.shape[1] / 16 + 2) * 2.0 ** -23 * (hh.abs() @ w.double().abs().t()).amax(-1) \
+            + 2.0 ** -20 + 2.0 ** -22 * zl.abs().amax(-1)
+        # sums of exponentials over the words: 32 in a row, then 4, 4 chunks, 7000 / 32 halves
+        out.append((loss, 2 * ez + 2.0 ** -22 * loss.abs() + 260 * 2.0 ** -24))
+    return [torch.cat(t) for t in zip(*out)]
+
+
 def close(got, want, tol, name):
     err = (got.double() - want).abs()
     assert bool((err <= tol + 1e-38).all()), (name, float((err / (tol + 1e-38)).max()))
@@ -113,6 +128,17 @@ def test_pieces_of_the_vocabulary(T, ws):
 def test_wide():
     check(40, 50021, 256)
     check(900, 3001, 4096, ignored=0.2)
+
+
+def test_rows_in_parts():
+    """More statistics than are held at a time (256 MB): 7000 half tiles of 128 words."""
+    T, V, H = 4300, 896000, 8
+    h, w, y = make(T, V, H, ignored=0.2)
+    rows = vocab_cross_entropy(h, w, y, reduction="none")
+    pick = torch.cat((torch.arange(0, T, 37), torch.arange(T - 70, T))).cuda()
+    loss, tol, *_ = oracle_loss(h[pick], w, y[pick])
+    close(rows[pick], loss, tol, "rows")
+    check_errors()
 
 
 def test_large_logits():
