@@ -313,18 +313,6 @@ __global__ void __launch_bounds__(384, 1)
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
-  const int M = ep.m_dev != nullptr ? max(0, min(M_max, __ldg(ep.m_dev) - ep.m_off)) : M_max;
-  const int K = ep.k_dev != nullptr ? min(K_max, __ldg(ep.k_dev)) : K_max;
-  const int num_m = (M + Cfg::TILE_M - 1) / Cfg::TILE_M;
-  // with the fused all-gather, this rank's own row tiles come first
-  const int m_shift = ep.ag.active ? (ep.sync.rank * ep.ag.rows) / Cfg::TILE_M : 0;
-  const int num_n = (N + BN - 1) / BN;
-  const int num_tiles = num_m * num_n;
-  const int nk = (K + kBK - 1) / kBK;
-  // work unit u = (tile u / ksplit, K slice u % ksplit); ksplit > 1 only with the
-  // fp32 atomic epilogue, which sums the partial products of the slices
-  const int total = num_tiles * ksplit * (ep.grp.mode == 2 ? ep.grp.ngroups : 1);
-
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -363,6 +351,20 @@ __global__ void __launch_bounds__(384, 1)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // launched before the end of the kernel before: its results are read from here on
+  if (ep.dependent) grid_dependency_wait();
+
+  const int M = ep.m_dev != nullptr ? max(0, min(M_max, *static_cast<const volatile int*>(ep.m_dev) - ep.m_off)) : M_max;
+  const int K = ep.k_dev != nullptr ? min(K_max, *static_cast<const volatile int*>(ep.k_dev)) : K_max;
+  const int num_m = (M + Cfg::TILE_M - 1) / Cfg::TILE_M;
+  // with the fused all-gather, this rank's own row tiles come first
+  const int m_shift = ep.ag.active ? (ep.sync.rank * ep.ag.rows) / Cfg::TILE_M : 0;
+  const int num_n = (N + BN - 1) / BN;
+  const int num_tiles = num_m * num_n;
+  const int nk = (K + kBK - 1) / kBK;
+  // work unit u = (tile u / ksplit, K slice u % ksplit); ksplit > 1 only with the
+  // fp32 atomic epilogue, which sums the partial products of the slices
+  const int total = num_tiles * ksplit * (ep.grp.mode == 2 ? ep.grp.ngroups : 1);
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -1023,7 +1025,7 @@ static int launch_impl(const SegMaps<NA>& ta, const SegMaps<NB>& tb, const CUten
   auto kern = gemm_tc_kernel<BN, A_MN, B_MN, EPI, PAIR, NA, NB>;
   static int max_units = -1;  // resident CTAs (or CTA pairs), one query per instantiation
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.blockDim = dim3(384, 1, 1);
   cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
   cfg.stream = stream;
@@ -1069,6 +1071,11 @@ static int launch_impl(const SegMaps<NA>& ta, const SegMaps<NB>& tb, const CUten
   const int work = tiles * ksplit;
   const int units = work < max_units ? work : max_units;
   cfg.gridDim = dim3(PAIR ? 2 * units : units, 1, 1);
+  if (ep.dependent) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, tc[0], tc[1], M, N, K, ksplit, ep, err);
   return static_cast<int>(e);
 }

@@ -133,6 +133,7 @@ struct GemmEpi {
   const int* k_dev = nullptr;
   int64_t split_stride = 0;  // EPI_F32 / EPI_F32_ACC: K slices write their own C, this far apart
   const float* alpha_dev = nullptr;  // EPI_STORE, EPI_F32, EPI_F32_ACC: a further factor of acc
+  int dependent = 0;         // launch before the end of the kernel before, and wait for it inside
   int group_m = 0;           // > 0: the schedule takes the row tiles in groups of this many, every
                              // column tile of a group before the next group
 };

@@ -668,6 +668,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
   }
   in.drain();
   if (a.partials == nullptr) return;
+  grid_dependents_go();
   // the groups of the CTA one after the other, through this CTA's part of the workspace
   float* p = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * a.H;
   for (int q = 0; q < groups; ++q) {
@@ -694,6 +695,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
 template <typename T>
 __global__ void __launch_bounds__(1024) join_cols_k(const JoinArgs a, int blocks, float f) {
   __shared__ float t1[32][33], t2[32][33];
+  grid_dependency_wait();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + tx;
   float s1 = 0.f, s2 = 0.f;
@@ -907,9 +909,10 @@ int join_bwd(const JoinArgs& a, int num_sms, cudaStream_t s) {
   return with_kernel<true>(a, num_sms, [&](auto t, auto kern, const JoinLaunch& l) {
     using T = decltype(t);
     kern<<<l.grid, l.threads, l.smem, s>>>(a, a.drop.factor(), l.stages);
-    if (a.partials != nullptr)
-      join_cols_k<T><<<(a.H + 31) / 32, 1024, 0, s>>>(a, l.grid, a.scale * a.drop.factor());
-    return static_cast<int>(cudaGetLastError());
+    const int rc = static_cast<int>(cudaGetLastError());
+    if (rc != 0 || a.partials == nullptr) return rc;
+    return launch_dependent(join_cols_k<T>, dim3((a.H + 31) / 32), 1024, s, a, l.grid,
+                            a.scale * a.drop.factor());
   });
 }
 

@@ -49,6 +49,7 @@ __device__ __forceinline__ float warp_max(float v) {
 __global__ void __launch_bounds__(256) vl_gather_k(const VlCall c, const VlForward f, int per) {
   __shared__ int warp_n[8];
   __shared__ int dest[256];
+  grid_dependents_go();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * per;
   const auto counts = [&](int64_t y) { return y != c.ignore && y >= 0 && y < c.V; };
@@ -139,10 +140,10 @@ __global__ void __launch_bounds__(256) vl_gather_k(const VlCall c, const VlForwa
 
 // Joins the half tiles' statistics of rows [first, first + n), a warp a row.
 __global__ void __launch_bounds__(256) vl_rows_k(const VlCall c, const VlForward f,
-                                                 const float2* __restrict__ stats,
-                                                 const float* __restrict__ zt,
-                                                 const float* __restrict__ zsum, int halves,
-                                                 int64_t first, int64_t n) {
+                                                 const float2* stats, const float* zt,
+                                                 const float* zsum, int halves, int64_t first,
+                                                 int64_t n) {
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int64_t row = first + at;
@@ -172,6 +173,7 @@ __global__ void __launch_bounds__(256) vl_rows_k(const VlCall c, const VlForward
 
 __global__ void __launch_bounds__(1024) vl_total_k(const VlCall c, const VlForward f) {
   __shared__ float part[32];
+  grid_dependency_wait();
   float s = 0.f;
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < c.T; i += 1024) s += f.rows[i];
@@ -187,11 +189,10 @@ __global__ void __launch_bounds__(1024) vl_total_k(const VlCall c, const VlForwa
 // dh in the call's order: the K slices' sum of a counted row, 0 of the others.  The target's
 // gradient, about -1 beside words' of some 1 / V, is most of a row's: what rounding it to bf16
 // took (resid) is added back as resid w_target, so that its error is not dh's.
-__global__ void __launch_bounds__(256) vl_scatter_k(const VlCall c, const float* __restrict__ acc,
-                                                    int ldc, int64_t slice, int slices,
-                                                    const float* __restrict__ resid,
-                                                    const float* __restrict__ alpha,
-                                                    __nv_bfloat16* __restrict__ dh) {
+__global__ void __launch_bounds__(256) vl_scatter_k(const VlCall c, const float* acc, int ldc,
+                                                    int64_t slice, int slices, const float* resid,
+                                                    const float* alpha, __nv_bfloat16* dh) {
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, nv = c.H >> 3;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < c.T;
        row += static_cast<int64_t>(gridDim.x) * 8) {
@@ -228,6 +229,7 @@ __global__ void __launch_bounds__(256) vl_scatter_k(const VlCall c, const float*
 // where the rows share it.
 __global__ void vl_alpha_k(const VlCall c, const float* gout, bool per_row, float unit,
                            float* alpha) {
+  grid_dependents_go();
   *alpha = c.scale * c.sign * unit * (per_row ? 1.f : *gout * *c.ginv);
 }
 float unit_of(const VlCall& c) { return c.smooth < 1.f ? 1.f - c.smooth : 1.f; }
@@ -242,6 +244,7 @@ GemmEpi epi_of(const VlCall& c) {
   ep.ce.target = c.target;
   ep.ce.n_valid = 0;
   ep.m_dev = c.cnt + 1;
+  ep.dependent = 1;
   return ep;
 }
 
@@ -290,12 +293,16 @@ int vl_forward(const VlCall& c, const VlForward& f, cudaStream_t s) {
     ep.ce.zsum = zsum;
     ep.ce.n_valid = c.V;
     ep.group_m = 8;
-    const int rc = gemm_tc_launch(g, ep, s, c.err);
+    int rc = gemm_tc_launch(g, ep, s, c.err);
     if (rc) return rc;
-    vl_rows_k<<<static_cast<unsigned>((n + 7) / 8), 256, 0, s>>>(c, f, stats, zt, zsum, halves, r0,
-                                                                 n);
+    rc = launch_dependent(vl_rows_k, dim3(static_cast<unsigned>((n + 7) / 8)), 256, s, c, f, stats,
+                          zt, zsum, halves, r0, n);
+    if (rc) return rc;
   }
-  if (f.total != nullptr) vl_total_k<<<1, 1024, 0, s>>>(c, f);
+  if (f.total != nullptr) {
+    const int rc = launch_dependent(vl_total_k, dim3(1), 1024, s, c, f);
+    if (rc) return rc;
+  }
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -402,6 +409,7 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
       e.ldc = ldh;
       e.split_stride = R * ldh;
       e.alpha_dev = b.alpha;
+      e.dependent = 1;
       rc = gemm_tc_launch(d, e, s, c.err);
       if (rc) return rc;
     }
@@ -422,6 +430,7 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
       GemmEpi e;
       e.k_dev = c.cnt + 1;
       e.alpha_dev = b.alpha;
+      e.dependent = 1;
       e.c = b.dw + static_cast<int64_t>(v0) * c.H;
       e.ldc = c.H;
       rc = gemm_tc_launch(d, e, s, c.err);
@@ -430,8 +439,10 @@ int vl_backward(const VlCall& c, const VlBackward& b, cudaStream_t s) {
   }
   if (b.dh != nullptr) {
     const int64_t want = (c.T + 7) / 8, most = static_cast<int64_t>(c.num_sms) * 8;
-    vl_scatter_k<<<static_cast<unsigned>(want < most ? want : most), 256, 0, s>>>(
-        c, b.acc, ldh, R * ldh, b.ksplit, b.resid, b.alpha, b.dh);
+    const int rc =
+        launch_dependent(vl_scatter_k, dim3(static_cast<unsigned>(want < most ? want : most)), 256, s,
+                         c, b.acc, ldh, R * ldh, b.ksplit, b.resid, b.alpha, b.dh);
+    if (rc) return rc;
   }
   return static_cast<int>(cudaGetLastError());
 }
