@@ -44,7 +44,7 @@ cfb::VlCall call_of(int64_t T, const Tensor& w, double scale, double smooth, dou
                     "too many rows or words");
   TORCH_CHECK_VALUE(w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(1) <= (1 << 20),
                     "the hidden size must be a multiple of 8, got ", w.size(1));
-  TORCH_CHECK_VALUE(std::isfinite(scale), "logit_scale must be finite");
+  TORCH_CHECK_VALUE(scale > 0.0 && std::isfinite(scale), "logit_scale must be positive and finite");
   TORCH_CHECK_VALUE(smooth >= 0.0 && smooth <= 1.0, "label_smoothing must be between 0 and 1");
   TORCH_CHECK_VALUE(z >= 0.0 && std::isfinite(z), "z_loss must not be negative");
   cfb::VlCall c;

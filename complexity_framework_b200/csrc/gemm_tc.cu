@@ -746,8 +746,9 @@ __global__ void __launch_bounds__(384, 1)
           st[static_cast<int64_t>(row) * num_n * 2 + n_blk * 2 + wg] = make_float2(mx, se);
         }
       } else if constexpr (EPI == EPI_CE_FWD) {
-        // Softmax statistics of the half tile in units of log 2; columns from n_valid on are
-        // padding.  A half tile of -inf alone has the maximum -inf and the sum 0.
+        // Softmax statistics of the half tile; columns from n_valid on are padding.  Exponents come
+        // from differences to the maximum, so their error goes with these and not with the size
+        // of the logits.  A half tile of -inf alone has the maximum -inf and the sum 0.
         const int half = 2 * n_blk + wg;
         const int64_t at = static_cast<int64_t>(row) * 2 * num_n + half;
         const int tgt = row_ok ? ep.ce.target[row] : -1;
@@ -763,33 +764,26 @@ __global__ void __launch_bounds__(384, 1)
           if (ti >= 0 && ti < 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (i == ti) ep.ce.zt[row] = v[i] * ep.ce.scale;
+              if (i == ti) ep.ce.zt[row] = v[i];
           }
           if (ep.ce.zsum != nullptr) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) zs += v[i];  // padding columns are 0
           }
-          float lm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (left >= 32) {
+          if (left < 32) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              v[i] *= ep.ce.k2;
-              lm[i & 3] = fmaxf(lm[i & 3], v[i]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              v[i] = i < left ? v[i] * ep.ce.k2 : -INFINITY;
-              lm[i & 3] = fmaxf(lm[i & 3], v[i]);
-            }
+            for (int i = 0; i < 32; ++i) v[i] = i < left ? v[i] : -INFINITY;
           }
-          const float nm = fmaxf(fmaxf(fmaxf(lm[0], lm[1]), fmaxf(lm[2], lm[3])), mx);
-          const float base = nm == -INFINITY ? 0.0f : nm;
-          float s[4] = {se * exp2_approx(mx - base), 0.0f, 0.0f, 0.0f};
+          float lm[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[i & 3] += exp2_approx(v[i] - base);
+          for (int i = 0; i < 32; ++i) lm[i & 3] = fmaxf(lm[i & 3], v[i]);
+          const float old = mx;
+          mx = fmaxf(fmaxf(lm[0], lm[1]), fmaxf(lm[2], lm[3]));
+          const float base = mx == -INFINITY ? 0.0f : mx;
+          float s[4] = {se * exp2_approx((old - base) * ep.ce.k2), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i & 3] += exp2_approx((v[i] - base) * ep.ce.k2);
           se = (s[0] + s[1]) + (s[2] + s[3]);
-          mx = nm;
         }
         if (row_ok) {
           ep.ce.stats[at] = make_float2(mx, se);

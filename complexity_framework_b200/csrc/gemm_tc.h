@@ -85,8 +85,8 @@ struct GemmCe {
   float k2 = 0.f;     // scale * log2(e)
   float scale = 1.f;  // logit scale
   const int* target = nullptr;  // [M] word of each row, < 0: none
-  // forward: (max t, sum 2^(t - max)) of a half tile, scale * acc of the target, and (where
-  // wanted) the sum of scale * acc over a half tile
+  // forward: (m, sum 2^(k2 (acc - m))) of a half tile with m its largest acc, acc of the
+  // target, and (where wanted) the sum of scale * acc over a half tile; scale > 0
   float2* stats = nullptr;  // [M][2 * ceil(N / 256)]
   float* zt = nullptr;      // [M]
   float* zsum = nullptr;    // [M][2 * ceil(N / 256)]

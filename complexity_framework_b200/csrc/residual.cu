@@ -882,8 +882,10 @@ static int with_kernel(const JoinArgs& a, int num_sms, F f) {
       if (l.stages > 0)
         return a.drop.threshold > 0 ? pick(std::true_type(), std::true_type())
                                     : pick(std::false_type(), std::true_type());
-      return a.drop.threshold > 0 ? pick(std::true_type(), std::false_type())
-                                  : pick(std::false_type(), std::false_type());
+      if constexpr (RT == 512)  // the widest rows alone can be without
+        return a.drop.threshold > 0 ? pick(std::true_type(), std::false_type())
+                                    : pick(std::false_type(), std::false_type());
+      return -2;
     });
   });
 }

@@ -152,22 +152,24 @@ __global__ void __launch_bounds__(256) vl_rows_k(const VlCall c, const VlForward
   float mx = -INFINITY;
   for (int i = lane; i < halves; i += 32) mx = fmaxf(mx, st[i].x);
   mx = warp_max(mx);
+  const float k2 = c.scale * kLog2e;
   float se = 0.f, zs = 0.f;
   for (int i = lane; i < halves; i += 32) {
     const float2 v = st[i];
-    se += v.y * exp2_approx(v.x - mx);
+    se += v.y * exp2_approx((v.x - mx) * k2);
     if (zsum != nullptr) zs += zsum[at * halves + i];
   }
   se = warp_sum(se);
   if (zsum != nullptr) zs = warp_sum(zs);
   if (lane != 0) return;
-  const float lse2 = mx + log2f(se);
+  const float log2_se = log2f(se), lse2 = fmaf(mx, k2, log2_se);
   c.lse2[row] = lse2;
   const int src = c.src[row];
   if (src < 0) return;
+  // lse - z_y from the difference to the maximum: the size of the logits does not enter its error
+  float loss = c.scale * (mx - zt[at]) + log2_se * kLn2;
   const float lse = lse2 * kLn2;
-  float loss = lse - zt[at];
-  if (c.smooth > 0.f) loss += c.smooth * (zt[at] - zs / static_cast<float>(c.V));
+  if (c.smooth > 0.f) loss += c.smooth * (c.scale * zt[at] - zs / static_cast<float>(c.V));
   f.rows[src] = c.sign * (loss + c.z * lse * lse);
 }
 

@@ -66,6 +66,8 @@ def _loss(hidden, weight, targets, ignore_index, label_smoothing, z_loss, logit_
         raise ValueError("label_smoothing must be between 0 and 1")
     if not 0.0 <= z_loss < float("inf"):
         raise ValueError("z_loss must not be negative")
+    if not 0.0 < logit_scale < float("inf"):
+        raise ValueError("logit_scale must be positive and finite")
     if workspace_bytes < 0:
         raise ValueError("workspace_bytes must not be negative")
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:

@@ -82,5 +82,8 @@ def test_refusals():
         vocab_cross_entropy(h, w.t(), y)
     with pytest.raises(ValueError, match="neither a word"):
         vocab_cross_entropy(h, w, torch.full_like(y, 11))
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="logit_scale"):
+            vocab_cross_entropy(h, w, y, logit_scale=scale)
     with pytest.raises(ValueError, match="workspace"):
         vocab_cross_entropy(h, w, y, workspace_bytes=-1)
