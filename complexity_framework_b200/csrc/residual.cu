@@ -11,11 +11,20 @@
 //   t = scale * m * g,   S = sum_rows t bh,                   dgate = w1 S,   dw1 = gate S
 //   db = (t gate w1 - bh mean(t gate w1 bh)) / rms(b)         (t gate without w1)
 //
-// All of it is bound by memory.  The forward reads x, b and writes x', y; the backward reads dx',
-// dy, x', b and writes dx, db; the dropout mask is drawn again from its counter instead of being
-// stored.  A row lies in the registers of RT threads; sums run in fp32; results are rounded once,
-// at their stores.  The columns' sums stay in registers over all rows of a CTA, and one small
-// kernel adds the CTAs' sums in a fixed order, so that equal calls give equal bits.
+// The forward reads x, b and writes x', y; the backward reads dx', dy, x', b and writes dx, db; the
+// dropout mask is drawn again from its counter instead of being stored.  Memory would bound both;
+// what does is the issue of instructions, as every element passes two sums in sequence: the
+// backward takes 400 warp instructions for 32 blocks of eight elements and 120 more for their
+// dropout, of which schedulers with four warps each issue one every other cycle.  So a row's
+// fixed work is spread over as many elements as registers allow, rows come through a ring of bulk
+// copies, and arithmetic is in pairs.  Sums run in fp32; results are rounded once, at their stores.
+// The columns' sums stay in registers over all rows of a CTA, and one small kernel adds the CTAs'
+// sums in a fixed order, so that equal calls give equal bits.
+//
+// us (TB/s), bf16, with norms and gate, on one B200 (a copy runs at 6.55 TB/s):
+//   32768 x 896   forward 41 (5.7), with dropout 51 (4.6); backward 92 (3.8), 113 (3.1)
+//   8191 x 4096   forward 49 (5.5), with dropout 56 (4.8); backward 81 (5.0), 110 (3.7)
+//   dropout alone of 32768 x 896: 21 (5.5)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -724,7 +733,7 @@ __global__ void __launch_bounds__(1024) join_cols_k(const JoinArgs a, int blocks
 }
 
 // y = m * x / kept share: kDropVecs blocks of eight elements a thread, loaded before the generator
-// runs for them.
+// runs for them (one a turn of a persistent grid: 31 us where four take 21, 32768 x 896 bf16).
 constexpr int kDropVecs = 4;
 
 template <typename T>

@@ -13,6 +13,11 @@
 // products of 2 T V H operations where three would do with the logits kept; all run on the
 // tensor cores from fp32 accumulators, and the logits are never rounded to bf16.
 //
+// The products of 8192 x 32000 x 896, ncu at the 1.46 GHz of the power limit: logits 289 us
+// with the tensor pipe active 92 % of the time, dz 328 us (79 %), dh 356 (75 %), dW 335 (79 %).  A
+// whole call with gradients: 32768 x 32000 x 896 in 6.8 ms, 4096 x 100000 x 4096 in 10.2 ms (1.1
+// and 1.3 PFLOP/s of the four products; cuBLAS runs 1.41 back to back).
+//
 // Rows that do not count (ignored targets) are left out before the first product: the others are
 // gathered in their order, and the products take their number from device memory.  A batch with
 // half of its tokens ignored costs half, and what an ignored row holds reaches nothing.
