@@ -53,6 +53,7 @@ template <>
 __device__ __forceinline__ float from_f(float v) { return v; }
 
 constexpr int kMaxStages = 4;
+constexpr int kMaxSmem = 226 * 1024;  // dynamic; the static part takes less than the last KB
 
 // Eight elements, a block of the dropout generator, in 16-byte accesses.
 template <typename T>
@@ -229,8 +230,8 @@ struct Cols {
 // row has to stay in registers from one of its sums to the next.  Without, a row is loaded into
 // registers (rows so wide that two do not fit).  A copy takes the row's whole blocks, which start
 // on 16-byte boundaries also where the row does not (the tensor's last block, where it is not
-// whole, is left out); a row's partial blocks are put right by the threads that read them.  A wait that runs out is reported and the rows that follow are
-// computed from what is there.
+// whole, is left out); a row's partial blocks are put right by the threads that read them.  A wait
+// that runs out is reported and the rows that follow are computed from what is there.
 template <typename T, int NV, int RT, int NT, bool ODD, bool RING>
 struct Feed {
   const T* p[NT];  // null: not read
@@ -873,9 +874,10 @@ static int with_kernel(const JoinArgs& a, int num_sms, F f) {
                Feed<T, NV, RT, tensors, ODD, true>::pitch(a.H) * static_cast<int>(sizeof(T));
       if (hold_of(NV, RT) == kInShared) l.smem += 8 * a.H;
       const auto go = [&](auto kern) {
-        if (l.smem > 40 * 1024) {  // 48 KB with the static part need no consent
+        if (l.smem > 40 * 1024) {  // up to 48 KB with the static part need no consent
+          // one value for every call: another thread's smaller one must not undo this one's
           const cudaError_t e = cudaFuncSetAttribute(
-              kern, cudaFuncAttributeMaxDynamicSharedMemorySize, l.smem);
+              kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
           if (e != cudaSuccess) return static_cast<int>(e);
         }
         l.grid = grid_of(kern, l, a, num_sms);

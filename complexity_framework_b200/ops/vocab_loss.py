@@ -8,7 +8,7 @@ target is the word ``y`` has the loss
 
 The logits exist a tile at a time: the forward pass leaves a row's log-sum-exp, the backward
 pass computes the logits again, for as much of the vocabulary at a time as ``workspace_bytes``
-holds gradients of (bf16).  They are fp32 throughout, where ``ops.fused.linear_cross_entropy``
+holds gradients of (bf16), beside an fp32 accumulator of ``hidden``'s gradient.  They are fp32 throughout, where ``ops.fused.linear_cross_entropy``
 keeps them, rounded to bf16, for the mean loss alone.
 
 Rows whose target is ``ignore_index`` have the loss 0, add nothing to a gradient whatever they

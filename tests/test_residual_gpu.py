@@ -166,6 +166,15 @@ def test_many_rows_are_deterministic():
         assert torch.equal(a[k], b[k]), k
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("H", [264, 903, 1000, 1017, 1024])
+def test_rows_for_every_warp(H, dtype):
+    """Enough rows that one or two warps take a row each."""
+    t = make(2501, H, DT[dtype], True, True, True, seed=H)
+    want, tol = oracle(t, 0.7, 0.1, 3, 0)
+    check(call(t, 0.7, 0.1, 3, 0), want, tol, DT[dtype])
+
+
 @pytest.mark.parametrize("which", ["x", "b", "w1", "gate", "w2"])
 def test_one_gradient_at_a_time(which):
     t = make(65, 136, torch.bfloat16, True, True, True)
@@ -305,6 +314,31 @@ def test_seed_changed_before_backward_is_refused():
     seed.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+def test_two_threads():
+    """Calls of one kernel with small and large rows from two threads at once."""
+    import threading
+
+    small = make(40, 1032, torch.bfloat16, True, True, True)
+    large = make(40, 2048, torch.bfloat16, True, True, True)
+    want = [call(t, 0.5, 0.1, 1, 0) for t in (small, large)]
+    bad = []
+
+    def go(t, w):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                got = call(t, 0.5, 0.1, 1, 0)
+                torch.cuda.current_stream().synchronize()
+                bad.extend(k for k in w if not torch.equal(got[k], w[k]))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=go, args=a) for a in zip((small, large), want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_another_stream():
