@@ -25,6 +25,9 @@ SOURCES = [
     "paged8_chunk.cu",
     "bind_stream.cpp",
     "residual.cu",
+    "residual_bf16.cu",
+    "residual_half.cu",
+    "residual_float.cu",
     "bind_vocab.cpp",
     "vocab_loss.cu",
     "dist_fused.cu",
