@@ -372,6 +372,13 @@ struct Feed {
   }
 };
 
+// CTAs an SM that a kernel's registers have to allow.  Odd widths' conditions would otherwise take
+// a fifth warp's registers: 20000 x 1111 with dropout, forward 121 us without the bound, 83 with
+// four CTAs, backward 149 and 121 with three; three for the smallest rows' backward spills.
+__host__ __device__ constexpr int ctas_of(int nv, int rt, int most) {
+  return rt == 512 ? 1 : nv == 1 && rt == 256 ? most : 2;
+}
+
 // The branch's factors f * w1 * gate and the norm's weights w2 (1 where there are none) of a
 // thread's columns: in registers for all rows (up to two blocks a thread), in shared memory as
 // fp32 (a warp a row: its four blocks would take 64 registers), or read again from L1 for every
@@ -457,7 +464,7 @@ struct Weights {
 };
 
 template <typename T, int NV, int RT, bool ODD, bool DROP, bool RING, bool FULL>
-__global__ void __launch_bounds__(RT > 256 ? RT : 256)
+__global__ void __launch_bounds__(RT > 256 ? RT : 256, ctas_of(NV, RT, 4))
     join_fwd_k(const JoinArgs a, float factor, int stages) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t bars[8][kMaxStages];
@@ -542,7 +549,7 @@ __global__ void __launch_bounds__(RT > 256 ? RT : 256)
 }
 
 template <typename T, int NV, int RT, bool ODD, bool DROP, bool RING, bool FULL>
-__global__ void __launch_bounds__(RT > 256 ? RT : 256)
+__global__ void __launch_bounds__(RT > 256 ? RT : 256, ctas_of(NV, RT, 3))
     join_bwd_k(const JoinArgs a, float factor, int stages) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t bars[8][kMaxStages];
