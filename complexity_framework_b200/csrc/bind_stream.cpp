@@ -1,4 +1,4 @@
-// Python bindings of the residual-stream kernels (residual.cu).  Shapes, dtypes and devices are
+// Python bindings of the residual-stream kernels (residual.cuh).  Shapes, dtypes and devices are
 // checked here; every entry allocates its outputs and launches on the current stream of its
 // tensors' device.
 #include <torch/extension.h>

@@ -14,16 +14,17 @@
 // The forward reads x, b and writes x', y; the backward reads dx', dy, x', b and writes dx, db; the
 // dropout mask is drawn again from its counter instead of being stored.  Memory would bound both;
 // what does is the issue of instructions, as every element passes two sums in sequence: the
-// backward takes 400 warp instructions for 32 blocks of eight elements and 120 more for their
+// backward takes 310 warp instructions for 32 blocks of eight elements and 120 more for their
 // dropout, of which schedulers with four warps each issue one every other cycle.  So a row's
 // fixed work is spread over as many elements as registers allow, rows come through a ring of bulk
-// copies, and arithmetic is in pairs.  Sums run in fp32; results are rounded once, at their stores.
+// copies, arithmetic is in pairs, and what a call leaves out is asked for outside the rows.  Sums run in fp32; results are rounded once, at their stores.
 // The columns' sums stay in registers over all rows of a CTA, and one small kernel adds the CTAs'
 // sums in a fixed order, so that equal calls give equal bits.
 //
 // us (TB/s), bf16, with norms and gate, on one B200 (a copy runs at 6.55 TB/s):
-//   32768 x 896   forward 41 (5.7), with dropout 51 (4.6); backward 92 (3.8), 113 (3.1)
-//   8191 x 4096   forward 49 (5.5), with dropout 56 (4.8); backward 81 (5.0), 110 (3.7)
+//   32768 x 896   forward 38 (6.2), with dropout 49 (4.8); backward 74 (4.8), 92 (3.8)
+//   8191 x 4096   forward 47 (5.7), with dropout 53 (5.1); backward 81 (5.0), 85 (4.7)
+//   20000 x 903   forward 40 (3.6), with dropout 53 (2.8); backward 81 (2.7), 93 (2.3)
 //   dropout alone of 32768 x 896: 21 (5.5)
 //
 // Templates of one element type each; residual_bf16.cu, residual_half.cu and residual_float.cu
@@ -792,8 +793,8 @@ __global__ void __launch_bounds__(256) dropout_k(const T* __restrict__ x, T* __r
 // Calls f with the (NV, RT, ODD) of a row: the fewest threads that hold it.  Up to 128 blocks of a
 // 16-bit type, with rows for every warp of the machine, take fewer threads with more blocks each:
 // a row's fixed work (its sums and barriers) is then one or two warps' instead of four's.  32768 x
-// 896 with dropout, us: forward 60 with four warps a row, 51 with one; backward 123 with four, 114
-// with two (one: 153, its columns' sums leave 8 warps an SM).
+// 896 with dropout, us, before what `full` saves: forward 60 with four warps a row, 51 with one;
+// backward 123 with four, 114 with two (one: 153, its columns' sums leave 8 warps an SM).
 template <typename T, bool BWD, typename F>
 int with_shape(const JoinArgs& a, int num_sms, F f) {
   const bool odd = a.H % 8 != 0;

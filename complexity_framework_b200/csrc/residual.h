@@ -1,4 +1,4 @@
-// Host interface of the residual-stream kernels (residual.cu).
+// Host interface of the residual-stream kernels (residual.cuh).
 #pragma once
 #include <cuda_runtime.h>
 #include <cstdint>

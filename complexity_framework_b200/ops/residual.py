@@ -1,4 +1,4 @@
-"""Operators of the residual stream (``csrc/residual.cu``): what joins a block's branch to the
+"""Operators of the residual stream (``csrc/residual.cuh``): what joins a block's branch to the
 stream, and dropout.
 
 ``residual_norm`` is one join of a decoder whose blocks have norms before and after them:
