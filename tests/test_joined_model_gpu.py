@@ -133,6 +133,21 @@ def test_decoding_follows_the_forward():
         assert float(row.max() - row[out[i]]) <= 2.0 ** -6 * max(1.0, float(row.abs().max()))
 
 
+def test_recomputed_blocks_draw_the_same_masks():
+    m = model(residual_dropout=0.3, embedding_dropout=0.1, **FULL).train()
+    ids = torch.randint(0, 1000, (2, 64), device="cuda")
+    grads = []
+    for ckpt in (False, True, True):
+        (m.gradient_checkpointing_enable if ckpt else m.gradient_checkpointing_disable)()
+        m.zero_grad()
+        torch.manual_seed(7)
+        m.loss(ids, label_smoothing=0.1).backward()
+        grads.append([p.grad.clone() for p in m.parameters()])
+    # the model's other kernels add some gradients by atomics: equal up to roundings to 8 bits
+    for a, b, c in zip(*grads):
+        assert cosine(a, b) >= 1 - (4 * 2.0 ** -8) ** 2 and cosine(b, c) >= 1 - (4 * 2.0 ** -8) ** 2
+
+
 @pytest.mark.parametrize("graph", [False, True])
 def test_training_steps(graph):
     m = model(residual_dropout=0.2, embedding_dropout=0.1, **FULL)

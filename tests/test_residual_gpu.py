@@ -263,6 +263,32 @@ def test_dropout(n, dtype):
         assert torch.equal(R.dropout(x, p, torch.tensor([seed], device="cuda"), stream=stream), y)
 
 
+def philox(block, stream, seed):
+    """Random bits of one block in Python's integers: 8 x 16 bits."""
+    c, k = [block & 0xFFFFFFFF, block >> 32, stream, 0], [seed & 0xFFFFFFFF, seed >> 32]
+    for _ in range(10):
+        a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return [v >> s & 0xFFFF for v in c for s in (0, 16)]
+
+
+@pytest.mark.parametrize("H", [520, 515])
+def test_more_elements_than_31_bits(H):
+    T = 2 ** 31 // H + 3
+    x = torch.ones(T, H, device="cuda", dtype=torch.bfloat16)
+    y = R.dropout(x, 0.5, 12345, stream=6)
+    new, n = R.residual_norm(x, x, norm_weight=x[0], p=0.5, seed=12345, stream=6)
+    for row in (0, T // 2, T - 1):
+        e = [row * H + c for c in range(H)]
+        bits = {b: philox(b, 6, 12345) for b in range(e[0] // 8, e[-1] // 8 + 1)}
+        want = torch.tensor([2.0 if bits[i // 8][i % 8] >= 32768 else 0.0 for i in e])
+        assert torch.equal(y[row].cpu().float(), want)
+        assert torch.equal(new[row].cpu().float(), 1 + want)
+        ref = (1 + want.double()) / ((1 + want.double()).square().mean() + 1e-6).sqrt()
+        assert bool(((n[row].cpu().double() - ref).abs() <= 2.0 ** -8 * ref).all())
+
+
 def test_dropout_layouts():
     base = torch.randn(9, 34, device="cuda", dtype=torch.float16)
     for x in (base[:, 1:], base.t(), base.reshape(-1)[1:], base[:0]):

@@ -138,6 +138,9 @@ def test_rows_in_parts():
     pick = torch.cat((torch.arange(0, T, 37), torch.arange(T - 70, T))).cuda()
     loss, tol, *_ = oracle_loss(h[pick], w, y[pick])
     close(rows[pick], loss, tol, "rows")
+    y[500:] = -100  # all counted rows in the first part
+    few = vocab_cross_entropy(h, w, y, reduction="none")
+    assert torch.equal(few[:500], rows[:500]) and bool((few[500:] == 0).all())
     check_errors()
 
 
