@@ -392,7 +392,7 @@ def build_parser() -> argparse.ArgumentParser:
     pr = sub.add_parser("profile")
     pr.add_argument("what", choices=["model", "kernels", "throughput"])
     pr.add_argument("--model", default="tr-hash-200m")
-    pr.add_argument("--case", default="gemm", choices=["gemm", "gemm_bn", "flash", "norms"])
+    pr.add_argument("--case", default="gemm", choices=["gemm", "gemm_bn", "flash", "norms", "stream"])
     pr.add_argument("--seq-len", type=int, default=2048)
     pr.add_argument("--batch", type=int, default=1)
     pr.add_argument("--device", default=None)

@@ -53,7 +53,8 @@ int type_of(const Tensor& t, const char* name) {
 }
 
 void like(const Tensor& t, const Tensor& x, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.get_device() == x.get_device(), name, " must be on x's CUDA device");
+  TORCH_CHECK_VALUE(t.is_cuda() && t.get_device() == x.get_device(), name,
+                    " must be on x's CUDA device");
   TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), name, " must have x's dtype ",
                    x.scalar_type(), ", got ", t.scalar_type());
 }
@@ -88,8 +89,8 @@ cfb::DropArgs drop_of(double p, const OptTensor& seed, int64_t seed_value, int64
   d.stream = static_cast<uint32_t>(stream);
   d.seed = static_cast<uint64_t>(seed_value);
   if (seed.has_value()) {
-    TORCH_CHECK(seed->is_cuda() && seed->get_device() == x.get_device(),
-                "seed must be on x's CUDA device");
+    TORCH_CHECK_VALUE(seed->is_cuda() && seed->get_device() == x.get_device(),
+                      "seed must be on x's CUDA device");
     TORCH_CHECK_TYPE(seed->scalar_type() == torch::kInt64, "seed must be int64");
     TORCH_CHECK_VALUE(seed->numel() == 1, "seed must have one element");
     d.seed_ptr = seed->data_ptr<int64_t>();

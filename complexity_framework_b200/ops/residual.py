@@ -157,11 +157,15 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, *,
     ``[H]`` of that type.  ``p`` > 0 drops elements of the branch and needs a ``seed``.
     """
     threshold = _threshold(p)
+    tensor, value = (None, 0) if threshold == 0 else _check_seed(seed, stream, x)
+    ts = (x, branch, branch_weight, gate, norm_weight)
+    if x.is_cuda:  # shapes, types and devices are checked in the extension
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+            return require().residual_norm_grad(*ts, scale, p, tensor, value, stream, eps)
+        return require().residual_norm_fwd(*ts, scale, p, tensor, value, stream, eps, False)[:2]
     if not x.is_floating_point():
         raise TypeError("x must be a floating-point tensor")
-    tensor, value = (None, 0) if threshold == 0 else _check_seed(seed, stream, x)
-    for name, t in (("branch", branch), ("branch_weight", branch_weight), ("gate", gate),
-                    ("norm_weight", norm_weight)):
+    for name, t in zip(("branch", "branch_weight", "gate", "norm_weight"), ts[1:]):
         if t is None:
             continue
         if t.dtype != x.dtype:
@@ -171,13 +175,8 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, *,
         want = x.shape if name == "branch" else x.shape[-1:]
         if t.shape != want:
             raise ValueError(f"{name} must be {list(want)}, got {list(t.shape)}")
-    if not x.is_cuda:
-        f = None
-        if threshold:
-            f = dropout_factors(x.shape, p, value if tensor is None else tensor, stream=stream,
-                                device=x.device)
-        return _residual_norm_torch(x, branch, branch_weight, gate, norm_weight, scale, f, eps)
-    ts = (x, branch, branch_weight, gate, norm_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        return require().residual_norm_grad(*ts, scale, p, tensor, value, stream, eps)
-    return require().residual_norm_fwd(*ts, scale, p, tensor, value, stream, eps, False)[:2]
+    f = None
+    if threshold:
+        f = dropout_factors(x.shape, p, value if tensor is None else tensor, stream=stream,
+                            device=x.device)
+    return _residual_norm_torch(*ts, scale, f, eps)

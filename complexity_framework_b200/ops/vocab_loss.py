@@ -76,12 +76,14 @@ def _loss(hidden, weight, targets, ignore_index, label_smoothing, z_loss, logit_
         raise ValueError(f"targets must be {list(hidden.shape[:-1])}, got {list(targets.shape)}")
     if targets.dtype != torch.int64:
         raise TypeError("targets must be int64")
-    h, y = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1)
+    h, y = hidden, targets
+    if hidden.dim() != 2:
+        h, y = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1)
     if h.is_cuda:
         grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
         loss = require().vocab_loss(h, weight, y, ignore_index, label_smoothing, z_loss, logit_scale,
                                     _REDUCTIONS[reduction], sign, workspace_bytes, grad)
-        return loss.view(targets.shape) if reduction == "none" else loss
+        return loss.view(targets.shape) if loss.dim() and targets.dim() != 1 else loss
     rows = sign * _rows_torch(h, weight, y, ignore_index, label_smoothing, z_loss, logit_scale)
     if reduction == "none":
         return rows.view(targets.shape)

@@ -3,6 +3,7 @@
     python -m complexity_framework_b200.profiling.kernel_cases gemm
     python -m complexity_framework_b200.profiling.kernel_cases flash
     python -m complexity_framework_b200.profiling.kernel_cases norms
+    python -m complexity_framework_b200.profiling.kernel_cases stream
 
 Each case runs the 200M-shape kernels (inputs larger than L2, a few GB at
 most) ``--iters`` times and prints CUDA-event timings with the fraction of
@@ -258,8 +259,37 @@ def case_decode(iters: int) -> None:
         del ws
 
 
+def case_stream(iters: int) -> None:
+    """Residual join, dropout and the vocabulary loss without logits, forward and backward."""
+    from ..ops.residual import dropout, residual_norm
+    from ..ops.vocab_loss import vocab_cross_entropy
+
+    T, H, V = 32768, 896, 32000
+    x, b, dy = (torch.randn(T, H, device="cuda").bfloat16().requires_grad_(i < 2)
+                for i in range(3))
+    w1, gate, w2 = (torch.ones(H, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+                    for _ in range(3))
+    row = 2.0 * T * H
+
+    def join(p):
+        outs = residual_norm(x, b, branch_weight=w1, gate=gate, norm_weight=w2, p=p, seed=1)
+        torch.autograd.grad(outs, (x, b, w1, gate, w2), (dy, dy))
+
+    for p in (0.0, 0.1):
+        _report(f"residual_norm p={p}", cuda_time(lambda: join(p), iters), nbytes=10 * row)
+    _report("dropout", cuda_time(lambda: dropout(dy, 0.1, 1), iters), nbytes=2 * row)
+    w = (torch.randn(V, H, device="cuda") * 0.05).bfloat16().requires_grad_()
+    y = torch.randint(0, V, (T,), device="cuda")
+
+    def loss():
+        out = vocab_cross_entropy(x, w, y, label_smoothing=0.1)
+        torch.autograd.grad(out, (x, w))
+
+    _report("vocab_cross_entropy", cuda_time(loss, max(3, iters // 4)), 8.0 * T * V * H)
+
+
 CASES = {"decode": case_decode, "gemm": case_gemm, "gemm_bn": case_gemm_bn, "flash": case_flash, "norms": case_norms,
-         "moe": case_moe}
+         "moe": case_moe, "stream": case_stream}
 
 
 def main(argv=None) -> None:

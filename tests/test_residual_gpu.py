@@ -387,6 +387,20 @@ def test_refusals():
         R.residual_norm(x.double(), x.double())
     with pytest.raises(ValueError, match="device"):
         R.residual_norm(x, x.cpu())
+    with pytest.raises(ValueError, match="branch must"):
+        R.residual_norm(x, x[:2])
+    with pytest.raises(ValueError, match="gate must"):
+        R.residual_norm(x, x, gate=x[0, :4])
+    with pytest.raises(TypeError, match="norm_weight must"):
+        R.residual_norm(x, x, norm_weight=x[0].bfloat16())
+    with pytest.raises(TypeError, match="bfloat16"):
+        R.residual_norm(x.long(), x.long())
+    with pytest.raises(ValueError, match="scale must"):
+        R.residual_norm(x, x, scale=float("nan"))
+    with pytest.raises(ValueError, match="eps must"):
+        R.residual_norm(x, x, norm_weight=x[0], eps=-1.0)
+    with pytest.raises(ValueError, match="seed"):
+        R.residual_norm(x, x, p=0.1)
     with pytest.raises(ValueError, match="device"):
         R.dropout(x, 0.1, torch.zeros(1, dtype=torch.int64))
     with pytest.raises(RuntimeError, match="once_differentiable|twice"):
