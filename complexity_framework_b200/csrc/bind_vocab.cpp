@@ -40,7 +40,7 @@ void check_rc(int rc) {
 
 cfb::VlCall call_of(int64_t T, const Tensor& w, double scale, double smooth, double z,
                     int64_t ignore) {
-  TORCH_CHECK_VALUE(T <= 0x7fffff00 && w.size(0) >= 1 && w.size(0) <= 0x7fffff00,
+  TORCH_CHECK_VALUE(T <= (1 << 30) && w.size(0) >= 1 && w.size(0) <= (1 << 30),
                     "too many rows or words");
   TORCH_CHECK_VALUE(w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(1) <= (1 << 20),
                     "the hidden size must be a multiple of 8, got ", w.size(1));

@@ -1017,7 +1017,11 @@ static int launch_impl(const SegMaps<NA>& ta, const SegMaps<NB>& tb, const CUten
                        int* err, int ksplit = 1) {
   using Cfg = GemmCfg<BN, PAIR, epi_slots(EPI), epi_loads(EPI), epi_depth(EPI)>;
   auto kern = gemm_tc_kernel<BN, A_MN, B_MN, EPI, PAIR, NA, NB>;
-  static int max_units = -1;  // resident CTAs (or CTA pairs), one query per instantiation
+  // resident CTAs (or CTA pairs), one query per instantiation and device
+  static int units_of[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int& max_units = units_of[dev & 63];
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.blockDim = dim3(384, 1, 1);
@@ -1029,7 +1033,7 @@ static int launch_impl(const SegMaps<NA>& ta, const SegMaps<NB>& tb, const CUten
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (max_units < 0) {
+  if (max_units <= 0) {
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
     if (PAIR) {
       cfg.gridDim = dim3(2 * (num_sms / 2), 1, 1);
