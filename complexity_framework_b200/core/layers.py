@@ -86,13 +86,15 @@ class ResidualJoin(nn.Module):
                      else nn.Parameter(torch.full((hidden_size,), float(gate_init))))
         self.scale, self.p, self.eps = scale, p, eps
 
-    def forward(self, x: torch.Tensor, branch: torch.Tensor, next_norm: Optional[nn.Module] = None):
-        """``(x', next_norm(x'))``; the second is None without ``next_norm``."""
+    def forward(self, x: torch.Tensor, branch: torch.Tensor, next_norm: Optional[nn.Module] = None,
+                drop: bool = True):
+        """``(x', next_norm(x'))``; the second is None without ``next_norm``.  ``drop=False``: no
+        dropout in training mode either (decoding)."""
         from ..ops.residual import new_seed, residual_norm
 
         fused = (isinstance(next_norm, RMSNorm) and next_norm.eps == self.eps
                  and next_norm.weight.dtype == x.dtype)
-        p = self.p if self.training else 0.0
+        p = self.p if self.training and drop else 0.0
         new, y = residual_norm(x, branch.to(x.dtype), branch_weight=self.weight, gate=self.gate,
                                norm_weight=next_norm.weight if fused else None, scale=self.scale,
                                p=p, seed=new_seed(x.device) if p > 0 else None, eps=self.eps)

@@ -157,8 +157,8 @@ class TransformerBlock(nn.Module):
                 raise NotImplementedError("tensor-parallel decoding adds its branches while it "
                                           "reduces them: no sandwich norms, residual gate or scale")
             a = self.self_attn.forward_paged(h, cache, self.layer_idx)
-            x, h = self.attn_join(hidden_states, a, self.post_attention_layernorm)
-            return self.mlp_join(x, self.mlp(h, token_ids=token_ids))[0]
+            x, h = self.attn_join(hidden_states, a, self.post_attention_layernorm, drop=False)
+            return self.mlp_join(x, self.mlp(h, token_ids=token_ids), drop=False)[0]
         x = self.self_attn.forward_paged(h, cache, self.layer_idx, residual=hidden_states)
         h = self.post_attention_layernorm(x)
         return self.mlp(h, token_ids=token_ids, residual=x)

@@ -97,6 +97,14 @@ def test_paged_decoding_follows_the_forward():
     assert out == ids
 
 
+def test_decoding_drops_nothing_in_training_mode():
+    from complexity_framework_b200.inference import beam_search
+
+    m = tiny(residual_dropout=0.5, embedding_dropout=0.5, **FULL)
+    want = beam_search(m.eval(), [3, 14, 15], num_beams=2, max_new_tokens=4)["tokens"]
+    assert beam_search(m.train(), [3, 14, 15], num_beams=2, max_new_tokens=4)["tokens"] == want
+
+
 def test_config_round_trip_and_refusals(tmp_path):
     m = tiny(residual_dropout=0.1, **FULL)
     m.save_pretrained(tmp_path)
