@@ -304,6 +304,7 @@ class ComplexityModel(nn.Module):
         n_total = (labels != ignore_index).sum().clamp_min(1)
         loss = causal_lm_loss_from_hidden(x.view(1, rows, -1), self.output_weight(),
                                           lab.view(1, rows), ignore_index=ignore_index,
+                                          logit_scale=self.logit_scale,
                                           label_smoothing=label_smoothing,
                                           z_loss_coef=z_loss_coef)
         return loss * (n_local / n_total)

@@ -79,7 +79,8 @@ class PipelineStage(nn.Module):
 
         labels = torch.roll(token_ids, -1, dims=1)
         labels[:, -1] = -100
-        return causal_lm_loss_from_hidden(hidden, self.output_weight(), labels)
+        return causal_lm_loss_from_hidden(hidden, self.output_weight(), labels,
+                                          logit_scale=self._model[0].logit_scale)
 
 
 class PipelineModel(nn.Module):

@@ -1,0 +1,49 @@
+"""Loss options and joined residuals on the paths beside the plain model: sequence-parallel and
+pipeline losses, data-parallel ranks, resumed runs, exports."""
+import types
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from complexity_framework_b200 import ComplexityModel
+from complexity_framework_b200.config import ModelConfig
+
+
+def tiny(**kw):
+    base = dict(hidden_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                intermediate_size=64, shared_intermediate_size=64, vocab_size=97, num_experts=2,
+                top_k=2, max_position_embeddings=64)
+    base.update(kw)
+    torch.manual_seed(0)
+    return ComplexityModel(ModelConfig(**base))
+
+
+FULL = dict(norm_placement="sandwich", residual_gate_init=0.5, residual_scale=0.7)
+MUP = dict(use_mup_output_mult=True, mup_base_width=16)  # logits times 1 / 4
+
+
+# ------------------------------------------------------------- the logit scale
+def test_sequence_parallel_loss_scales_the_logits():
+    """The sequence-parallel loss of one rank that holds every token is the model's loss."""
+    m = tiny(**MUP).train()
+    with torch.no_grad():
+        m.embed_tokens.weight.mul_(50)  # logits large enough that their scale matters
+    ids = torch.randint(0, 97, (2, 9))
+    m.sp_ws = types.SimpleNamespace(world=1, rank=0, begin_step=lambda: None)
+    for layer in m.layers:
+        layer.forward_sp = lambda x, ids, B, S, ws, f=layer: f(
+            x.view(B, S, -1), token_ids=ids)[0].view(B * S, -1)
+    for kw in ({}, dict(label_smoothing=0.1, z_loss_coef=1e-2)):
+        torch.testing.assert_close(m._loss_sp(ids, None, -100, **kw), m.loss(ids, **kw))
+
+
+def test_pipeline_stage_loss_scales_the_logits():
+    from complexity_framework_b200.parallel.pipeline_parallel import PipelineStage
+
+    m = tiny(**MUP)
+    with torch.no_grad():
+        m.embed_tokens.weight.mul_(50)
+    ids = torch.randint(0, 97, (2, 9))
+    stage = PipelineStage(m, 0, 2, True, True)
+    torch.testing.assert_close(stage.loss(stage(None, ids), ids), m.loss(ids))
