@@ -125,9 +125,10 @@ def weighted_sft_loss(model, input_ids, packed_labels):
     y = labels.reshape(-1)
     w = weights.reshape(-1)
     valid = y != IGNORE_INDEX
+    scale = getattr(model, "logit_scale", 1.0)
     total = h.new_zeros((), dtype=torch.float32)
     for s in range(0, h.shape[0], 4096):
-        logits = (h[s:s + 4096] @ W.t()).float()
+        logits = (h[s:s + 4096] @ W.t()).float() * scale
         ce = torch.nn.functional.cross_entropy(logits, y[s:s + 4096].clamp_min(0),
                                                reduction="none")
         total = total + (ce * w[s:s + 4096] * valid[s:s + 4096]).sum()

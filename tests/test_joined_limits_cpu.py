@@ -47,3 +47,17 @@ def test_pipeline_stage_loss_scales_the_logits():
     ids = torch.randint(0, 97, (2, 9))
     stage = PipelineStage(m, 0, 2, True, True)
     torch.testing.assert_close(stage.loss(stage(None, ids), ids), m.loss(ids))
+
+
+def test_weighted_fine_tuning_loss_scales_the_logits():
+    from complexity_framework_b200.training.sft import weighted_sft_loss
+
+    m = tiny(**MUP)
+    with torch.no_grad():
+        m.embed_tokens.weight.mul_(50)
+    ids = torch.randint(0, 97, (2, 9))
+    labels = torch.randint(0, 97, (2, 9))
+    labels[0, :3] = -100
+    ones = torch.ones(2, 9, dtype=torch.long)
+    got = weighted_sft_loss(m, ids, torch.stack((labels, ones), -1))
+    torch.testing.assert_close(got, m.loss(ids, labels))
