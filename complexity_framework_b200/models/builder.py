@@ -200,6 +200,9 @@ class ComplexityModel(nn.Module):
                 past_len = past_key_values[0][0].shape[2]
             hidden = self.embed_positions(hidden, offset=past_len)
         if self.training and self.config.embedding_dropout > 0:
+            if getattr(self, "tp_group", None) is not None:
+                raise NotImplementedError("embedding_dropout under tensor parallelism: the ranks "
+                                          "of a group would draw different masks")
             from ..ops.residual import dropout, new_seed
 
             hidden = dropout(hidden, self.config.embedding_dropout, new_seed(hidden.device))

@@ -80,7 +80,7 @@ class PipelineStage(nn.Module):
         labels = torch.roll(token_ids, -1, dims=1)
         labels[:, -1] = -100
         return causal_lm_loss_from_hidden(hidden, self.output_weight(), labels,
-                                          logit_scale=self._model[0].logit_scale)
+                                          logit_scale=getattr(self._model[0], "logit_scale", 1.0))
 
 
 class PipelineModel(nn.Module):

@@ -61,3 +61,14 @@ def test_weighted_fine_tuning_loss_scales_the_logits():
     ones = torch.ones(2, 9, dtype=torch.long)
     got = weighted_sft_loss(m, ids, torch.stack((labels, ones), -1))
     torch.testing.assert_close(got, m.loss(ids, labels))
+
+
+# -------------------------------------------------------- dropout across ranks
+def test_embedding_dropout_is_refused_under_tensor_parallelism():
+    """The ranks of a group hold one replicated stream, which different masks would part."""
+    m = tiny(embedding_dropout=0.1).train()
+    m.tp_group = object()
+    with pytest.raises(NotImplementedError, match="embedding_dropout under tensor parallelism"):
+        m(torch.randint(0, 97, (1, 4)))
+    m.eval()
+    m(torch.randint(0, 97, (1, 4)))
