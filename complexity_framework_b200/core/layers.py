@@ -70,12 +70,20 @@ class IdentityNorm(nn.Module):
         return x
 
 
+def dropout_stream() -> int:
+    """Generator stream of this process's dropout masks: its rank, so that data-parallel ranks
+    whose generators are seeded alike still draw masks of their own."""
+    dist = torch.distributed
+    return dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
+
+
 class ResidualJoin(nn.Module):
     """``x + scale * dropout(gate * rmsnorm(branch))`` and, of the sum, the next block's norm.
 
     ``norm``: the branch is normalised, with a learned weight; ``gate_init``: a learned gate of
     each channel starts there; ``p``: dropout in training, from a seed drawn for each call from
-    PyTorch's generator.  One ``ops.residual.residual_norm`` on any device.
+    PyTorch's generator and the rank (``dropout_stream``).  One ``ops.residual.residual_norm`` on
+    any device.
     """
 
     def __init__(self, hidden_size: int, *, norm: bool = True, gate_init: Optional[float] = None,
@@ -97,7 +105,8 @@ class ResidualJoin(nn.Module):
         p = self.p if self.training and drop else 0.0
         new, y = residual_norm(x, branch.to(x.dtype), branch_weight=self.weight, gate=self.gate,
                                norm_weight=next_norm.weight if fused else None, scale=self.scale,
-                               p=p, seed=new_seed(x.device) if p > 0 else None, eps=self.eps)
+                               p=p, seed=new_seed(x.device) if p > 0 else None,
+                               stream=dropout_stream(), eps=self.eps)
         if next_norm is not None and not fused:
             y = next_norm(new)
         return new, y

@@ -24,7 +24,7 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint as activation_checkpoint
 
 from ..config.model_config import ModelConfig, get_preset
-from ..core.layers import use_fused
+from ..core.layers import dropout_stream, use_fused
 from ..core.registry import NORMALIZATION_REGISTRY
 from .block import TransformerBlock
 
@@ -205,7 +205,8 @@ class ComplexityModel(nn.Module):
                                           "of a group would draw different masks")
             from ..ops.residual import dropout, new_seed
 
-            hidden = dropout(hidden, self.config.embedding_dropout, new_seed(hidden.device))
+            hidden = dropout(hidden, self.config.embedding_dropout, new_seed(hidden.device),
+                             stream=dropout_stream())
         token_ids = routing_ids if routing_ids is not None else input_ids
         if token_ids is None:
             token_ids = torch.zeros(B, S, dtype=torch.long, device=hidden.device)

@@ -72,3 +72,53 @@ def test_embedding_dropout_is_refused_under_tensor_parallelism():
         m(torch.randint(0, 97, (1, 4)))
     m.eval()
     m(torch.randint(0, 97, (1, 4)))
+
+
+def _rank_masks(rank, port, out):
+    import torch.distributed as dist
+
+    from complexity_framework_b200.core.layers import ResidualJoin
+
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=2)
+    try:
+        out[rank] = _masks(ResidualJoin)
+    finally:
+        dist.destroy_process_group()
+
+
+def _masks(ResidualJoin):
+    """What a join and a model's embedding dropout keep, under one seed."""
+    torch.manual_seed(3)
+    x = torch.zeros(16, 64)
+    join = ResidualJoin(64, norm=False, p=0.5).train()(x, torch.ones(16, 64))[0]
+    m = tiny(embedding_dropout=0.5).train()
+    kept = []
+    m.layers[0].register_forward_pre_hook(lambda _, args: kept.append(args[0] != 0))
+    m(torch.arange(8).view(1, 8))
+    return (join != 0).tolist(), kept[0].tolist()
+
+
+def test_data_parallel_ranks_draw_masks_of_their_own():
+    """Ranks that are seeded alike, as the training scripts seed them."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    from complexity_framework_b200.core.layers import ResidualJoin
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    with ctx.Manager() as manager:
+        out = manager.dict()
+        procs = [ctx.Process(target=_rank_masks, args=(r, port, out)) for r in range(2)]
+        for p in procs:
+            p.start()
+        for p in procs:
+            p.join(180)
+        assert [p.exitcode for p in procs] == [0, 0]
+        a, b = out[0], out[1]
+    for i in range(2):
+        assert a[i] != b[i]
+    assert a == _masks(ResidualJoin)  # the first rank's are those of a process by itself
