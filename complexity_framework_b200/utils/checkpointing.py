@@ -2,7 +2,8 @@
 
 Directory layout per checkpoint (reference: complexity/utils/checkpointing.py:127-579):
 ``checkpoint.pt`` = {"model": full state dict, "scheduler": state}, ``model.safetensors``,
-``optimizer_rank{r}.pt`` (each rank's optimizer shard), ``training_state.json``
+``optimizer_rank{r}.pt`` (each rank's optimizer shard), ``rng_rank{r}.pt`` (each rank's PyTorch
+generators, which dropout draws from), ``training_state.json``
 = {step, epoch, best_loss, total_tokens, learning_rate} written LAST so a
 directory without it is incomplete and skipped on resume.  Files are written
 to a temporary name and renamed (atomic on POSIX).  ``save_total_limit`` keeps
@@ -62,6 +63,25 @@ def _atomic_save(obj: Any, path: Path) -> None:
     os.replace(tmp, path)
 
 
+def _cuda_device(model: torch.nn.Module) -> Optional[torch.device]:
+    p = next(model.parameters(), None)
+    return p.device if p is not None and p.is_cuda else None
+
+
+def _generator_states(model: torch.nn.Module) -> Dict[str, torch.Tensor]:
+    st, dev = {"torch": torch.get_rng_state()}, _cuda_device(model)
+    if dev is not None:
+        st["cuda"] = torch.cuda.get_rng_state(dev)
+    return st
+
+
+def _set_generator_states(model: torch.nn.Module, st: Dict[str, torch.Tensor]) -> None:
+    torch.set_rng_state(st["torch"])
+    dev = _cuda_device(model)
+    if "cuda" in st and dev is not None:
+        torch.cuda.set_rng_state(st["cuda"], dev)
+
+
 def _atomic_json(obj: Any, path: Path) -> None:
     tmp = path.with_suffix(path.suffix + ".tmp")
     with open(tmp, "w") as fh:
@@ -99,6 +119,7 @@ class CheckpointManager:
         if optimizer is not None:
             path.mkdir(parents=True, exist_ok=True)
             _atomic_save(optimizer.state_dict(), path / f"optimizer_rank{rank}.pt")
+            _atomic_save(_generator_states(model), path / f"rng_rank{rank}.pt")
         if on:
             dist.barrier()
         if is_main:
@@ -156,6 +177,11 @@ class CheckpointManager:
         if optimizer is not None and opt_path.exists():
             optimizer.load_state_dict(torch.load(opt_path, map_location=map_location,
                                                  weights_only=False))
+        # a rank that the saved run did not have goes on from the first one's generators
+        rng = [path / f"rng_rank{r}.pt" for r in (rank, 0)]
+        rng = next((p for p in rng if p.exists()), None)
+        if optimizer is not None and rng is not None:
+            _set_generator_states(model, torch.load(rng, map_location="cpu", weights_only=True))
         with open(path / STATE_FILE) as fh:
             return json.load(fh)
 

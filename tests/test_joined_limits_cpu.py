@@ -122,3 +122,31 @@ def test_data_parallel_ranks_draw_masks_of_their_own():
     for i in range(2):
         assert a[i] != b[i]
     assert a == _masks(ResidualJoin)  # the first rank's are those of a process by itself
+
+
+# ------------------------------------------------------------------ resumed runs
+def test_resumed_run_goes_on_with_the_masks(tmp_path):
+    """Two steps, a checkpoint and two more steps of another process are four steps of one."""
+    from complexity_framework_b200.training import Trainer, TrainingConfig
+
+    ids = torch.randint(0, 97, (2, 9), generator=torch.Generator().manual_seed(1))
+
+    def trainer():
+        m = tiny(residual_dropout=0.3, embedding_dropout=0.2, **FULL)
+        return Trainer(m, TrainingConfig(max_steps=8, learning_rate=1e-3, precision="fp32",
+                                         warmup_steps=0, checkpoint_dir=str(tmp_path)),
+                       device=torch.device("cpu"))
+
+    a = trainer()
+    for _ in range(2):
+        a.train_step(ids)
+    a.save_checkpoint()
+    want = [a.train_step(ids) for _ in range(2)]
+    b = trainer()
+    torch.manual_seed(77)
+    assert b.resume("auto") and b.global_step == 2
+    assert [b.train_step(ids) for _ in range(2)] == want
+    # a checkpoint without the generators' state, as older ones are, still resumes
+    for f in tmp_path.glob("*/rng_rank*.pt"):
+        f.unlink()
+    assert trainer().resume("auto")
