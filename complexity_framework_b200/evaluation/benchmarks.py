@@ -30,10 +30,14 @@ class BenchmarkResult:
 @torch.no_grad()
 def choice_logprobs(model, tokenizer, context: str, choices: Sequence[str],
                     normalize: bool = True) -> List[float]:
-    """Sum (or per-token mean) log p(choice | context) for every choice."""
+    """Sum (or per-token mean) log p(choice | context) for every choice.  Without a context a
+    choice's first token follows nothing: it is not scored, and a choice needs two."""
     dev = next(model.parameters()).device
     ctx = tokenizer.encode(context)
     seqs = [ctx + tokenizer.encode(c) for c in choices]
+    first = max(len(ctx), 1)  # scored from here on
+    if not ctx and any(len(s) < 2 for s in seqs):
+        raise ValueError("a choice of one token without a context has nothing to score")
     L = max(len(s) for s in seqs)
     pad = tokenizer.pad_token_id or 0
     ids = torch.full((len(seqs), L), pad, dtype=torch.long)
@@ -41,9 +45,9 @@ def choice_logprobs(model, tokenizer, context: str, choices: Sequence[str],
         ids[i, :len(s)] = torch.tensor(s)
     targets = torch.full((len(seqs), L), -100, dtype=torch.long)
     for i, s in enumerate(seqs):
-        targets[i, len(ctx) - 1:len(s) - 1] = torch.tensor(s[len(ctx):], dtype=torch.long)
+        targets[i, first - 1:len(s) - 1] = torch.tensor(s[first:], dtype=torch.long)
     sums = model_token_logprobs(model, ids.to(dev), targets.to(dev)).sum(-1).tolist()
-    return [v / (len(s) - len(ctx) if normalize and len(s) > len(ctx) else 1)
+    return [v / (len(s) - first if normalize and len(s) > first else 1)
             for v, s in zip(sums, seqs)]
 
 

@@ -150,3 +150,30 @@ def test_resumed_run_goes_on_with_the_masks(tmp_path):
     for f in tmp_path.glob("*/rng_rank*.pt"):
         f.unlink()
     assert trainer().resume("auto")
+
+
+# ------------------------------------------------------------- scoring of choices
+class _Words:
+    pad_token_id = 0
+
+    @staticmethod
+    def encode(text):
+        return [int(t) for t in text.split()]
+
+
+def test_choices_without_a_context():
+    """The first token of a sequence follows nothing and is not scored."""
+    from complexity_framework_b200.evaluation.benchmarks import choice_logprobs
+
+    m = tiny().eval()
+    with torch.no_grad():
+        lp = torch.log_softmax(m(torch.tensor([[5, 6, 7]]))["logits"][0], -1)
+        one = float(lp[0, 6])
+        two = one + float(lp[1, 7])
+    for normalize, want in ((False, [one, two]), (True, [one, two / 2])):
+        got = choice_logprobs(m, _Words, "", ["5 6", "5 6 7"], normalize)
+        assert got == pytest.approx(want, abs=1e-5)
+    with pytest.raises(ValueError, match="nothing to score"):
+        choice_logprobs(m, _Words, "", ["5", "5 6"])
+    want = choice_logprobs(m, _Words, "5", ["6", "6 7"])
+    assert want == pytest.approx([one, two / 2], abs=1e-5)
