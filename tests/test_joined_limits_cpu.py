@@ -177,3 +177,17 @@ def test_choices_without_a_context():
         choice_logprobs(m, _Words, "", ["5", "5 6"])
     want = choice_logprobs(m, _Words, "5", ["6", "6 7"])
     assert want == pytest.approx([one, two / 2], abs=1e-5)
+
+
+# ---------------------------------------------------------------- joins in a model
+@pytest.mark.parametrize("kind", ["adamw", "lion"])
+def test_weight_decay_leaves_the_joins_vectors_alone(kind):
+    """As it leaves every other norm's weight alone."""
+    from complexity_framework_b200.training.optim import default_param_groups
+    from complexity_framework_b200.training.optimizers import _decay_groups
+
+    m = tiny(**FULL)
+    groups = (default_param_groups if kind == "adamw" else _decay_groups)(m, 0.1)
+    decayed = {id(p) for g in groups if g["weight_decay"] > 0 for p in g["params"]}
+    names = [n for n, p in m.named_parameters() if p.dim() == 1 and id(p) in decayed]
+    assert not names, names
