@@ -97,13 +97,20 @@ class ResidualJoin(nn.Module):
     def forward(self, x: torch.Tensor, branch: torch.Tensor, next_norm: Optional[nn.Module] = None,
                 drop: bool = True):
         """``(x', next_norm(x'))``; the second is None without ``next_norm``.  ``drop=False``: no
-        dropout in training mode either (decoding)."""
+        dropout in training mode either (decoding).  Where the join's own weights have another
+        type than ``x``, both are taken in the wider one."""
         from ..ops.residual import new_seed, residual_norm
 
+        own = (self.weight, self.gate)
+        wide = x.dtype
+        for t in own:
+            wide = wide if t is None else torch.promote_types(wide, t.dtype)
+        x = x.to(wide)
+        weight, gate = (None if t is None else t.to(wide) for t in own)
         fused = (isinstance(next_norm, RMSNorm) and next_norm.eps == self.eps
                  and next_norm.weight.dtype == x.dtype)
         p = self.p if self.training and drop else 0.0
-        new, y = residual_norm(x, branch.to(x.dtype), branch_weight=self.weight, gate=self.gate,
+        new, y = residual_norm(x, branch.to(wide), branch_weight=weight, gate=gate,
                                norm_weight=next_norm.weight if fused else None, scale=self.scale,
                                p=p, seed=new_seed(x.device) if p > 0 else None,
                                stream=dropout_stream(), eps=self.eps)

@@ -191,3 +191,23 @@ def test_weight_decay_leaves_the_joins_vectors_alone(kind):
     decayed = {id(p) for g in groups if g["weight_decay"] > 0 for p in g["params"]}
     names = [n for n, p in m.named_parameters() if p.dim() == 1 and id(p) in decayed]
     assert not names, names
+
+
+@pytest.mark.parametrize("stream,weights", [(torch.bfloat16, torch.float32),
+                                            (torch.float32, torch.bfloat16)])
+def test_join_with_weights_of_another_type(stream, weights):
+    """The wider type of the two, as the plain norms compute."""
+    from complexity_framework_b200.core.layers import ResidualJoin, RMSNorm
+
+    torch.manual_seed(0)
+    j = ResidualJoin(8, gate_init=0.7).to(weights).eval()
+    j.weight.data.add_(0.1 * torch.randn(8))
+    n = RMSNorm(8).to(weights)
+    x, b = torch.randn(3, 8).to(stream), torch.randn(3, 8).to(stream)
+    new, y = j(x, b, n)
+    want = ResidualJoin(8, gate_init=0.7).eval()
+    want.load_state_dict({k: v.float() for k, v in j.state_dict().items()})
+    a, c = want(x.float(), b.float(), RMSNorm(8))
+    assert new.dtype == y.dtype == torch.float32
+    torch.testing.assert_close(new, a)
+    torch.testing.assert_close(y, c)
