@@ -44,7 +44,7 @@ class PipelineStage(nn.Module):
         self.first, self.last = first, last
         self.start, self.end = start, end
         self.layers = nn.ModuleList(list(model.layers)[start:end])
-        if model.config.embedding_dropout > 0:
+        if getattr(model.config, "embedding_dropout", 0.0) > 0:
             raise NotImplementedError("embedding_dropout in a pipeline stage")
         self.embed_tokens = model.embed_tokens if first else None
         self.norm = model.norm if last else None

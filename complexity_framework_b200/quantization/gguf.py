@@ -174,7 +174,7 @@ def _gguf_name(name: str) -> str:
 
 def export_gguf(model, path, qtype: GGUFQuantType = GGUFQuantType.Q8_0) -> Path:
     cfg = model.config
-    if cfg.joined_residual:
+    if getattr(cfg, "joined_residual", False):
         raise ValueError("the GGUF layout has no norms, gates or factors of the branches")
     w = GGUFWriter(path)
     a = w.arch

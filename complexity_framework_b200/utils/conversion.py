@@ -301,7 +301,7 @@ def save_to_huggingface(model, save_path: str, model_type: str = "llama", config
     from safetensors.torch import save_file
 
     cfg = config or model.config
-    if cfg.joined_residual:
+    if getattr(getattr(model, "config", None), "joined_residual", False):
         raise ValueError("the Llama layout has no norms, gates or factors of the branches")
     out = Path(save_path)
     out.mkdir(parents=True, exist_ok=True)

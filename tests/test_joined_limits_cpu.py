@@ -211,3 +211,29 @@ def test_join_with_weights_of_another_type(stream, weights):
     assert new.dtype == y.dtype == torch.float32
     torch.testing.assert_close(new, a)
     torch.testing.assert_close(y, c)
+
+
+# ------------------------------------------------------------------------- exports
+def test_exports_ask_the_model_about_its_joins(tmp_path):
+    """A configuration that is handed over may be any object with the layout's fields; what the
+    layout cannot hold is the model's."""
+    from complexity_framework_b200.quantization.gguf import export_gguf
+    from complexity_framework_b200.utils.conversion import save_to_huggingface
+
+    m = tiny(mlp_type="swiglu", tie_word_embeddings=False)
+    fields = {k: v for k, v in m.config.to_dict().items()
+              if not k.startswith("residual") and k not in ("norm_placement", "embedding_dropout")}
+    plain = types.SimpleNamespace(**fields)
+    save_to_huggingface(m, str(tmp_path / "a"), config=plain)
+    m.config = plain
+    export_gguf(m, tmp_path / "m.gguf")
+    with pytest.raises(ValueError, match="branches"):
+        save_to_huggingface(tiny(**FULL), str(tmp_path / "b"), config=plain)
+
+
+def test_pipeline_stage_of_a_model_with_a_plain_configuration():
+    from complexity_framework_b200.parallel.pipeline_parallel import PipelineStage
+
+    m = tiny()
+    m.config = types.SimpleNamespace(hidden_size=64, num_hidden_layers=2)
+    PipelineStage(m, 0, 1, True, False)
