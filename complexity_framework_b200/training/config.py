@@ -26,7 +26,8 @@ class TrainingConfig:
     wsd_decay_ratio: float = 0.2
     precision: str = "bf16"
     grad_clip: float = 1.0
-    # of the training loss only; evaluation reports the plain cross-entropy
+    # of the model's training loss only: evaluation reports the plain cross-entropy, and a
+    # compute_loss given to the trainer is called without them
     label_smoothing: float = 0.0
     z_loss_coef: float = 0.0
     skip_param_update_check: bool = False

@@ -97,6 +97,10 @@ class Trainer:
         self.total_tokens = 0
         self.best_loss = float("inf")
         self._compute_loss = compute_loss
+        if compute_loss is not None and (self.config.label_smoothing > 0
+                                         or self.config.z_loss_coef > 0):
+            logger.warning("label_smoothing and z_loss_coef are options of the model's own loss: "
+                           "the given compute_loss does not receive them")
         self._graphed = None
         self._canary = None
         self.should_stop = False

@@ -237,3 +237,20 @@ def test_pipeline_stage_of_a_model_with_a_plain_configuration():
     m = tiny()
     m.config = types.SimpleNamespace(hidden_size=64, num_hidden_layers=2)
     PipelineStage(m, 0, 1, True, False)
+
+
+# ------------------------------------------------------------------ training options
+def test_loss_options_beside_a_loss_of_ones_own_are_told(caplog):
+    from complexity_framework_b200.training import Trainer, TrainingConfig
+
+    def own(model, ids, labels):
+        return model.loss(ids, labels)
+
+    kw = dict(device=torch.device("cpu"), compute_loss=own)
+    for opt in (dict(label_smoothing=0.1), dict(z_loss_coef=1e-4)):
+        caplog.clear()
+        Trainer(tiny(), TrainingConfig(precision="fp32", **opt), **kw)
+        assert "compute_loss" in caplog.text and next(iter(opt)) in caplog.text
+    caplog.clear()
+    Trainer(tiny(), TrainingConfig(precision="fp32"), **kw)
+    assert "compute_loss" not in caplog.text
