@@ -220,7 +220,7 @@ def test_exports_ask_the_model_about_its_joins(tmp_path):
     from complexity_framework_b200.quantization.gguf import export_gguf
     from complexity_framework_b200.utils.conversion import save_to_huggingface
 
-    m = tiny(mlp_type="swiglu", tie_word_embeddings=False)
+    m = tiny(tie_word_embeddings=False)
     fields = {k: v for k, v in m.config.to_dict().items()
               if not k.startswith("residual") and k not in ("norm_placement", "embedding_dropout")}
     plain = types.SimpleNamespace(**fields)
