@@ -5,9 +5,10 @@
 * ``causal_lm_loss_from_hidden`` / ``fused_linear_causal_lm_loss``: CE of
   ``hidden @ W^T`` without materialising all logits.  On CUDA bf16 it is the
   sm_100a fused linear-CE (ops.fused.linear_cross_entropy) for the plain mean, and
-  ops.vocab_loss with label smoothing, z-loss, a logit scale or a vocabulary that is no
-  multiple of 32; elsewhere a chunked PyTorch loop with per-chunk recomputation
-  (complexity/core/losses/causal_lm.py:106-191, fused_ce.py:95-204).
+  ops.vocab_loss with label smoothing, z-loss, a positive logit scale or a vocabulary that is
+  no multiple of 32; elsewhere, and under torch.func or forward-mode differentiation, a chunked
+  PyTorch loop with per-chunk recomputation (complexity/core/losses/causal_lm.py:106-191,
+  fused_ce.py:95-204).
 * ``model_token_logprobs``: log-probabilities of given next tokens, without logits where
   ops.vocab_loss applies.
 """
@@ -18,6 +19,7 @@ from typing import Tuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint as activation_checkpoint
 
 from .layers import use_fused
@@ -68,6 +70,15 @@ def _chunk_ce(h: torch.Tensor, w: torch.Tensor, y: torch.Tensor, ignore_index: i
     return ce
 
 
+def _transformed(*tensors: torch.Tensor) -> bool:
+    """Whether torch.func transforms or forward-mode differentiation are at work, which the
+    kernels take no part in."""
+    if torch._C._are_functorch_transforms_active():
+        return True
+    return forward_ad._current_level >= 0 and any(
+        forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def causal_lm_loss_from_hidden(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                                *, ignore_index: int = -100, chunk_tokens: int = 8192,
                                logit_scale: float = 1.0, checkpoint_chunks: bool = True,
@@ -87,11 +98,12 @@ def causal_lm_loss_from_hidden(hidden: torch.Tensor, weight: torch.Tensor, label
             from ..ops.fused import linear_cross_entropy
 
             return linear_cross_entropy(h, weight, y, ignore_index=ignore_index)
-        from ..ops.vocab_loss import vocab_cross_entropy
+        if 0.0 < logit_scale < float("inf") and not _transformed(h, weight):
+            from ..ops.vocab_loss import vocab_cross_entropy
 
-        return vocab_cross_entropy(h, weight, y.long(), ignore_index=ignore_index,
-                                   label_smoothing=label_smoothing, z_loss=z_loss_coef,
-                                   logit_scale=logit_scale)
+            return vocab_cross_entropy(h, weight, y.long(), ignore_index=ignore_index,
+                                       label_smoothing=label_smoothing, z_loss=z_loss_coef,
+                                       logit_scale=logit_scale)
     total = h.new_zeros((), dtype=torch.float32)
     for s in range(0, h.shape[0], chunk_tokens):
         hc, yc = h[s:s + chunk_tokens], y[s:s + chunk_tokens]

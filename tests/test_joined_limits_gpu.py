@@ -2,10 +2,62 @@
 import pytest
 import torch
 
+from complexity_framework_b200.core.losses import causal_lm_loss_from_hidden
 from complexity_framework_b200.ops import check_errors
 from complexity_framework_b200.ops.vocab_loss import vocab_cross_entropy
 
 pytestmark = pytest.mark.gpu
+
+
+def rows(T=70, V=333, H=64, seed=0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    h = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(V, H, generator=g, device="cuda") * 0.2).bfloat16()
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    y[::5] = -100
+    return h, w, y
+
+
+# ------------------------------------------- calls of the loss that have no kernel
+@pytest.mark.parametrize("scale", [0.0, -0.5])
+def test_any_logit_scale(scale):
+    """A scale that is not positive is PyTorch's: the loop rounds the logits to bf16 (2^-9 of
+    some 3 at most) before it scales them, and the mean loss is off by no more."""
+    h, w, y = rows()
+    h.requires_grad_()
+    w.requires_grad_()
+    got = causal_lm_loss_from_hidden(h, w, y, logit_scale=scale)
+    want = torch.nn.functional.cross_entropy(scale * h.double() @ w.double().t(), y)
+    z = (h.double() @ w.double().t()).abs().max()
+    assert abs(float(got.detach()) - float(want.detach())) <= 2 * abs(scale) * 2.0 ** -8 * float(z) + 1e-5
+    for a, b in zip(torch.autograd.grad(got, (h, w)), torch.autograd.grad(want, (h, w))):
+        assert float((a.double() - b).norm()) <= 2.0 ** -6 * float(b.norm())
+
+
+def test_transforms_and_forward_derivatives():
+    """torch.func and forward-mode differentiation, which the kernels take no part in."""
+    import torch.autograd.forward_ad as fa
+
+    h, w, y = rows()
+
+    def loss(h):
+        return causal_lm_loss_from_hidden(h, w, y, checkpoint_chunks=False)
+
+    a = h.clone().requires_grad_()
+    want = torch.autograd.grad(loss(a), a)[0].double()
+    got = torch.func.grad(loss)(h).double()
+    # two ways of rounding a gradient: each off by two roundings to 8 bits at most
+    assert float((got - want).norm()) <= 4 * 2.0 ** -8 * float(want.norm())
+    three = torch.func.vmap(loss)(torch.stack((h, h * 2, h)))
+    one = torch.stack([loss(v) for v in (h, h * 2, h)])
+    # logits of up to some 6 rounded to 8 bits by one of the two
+    assert float((three - one).abs().max()) <= 6 * 2.0 ** -8
+    t = torch.randn(h.shape, device="cuda").bfloat16()
+    with fa.dual_level():
+        out = fa.unpack_dual(loss(fa.make_dual(h, t)))
+    slope = float((want * t.double()).sum())
+    mag = float((want * t.double()).abs().sum())
+    assert abs(float(out.tangent) - slope) <= 4 * 2.0 ** -8 * mag
 
 
 # ----------------------------------------------------------------- very many rows
