@@ -11,7 +11,6 @@
 
 int* cfb_err_ptr(int device);
 int cfb_num_sms(int device);
-torch::autograd::variable_list cfb_once_differentiable(torch::autograd::variable_list grads);
 
 namespace {
 
@@ -178,7 +177,128 @@ std::tuple<OptTensor, OptTensor> vocab_loss_bwd(const Tensor& gout_in, const Ten
 }
 
 using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
 using torch::autograd::variable_list;
+
+// What a backward pass knows beside its tensors.
+struct Options {
+  int64_t rows = 0;
+  double smooth = 0, z = 0, scale = 1, sign = 1;
+  bool per_row = false;
+  int64_t workspace = 0;
+  void put(AutogradContext* ctx) const {
+    ctx->saved_data["rows"] = rows;
+    ctx->saved_data["smooth"] = smooth;
+    ctx->saved_data["z"] = z;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["per_row"] = per_row;
+    ctx->saved_data["sign"] = sign;
+    ctx->saved_data["workspace"] = workspace;
+  }
+  static Options of(AutogradContext* ctx) {
+    const auto num = [&](const char* key) { return ctx->saved_data[key].toDouble(); };
+    Options o;
+    o.rows = ctx->saved_data["rows"].toInt();
+    o.smooth = num("smooth");
+    o.z = num("z");
+    o.scale = num("scale");
+    o.per_row = ctx->saved_data["per_row"].toBool();
+    o.sign = num("sign");
+    o.workspace = ctx->saved_data["workspace"].toInt();
+    return o;
+  }
+};
+
+// A part of the saved buffer (see place_saved) as a tensor.
+Tensor part(const Tensor& saved, const void* at, int64_t n, torch::ScalarType type) {
+  const int64_t first = static_cast<const char*>(at) - static_cast<const char*>(saved.data_ptr());
+  return saved.slice(0, first, first + n * static_cast<int64_t>(c10::elementSize(type))).view(type);
+}
+
+cfb::VlCall saved_call(const Tensor& saved, const Tensor& w, const Options& o) {
+  cfb::VlCall c = call_of(o.rows, w, o.scale, o.smooth, o.z, 0);
+  place_saved(&c, static_cast<char*>(saved.data_ptr()));
+  return c;
+}
+
+// hidden as the forward pass read it, rows that do not count 0.
+Tensor hidden_of(const Tensor& saved, const Tensor& w, const Options& o) {
+  const cfb::VlCall c = saved_call(saved, w, o);
+  const Tensor pos = part(saved, c.pos, o.rows, torch::kInt32).to(torch::kInt64);
+  const Tensor compact =
+      part(saved, c.hc, cfb::vl_rows(o.rows) * c.H, torch::kBFloat16).view({-1, c.H});
+  return compact.index_select(0, pos.clamp_min(0)).masked_fill_((pos < 0).unsqueeze(1), 0);
+}
+
+// The gradients in ATen operations, 32 bits, with all logits: what their own derivatives are taken
+// of.
+std::pair<Tensor, Tensor> plain_gradients(const Tensor& gout, const Tensor& h, const Tensor& w,
+                                          const Tensor& saved, const Options& o) {
+  const cfb::VlCall c = saved_call(saved, w, o);
+  const Tensor pos = part(saved, c.pos, o.rows, torch::kInt32).to(torch::kInt64);
+  const Tensor on = (pos >= 0).unsqueeze(1);
+  const Tensor target = part(saved, c.target, cfb::vl_rows(o.rows), torch::kInt32)
+                            .to(torch::kInt64)
+                            .index_select(0, pos.clamp_min(0))
+                            .clamp_min(0)
+                            .unsqueeze(1);
+  const Tensor hf = h.to(torch::kFloat32).masked_fill(~on, 0), wf = w.to(torch::kFloat32);
+  const Tensor z = at::matmul(hf, wf.t()) * o.scale;
+  const Tensor lse = z.logsumexp({1}, true);
+  Tensor g = o.per_row ? gout.unsqueeze(1)
+                       : (gout * part(saved, c.ginv, 1, torch::kFloat32)).expand({o.rows, 1});
+  g = (g * (o.sign * o.scale)).masked_fill(~on, 0);
+  Tensor dz = (z - lse).exp() * (1 + 2 * o.z * lse) - o.smooth / static_cast<double>(c.V);
+  dz = (g * dz).scatter_add(1, target, -(1 - o.smooth) * g);
+  return {at::matmul(dz, wf).to(h.scalar_type()), at::matmul(dz.t(), hf).to(w.scalar_type())};
+}
+
+// The gradients as a function of the loss's gradient, hidden and weight: the kernels' values, and
+// derivatives from plain_gradients.
+struct VocabLossGradNode : torch::autograd::Function<VocabLossGradNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& gout, const Tensor& h,
+                               const Tensor& w, const Tensor& saved, const Options& o, bool need_h,
+                               bool need_w) {
+    ctx->save_for_backward({gout, h, w, saved});
+    o.put(ctx);
+    ctx->saved_data["need_h"] = need_h;
+    ctx->saved_data["need_w"] = need_w;
+    ctx->set_materialize_grads(false);
+    const auto grads = vocab_loss_bwd(gout, saved, w, o.rows, o.smooth, o.z, o.scale, o.per_row,
+                                      o.sign, need_h, need_w, o.workspace);
+    variable_list out;
+    if (need_h) out.push_back(*std::get<0>(grads));
+    if (need_w) out.push_back(*std::get<1>(grads));
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list up) {
+    const Options o = Options::of(ctx);
+    const bool need_h = ctx->saved_data["need_h"].toBool(),
+               need_w = ctx->saved_data["need_w"].toBool(), again = at::GradMode::is_enabled();
+    auto saved = ctx->get_saved_variables();
+    variable_list out(7), outputs, factors, inputs;
+    std::vector<int> which;
+    at::AutoGradMode on(true);
+    for (int i = 0; i < 3; ++i) {
+      if (!ctx->needs_input_grad(i)) continue;
+      if (!again) saved[i] = saved[i].detach().requires_grad_();
+      inputs.push_back(saved[i]);
+      which.push_back(i);
+    }
+    const auto grads = plain_gradients(saved[0], saved[1], saved[2], saved[3], o);
+    const auto take = [&](const Tensor& value, const Tensor& factor) {
+      if (!factor.defined()) return;
+      outputs.push_back(value);
+      factors.push_back(factor);
+    };
+    if (need_h) take(grads.first, up[0]);
+    if (need_w) take(grads.second, up[need_h ? 1 : 0]);
+    if (outputs.empty() || inputs.empty()) return out;
+    const auto got = torch::autograd::grad(outputs, inputs, factors, again, again, true);
+    for (size_t k = 0; k < which.size(); ++k) out[which[k]] = got[k];
+    return out;
+  }
+};
 
 struct VocabLossNode : torch::autograd::Function<VocabLossNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& y,
@@ -189,26 +309,51 @@ struct VocabLossNode : torch::autograd::Function<VocabLossNode> {
     // the caller's weight itself where it was read in place, so that a change to it before the
     // backward pass is noticed
     ctx->save_for_backward({saved, read.data_ptr() == w.data_ptr() ? w : read});
-    ctx->saved_data["rows"] = h.size(0);
-    ctx->saved_data["smooth"] = smooth;
-    ctx->saved_data["z"] = z;
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["per_row"] = reduction == 0;
-    ctx->saved_data["sign"] = sign;
-    ctx->saved_data["workspace"] = workspace_bytes;
+    Options o;
+    o.rows = h.size(0);
+    o.smooth = smooth;
+    o.z = z;
+    o.scale = scale;
+    o.sign = sign;
+    o.per_row = reduction == 0;
+    o.workspace = workspace_bytes;
+    o.put(ctx);
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list gout) {
-    const auto saved = ctx->get_saved_variables();
-    const auto num = [&](const char* key) { return ctx->saved_data[key].toDouble(); };
-    const auto grads = vocab_loss_bwd(
-        gout[0].detach(), saved[0], saved[1].detach(), ctx->saved_data["rows"].toInt(),
-        num("smooth"), num("z"), num("scale"), ctx->saved_data["per_row"].toBool(), num("sign"),
-        ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->saved_data["workspace"].toInt());
+    const auto v = ctx->get_saved_variables();
+    const Options o = Options::of(ctx);
+    const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     variable_list out(10);
-    if (std::get<0>(grads).has_value()) out[0] = *std::get<0>(grads);
-    if (std::get<1>(grads).has_value()) out[1] = *std::get<1>(grads);
-    return cfb_once_differentiable(std::move(out));
+    if (!at::GradMode::is_enabled() || o.rows == 0) {
+      const auto grads =
+          vocab_loss_bwd(gout[0].detach(), v[0], v[1].detach(), o.rows, o.smooth, o.z, o.scale,
+                         o.per_row, o.sign, need_h, need_w, o.workspace);
+      if (std::get<0>(grads).has_value()) out[0] = *std::get<0>(grads);
+      if (std::get<1>(grads).has_value()) out[1] = *std::get<1>(grads);
+      return out;
+    }
+    // Under create_graph the gradients stay part of the graph.  hidden, and a weight that was
+    // copied, take the edges of the call's own tensors.
+    const auto node = torch::autograd::get_current_node();
+    const auto joined = [&](Tensor t, int i) {
+      const auto edge = node->next_edge(i);
+      if (edge.is_valid()) torch::autograd::impl::set_gradient_edge(t, edge);
+      return t;
+    };
+    Tensor h, w = v[1];
+    {
+      at::NoGradGuard no_grad;
+      h = hidden_of(v[0], w, o);
+      if (need_w && !w.requires_grad()) w = w.clone();
+    }
+    h = joined(h, 0);
+    if (need_w && !w.requires_grad()) w = joined(w, 1);
+    const auto grads = VocabLossGradNode::apply(gout[0], h, w, v[0], o, need_h, need_w);
+    size_t k = 0;
+    if (need_h) out[0] = grads[k++];
+    if (need_w) out[1] = grads[k++];
+    return out;
   }
 };
 

@@ -60,6 +60,60 @@ def test_transforms_and_forward_derivatives():
     assert abs(float(out.tangent) - slope) <= 4 * 2.0 ** -8 * mag
 
 
+def test_second_derivatives():
+    """Gradients of gradients, against the formula in 64 bits."""
+    h, w, y = rows()
+    gen = torch.Generator("cuda").manual_seed(5)
+    u, v = (torch.randn(t.shape, generator=gen, device="cuda") for t in (h, w))
+    up = torch.randn(70, generator=gen, device="cuda")
+
+    def second(f, h, w, factor):
+        h, w, factor = (t.detach().clone().requires_grad_() for t in (h, w, factor))
+        hh = h * 1.0  # not a leaf
+        loss = f(hh, w)
+        if loss.dim():
+            first = torch.autograd.grad(loss, (hh, w), factor.to(loss.dtype), create_graph=True)
+        else:
+            first = torch.autograd.grad(loss, (hh, w), factor[0].to(loss.dtype), create_graph=True)
+        dot = (first[0] * u.to(first[0].dtype)).sum() + (first[1] * v.to(first[1].dtype)).sum()
+        return [t.detach().double() for t in first], \
+            [t.double() for t in torch.autograd.grad(dot, (h, w, factor))]
+
+    def kernel(**kw):
+        return lambda h, w: vocab_cross_entropy(h, w, y, **kw)
+
+    def formula(smooth=0.0, z=0.0, scale=1.0, reduction="mean"):
+        def f(h, w):
+            zl = scale * h @ w.t()
+            keep = y != -100
+            lse = torch.logsumexp(zl, -1)
+            loss = lse - (1 - smooth) * zl.gather(1, y.clamp_min(0)[:, None])[:, 0] \
+                - smooth * zl.mean(-1) + z * lse ** 2
+            loss = torch.where(keep, loss, 0.0)
+            return {"none": loss, "sum": loss.sum(), "mean": loss.sum() / keep.sum()}[reduction]
+        return f
+
+    for red in ("none", "sum", "mean"):
+        for smooth, z, scale in ((0.0, 0.0, 1.0), (0.1, 1e-2, 0.5)):
+            got = second(kernel(label_smoothing=smooth, z_loss=z, logit_scale=scale,
+                                reduction=red), h, w, up)
+            want = second(formula(smooth, z, scale, red), h.double(), w.double(), up.double())
+            # the first gradient is the kernels': dz and the result rounded to 8 bits
+            for a, b in zip(got[0], want[0]):
+                assert float((a - b).norm()) <= 2 * 2.0 ** -8 * float(b.norm())
+            # u and v are rounded to 8 bits, then the result: 2^-9 each in the mean
+            for a, b in zip(got[1], want[1]):
+                assert float((a - b).norm()) <= 4 * 2.0 ** -8 * float(b.norm())
+    a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+    plain = torch.autograd.grad(vocab_cross_entropy(a, b, y), (a, b))
+    graph = torch.autograd.grad(vocab_cross_entropy(a, b, y), (a, b), create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(plain, graph))
+    # the frozen one has no part
+    only = torch.autograd.grad(vocab_cross_entropy(a, w, y), a, create_graph=True)[0]
+    assert torch.autograd.grad(only.float().square().sum(), a)[0].isfinite().all()
+    check_errors()
+
+
 # ----------------------------------------------------------------- very many rows
 def test_losses_of_very_many_rows():
     """More rows than the blocks of the gathering kernel take at a time, ignored ones among them:
