@@ -164,3 +164,73 @@ def test_time_grows_with_the_rows():
 
     few, many = best(1 << 20), best(1 << 22)
     assert many <= 7 * few, (few, many)
+
+
+# ------------------------------------------------------- joins of many rows, in parts
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+LEFT_OUT = ["none", "w1", "gate", "w2", "dy", "dx", "w1 w2", "w1 gate w2"]
+
+
+@pytest.mark.parametrize("left_out", LEFT_OUT)
+@pytest.mark.parametrize("H", [264, 896, 903, 2048, 8192])
+@pytest.mark.parametrize("dtype,p", [("bf16", 0.0), ("bf16", 0.2), ("fp32", 0.2)])
+def test_join_parts_with_many_rows(left_out, H, dtype, p):
+    """Rows enough that one or two warps take a row each, without a norm, gate or gradient."""
+    from test_residual_gpu import call, check, make, oracle
+
+    off = left_out.split()
+    t = make(2501, H, DT[dtype], "w1" not in off, "gate" not in off, "w2" not in off, seed=H)
+    if "dy" in off or "dx" in off:
+        from complexity_framework_b200.ops import residual as R
+
+        one = {**t, **{k: torch.zeros_like(t[k]) for k in ("dx", "dy") if k in off}}
+        want, tol = oracle(one, 0.7, p, 3, 0)
+        leaf = {k: t[k].detach().clone().requires_grad_() for k in ("x", "b", "w1", "gate", "w2")}
+        new, y = R.residual_norm(leaf["x"], leaf["b"], branch_weight=leaf["w1"],
+                                 gate=leaf["gate"], norm_weight=leaf["w2"], scale=0.7, p=p,
+                                 seed=3)
+        (new if "dy" in off else y).backward(t["dx" if "dy" in off else "dy"])
+        got = {"d" + k: v.grad for k, v in leaf.items() if v.grad is not None}
+        assert ("dw2" in got) == ("dx" in off)
+    else:
+        want, tol = oracle(t, 0.7, p, 3, 0)
+        got = call(t, 0.7, p, 3 if p else None, 0)
+    check(got, want, tol, DT[dtype])
+    check_errors()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_resumed_run_goes_on_with_the_masks(tmp_path, graph):
+    """A learning rate of nearly nothing: the losses of a step differ by their masks alone.  The
+    model's other kernels add some gradients by atomics, which reach a loss by less than 1e-3."""
+    from complexity_framework_b200 import ComplexityModel
+    from complexity_framework_b200.config import ModelConfig
+    from complexity_framework_b200.training import Trainer, TrainingConfig
+
+    def trainer():
+        torch.manual_seed(0)
+        m = ComplexityModel(ModelConfig(
+            hidden_size=256, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+            intermediate_size=256, shared_intermediate_size=256, vocab_size=1000, num_experts=2,
+            top_k=2, max_position_embeddings=256, residual_dropout=0.3, embedding_dropout=0.2,
+            norm_placement="sandwich"))
+        return Trainer(m, TrainingConfig(learning_rate=1e-8, precision="bf16", warmup_steps=0,
+                                         lr_scheduler="constant", weight_decay=0.0,
+                                         cuda_graph=graph, cuda_graph_warmup=2,
+                                         skip_param_update_check=True,
+                                         checkpoint_dir=str(tmp_path)))
+
+    ids = torch.randint(0, 1000, (2, 64)).pin_memory()
+    a = trainer()
+    for _ in range(4):
+        a.train_step(ids)
+    a.save_checkpoint()
+    want = [a.train_step(ids) for _ in range(4)]
+    b = trainer()
+    torch.cuda.manual_seed(77)
+    assert b.resume("auto")
+    got = [b.train_step(ids) for _ in range(4)]
+    spread = max(abs(p - q) for p in want for q in want)
+    assert spread > 5e-3
+    assert max(abs(p - q) for p, q in zip(got, want)) <= 1e-3, (got, want)
+    check_errors()
