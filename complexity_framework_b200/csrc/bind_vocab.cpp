@@ -11,6 +11,7 @@
 
 int* cfb_err_ptr(int device);
 int cfb_num_sms(int device);
+torch::autograd::variable_list cfb_once_differentiable(torch::autograd::variable_list grads);
 
 namespace {
 
@@ -325,17 +326,19 @@ struct VocabLossNode : torch::autograd::Function<VocabLossNode> {
     const Options o = Options::of(ctx);
     const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     variable_list out(10);
-    if (!at::GradMode::is_enabled() || o.rows == 0) {
+    // under create_graph the engine runs this node; a node that is called by itself is not known
+    const auto node = std::dynamic_pointer_cast<torch::autograd::CppNode<VocabLossNode>>(
+        torch::autograd::get_current_node());
+    if (!at::GradMode::is_enabled() || o.rows == 0 || node == nullptr) {
       const auto grads =
           vocab_loss_bwd(gout[0].detach(), v[0], v[1].detach(), o.rows, o.smooth, o.z, o.scale,
                          o.per_row, o.sign, need_h, need_w, o.workspace);
       if (std::get<0>(grads).has_value()) out[0] = *std::get<0>(grads);
       if (std::get<1>(grads).has_value()) out[1] = *std::get<1>(grads);
-      return out;
+      return cfb_once_differentiable(std::move(out));
     }
-    // Under create_graph the gradients stay part of the graph.  hidden, and a weight that was
-    // copied, take the edges of the call's own tensors.
-    const auto node = torch::autograd::get_current_node();
+    // The gradients stay part of the graph: hidden, and a weight that was copied, take the edges
+    // of the call's own tensors.
     const auto joined = [&](Tensor t, int i) {
       const auto edge = node->next_edge(i);
       if (edge.is_valid()) torch::autograd::impl::set_gradient_edge(t, edge);

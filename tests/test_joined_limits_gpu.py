@@ -114,6 +114,26 @@ def test_second_derivatives():
     check_errors()
 
 
+def test_second_derivatives_in_other_layouts():
+    """A weight that is copied for the call, three dimensions, a node that is called by itself."""
+    h, w, y = rows()
+    wt = w.t().contiguous().requires_grad_()
+    a = h.clone().requires_grad_()
+    b, c = w.clone().requires_grad_(), h.view(2, 35, 64).clone().requires_grad_()
+    out = []
+    for x, m, leaf, t in ((a, wt.t(), wt, y), (c, b, b, y.view(2, 35))):
+        loss = vocab_cross_entropy(x, m, t, z_loss=1e-3)
+        gx, gm = torch.autograd.grad(loss, (x, m), create_graph=True)
+        out.append(torch.autograd.grad(gx.float().square().sum() + gm.float().square().sum(),
+                                       (x, leaf)))
+    assert torch.equal(out[0][0], out[1][0].view(70, 64)) and torch.equal(out[0][1].t(), out[1][1])
+    loss = vocab_cross_entropy(a, b, y)
+    want = torch.autograd.grad(loss, (a, b), retain_graph=True)
+    got = loss.grad_fn(torch.ones((), device="cuda"))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    check_errors()
+
+
 # ----------------------------------------------------------------- very many rows
 def test_losses_of_very_many_rows():
     """More rows than the blocks of the gathering kernel take at a time, ignored ones among them:
