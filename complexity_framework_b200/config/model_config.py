@@ -147,8 +147,9 @@ class ModelConfig:
     # normalisation
     norm_type: str = "rmsnorm"
     norm_eps: float = 1e-6
-    # residual stream: "sandwich" also normalises what a branch adds; a learned gate of each
-    # channel (from this value), a factor and dropout of the branches, dropout of the embedding
+    # residual stream: "sandwich" also normalises what a branch adds, by its rms whatever
+    # norm_type is; a learned gate of each channel (from this value), a factor and dropout of the
+    # branches, dropout of the embedding
     norm_placement: str = "pre"
     residual_gate_init: Optional[float] = None
     residual_scale: float = 1.0

@@ -578,15 +578,17 @@ __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float 
                : "memory");
 }
 
-// fast-math intrinsics: results are rounded to bf16 right after
-// sigmoid(x) = 0.5 * tanh(x / 2) + 0.5: one MUFU op (tanh.approx, max relative
-// error about 2^-11) instead of ex2 + reciprocal; the SwiGLU GEMM epilogues are
-// bound by their per-element work.
+// 2^x, off by some 2^-22 of itself
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// fast-math intrinsics: results are rounded to bf16 right after
+// sigmoid(x) = 0.5 * tanh(x / 2) + 0.5: one MUFU op (tanh.approx, max relative
+// error about 2^-11) instead of ex2 + reciprocal; the SwiGLU GEMM epilogues are
+// bound by their per-element work.
 __device__ __forceinline__ float tanh_approx(float x) {
   float y;
   asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -15,17 +15,22 @@
 //
 // The products of 8192 x 32000 x 896, ncu at the 1.46 GHz of the power limit: logits 289 us
 // with the tensor pipe active 92 % of the time, dz 328 us (79 %), dh 356 (75 %), dW 335 (79 %).  A
-// whole call with gradients: 32768 x 32000 x 896 in 6.8 ms, 4096 x 100000 x 4096 in 10.2 ms (1.1
+// whole call with gradients: 32768 x 32000 x 896 in 7.0 ms, 4096 x 100000 x 4096 in 10.4 ms (1.1
 // and 1.3 PFLOP/s of the four products; cuBLAS runs 1.41 back to back).
 //
 // Rows that do not count (ignored targets) are left out before the first product: the others are
 // gathered in their order, and the products take their number from device memory.  A batch with
 // half of its tokens ignored costs half, and what an ignored row holds reaches nothing.
 //
-// dz is rounded to bf16, as the tensor cores' operand; its sums are fp32.  The factors that all
+// dz is rounded to bf16, as the tensor cores' operand (gradients are off by up to 0.0024, root mean
+// square, where their own rounding gives 0.0017); its sums are fp32.  The factors that all
 // rows share (1 / counted rows, the incoming gradient, scale, 1 - eps) are left to the products'
 // epilogues, so that a target's term is p - 1 and the -1 is exact: scaled first, every target's
-// term would be off by the same part of up to 2^-9.  No sum depends on the order of atomics: equal calls give equal bits.
+// term would be off by the same part of up to 2^-9.  What rounding the target's term takes is put back
+// into dh (vl_scatter_k); in dW, a sum over rows with errors of either sign, it stays.  The
+// exponentials are ex2.approx's (2^-22): row losses are off by 3.4e-7 of their size where fp32
+// elementary operations give 1.3e-7.  No sum depends on the order of atomics: equal calls give
+// equal bits.
 #include <algorithm>
 #include <cmath>
 
@@ -325,10 +330,11 @@ int vl_forward(const VlCall& c, const VlForward& f, cudaStream_t s) {
 //
 // One piece where the workspace holds all of dz; else about 256 MB of it, but at least 4096 words:
 // of two L2 caches' worth the next product still finds some, while every piece costs three launches
-// and dh read and written once more.  32768 x 32000 x 896 in 128, 256, 512, 2048 MB: 9.8, 6.4, 6.5,
-// 6.9 ms; 4096 x 100000 x 4096 in 64, 192, 256, 512 MB: 11.0, 10.1, 10.1, 10.5 ms; one piece against
-// two of 3001 x 50021 x 1024: 0.93, 1.01 ms.  (Back to back for a second, a card at its power limit
-// takes 6.7 to 6.9 ms for the first whatever the piece.)
+// and dh read and written once more.  Back to back at the power limit, 32768 x 32000 x 896 in 128,
+// 256, 512, 2048 MB of workspace: 8.8, 6.9, 6.9, 6.5 ms (the last is one piece, in four times the
+// memory); 4096 x 100000 x 4096 in 64, 192, 256, 512 MB: 10.5, 10.2, 10.1, 10.1 ms; one piece against
+// two of 3001 x 50021 x 1024: 0.93, 1.01 ms.  With more rows the pieces get smaller: 131072 rows of
+// 32000 x 896 take 16 of them, 34.7 ms, of which the 470 MB of dh that each reads and writes are 2.
 //
 // dh has few tiles (256 x 256, one CTA pair each): 48 at 3000 x 1024 for 74 pairs.  It is cut along
 // the words into the slices that fill the waves of pairs best; as the counted rows may be any part

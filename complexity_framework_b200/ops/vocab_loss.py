@@ -8,16 +8,20 @@ target is the word ``y`` has the loss
 
 The logits exist a tile at a time: the forward pass leaves a row's log-sum-exp, the backward
 pass computes the logits again, for as much of the vocabulary at a time as ``workspace_bytes``
-holds gradients of (bf16), beside an fp32 accumulator of ``hidden``'s gradient.  They are fp32 throughout, where ``ops.fused.linear_cross_entropy``
-keeps them, rounded to bf16, for the mean loss alone.
+holds gradients of (bf16), but 256 words at least.  Beside it are a copy of the counted rows and
+one or more fp32 accumulators of ``hidden``'s gradient (few rows of few channels take more, so
+that their products fill the GPU: 18 at 2048 x 50000 x 256), which ``workspace_bytes`` does not
+count.  The logits are fp32 throughout, where ``ops.fused.linear_cross_entropy`` keeps them,
+rounded to bf16, for the mean loss alone.
 
 Rows whose target is ``ignore_index`` have the loss 0, add nothing to a gradient whatever they
 hold, and cost nothing in the products.  A target that is neither a word nor ``ignore_index`` is
 reported by ``ops.check_errors`` and its row's loss is NaN.
 
 On CUDA ``hidden`` and ``weight`` are bfloat16 with a hidden size that is a multiple of 8 (any
-number of rows and words); the gradients are bfloat16, and equal calls give equal bits.  On the
-CPU the same formulas run in PyTorch, any floating-point type.
+number of rows and words); the gradients are bfloat16, and equal calls give equal bits.  The
+gradients' own derivatives (``create_graph``) are computed in PyTorch from all logits in fp32.  On
+the CPU the same formulas run in PyTorch, any floating-point type.
 """
 from __future__ import annotations
 
