@@ -28,15 +28,14 @@ import torch
 
 
 def default_param_groups(model: torch.nn.Module, weight_decay: float) -> List[dict]:
-    """Decay / no-decay split by name, as the reference trainer does; a residual join's norm
-    weight and gate go with the norms."""
+    """Decay / no-decay split by name, as the reference trainer does."""
     decay, no_decay, local = [], [], []
     for name, p in model.named_parameters():
         if not p.requires_grad:
             continue
         if getattr(p, "_ep_local", False):
             local.append(p)
-        elif "bias" in name or "norm" in name or ".mu" in name or "_join." in name:
+        elif "bias" in name or "norm" in name or ".mu" in name:
             no_decay.append(p)
         else:
             decay.append(p)

@@ -800,7 +800,7 @@ def _decay_groups(model: torch.nn.Module, weight_decay: float) -> List[dict]:
     for name, p in model.named_parameters():
         if not p.requires_grad:
             continue
-        if "bias" in name or "norm" in name or "embed" in name or "_join." in name:
+        if "bias" in name or "norm" in name or "embed" in name:
             nodecay.append(p)
         else:
             decay.append(p)

@@ -180,19 +180,6 @@ def test_choices_without_a_context():
 
 
 # ---------------------------------------------------------------- joins in a model
-@pytest.mark.parametrize("kind", ["adamw", "lion"])
-def test_weight_decay_leaves_the_joins_vectors_alone(kind):
-    """As it leaves every other norm's weight alone."""
-    from complexity_framework_b200.training.optim import default_param_groups
-    from complexity_framework_b200.training.optimizers import _decay_groups
-
-    m = tiny(**FULL)
-    groups = (default_param_groups if kind == "adamw" else _decay_groups)(m, 0.1)
-    decayed = {id(p) for g in groups if g["weight_decay"] > 0 for p in g["params"]}
-    names = [n for n, p in m.named_parameters() if p.dim() == 1 and id(p) in decayed]
-    assert not names, names
-
-
 @pytest.mark.parametrize("stream,weights", [(torch.bfloat16, torch.float32),
                                             (torch.float32, torch.bfloat16)])
 def test_join_with_weights_of_another_type(stream, weights):
